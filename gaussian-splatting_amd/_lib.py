@@ -22,9 +22,10 @@ SYMBOLS = [
     "gsx_keep_flags", "gsx_compact_rows", "gsx_clamp_inplace",
     "gsx_merge_workspace_bytes", "gsx_merge_count", "gsx_merge_fill", "gsx_merge_greedy_host", "gsx_train_step", "gsx_train_step_grads", "gsx_train_step_apply",
     "gsx_comm_available", "gsx_comm_unique_id", "gsx_comm_init", "gsx_allreduce_avg", "gsx_bcast", "gsx_comm_destroy",
+    "gsx_gated_marks_floats", "gsx_gated_scan_fwd", "gsx_gated_scan_bwd", "gsx_gated_step", "gsx_draw_workspace_bytes", "gsx_draw_indices",
 ]
 
-ABI_VERSION = 20            # GSX_ABI_VERSION of include/gsx.h (tests check that the two agree)
+ABI_VERSION = 21            # GSX_ABI_VERSION of include/gsx.h (tests check that the two agree)
 GSX_OK, GSX_E_INVALID, GSX_E_CAPACITY, GSX_E_HIP, GSX_E_RANGE, GSX_E_AGAIN, GSX_E_COMM = 0, -1, -2, -3, -4, -5, -6
 RANK_NONE = 0xFFFFFFFF
 REC_FLOATS = int(os.environ.get("GSX_REC_FLOATS", "12"))      # (16 only with a library built for the 64-byte-stride experiment)
@@ -62,6 +63,21 @@ class GsxStep(C.Structure):
                 ("mean2d", _p), ("depth", _p), ("cov2d", _p), ("rgb", _p), ("alpha", _p), ("state", _p), ("d_rgb", _p), ("loss", _p),
                 ("loss_ws", _p), ("loss_ws_bytes", _sz), ("adam_ws", _p), ("adam_ws_bytes", _sz),
                 ("counts_pinned_host", _p), ("count_event", _p)]
+
+
+class GsxGated(C.Structure):
+    """struct gsx_gated of include/gsx.h"""
+    _fields_ = [("dtype", _i32), ("form", _i32), ("reverse", _i32), ("planes", _i32), ("B", _i64), ("T", _i64), ("D", _i64),
+                ("gate", _p), ("gate_stride", _i64 * 2), ("x", _p), ("x_stride", _i64 * 3), ("initial", _p), ("lengths", _p),
+                ("states", _p), ("last", _p), ("marks", _p), ("d_states", _p), ("d_states_stride", _i64 * 3), ("d_last", _p),
+                ("d_gate", _p), ("d_x", _p), ("d_initial", _p)]
+
+
+class GsxDraw(C.Structure):
+    """struct gsx_draw of include/gsx.h"""
+    _fields_ = [("dtype", _i32), ("uniforms_f64", _i32), ("R", _i64), ("V", _i64), ("S", _i64), ("logits", _p), ("row_stride", _i64), ("uniforms", _p),
+                ("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("top_k", _i32),
+                ("temperatures", _p), ("top_ps", _p), ("min_ps", _p), ("top_ks", _p), ("indices", _p), ("logprobs", _p), ("ws", _p), ("ws_bytes", _sz)]
 
 
 def lib():
@@ -122,9 +138,15 @@ def lib():
     L.gsx_l1_ssim_workspace_bytes.restype = _sz; L.gsx_l1_ssim_workspace_bytes.argtypes = [_i32, _i32, _i32]
     L.gsx_l1_ssim_fwd.argtypes = [_p, _p, _i32, _i32, _i32, C.c_float, _p, _p, _sz, _p]
     L.gsx_l1_ssim_bwd.argtypes = [_p, _p, _i32, _i32, _i32, C.c_float, _p, _p, _sz, _p, _p]
+    L.gsx_gated_marks_floats.restype = _i64; L.gsx_gated_marks_floats.argtypes = [_i64, _i64, _i32, _i64]
+    L.gsx_gated_scan_fwd.argtypes = [C.POINTER(GsxGated), _p]
+    L.gsx_gated_scan_bwd.argtypes = [C.POINTER(GsxGated), _p]
+    L.gsx_gated_step.argtypes = [_i32, _i32, _i64, _p, _p, _p, _p]
+    L.gsx_draw_workspace_bytes.restype = _sz; L.gsx_draw_workspace_bytes.argtypes = [C.POINTER(GsxDraw)]
+    L.gsx_draw_indices.argtypes = [C.POINTER(GsxDraw), _p]
     for name in SYMBOLS:
         getattr(L, name)
-        if name not in ("gsx_strerror", "gsx_last_hip_error", "gsx_abi_version") and not name.endswith("_bytes") and name not in ("gsx_max_chunks", "gsx_view_layout", "gsx_chunk_state_floats"):
+        if name not in ("gsx_strerror", "gsx_last_hip_error", "gsx_abi_version") and not name.endswith("_bytes") and name not in ("gsx_max_chunks", "gsx_view_layout", "gsx_chunk_state_floats", "gsx_gated_marks_floats"):
             getattr(L, name).restype = C.c_int
     _lib = L
     return L

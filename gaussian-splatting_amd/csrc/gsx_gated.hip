@@ -1,0 +1,380 @@
+// gsx_gated.hip -- the gated linear recurrence h_t = a_t h_(t-1) + b_t along one axis, and its gradients: the compositing formula
+// ("over", front index 0, last layer first) without the splats, for layers, traces and sequences of any length.
+//   linear  a = z,     b = x         blend  a = 1 - z, b = z x         over  a = 1 - z, b = x
+// Backward, from the last step to the first with c = dL/dh flowing back:  g_t = d_t + c,  dx = g (z g for blend),
+// dz = g h_(t-1) (linear), g (x - h_(t-1)) (blend), -g h_(t-1) (over),  c = a_t g_t;  dL/dinitial is the c that leaves the first step.
+// Three to eight flops per element against 6 to 16 bytes: HBM bounds it.  A lane owns a channel (NV neighbouring ones, or R planes that
+// share a gate) and walks the steps in batches of K whose loads are all in flight together; the state stays in a 32-bit register.
+// The backward needs h_(t-1) in 32 bits, not as `states` rounds it: the forward leaves the state in front of every K-th step ("marks",
+// 4 / K bytes per element) and the backward runs each batch forward again from its mark, in registers.  It then reads gate, x and
+// the states' gradient, once each -- as much as a backward that reads `states` instead of x, and `states` need not exist.
+#include "gsx_common.h"
+
+namespace gsx {
+
+constexpr int kGatedWaves = 4;
+
+template <int R>
+struct GatedBatch { static constexpr int value = R == 1 ? 16 : 8; };        // K: steps in flight; planes multiply the registers
+
+struct GatedArgs {
+    const void* gate; const void* x; const float* initial; const int32_t* lengths;
+    void* states; float* last; float* marks;
+    const void* d_states; const float* d_last; void* d_gate; void* d_x; float* d_initial;
+    long long T, groups, row;                  // steps, lanes' groups of NV channels in all, groups of one sequence
+    long long D;
+    long long gate_b, gate_t, x_b, x_t, x_r, ds_b, ds_t, ds_r;
+    int form, reverse;
+};
+
+template <typename T, int NV>
+struct alignas(sizeof(T) * NV) Pack { T v[NV]; };
+
+template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }         // round to nearest even
+
+// coefficients of one step: a, and m of b = m x
+__device__ __forceinline__ void gated_am(int form, float z, float& a, float& m)
+{
+    a = form == GSX_GATED_LINEAR ? z : 1.0f - z;
+    m = form == GSX_GATED_BLEND ? z : 1.0f;
+}
+
+// A lane's place: which sequence and channels, and where its steps lie.  Scan position s is memory step s, or T - 1 - s in reverse;
+// the sequence's own steps are scan positions [lo, hi) (a padded sequence in reverse starts behind its padding).
+struct Lane {
+    long long b, d, lo, hi;
+    bool on;
+};
+
+template <int NV>
+__device__ __forceinline__ Lane lane_of(const GatedArgs& p, long long group)
+{
+    Lane l;
+    l.on = group < p.groups;
+    const long long g = l.on ? group : p.groups - 1;
+    if (p.groups < (1ll << 31)) {                                            // 32-bit division where it is enough
+        const uint32_t q = (uint32_t)g / (uint32_t)p.row;
+        l.b = q; l.d = (long long)((uint32_t)g - q * (uint32_t)p.row) * NV;
+    } else {
+        l.b = g / p.row; l.d = (g - l.b * p.row) * NV;
+    }
+    long long len = p.T;
+    if (p.lengths) { const int n = p.lengths[l.b]; len = n < 0 ? 0 : n < p.T ? n : p.T; }
+    l.lo = p.reverse ? p.T - len : 0;
+    l.hi = p.reverse ? p.T : len;
+    if (!l.on) { l.lo = 0; l.hi = 0; }
+    return l;
+}
+
+template <typename T, int NV, int R, int K, bool WHOLE>
+__device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& l, long long s0, float (&h)[R][NV])
+{
+    using P = Pack<T, NV>;
+    P z[K], x[K][R];
+    const long long dir = p.reverse ? -1 : 1, m0 = p.reverse ? p.T - 1 - s0 : s0;
+    const T* gp = (const T*)p.gate + l.b * p.gate_b + m0 * p.gate_t + l.d;
+    const T* xp = (const T*)p.x + l.b * p.x_b + m0 * p.x_t + l.d;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+        if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
+            z[k] = *(const P*)(gp + dir * k * p.gate_t);
+#pragma unroll
+            for (int r = 0; r < R; r++) x[k][r] = *(const P*)(xp + dir * k * p.x_t + r * p.x_r);
+        }
+    T* sp = p.states ? (T*)p.states + ((l.b * p.T + m0) * R) * p.D + l.d : nullptr;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const bool in = WHOLE || (s0 + k >= l.lo && s0 + k < l.hi);
+        if (in) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                float a, m;
+                gated_am(p.form, to_f(z[k].v[i]), a, m);
+#pragma unroll
+                for (int r = 0; r < R; r++) h[r][i] = __builtin_fmaf(a, h[r][i], m * to_f(x[k][r].v[i]));
+            }
+        }
+        if (sp && (WHOLE || (l.on && s0 + k < p.T))) {
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                P o;
+#pragma unroll
+                for (int i = 0; i < NV; i++) o.v[i] = in ? from_f<T>(h[r][i]) : from_f<T>(0.0f);
+                *(P*)(sp + (dir * k * R + r) * p.D) = o;
+            }
+        }
+    }
+}
+
+template <typename T, int NV, int R>
+__global__ __launch_bounds__(64 * kGatedWaves) void gated_fwd_kernel(GatedArgs p)
+{
+    constexpr int K = GatedBatch<R>::value;
+    const long long group = (long long)blockIdx.x * (64 * kGatedWaves) + threadIdx.x;
+    const Lane l = lane_of<NV>(p, group);
+    const long long out = (l.b * R) * p.D + l.d;                             // in B x R x D
+    float h[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int i = 0; i < NV; i++) h[r][i] = p.initial ? p.initial[out + r * p.D + i] : 0.0f;
+    for (long long s0 = 0; s0 < p.T; s0 += K) {
+        if (p.marks && l.on) {
+            float* mk = p.marks + (s0 / K) * R * p.groups * NV + group * NV;
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                Pack<float, NV> o;
+#pragma unroll
+                for (int i = 0; i < NV; i++) o.v[i] = h[r][i];
+                *(Pack<float, NV>*)(mk + r * p.groups * NV) = o;
+            }
+        }
+        if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fwd_batch<T, NV, R, K, true>(p, l, s0, h);
+        else gated_fwd_batch<T, NV, R, K, false>(p, l, s0, h);
+    }
+    if (l.on)
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < NV; i++) p.last[out + r * p.D + i] = h[r][i];
+}
+
+template <typename T, int NV, int R, int K, bool WHOLE>
+__device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& l, long long group, long long s0, float (&c)[R][NV])
+{
+    using P = Pack<T, NV>;
+    P z[K], x[K][R], d[K][R];
+    const long long dir = p.reverse ? -1 : 1, m0 = p.reverse ? p.T - 1 - s0 : s0;
+    const T* gp = (const T*)p.gate + l.b * p.gate_b + m0 * p.gate_t + l.d;
+    const T* xp = (const T*)p.x + l.b * p.x_b + m0 * p.x_t + l.d;
+    const T* dp = p.d_states ? (const T*)p.d_states + l.b * p.ds_b + m0 * p.ds_t + l.d : nullptr;
+    float h[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        Pack<float, NV> o;
+        if (l.on) o = *(const Pack<float, NV>*)(p.marks + ((s0 / K) * R + r) * p.groups * NV + group * NV);
+#pragma unroll
+        for (int i = 0; i < NV; i++) h[r][i] = l.on ? o.v[i] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < K; k++)
+        if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
+            z[k] = *(const P*)(gp + dir * k * p.gate_t);
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                x[k][r] = *(const P*)(xp + dir * k * p.x_t + r * p.x_r);
+                if (dp) d[k][r] = *(const P*)(dp + dir * k * p.ds_t + r * p.ds_r);
+            }
+        }
+    float before[K][R][NV];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < NV; i++) before[k][r][i] = h[r][i];
+        if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                float a, m;
+                gated_am(p.form, to_f(z[k].v[i]), a, m);
+#pragma unroll
+                for (int r = 0; r < R; r++) h[r][i] = __builtin_fmaf(a, h[r][i], m * to_f(x[k][r].v[i]));
+            }
+        }
+    }
+    T* ogp = p.d_gate ? (T*)p.d_gate + (l.b * p.T + m0) * p.D + l.d : nullptr;
+    T* oxp = p.d_x ? (T*)p.d_x + ((l.b * p.T + m0) * R) * p.D + l.d : nullptr;
+#pragma unroll
+    for (int k = K - 1; k >= 0; k--) {
+        const bool in = WHOLE || (s0 + k >= l.lo && s0 + k < l.hi);
+        P oz, ox[R];
+#pragma unroll
+        for (int i = 0; i < NV; i++) { oz.v[i] = from_f<T>(0.0f); for (int r = 0; r < R; r++) ox[r].v[i] = from_f<T>(0.0f); }
+        if (in) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                float a, m, dz = 0.0f;
+                gated_am(p.form, to_f(z[k].v[i]), a, m);
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float g = c[r][i] + (dp ? to_f(d[k][r].v[i]) : 0.0f);
+                    const float h0 = before[k][r][i];
+                    dz = __builtin_fmaf(g, p.form == GSX_GATED_LINEAR ? h0 : p.form == GSX_GATED_BLEND ? to_f(x[k][r].v[i]) - h0 : -h0, dz);
+                    ox[r].v[i] = from_f<T>(m * g);
+                    c[r][i] = a * g;
+                }
+                oz.v[i] = from_f<T>(dz);
+            }
+        }
+        if (WHOLE || (l.on && s0 + k < p.T)) {
+            if (ogp) *(P*)(ogp + dir * k * p.D) = oz;
+            if (oxp)
+#pragma unroll
+                for (int r = 0; r < R; r++) *(P*)(oxp + (dir * k * R + r) * p.D) = ox[r];
+        }
+    }
+}
+
+template <typename T, int NV, int R>
+__global__ __launch_bounds__(64 * kGatedWaves) void gated_bwd_kernel(GatedArgs p)
+{
+    constexpr int K = GatedBatch<R>::value;
+    const long long group = (long long)blockIdx.x * (64 * kGatedWaves) + threadIdx.x;
+    const Lane l = lane_of<NV>(p, group);
+    const long long out = (l.b * R) * p.D + l.d;
+    float c[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int i = 0; i < NV; i++) c[r][i] = p.d_last ? p.d_last[out + r * p.D + i] : 0.0f;
+    for (long long s0 = ((p.T + K - 1) / K - 1) * K; s0 >= 0; s0 -= K) {           // no steps: none
+        if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_bwd_batch<T, NV, R, K, true>(p, l, group, s0, c);
+        else gated_bwd_batch<T, NV, R, K, false>(p, l, group, s0, c);
+    }
+    if (p.d_initial && l.on)
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < NV; i++) p.d_initial[out + r * p.D + i] = c[r][i];
+}
+
+// One step in place, for a state that lives between calls: 12 bytes and more per element, and at a serving batch's size (64 x 2048)
+// nothing but the launch.
+template <typename T, int NV>
+__global__ __launch_bounds__(kBlock) void gated_step_kernel(float* __restrict__ state, const T* __restrict__ gate, const T* __restrict__ x, long long n, int form)
+{
+    const long long i = ((long long)blockIdx.x * kBlock + threadIdx.x) * NV;
+    if (i >= n) return;                                                      // NV divides n
+    Pack<float, NV> h = *(const Pack<float, NV>*)(state + i);
+    const Pack<T, NV> z = *(const Pack<T, NV>*)(gate + i), v = *(const Pack<T, NV>*)(x + i);
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        float a, m;
+        gated_am(form, to_f(z.v[k]), a, m);
+        h.v[k] = __builtin_fmaf(a, h.v[k], m * to_f(v.v[k]));
+    }
+    *(Pack<float, NV>*)(state + i) = h;
+}
+
+static int gated_check(const gsx_gated* s)
+{
+    if (!s || s->B < 0 || s->T < 0 || s->D < 0 || s->planes < 1 || s->planes > GSX_GATED_MAX_PLANES) return GSX_E_INVALID;
+    if (s->dtype != GSX_F32 && s->dtype != GSX_BF16 && s->dtype != GSX_F16) return GSX_E_INVALID;
+    if (s->form != GSX_GATED_LINEAR && s->form != GSX_GATED_BLEND && s->form != GSX_GATED_OVER) return GSX_E_INVALID;
+    if (s->T >= (1ll << 40) || s->B >= (1ll << 31) || s->D >= (1ll << 31) || (s->B && s->D > (1ll << 40) / s->B)) return GSX_E_RANGE;
+    return GSX_OK;
+}
+
+static size_t size_of(int dtype) { return dtype == GSX_F32 ? 4 : 2; }
+
+// NV channels per lane want every row of every array on a boundary of NV elements
+static bool aligned_for(const gsx_gated* s, int nv, bool backward)
+{
+    const int64_t e = (int64_t)size_of(s->dtype);
+    auto at = [&](const void* p, int64_t size) { return ((uintptr_t)p & (uintptr_t)(size * nv - 1)) == 0; };
+    auto by = [&](int64_t stride) { return stride % nv == 0; };
+    if (s->D % nv || !at(s->gate, e) || !at(s->x, e)) return false;
+    if (!by(s->gate_stride[0]) || !by(s->gate_stride[1]) || !by(s->x_stride[0]) || !by(s->x_stride[1]) || !by(s->x_stride[2])) return false;
+    if (!at(s->marks, 4)) return false;
+    if (!backward) return at(s->states, e);
+    if (!at(s->d_gate, e) || !at(s->d_x, e)) return false;
+    return !s->d_states || (at(s->d_states, e) && by(s->d_states_stride[0]) && by(s->d_states_stride[1]) && by(s->d_states_stride[2]));
+}
+
+static GatedArgs gated_args(const gsx_gated* s, int nv)
+{
+    GatedArgs p;
+    p.gate = s->gate; p.x = s->x; p.initial = s->initial; p.lengths = s->lengths;
+    p.states = s->states; p.last = s->last; p.marks = s->marks;
+    p.d_states = s->d_states; p.d_last = s->d_last; p.d_gate = s->d_gate; p.d_x = s->d_x; p.d_initial = s->d_initial;
+    p.T = s->T; p.D = s->D; p.row = s->D / nv; p.groups = s->B * p.row;
+    p.gate_b = s->gate_stride[0]; p.gate_t = s->gate_stride[1];
+    p.x_b = s->x_stride[0]; p.x_t = s->x_stride[1]; p.x_r = s->x_stride[2];
+    p.ds_b = s->d_states_stride[0]; p.ds_t = s->d_states_stride[1]; p.ds_r = s->d_states_stride[2];
+    p.form = s->form; p.reverse = s->reverse != 0;
+    return p;
+}
+
+template <typename T, int NV, int R>
+static int gated_launch(const gsx_gated* s, bool backward, hipStream_t stream)
+{
+    const GatedArgs p = gated_args(s, NV);
+    const int64_t blocks = ceil_div(p.groups, 64 * kGatedWaves);
+    if (blocks > 0x7fffffffll) return GSX_E_RANGE;
+    if (backward) gated_bwd_kernel<T, NV, R><<<dim3((unsigned)blocks), dim3(64 * kGatedWaves), 0, stream>>>(p);
+    else gated_fwd_kernel<T, NV, R><<<dim3((unsigned)blocks), dim3(64 * kGatedWaves), 0, stream>>>(p);
+    GSX_LAUNCH_CHECK();
+    return GSX_OK;
+}
+
+template <typename T>
+static int gated_by_planes(const gsx_gated* s, bool backward, hipStream_t stream)
+{
+    switch (s->planes) {
+    case 1: return aligned_for(s, 2, backward) ? gated_launch<T, 2, 1>(s, backward, stream) : gated_launch<T, 1, 1>(s, backward, stream);
+    case 2: return gated_launch<T, 1, 2>(s, backward, stream);
+    case 3: return gated_launch<T, 1, 3>(s, backward, stream);
+    default: return gated_launch<T, 1, 4>(s, backward, stream);
+    }
+}
+
+static int gated_run(const gsx_gated* s, bool backward, void* stream)
+{
+    switch (s->dtype) {
+    case GSX_F32: return gated_by_planes<float>(s, backward, (hipStream_t)stream);
+    case GSX_BF16: return gated_by_planes<__bf16>(s, backward, (hipStream_t)stream);
+    default: return gated_by_planes<_Float16>(s, backward, (hipStream_t)stream);
+    }
+}
+
+}  // namespace gsx
+
+using namespace gsx;
+
+GSX_API int64_t gsx_gated_marks_floats(int64_t B, int64_t T, int32_t planes, int64_t D)
+{
+    if (B < 0 || T < 0 || D < 0 || planes < 1 || planes > GSX_GATED_MAX_PLANES) return GSX_E_INVALID;
+    return ceil_div(T, planes == 1 ? GatedBatch<1>::value : GatedBatch<2>::value) * planes * B * D;
+}
+
+GSX_API int gsx_gated_scan_fwd(const gsx_gated* s, void* stream)
+{
+    const int st = gated_check(s);
+    if (st != GSX_OK) return st;
+    if (s->B == 0 || s->D == 0) return GSX_OK;
+    if (!s->last || (s->T && (!s->gate || !s->x))) return GSX_E_INVALID;
+    return gated_run(s, false, stream);
+}
+
+GSX_API int gsx_gated_scan_bwd(const gsx_gated* s, void* stream)
+{
+    const int st = gated_check(s);
+    if (st != GSX_OK) return st;
+    if (s->B == 0 || s->D == 0) return GSX_OK;
+    if (s->T && (!s->gate || !s->x || !s->marks)) return GSX_E_INVALID;
+    return gated_run(s, true, stream);
+}
+
+GSX_API int gsx_gated_step(int32_t dtype, int32_t form, int64_t n, float* state, const void* gate, const void* x, void* stream)
+{
+    if (n < 0 || (dtype != GSX_F32 && dtype != GSX_BF16 && dtype != GSX_F16)) return GSX_E_INVALID;
+    if (form != GSX_GATED_LINEAR && form != GSX_GATED_BLEND && form != GSX_GATED_OVER) return GSX_E_INVALID;
+    if (n == 0) return GSX_OK;
+    if (!state || !gate || !x) return GSX_E_INVALID;
+    const uintptr_t e = size_of(dtype);
+    const bool four = n % 4 == 0 && ((uintptr_t)state & 15) == 0 && ((uintptr_t)gate & (4 * e - 1)) == 0 && ((uintptr_t)x & (4 * e - 1)) == 0;
+    const int64_t blocks = ceil_div(n, four ? 4 * kBlock : kBlock);
+    if (blocks > 0x7fffffffll) return GSX_E_RANGE;
+    const dim3 grid((unsigned)blocks), block(kBlock);
+    hipStream_t st = (hipStream_t)stream;
+#define GSX_STEP(T) do { if (four) gated_step_kernel<T, 4><<<grid, block, 0, st>>>(state, (const T*)gate, (const T*)x, n, form); \
+                         else gated_step_kernel<T, 1><<<grid, block, 0, st>>>(state, (const T*)gate, (const T*)x, n, form); } while (0)
+    if (dtype == GSX_F32) GSX_STEP(float);
+    else if (dtype == GSX_BF16) GSX_STEP(__bf16);
+    else GSX_STEP(_Float16);
+#undef GSX_STEP
+    GSX_LAUNCH_CHECK();
+    return GSX_OK;
+}

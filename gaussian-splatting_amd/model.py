@@ -210,8 +210,26 @@ class GaussianSplat(nn.Module):
         torch.autograd.graph.increment_version(self.scales)      # written through a raw pointer: autograd must see it
 
     @torch.no_grad()
-    def get_dense_points(self, num_points: int = 1000000) -> torch.Tensor:
-        """(num_points, 6) xyz+rgb samples, Gaussians drawn with probability softmax(opacity) (:420-443)."""
+    def get_dense_points(self, num_points: int = 1000000, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                         min_p: float = 0.0, uniforms: torch.Tensor = None, logits: torch.Tensor = None) -> torch.Tensor:
+        """(num_points, 6) xyz+rgb samples, Gaussians drawn with probability softmax(opacity) (:420-443).
+        With any of the other arguments the draws come from sampling.sample (GPU tensors only): softmax(logits / temperature), `logits` (N)
+        in place of the opacities (a score of the Gaussians over views, say), cut to the top_k most opaque Gaussians, to the
+        fewest that hold top_p of the mass, to those at least min_p times as likely as the first; `uniforms` (num_points) in [0, 1) are
+        the random numbers (default: torch.rand in 64 bits, enough to tell millions of Gaussians apart)."""
+        if logits is not None or uniforms is not None or temperature != 1.0 or top_k != 0 or top_p != 1.0 or min_p != 0.0:
+            from .sampling import sample
+            row = (self.opacity.data if logits is None else logits.detach()).reshape(1, -1)
+            if row.shape[1] != self.positions.shape[0]:
+                raise ValueError(f"one logit per Gaussian is wanted ({self.positions.shape[0]}), got {row.shape[1]}")
+            if uniforms is None:
+                uniforms = torch.rand(num_points, dtype=torch.float64, device=row.device)
+            if uniforms.shape != (num_points,):
+                raise ValueError(f"one uniform per point is wanted ({num_points}), got {tuple(uniforms.shape)}")
+            indices = sample(row, uniforms[None], temperature, top_k, top_p, min_p)[0]
+            if num_points and int(indices[0]) < 0:
+                raise ValueError("no Gaussian is left to draw from: every logit is -inf or NaN")
+            return torch.cat([self.positions[indices], self.features[indices]], dim=1)
         weights = F.softmax(self.opacity.squeeze(-1), dim=0)
         indices = torch.multinomial(weights, num_points, replacement=True)
         return torch.cat([self.positions[indices], self.features[indices]], dim=1)

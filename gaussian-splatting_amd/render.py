@@ -622,3 +622,23 @@ def _orbit_streams(dev, count):
     while len(pool) < count:
         pool.append(torch.cuda.Stream(device=dev))
     return pool[:count]
+
+
+def composite_layers(rgb, alpha, background=None, straight=False):
+    """Renders over each other: rgb (L, B, P, H, W) of P <= 4 planes, alpha (L, B, 1, H, W), layer 0 in front -> (B, P, H, W).  The compositing
+    formula of one view (/root/reference/model/gaussian_splatting.py:143-144) with whole layers in place of splats, from the last layer
+    to the first: C = (1 - alpha) C + rgb for premultiplied colours, as `forward` returns them in 'rendered_images' and 'alpha', or
+    C = (1 - alpha) C + alpha rgb with straight=True.  background (B, P, H, W) lies behind the last layer (default 0).  One HIP
+    pass each way (csrc/gsx_gated.hip); differentiable in all three."""
+    from .recurrence import gated_scan, MAX_PLANES
+    if rgb.dim() != 5 or alpha.shape != rgb.shape[:2] + (1,) + rgb.shape[3:]:
+        raise ValueError(f"rgb (L, B, P, H, W) and alpha (L, B, 1, H, W) are wanted, got {tuple(rgb.shape)} and {tuple(alpha.shape)}")
+    n, B, P, H, W = rgb.shape
+    if not 1 <= P <= MAX_PLANES:
+        raise ValueError(f"a layer has 1 to {MAX_PLANES} planes, got {P}")
+    if background is not None and background.shape != rgb.shape[1:]:
+        raise ValueError(f"background must be {tuple(rgb.shape[1:])}, got {tuple(background.shape)}")
+    _, last = gated_scan(alpha.reshape(n, B, H * W).transpose(0, 1), rgb.reshape(n, B, P, H * W).transpose(0, 1),
+                         None if background is None else background.reshape(B, P, H * W),
+                         form="blend" if straight else "over", reverse=True, return_states=False)
+    return last.reshape(B, P, H, W).to(rgb.dtype)

@@ -45,7 +45,7 @@ extern "C" {
 const char* gsx_strerror(int status);
 int gsx_last_hip_error(void);
 /* ABI version; bumped on any signature change */
-#define GSX_ABI_VERSION 20
+#define GSX_ABI_VERSION 21
 int gsx_abi_version(void);
 
 /* ---- a5-a8 + sort key: replaces _project_positions, _project_scales,
@@ -408,6 +408,77 @@ int gsx_merge_fill(const float* positions, int32_t N, float threshold, const uin
                    const void* ws, size_t ws_bytes, void* stream);
 int gsx_merge_greedy_host(int32_t N, const uint32_t* offsets_host, const uint32_t* partners_host,
                           float* positions_host, float* features_host, float* opacity_host, uint8_t* removed_host);
+
+/* ---- the gated linear recurrence, forward and backward: h_t = a_t h_(t-1) + b_t along the steps, every channel on its own.
+ * NO counterpart as a call in the reference; it is the compositing formula of _render_chunk (:143-144) by itself -- layers, traces
+ * over views, sequences -- with the gate z given per step and channel:
+ *   GSX_GATED_LINEAR  a = z,     b = x
+ *   GSX_GATED_BLEND   a = 1 - z, b = z x       (straight colours over each other: z = alpha)
+ *   GSX_GATED_OVER    a = 1 - z, b = x         (premultiplied colours, what this library renders)
+ * Shapes: gate B x T x D, x and states B x T x planes x D (the planes of a channel share its gate; 1 <= planes <= 4), initial and last
+ * B x planes x D.  Channels are consecutive in memory; the other strides are in ELEMENTS and free (0 and negative ones too).
+ * gate, x, states and their gradients are `dtype`; the state itself is 32 bits all the way, and so are initial, last, the marks, d_last
+ * and d_initial.  reverse: the steps are taken from T - 1 down to 0, and last is the state behind step 0.
+ * lengths: sequence b consists of steps 0 .. lengths[b] - 1 only (clamped to 0 .. T); the steps behind it are not read, change no
+ * state, and get zeros in states, d_gate and d_x.
+ * fwd writes states (NULL: not wanted), last and marks (NULL: no backward follows; else gsx_gated_marks_floats floats: the 32-bit
+ * state in front of every batch of steps, from which bwd runs the batch again).  bwd reads gate, x, lengths and marks as fwd left
+ * them, d_states and d_last (each may be NULL: zeros), and writes d_gate (B x T x D), d_x (B x T x planes x D) and d_initial, all
+ * contiguous, each NULL if not wanted.  No atomics: results are the same bits every time.
+ * gsx_gated_step: one step in place on n contiguous elements, for a state that lives between calls (a served stream). */
+#define GSX_F32 0
+#define GSX_BF16 1
+#define GSX_F16 2
+#define GSX_GATED_LINEAR 0
+#define GSX_GATED_BLEND 1
+#define GSX_GATED_OVER 2
+#define GSX_GATED_MAX_PLANES 4
+typedef struct gsx_gated {
+    int32_t dtype, form, reverse, planes;
+    int64_t B, T, D;
+    const void* gate; int64_t gate_stride[2];          /* sequence, step */
+    const void* x; int64_t x_stride[3];                /* sequence, step, plane */
+    const float* initial;                              /* NULL: zeros */
+    const int32_t* lengths;                            /* NULL: all steps */
+    void* states;
+    float* last;
+    float* marks;
+    const void* d_states; int64_t d_states_stride[3];  /* sequence, step, plane */
+    const float* d_last;
+    void* d_gate; void* d_x; float* d_initial;
+} gsx_gated;
+int64_t gsx_gated_marks_floats(int64_t B, int64_t T, int32_t planes, int64_t D);
+int gsx_gated_scan_fwd(const gsx_gated* s, void* stream);
+int gsx_gated_scan_bwd(const gsx_gated* s, void* stream);
+int gsx_gated_step(int32_t dtype, int32_t form, int64_t n, float* state, const void* gate, const void* x, void* stream);
+
+/* ---- draws from softmax(logits / temperature) cut to the top k, the top p and the min p, by given random numbers: what
+ * get_dense_points gets from softmax + torch.multinomial (model/gaussian_splatting.py:420-443), with the cuts, reproducible, for rows of up to
+ * GSX_DRAW_MAX_V tokens (multinomial stops at 2^24) and for many rows.
+ * logits R x V of `dtype`, rows row_stride elements apart; NaN and -inf are masked tokens, never drawn; +inf takes all mass.
+ * Per row (the array) or for all rows (the number, where the array is NULL): temperature >= 0 (0: the lowest index of the largest logit), top_k
+ * (<= 0: off), top_p > 0 (>= 1: off), 0 <= min_p <= 1 (0: off).  Tokens are ranked by (logit descending, index ascending).  Kept are the
+ * first top_k; of these the fewest whose mass reaches top_p of their mass; of these the ones whose probability is at least min_p
+ * times the largest.
+ * uniforms R x S, contiguous, floats or (uniforms_f64) doubles in [0, 1) (outside: clamped; NaN: 0).  24 random bits cannot tell 2^24 tokens apart: give
+ * doubles where V is large.  indices[r][s] = the lowest index whose inclusive mass over the kept tokens, in index order, exceeds
+ * u * (all kept mass); logprobs (nullable) = the log of its share of the kept mass.  A row with nothing left, or with settings of its own
+ * out of range, gets -1 and -inf.  Masses are summed in 64 bits in a fixed order: the same bits every time.
+ * ws: gsx_draw_workspace_bytes (0: the arguments are refused), 256-byte aligned. */
+#define GSX_DRAW_MAX_V (1ll << 27)
+typedef struct gsx_draw {
+    int32_t dtype, uniforms_f64;
+    int64_t R, V, S;
+    const void* logits; int64_t row_stride;
+    const void* uniforms;
+    float temperature, top_p, min_p; int32_t top_k;
+    const float* temperatures; const float* top_ps; const float* min_ps; const int32_t* top_ks;
+    int64_t* indices;
+    float* logprobs;
+    void* ws; size_t ws_bytes;
+} gsx_draw;
+size_t gsx_draw_workspace_bytes(const gsx_draw* s);
+int gsx_draw_indices(const gsx_draw* s, void* stream);
 
 #ifdef __cplusplus
 }

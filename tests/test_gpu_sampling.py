@@ -1,0 +1,242 @@
+"""Draws (gaussian_splatting_amd.sampling, csrc/gsx_draw.hip) against the definition in 64 bits on the host, index for index: a random u lies within
+1e-15 of a border between two tokens about once in 1e12 draws, and where borders are met on purpose (equal logits) all sums are whole numbers."""
+import math
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def oracle_row(l, u, T, k, p, m):
+    """one row, doubles -> (indices, log probabilities)"""
+    V = len(l)
+    l = np.where(np.isnan(l), -np.inf, l)
+    none = np.full(len(u), -1, np.int64), np.full(len(u), -np.inf)
+    if V == 0 or not (T >= 0 and p > 0 and 0 <= m <= 1) or l.max() == -np.inf:
+        return none
+    top = l.max()
+    order = sorted(range(V), key=lambda i: (-l[i], i)) if V < 5000 else list(np.argsort(-l, kind="stable"))
+    order = np.array(order)
+    if T == 0:
+        kept, w = order[:1], np.ones(1)
+        full = np.zeros(V)
+        full[kept] = 1.0
+    else:
+        with np.errstate(invalid="ignore", over="ignore"):
+            w = np.where(l == top, 1.0, np.where(np.isneginf(l) | np.isposinf(top), 0.0, np.exp((l - top) / T)))
+        if 0 < k < V:
+            order = order[:k]
+        if p < 1:
+            run = np.cumsum(w[order])
+            order = order[:1 + int(np.sum(run < p * run[-1]))]
+        order = order[w[order] >= m]
+        full = np.zeros(V)
+        full[order] = w[order]
+    c = np.cumsum(full)
+    u = np.where(np.isnan(u), 0.0, np.clip(u, 0.0, 1.0))
+    i = np.searchsorted(c, u * c[-1], side="right")
+    i = np.minimum(i, np.nonzero(full)[0].max())
+    with np.errstate(divide="ignore"):
+        return i, np.log(full[i]) - np.log(c[-1])
+
+
+def check(logits, u, T=1.0, k=0, p=1.0, m=0.0):
+    from gaussian_splatting_amd import sample
+    R = logits.shape[0]
+    f = lambda v, r: float(v[r]) if torch.is_tensor(v) else float(np.float32(v))  # noqa: E731
+    got, lp = sample(logits, u, temperature=T, top_k=k, top_p=p, min_p=m, return_logprobs=True)
+    assert got.dtype == torch.int64 and got.shape == u.shape and lp.dtype == torch.float32 and lp.shape == u.shape
+    assert torch.equal(sample(logits, u, temperature=T, top_k=k, top_p=p, min_p=m), got)
+    lh, uh = logits.double().cpu().numpy(), u.double().cpu().numpy()
+    got, lp = got.cpu().numpy(), lp.cpu().numpy()
+    for r in range(R):
+        want, wl = oracle_row(lh[r], uh[r], f(T, r), int(k[r]) if torch.is_tensor(k) else k, f(p, r), f(m, r))
+        bad = np.nonzero(got[r] != want)[0]
+        assert len(bad) == 0, (r, len(bad), got[r][bad[:4]], want[bad[:4]], uh[r][bad[:4]])
+        # one rounding to 32 bits of a difference of 64-bit logarithms
+        fin = np.isfinite(wl)
+        assert np.array_equal(np.isfinite(lp[r]), fin) and bool((np.abs(lp[r][fin] - wl[fin]) <= 2.0 ** -24 * np.abs(wl[fin]) + 1e-12).all())
+
+
+def rand(seed, R, V, S, t=torch.float32, sigma=2.0, f64=False):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (sigma * torch.randn(R, V, generator=g, device="cuda")).to(t), torch.rand(R, S, generator=g, device="cuda", dtype=torch.float64 if f64 else torch.float32)
+
+
+CUTS = [dict(), dict(k=1), dict(k=7, T=0.5), dict(p=0.6), dict(m=0.1, T=1.7), dict(k=40, p=0.9, m=0.02, T=0.8), dict(T=0.0), dict(p=1e-6), dict(p=0.9999), dict(k=1000000), dict(m=1.0)]
+
+
+@pytest.mark.parametrize("V", [1, 2, 3, 31, 32, 33, 63, 64, 65, 127, 250, 300, 512, 513, 1000, 1025, 4097, 20011])
+@pytest.mark.parametrize("cut", CUTS, ids=str)
+def test_rows(V, cut):
+    dtype = list(DT.values())[V % 3]
+    logits, u = rand(V, 5, V, 9, dtype)
+    check(logits, u, **cut)
+
+
+@pytest.mark.parametrize("R,V,S", [(1, 5, 1), (300, 3, 1), (1000, 40, 2), (7, 70001, 33), (2, 200003, 5), (1, 300000, 70000), (600, 1500, 1), (1, 1100003, 100)])
+@pytest.mark.parametrize("cut", [dict(), dict(p=0.8), dict(k=300, p=0.95, m=0.001, T=0.9)], ids=str)
+def test_sizes(R, V, S, cut):
+    logits, u = rand(R + V, R, V, S, sigma=1.5, f64=V > 100000)
+    check(logits, u, **cut)
+
+
+@pytest.mark.parametrize("V", [5, 64, 300, 5000, 100001])
+def test_equal_logits_and_borders(V):
+    """all sums are whole numbers: every border is met exactly"""
+    for value in (0.0, -3.0, torch.finfo(torch.float32).min):
+        logits = torch.full((3, V), value, device="cuda")
+        grid = torch.arange(0, V + 1, max(1, V // 50), device="cuda", dtype=torch.float64)
+        u = (grid / V).clamp(max=1 - 2.0 ** -53).repeat(3, 1)
+        exact = torch.floor(u * V)                                    # u * V in doubles, as the definition has it
+        from gaussian_splatting_amd import sample
+        assert torch.equal(sample(logits, u), exact.long())
+        check(logits, u)
+        for cut in (dict(k=max(1, V // 3)), dict(p=0.5), dict(p=0.25, k=max(1, V // 2)), dict(m=1.0), dict(T=0.0), dict(p=0.5, m=0.5)):
+            check(logits, u, **cut)
+
+
+def test_ties_at_the_cut():
+    """few values, many times each, in bf16: the last kept ones are the first in index order"""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for V in (50, 700, 9000):
+        logits = torch.randint(0, 4, (6, V), generator=g, device="cuda").to(torch.bfloat16)
+        logits[:, ::7] = -logits[:, ::7]                              # -0 among the zeros
+        u = torch.rand(6, 40, generator=g, device="cuda")
+        for k in (1, 2, V // 5, V // 3, V - 1):
+            check(logits, u, k=k)
+            check(logits, u, k=k, p=0.7)
+        for p in (0.1, 0.33, 0.5, 0.77, 0.95):
+            check(logits, u, p=p)
+
+
+def test_masked_tokens_and_empty_rows():
+    inf, nan, lowest = math.inf, math.nan, torch.finfo(torch.float32).min
+    for V in (6, 130, 3000, 70000):
+        base, u = rand(V, 8, V, 12)
+        base[0] = -inf
+        base[1] = nan
+        base[2, ::2] = nan
+        base[2, 1::2] = -inf
+        base[3] = lowest
+        base[4, : V // 2] = -inf
+        base[4, V // 2] = nan
+        base[5, : V - 1] = lowest
+        base[6, V // 3] = inf
+        base[6, V - 1] = inf
+        base[7, 1:] = -inf
+        for cut in CUTS:
+            check(base, u, **cut)
+
+
+def test_settings_by_row_and_refused_rows():
+    R, V = 10, 900
+    logits, u = rand(3, R, V, 6)
+    dev = logits.device
+    T = torch.tensor([1, 0.5, 0, -1, math.nan, 2, 1, 1, 1, 3.0], device=dev)
+    k = torch.tensor([0, 5, 3, 0, 0, -4, 900, 901, 1, 100], dtype=torch.int32, device=dev)
+    p = torch.tensor([0.5, 1, 0.9, 0.5, 0.5, 1.5, 0.0, math.nan, 0.7, 0.3], device=dev)
+    m = torch.tensor([0, 0.1, 0, 0, 0, 0.01, 0, 0, 2.0, 0.0], device=dev)
+    check(logits, u, T=T, k=k, p=p, m=m)
+    check(logits, u, T=T)
+    check(logits, u, k=k)
+    check(logits, u, p=p)
+    check(logits, u, m=m)
+
+
+def test_numbers_at_the_ends():
+    for V in (9, 200, 20000):
+        logits, _ = rand(1, 2, V, 1)
+        logits[:, -1] = -math.inf
+        u = torch.tensor([[0.0, -0.5, 1.0, 7.0, math.nan, 1 - 2.0 ** -24, math.inf, -math.inf]] * 2, device="cuda")
+        check(logits, u)
+        check(logits, u.double(), p=0.5)
+
+
+def test_extreme_temperatures():
+    logits, u = rand(5, 4, 400, 8)
+    for T in (1e-30, 1e-4, 1e4, 1e30, 3e38):
+        check(logits, u, T=T)
+        check(logits, u, T=T, p=0.5)
+    check(logits * 1e37, u, T=0.01)
+    check(logits * 1e37, u, T=1e36, p=0.9, k=30)
+
+
+def test_strides_and_types():
+    big, u = rand(6, 12, 1003, 4)
+    check(big[::3, 5:700], u[::3], p=0.9)
+    check(big[:, 1:], u, k=20)
+    check(big.t()[:12, :].t()[:, :12], u, m=0.01)                     # tokens that are not consecutive
+    check(big.to(torch.bfloat16)[:, 3:], u.double(), p=0.5)
+    check(big[:, :640].to(torch.float16)[:, 1:33], u, p=0.5)
+    check(big[:1].expand(12, 1003), u, p=0.8)
+
+
+def test_no_rows_no_tokens_no_draws():
+    from gaussian_splatting_amd import sample
+    z = lambda *s: torch.zeros(s, device="cuda")  # noqa: E731
+    assert sample(z(0, 5), z(0, 3)).shape == (0, 3)
+    assert sample(z(4, 5), z(4, 0)).shape == (4, 0)
+    i, lp = sample(z(4, 0), z(4, 3), top_k=3, top_p=0.5, return_logprobs=True)
+    assert bool((i == -1).all()) and bool((lp == -math.inf).all())
+
+
+def test_many_short_rows():
+    g = torch.Generator(device="cuda").manual_seed(8)
+    for V in (2, 17, 32, 48, 100):
+        logits = torch.log(torch.rand(3000, V, generator=g, device="cuda"))
+        logits[torch.rand(3000, V, generator=g, device="cuda") < 0.5] = -math.inf
+        u = torch.rand(3000, 3, generator=g, device="cuda")
+        check(logits, u, m=0.01)
+        check(logits[:500], u[:500], p=0.9, k=3)
+
+
+def test_the_same_bits_on_another_stream_and_when_replayed():
+    from gaussian_splatting_amd import sample
+    shapes = [(3, 50000, 4), (200, 30, 2), (1, 400000, 5000), (300, 2000, 1)]
+    sets = [rand(n, R, V, S) for n, (R, V, S) in enumerate(shapes)]
+    work = lambda: [sample(l, u, temperature=0.8, top_k=5000, top_p=0.9, min_p=1e-4, return_logprobs=True) for l, u in sets]  # noqa: E731
+    flat = lambda r: [t.clone() for pair in r for t in pair]  # noqa: E731
+    first = flat(work())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = flat(work())
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for n in range(4):
+        for l, u in sets:
+            l.copy_(2 * torch.randn(l.shape, device="cuda"))
+            u.copy_(torch.rand(u.shape, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = flat(out)
+        assert all(torch.equal(a, b) for a, b in zip(got, flat(work()))), n
+
+
+def test_dense_points():
+    from gaussian_splatting_amd import GaussianSplat
+    torch.manual_seed(3)
+    m = GaussianSplat(5000).cuda()
+    u = torch.rand(2000, device="cuda", dtype=torch.float64)
+    pts = m.get_dense_points(2000, temperature=0.1, top_p=0.8, uniforms=u)
+    want, _ = oracle_row(m.opacity.detach().double().cpu().numpy()[:, 0], u.cpu().numpy(), float(np.float32(0.1)), 0, float(np.float32(0.8)), 0.0)
+    want = torch.from_numpy(want).cuda()
+    assert torch.equal(pts, torch.cat([m.positions[want], m.features[want]], 1))
+    assert m.get_dense_points(100, min_p=0.5).shape == (100, 6) and m.get_dense_points(0, min_p=0.5).shape == (0, 6)
+    # without any of the new arguments: the draws that it made before
+    torch.manual_seed(7)
+    a = m.get_dense_points(300)
+    torch.manual_seed(7)
+    i = torch.multinomial(torch.softmax(m.opacity.detach().squeeze(-1), 0), 300, replacement=True)
+    assert torch.equal(a, torch.cat([m.positions[i], m.features[i]], 1))
+    with torch.no_grad():
+        m.opacity.fill_(math.nan)
+    with pytest.raises(ValueError, match="no Gaussian is left"):
+        m.get_dense_points(10, top_k=5)
