@@ -22,10 +22,10 @@ SYMBOLS = [
     "gsx_keep_flags", "gsx_compact_rows", "gsx_clamp_inplace",
     "gsx_merge_workspace_bytes", "gsx_merge_count", "gsx_merge_fill", "gsx_merge_greedy_host", "gsx_train_step", "gsx_train_step_grads", "gsx_train_step_apply",
     "gsx_comm_available", "gsx_comm_unique_id", "gsx_comm_init", "gsx_allreduce_avg", "gsx_bcast", "gsx_comm_destroy",
-    "gsx_gated_marks_floats", "gsx_gated_scan_fwd", "gsx_gated_scan_bwd", "gsx_gated_step", "gsx_draw_workspace_bytes", "gsx_draw_indices",
+    "gsx_gated_marks_floats", "gsx_gated_workspace_bytes", "gsx_gated_scan_fwd", "gsx_gated_scan_bwd", "gsx_gated_step", "gsx_draw_workspace_bytes", "gsx_draw_indices",
 ]
 
-ABI_VERSION = 21            # GSX_ABI_VERSION of include/gsx.h (tests check that the two agree)
+ABI_VERSION = 22            # GSX_ABI_VERSION of include/gsx.h (tests check that the two agree)
 GSX_OK, GSX_E_INVALID, GSX_E_CAPACITY, GSX_E_HIP, GSX_E_RANGE, GSX_E_AGAIN, GSX_E_COMM = 0, -1, -2, -3, -4, -5, -6
 RANK_NONE = 0xFFFFFFFF
 REC_FLOATS = int(os.environ.get("GSX_REC_FLOATS", "12"))      # (16 only with a library built for the 64-byte-stride experiment)
@@ -70,7 +70,7 @@ class GsxGated(C.Structure):
     _fields_ = [("dtype", _i32), ("form", _i32), ("reverse", _i32), ("planes", _i32), ("B", _i64), ("T", _i64), ("D", _i64),
                 ("gate", _p), ("gate_stride", _i64 * 2), ("x", _p), ("x_stride", _i64 * 3), ("initial", _p), ("lengths", _p),
                 ("states", _p), ("last", _p), ("marks", _p), ("d_states", _p), ("d_states_stride", _i64 * 3), ("d_last", _p),
-                ("d_gate", _p), ("d_x", _p), ("d_initial", _p)]
+                ("d_gate", _p), ("d_x", _p), ("d_initial", _p), ("ws", _p), ("ws_bytes", _sz)]
 
 
 class GsxDraw(C.Structure):
@@ -139,6 +139,7 @@ def lib():
     L.gsx_l1_ssim_fwd.argtypes = [_p, _p, _i32, _i32, _i32, C.c_float, _p, _p, _sz, _p]
     L.gsx_l1_ssim_bwd.argtypes = [_p, _p, _i32, _i32, _i32, C.c_float, _p, _p, _sz, _p, _p]
     L.gsx_gated_marks_floats.restype = _i64; L.gsx_gated_marks_floats.argtypes = [_i64, _i64, _i32, _i64]
+    L.gsx_gated_workspace_bytes.restype = _sz; L.gsx_gated_workspace_bytes.argtypes = [C.POINTER(GsxGated), _i32]
     L.gsx_gated_scan_fwd.argtypes = [C.POINTER(GsxGated), _p]
     L.gsx_gated_scan_bwd.argtypes = [C.POINTER(GsxGated), _p]
     L.gsx_gated_step.argtypes = [_i32, _i32, _i64, _p, _p, _p, _p]

@@ -8,11 +8,14 @@
 // The backward needs h_(t-1) in 32 bits, not as `states` rounds it: the forward leaves the state in front of every K-th step ("marks",
 // 4 / K bytes per element) and the backward runs each batch forward again from its mark, in registers.  It then reads gate, x and
 // the states' gradient, once each -- as much as a backward that reads `states` instead of x, and `states` need not exist.
+// Few channels and many steps: the steps are split into spans, one per wave.  A first kernel folds every span to the (A, H) of
+// h -> A h + H, and every workgroup's spans to one; the second begins each span from what the spans in front of it come to.
 #include "gsx_common.h"
 
 namespace gsx {
 
 constexpr int kGatedWaves = 4;
+constexpr int kGatedSpans = 8;                      // spans (waves) of a workgroup where the steps are split
 
 template <int R>
 struct GatedBatch { static constexpr int value = R == 1 ? 16 : 8; };        // K: steps in flight; planes multiply the registers
@@ -25,6 +28,10 @@ struct GatedArgs {
     long long D;
     long long gate_b, gate_t, x_b, x_t, x_r, ds_b, ds_t, ds_r;
     int form, reverse;
+    // split steps: `span` steps each (a multiple of K), kGatedSpans of them to a workgroup, `blocks` workgroups per 64 groups
+    long long span, blocks, columns;
+    double* span_a; double* span_h;            // [span][B D], [span][planes][B D]
+    double* block_a; double* block_h;           // the same of whole workgroups
 };
 
 template <typename T, int NV>
@@ -107,11 +114,170 @@ __device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& 
     }
 }
 
-template <typename T, int NV, int R>
-__global__ __launch_bounds__(64 * kGatedWaves) void gated_fwd_kernel(GatedArgs p)
+// A product of gates in 64 bits that stays finite: times a zero state it is a zero, times any other one it leaves 32 bits, as the walk would
+__device__ __forceinline__ double gated_times(double A, double a) { return fmin(fmax(A * a, -1e300), 1e300); }
+
+// Folds steps [s0, s0 + K) to h -> A h + H, in 64 bits: H and A h may be far larger than the state that they add up to, and a 32-bit H would
+// then be less exact than the walk itself (its 64-bit FMA is as fast on this card as the 32-bit one).  Backward: c -> A c + H of c_t = a_t (d_t + c_(t+1)), from the last step to the first.
+template <typename T, int NV, int R, int K, bool BACK, bool WHOLE>
+__device__ __forceinline__ void gated_fold_batch(const GatedArgs& p, const Lane& l, long long s0, double (&A)[NV], double (&H)[R][NV])
+{
+    using P = Pack<T, NV>;
+    P z[K], v[K][R];
+    const long long dir = p.reverse ? -1 : 1, m0 = p.reverse ? p.T - 1 - s0 : s0;
+    const T* gp = (const T*)p.gate + l.b * p.gate_b + m0 * p.gate_t + l.d;
+    const T* vp = BACK ? (p.d_states ? (const T*)p.d_states + l.b * p.ds_b + m0 * p.ds_t + l.d : nullptr) : (const T*)p.x + l.b * p.x_b + m0 * p.x_t + l.d;
+    const long long v_t = BACK ? p.ds_t : p.x_t, v_r = BACK ? p.ds_r : p.x_r;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+        if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
+            z[k] = *(const P*)(gp + dir * k * p.gate_t);
+            if (!BACK || vp)
+#pragma unroll
+                for (int r = 0; r < R; r++) v[k][r] = *(const P*)(vp + dir * k * v_t + r * v_r);
+        }
+#pragma unroll
+    for (int q = 0; q < K; q++) {
+        const int k = BACK ? K - 1 - q : q;
+        if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi))
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const double zd = (double)to_f(z[k].v[i]), a = p.form == GSX_GATED_LINEAR ? zd : 1.0 - zd;
+                A[i] = gated_times(A[i], a);
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const double vd = BACK && !vp ? 0.0 : (double)to_f(v[k][r].v[i]);
+                    H[r][i] = BACK ? a * (H[r][i] + vd) : fma(a, H[r][i], p.form == GSX_GATED_BLEND ? zd * vd : vd);
+                }
+            }
+    }
+}
+
+// where the spans of a split walk lie: the workgroup's and wave's place in the order of the walk (backward: from the end), and its steps
+struct Span { long long group, block, index, s0, s1; };
+
+template <bool BACK>
+__device__ __forceinline__ Span span_of(const GatedArgs& p)
+{
+    Span s;
+    const long long column = blockIdx.x % p.columns;
+    s.block = blockIdx.x / p.columns;
+    s.group = column * 64 + (threadIdx.x & 63);
+    s.index = s.block * kGatedSpans + (threadIdx.x >> 6);
+    const long long at = BACK ? p.blocks * kGatedSpans - 1 - s.index : s.index;
+    s.s0 = at * p.span < p.T ? at * p.span : p.T;
+    s.s1 = s.s0 + p.span < p.T ? s.s0 + p.span : p.T;
+    return s;
+}
+
+// (A, H) behind (A0, H0): h -> A (A0 h + H0) + H
+__device__ __forceinline__ double gated_apply(double A, double h, double H) { return h == 0.0 ? H : fma(A, h, H); }
+
+template <typename T, int NV, int R, bool BACK>
+__global__ __launch_bounds__(64 * kGatedSpans) void gated_fold_kernel(GatedArgs p)
 {
     constexpr int K = GatedBatch<R>::value;
-    const long long group = (long long)blockIdx.x * (64 * kGatedWaves) + threadIdx.x;
+    __shared__ double s_a[kGatedSpans][64 * NV];
+    __shared__ double s_h[kGatedSpans][R][64 * NV];
+    const Span sp = span_of<BACK>(p);
+    const Lane l = lane_of<NV>(p, sp.group);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double A[NV], H[R][NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) { A[i] = 1.0; for (int r = 0; r < R; r++) H[r][i] = 0.0; }
+    for (long long n = 0; n < p.span; n += K) {
+        const long long s0 = sp.s0 + (BACK ? p.span - K - n : n);
+        if (s0 >= sp.s1) continue;
+        if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fold_batch<T, NV, R, K, BACK, true>(p, l, s0, A, H);
+        else gated_fold_batch<T, NV, R, K, BACK, false>(p, l, s0, A, H);
+    }
+    const long long BD = p.groups * NV, at = sp.group * NV;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        s_a[wave][lane * NV + i] = A[i];
+        if (l.on) p.span_a[sp.index * BD + at + i] = A[i];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            s_h[wave][r][lane * NV + i] = H[r][i];
+            if (l.on) p.span_h[(sp.index * R + r) * BD + at + i] = H[r][i];
+        }
+    }
+    __syncthreads();
+    if (wave == 0 && l.on)
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            double a = 1.0, h[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) h[r] = 0.0;
+            for (int w = 0; w < kGatedSpans; w++) {
+                const double aw = s_a[w][lane * NV + i];
+                a = gated_times(a, aw);
+#pragma unroll
+                for (int r = 0; r < R; r++) h[r] = gated_apply(aw, h[r], s_h[w][r][lane * NV + i]);
+            }
+            p.block_a[sp.block * BD + at + i] = a;
+#pragma unroll
+            for (int r = 0; r < R; r++) p.block_h[(sp.block * R + r) * BD + at + i] = h[r];
+        }
+}
+
+// The state in front of this wave's span: the workgroups in front of its own, folded by all waves together, then the spans in front of it in its own.
+template <int NV, int R>
+__device__ __forceinline__ void gated_carry(const GatedArgs& p, const Span& sp, bool on, float (&h)[R][NV])
+{
+    __shared__ double s_a[kGatedSpans][64 * NV];
+    __shared__ double s_h[kGatedSpans][R][64 * NV];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long BD = p.groups * NV, at = sp.group * NV;
+    const long long each = (sp.block + kGatedSpans - 1) / kGatedSpans;
+    const long long b0 = wave * each, b1 = b0 + each < sp.block ? b0 + each : sp.block;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        double a = 1.0, c[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) c[r] = 0.0;
+        if (on) {
+#pragma unroll 4
+            for (long long b = b0; b < b1; b++) {
+                const double ab = p.block_a[b * BD + at + i];
+                a = gated_times(a, ab);
+#pragma unroll
+                for (int r = 0; r < R; r++) c[r] = gated_apply(ab, c[r], p.block_h[(b * R + r) * BD + at + i]);
+            }
+        }
+        s_a[wave][lane * NV + i] = a;
+#pragma unroll
+        for (int r = 0; r < R; r++) s_h[wave][r][lane * NV + i] = c[r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        double c[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) c[r] = h[r][i];
+        for (int w = 0; w < kGatedSpans; w++)
+#pragma unroll
+            for (int r = 0; r < R; r++) c[r] = gated_apply(s_a[w][lane * NV + i], c[r], s_h[w][r][lane * NV + i]);
+        if (on)
+            for (int w = 0; w < wave; w++) {
+                const long long q = sp.block * kGatedSpans + w;
+                const double aq = p.span_a[q * BD + at + i];
+#pragma unroll
+                for (int r = 0; r < R; r++) c[r] = gated_apply(aq, c[r], p.span_h[(q * R + r) * BD + at + i]);
+            }
+#pragma unroll
+        for (int r = 0; r < R; r++) h[r][i] = (float)c[r];
+    }
+}
+
+template <typename T, int NV, int R, bool SPLIT>
+__global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gated_fwd_kernel(GatedArgs p)
+{
+    constexpr int K = GatedBatch<R>::value;
+    Span sp;
+    if (SPLIT) sp = span_of<false>(p);
+    else { sp.group = (long long)blockIdx.x * (64 * kGatedWaves) + threadIdx.x; sp.s0 = 0; sp.s1 = p.T; }
+    const long long group = sp.group;
     const Lane l = lane_of<NV>(p, group);
     const long long out = (l.b * R) * p.D + l.d;                             // in B x R x D
     float h[R][NV];
@@ -119,7 +285,8 @@ __global__ __launch_bounds__(64 * kGatedWaves) void gated_fwd_kernel(GatedArgs p
     for (int r = 0; r < R; r++)
 #pragma unroll
         for (int i = 0; i < NV; i++) h[r][i] = p.initial ? p.initial[out + r * p.D + i] : 0.0f;
-    for (long long s0 = 0; s0 < p.T; s0 += K) {
+    if (SPLIT) gated_carry<NV, R>(p, sp, l.on, h);
+    for (long long s0 = sp.s0; s0 < sp.s1; s0 += K) {
         if (p.marks && l.on) {
             float* mk = p.marks + (s0 / K) * R * p.groups * NV + group * NV;
 #pragma unroll
@@ -133,7 +300,7 @@ __global__ __launch_bounds__(64 * kGatedWaves) void gated_fwd_kernel(GatedArgs p
         if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fwd_batch<T, NV, R, K, true>(p, l, s0, h);
         else gated_fwd_batch<T, NV, R, K, false>(p, l, s0, h);
     }
-    if (l.on)
+    if (l.on && (!SPLIT || sp.index == p.blocks * kGatedSpans - 1))
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
@@ -217,11 +384,14 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
     }
 }
 
-template <typename T, int NV, int R>
-__global__ __launch_bounds__(64 * kGatedWaves) void gated_bwd_kernel(GatedArgs p)
+template <typename T, int NV, int R, bool SPLIT>
+__global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gated_bwd_kernel(GatedArgs p)
 {
     constexpr int K = GatedBatch<R>::value;
-    const long long group = (long long)blockIdx.x * (64 * kGatedWaves) + threadIdx.x;
+    Span sp;
+    if (SPLIT) sp = span_of<true>(p);
+    else { sp.group = (long long)blockIdx.x * (64 * kGatedWaves) + threadIdx.x; sp.s0 = 0; sp.s1 = p.T; }
+    const long long group = sp.group;
     const Lane l = lane_of<NV>(p, group);
     const long long out = (l.b * R) * p.D + l.d;
     float c[R][NV];
@@ -229,11 +399,13 @@ __global__ __launch_bounds__(64 * kGatedWaves) void gated_bwd_kernel(GatedArgs p
     for (int r = 0; r < R; r++)
 #pragma unroll
         for (int i = 0; i < NV; i++) c[r][i] = p.d_last ? p.d_last[out + r * p.D + i] : 0.0f;
-    for (long long s0 = ((p.T + K - 1) / K - 1) * K; s0 >= 0; s0 -= K) {           // no steps: none
+    if (SPLIT) gated_carry<NV, R>(p, sp, l.on, c);
+    for (long long n = (sp.s1 - sp.s0 + K - 1) / K; n > 0; n--) {
+        const long long s0 = sp.s0 + (n - 1) * K;
         if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_bwd_batch<T, NV, R, K, true>(p, l, group, s0, c);
         else gated_bwd_batch<T, NV, R, K, false>(p, l, group, s0, c);
     }
-    if (p.d_initial && l.on)
+    if (p.d_initial && l.on && (!SPLIT || sp.index == p.blocks * kGatedSpans - 1))
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
@@ -297,35 +469,86 @@ static GatedArgs gated_args(const gsx_gated* s, int nv)
     return p;
 }
 
-template <typename T, int NV, int R>
-static int gated_launch(const gsx_gated* s, bool backward, hipStream_t stream)
+struct GatedPlan { int nv; int64_t span, blocks, columns; size_t span_a, span_h, block_a, block_h, bytes; };
+
+// How a call is laid out.  Two channels per lane where the rows allow it.  The steps are split when whole columns alone would leave the card
+// short of kGatedWant waves (8 per CU), down to spans of two batches: a split walk reads its inputs twice.
+constexpr int64_t kGatedWant = 2048;
+
+static GatedPlan gated_plan(const gsx_gated* s, bool backward)
 {
-    const GatedArgs p = gated_args(s, NV);
-    const int64_t blocks = ceil_div(p.groups, 64 * kGatedWaves);
-    if (blocks > 0x7fffffffll) return GSX_E_RANGE;
-    if (backward) gated_bwd_kernel<T, NV, R><<<dim3((unsigned)blocks), dim3(64 * kGatedWaves), 0, stream>>>(p);
-    else gated_fwd_kernel<T, NV, R><<<dim3((unsigned)blocks), dim3(64 * kGatedWaves), 0, stream>>>(p);
+    GatedPlan g;
+    g.nv = s->planes == 1 && aligned_for(s, 2, backward) ? 2 : 1;
+    const int64_t K = s->planes == 1 ? GatedBatch<1>::value : GatedBatch<2>::value, BD = s->B * s->D;
+    g.columns = ceil_div(BD / g.nv, 64);
+    g.blocks = 1; g.span = s->T;
+    g.span_a = g.span_h = g.block_a = g.block_h = g.bytes = 0;
+    const int64_t spans = g.columns < kGatedWant ? ceil_div(kGatedWant, g.columns) : 1;
+    int64_t span = ceil_div(ceil_div(s->T, spans), K) * K;
+    if (span < 2 * K) span = 2 * K;
+    if (spans == 1 || span * 2 > s->T) return g;
+    g.span = span;
+    g.blocks = ceil_div(ceil_div(s->T, span), kGatedSpans);
+    const size_t n = (size_t)g.blocks * kGatedSpans;
+    g.span_a = 0; g.bytes = align_up(n * BD * 8);
+    g.span_h = g.bytes; g.bytes += align_up(n * s->planes * BD * 8);
+    g.block_a = g.bytes; g.bytes += align_up((size_t)g.blocks * BD * 8);
+    g.block_h = g.bytes; g.bytes += align_up((size_t)g.blocks * s->planes * BD * 8);
+    return g;
+}
+
+template <typename T, int NV, int R>
+static int gated_launch(const gsx_gated* s, const GatedPlan& g, bool backward, hipStream_t stream)
+{
+    GatedArgs p = gated_args(s, NV);
+    if (g.bytes) {
+        char* ws = (char*)s->ws;
+        p.span = g.span; p.blocks = g.blocks; p.columns = g.columns;
+        p.span_a = (double*)(ws + g.span_a); p.span_h = (double*)(ws + g.span_h);
+        p.block_a = (double*)(ws + g.block_a); p.block_h = (double*)(ws + g.block_h);
+        const int64_t grid = g.columns * g.blocks;
+        if (grid > 0x7fffffffll) return GSX_E_RANGE;
+        const dim3 dg((unsigned)grid), db(64 * kGatedSpans);
+        if (backward) {
+            gated_fold_kernel<T, NV, R, true><<<dg, db, 0, stream>>>(p);
+            GSX_LAUNCH_CHECK();
+            gated_bwd_kernel<T, NV, R, true><<<dg, db, 0, stream>>>(p);
+        } else {
+            gated_fold_kernel<T, NV, R, false><<<dg, db, 0, stream>>>(p);
+            GSX_LAUNCH_CHECK();
+            gated_fwd_kernel<T, NV, R, true><<<dg, db, 0, stream>>>(p);
+        }
+    } else {
+        const int64_t grid = ceil_div(p.groups, 64 * kGatedWaves);
+        if (grid > 0x7fffffffll) return GSX_E_RANGE;
+        const dim3 dg((unsigned)grid), db(64 * kGatedWaves);
+        if (backward) gated_bwd_kernel<T, NV, R, false><<<dg, db, 0, stream>>>(p);
+        else gated_fwd_kernel<T, NV, R, false><<<dg, db, 0, stream>>>(p);
+    }
     GSX_LAUNCH_CHECK();
     return GSX_OK;
 }
 
 template <typename T>
-static int gated_by_planes(const gsx_gated* s, bool backward, hipStream_t stream)
+static int gated_by_planes(const gsx_gated* s, const GatedPlan& g, bool backward, hipStream_t stream)
 {
     switch (s->planes) {
-    case 1: return aligned_for(s, 2, backward) ? gated_launch<T, 2, 1>(s, backward, stream) : gated_launch<T, 1, 1>(s, backward, stream);
-    case 2: return gated_launch<T, 1, 2>(s, backward, stream);
-    case 3: return gated_launch<T, 1, 3>(s, backward, stream);
-    default: return gated_launch<T, 1, 4>(s, backward, stream);
+    case 1: return g.nv == 2 ? gated_launch<T, 2, 1>(s, g, backward, stream) : gated_launch<T, 1, 1>(s, g, backward, stream);
+    case 2: return gated_launch<T, 1, 2>(s, g, backward, stream);
+    case 3: return gated_launch<T, 1, 3>(s, g, backward, stream);
+    default: return gated_launch<T, 1, 4>(s, g, backward, stream);
     }
 }
 
 static int gated_run(const gsx_gated* s, bool backward, void* stream)
 {
+    const GatedPlan g = gated_plan(s, backward);
+    if (g.bytes && (!s->ws || ((uintptr_t)s->ws & 255))) return GSX_E_INVALID;
+    if (s->ws_bytes < g.bytes) return GSX_E_CAPACITY;
     switch (s->dtype) {
-    case GSX_F32: return gated_by_planes<float>(s, backward, (hipStream_t)stream);
-    case GSX_BF16: return gated_by_planes<__bf16>(s, backward, (hipStream_t)stream);
-    default: return gated_by_planes<_Float16>(s, backward, (hipStream_t)stream);
+    case GSX_F32: return gated_by_planes<float>(s, g, backward, (hipStream_t)stream);
+    case GSX_BF16: return gated_by_planes<__bf16>(s, g, backward, (hipStream_t)stream);
+    default: return gated_by_planes<_Float16>(s, g, backward, (hipStream_t)stream);
     }
 }
 
@@ -337,6 +560,12 @@ GSX_API int64_t gsx_gated_marks_floats(int64_t B, int64_t T, int32_t planes, int
 {
     if (B < 0 || T < 0 || D < 0 || planes < 1 || planes > GSX_GATED_MAX_PLANES) return GSX_E_INVALID;
     return ceil_div(T, planes == 1 ? GatedBatch<1>::value : GatedBatch<2>::value) * planes * B * D;
+}
+
+GSX_API size_t gsx_gated_workspace_bytes(const gsx_gated* s, int32_t backward)
+{
+    if (gated_check(s) != GSX_OK || s->B == 0 || s->D == 0) return 0;
+    return gated_plan(s, backward != 0).bytes;
 }
 
 GSX_API int gsx_gated_scan_fwd(const gsx_gated* s, void* stream)

@@ -33,6 +33,15 @@ def _shape(gate, x, lengths, form, reverse):
     return s
 
 
+def _workspace(lib, s, backward, dev):
+    n = lib.gsx_gated_workspace_bytes(s, backward)
+    if not n:
+        return None
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    s.ws = _ptr(ws); s.ws_bytes = n
+    return ws
+
+
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, initial, lengths, form, reverse, want_states, want_grad):
@@ -48,6 +57,7 @@ class _GatedScan(torch.autograd.Function):
         if want_grad:
             marks = torch.empty(lib.gsx_gated_marks_floats(s.B, s.T, s.planes, s.D), dtype=torch.float32, device=dev)
         s.initial = _ptr(h0); s.states = _ptr(states); s.last = _ptr(last); s.marks = _ptr(marks)
+        ws = _workspace(lib, s, 0, dev)
         with L.on_device(dev):
             L.check(lib.gsx_gated_scan_fwd(s, L.stream_ptr(dev)), "gsx_gated_scan_fwd")
         if marks is not None:
@@ -76,6 +86,7 @@ class _GatedScan(torch.autograd.Function):
         d_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[1] else None
         d_initial = torch.empty(x.shape[:1] + x.shape[2:], dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
         s.d_gate = _ptr(d_gate); s.d_x = _ptr(d_x); s.d_initial = _ptr(d_initial)
+        ws = _workspace(lib, s, 1, dev)
         with L.on_device(dev):
             L.check(lib.gsx_gated_scan_bwd(s, L.stream_ptr(dev)), "gsx_gated_scan_bwd")
         if d_initial is not None:

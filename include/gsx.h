@@ -45,7 +45,7 @@ extern "C" {
 const char* gsx_strerror(int status);
 int gsx_last_hip_error(void);
 /* ABI version; bumped on any signature change */
-#define GSX_ABI_VERSION 21
+#define GSX_ABI_VERSION 22
 int gsx_abi_version(void);
 
 /* ---- a5-a8 + sort key: replaces _project_positions, _project_scales,
@@ -425,6 +425,7 @@ int gsx_merge_greedy_host(int32_t N, const uint32_t* offsets_host, const uint32_
  * state in front of every batch of steps, from which bwd runs the batch again).  bwd reads gate, x, lengths and marks as fwd left
  * them, d_states and d_last (each may be NULL: zeros), and writes d_gate (B x T x D), d_x (B x T x planes x D) and d_initial, all
  * contiguous, each NULL if not wanted.  No atomics: results are the same bits every time.
+ * ws: gsx_gated_workspace_bytes of the struct as it is handed over otherwise (often 0), 256-byte aligned; each call may have its own.
  * gsx_gated_step: one step in place on n contiguous elements, for a state that lives between calls (a served stream). */
 #define GSX_F32 0
 #define GSX_BF16 1
@@ -446,7 +447,9 @@ typedef struct gsx_gated {
     const void* d_states; int64_t d_states_stride[3];  /* sequence, step, plane */
     const float* d_last;
     void* d_gate; void* d_x; float* d_initial;
+    void* ws; size_t ws_bytes;
 } gsx_gated;
+size_t gsx_gated_workspace_bytes(const gsx_gated* s, int32_t backward);
 int64_t gsx_gated_marks_floats(int64_t B, int64_t T, int32_t planes, int64_t D);
 int gsx_gated_scan_fwd(const gsx_gated* s, void* stream);
 int gsx_gated_scan_bwd(const gsx_gated* s, void* stream);
