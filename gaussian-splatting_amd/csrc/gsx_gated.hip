@@ -70,7 +70,6 @@ __device__ __forceinline__ Lane lane_of(const GatedArgs& p, long long group)
     if (p.lengths) { const int n = p.lengths[l.b]; len = n < 0 ? 0 : n < p.T ? n : p.T; }
     l.lo = p.reverse ? p.T - len : 0;
     l.hi = p.reverse ? p.T : len;
-    if (!l.on) { l.lo = 0; l.hi = 0; }
     return l;
 }
 
@@ -102,7 +101,7 @@ __device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& 
                 for (int r = 0; r < R; r++) h[r][i] = __builtin_fmaf(a, h[r][i], m * to_f(x[k][r].v[i]));
             }
         }
-        if (sp && (WHOLE || (l.on && s0 + k < p.T))) {
+        if (sp && (WHOLE || s0 + k < p.T)) {
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 P o;
@@ -119,20 +118,20 @@ __device__ __forceinline__ double gated_times(double A, double a) { return fmin(
 
 // Folds steps [s0, s0 + K) to h -> A h + H, in 64 bits: H and A h may be far larger than the state that they add up to, and a 32-bit H would
 // then be less exact than the walk itself (its 64-bit FMA is as fast on this card as the 32-bit one).  Backward: c -> A c + H of c_t = a_t (d_t + c_(t+1)), from the last step to the first.
-template <typename T, int NV, int R, int K, bool BACK, bool WHOLE>
+template <typename T, int NV, int R, int K, bool BACK, bool HASV, bool WHOLE>
 __device__ __forceinline__ void gated_fold_batch(const GatedArgs& p, const Lane& l, long long s0, double (&A)[NV], double (&H)[R][NV])
 {
     using P = Pack<T, NV>;
     P z[K], v[K][R];
     const long long dir = p.reverse ? -1 : 1, m0 = p.reverse ? p.T - 1 - s0 : s0;
     const T* gp = (const T*)p.gate + l.b * p.gate_b + m0 * p.gate_t + l.d;
-    const T* vp = BACK ? (p.d_states ? (const T*)p.d_states + l.b * p.ds_b + m0 * p.ds_t + l.d : nullptr) : (const T*)p.x + l.b * p.x_b + m0 * p.x_t + l.d;
+    const T* vp = BACK ? (const T*)p.d_states + l.b * p.ds_b + m0 * p.ds_t + l.d : (const T*)p.x + l.b * p.x_b + m0 * p.x_t + l.d;       // !HASV: not read
     const long long v_t = BACK ? p.ds_t : p.x_t, v_r = BACK ? p.ds_r : p.x_r;
 #pragma unroll
     for (int k = 0; k < K; k++)
         if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
             z[k] = *(const P*)(gp + dir * k * p.gate_t);
-            if (!BACK || vp)
+            if (HASV)
 #pragma unroll
                 for (int r = 0; r < R; r++) v[k][r] = *(const P*)(vp + dir * k * v_t + r * v_r);
         }
@@ -146,7 +145,7 @@ __device__ __forceinline__ void gated_fold_batch(const GatedArgs& p, const Lane&
                 A[i] = gated_times(A[i], a);
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    const double vd = BACK && !vp ? 0.0 : (double)to_f(v[k][r].v[i]);
+                    const double vd = HASV ? (double)to_f(v[k][r].v[i]) : 0.0;
                     H[r][i] = BACK ? a * (H[r][i] + vd) : fma(a, H[r][i], p.form == GSX_GATED_BLEND ? zd * vd : vd);
                 }
             }
@@ -173,7 +172,7 @@ __device__ __forceinline__ Span span_of(const GatedArgs& p)
 // (A, H) behind (A0, H0): h -> A (A0 h + H0) + H
 __device__ __forceinline__ double gated_apply(double A, double h, double H) { return h == 0.0 ? H : fma(A, h, H); }
 
-template <typename T, int NV, int R, bool BACK>
+template <typename T, int NV, int R, bool BACK, bool HASV>
 __global__ __launch_bounds__(64 * kGatedSpans) void gated_fold_kernel(GatedArgs p)
 {
     constexpr int K = GatedBatch<R>::value;
@@ -185,12 +184,13 @@ __global__ __launch_bounds__(64 * kGatedSpans) void gated_fold_kernel(GatedArgs 
     double A[NV], H[R][NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) { A[i] = 1.0; for (int r = 0; r < R; r++) H[r][i] = 0.0; }
-    for (long long n = 0; n < p.span; n += K) {
-        const long long s0 = sp.s0 + (BACK ? p.span - K - n : n);
-        if (s0 >= sp.s1) continue;
-        if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fold_batch<T, NV, R, K, BACK, true>(p, l, s0, A, H);
-        else gated_fold_batch<T, NV, R, K, BACK, false>(p, l, s0, A, H);
-    }
+    if (l.on)
+        for (long long n = 0; n < p.span; n += K) {
+            const long long s0 = sp.s0 + (BACK ? p.span - K - n : n);
+            if (s0 >= sp.s1) continue;
+            if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fold_batch<T, NV, R, K, BACK, HASV, true>(p, l, s0, A, H);
+            else gated_fold_batch<T, NV, R, K, BACK, HASV, false>(p, l, s0, A, H);
+        }
     const long long BD = p.groups * NV, at = sp.group * NV;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
@@ -286,8 +286,9 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
 #pragma unroll
         for (int i = 0; i < NV; i++) h[r][i] = p.initial ? p.initial[out + r * p.D + i] : 0.0f;
     if (SPLIT) gated_carry<NV, R>(p, sp, l.on, h);
+    if (!l.on) return;
     for (long long s0 = sp.s0; s0 < sp.s1; s0 += K) {
-        if (p.marks && l.on) {
+        if (p.marks) {
             float* mk = p.marks + (s0 / K) * R * p.groups * NV + group * NV;
 #pragma unroll
             for (int r = 0; r < R; r++) {
@@ -300,14 +301,14 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
         if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fwd_batch<T, NV, R, K, true>(p, l, s0, h);
         else gated_fwd_batch<T, NV, R, K, false>(p, l, s0, h);
     }
-    if (l.on && (!SPLIT || sp.index == p.blocks * kGatedSpans - 1))
+    if (!SPLIT || sp.index == p.blocks * kGatedSpans - 1)
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int i = 0; i < NV; i++) p.last[out + r * p.D + i] = h[r][i];
 }
 
-template <typename T, int NV, int R, int K, bool WHOLE>
+template <typename T, int NV, int R, int K, bool HASD, bool WHOLE>
 __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& l, long long group, long long s0, float (&c)[R][NV])
 {
     using P = Pack<T, NV>;
@@ -315,14 +316,13 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
     const long long dir = p.reverse ? -1 : 1, m0 = p.reverse ? p.T - 1 - s0 : s0;
     const T* gp = (const T*)p.gate + l.b * p.gate_b + m0 * p.gate_t + l.d;
     const T* xp = (const T*)p.x + l.b * p.x_b + m0 * p.x_t + l.d;
-    const T* dp = p.d_states ? (const T*)p.d_states + l.b * p.ds_b + m0 * p.ds_t + l.d : nullptr;
+    const T* dp = (const T*)p.d_states + l.b * p.ds_b + m0 * p.ds_t + l.d;           // !HASD: not read
     float h[R][NV];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        Pack<float, NV> o;
-        if (l.on) o = *(const Pack<float, NV>*)(p.marks + ((s0 / K) * R + r) * p.groups * NV + group * NV);
+        const Pack<float, NV> o = *(const Pack<float, NV>*)(p.marks + ((s0 / K) * R + r) * p.groups * NV + group * NV);
 #pragma unroll
-        for (int i = 0; i < NV; i++) h[r][i] = l.on ? o.v[i] : 0.0f;
+        for (int i = 0; i < NV; i++) h[r][i] = o.v[i];
     }
 #pragma unroll
     for (int k = 0; k < K; k++)
@@ -331,7 +331,7 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 x[k][r] = *(const P*)(xp + dir * k * p.x_t + r * p.x_r);
-                if (dp) d[k][r] = *(const P*)(dp + dir * k * p.ds_t + r * p.ds_r);
+                if (HASD) d[k][r] = *(const P*)(dp + dir * k * p.ds_t + r * p.ds_r);
             }
         }
     float before[K][R][NV];
@@ -366,7 +366,7 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
                 gated_am(p.form, to_f(z[k].v[i]), a, m);
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    const float g = c[r][i] + (dp ? to_f(d[k][r].v[i]) : 0.0f);
+                    const float g = c[r][i] + (HASD ? to_f(d[k][r].v[i]) : 0.0f);
                     const float h0 = before[k][r][i];
                     dz = __builtin_fmaf(g, p.form == GSX_GATED_LINEAR ? h0 : p.form == GSX_GATED_BLEND ? to_f(x[k][r].v[i]) - h0 : -h0, dz);
                     ox[r].v[i] = from_f<T>(m * g);
@@ -375,7 +375,7 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
                 oz.v[i] = from_f<T>(dz);
             }
         }
-        if (WHOLE || (l.on && s0 + k < p.T)) {
+        if (WHOLE || s0 + k < p.T) {
             if (ogp) *(P*)(ogp + dir * k * p.D) = oz;
             if (oxp)
 #pragma unroll
@@ -384,7 +384,7 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
     }
 }
 
-template <typename T, int NV, int R, bool SPLIT>
+template <typename T, int NV, int R, bool SPLIT, bool HASD>
 __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gated_bwd_kernel(GatedArgs p)
 {
     constexpr int K = GatedBatch<R>::value;
@@ -400,12 +400,13 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
 #pragma unroll
         for (int i = 0; i < NV; i++) c[r][i] = p.d_last ? p.d_last[out + r * p.D + i] : 0.0f;
     if (SPLIT) gated_carry<NV, R>(p, sp, l.on, c);
+    if (!l.on) return;
     for (long long n = (sp.s1 - sp.s0 + K - 1) / K; n > 0; n--) {
         const long long s0 = sp.s0 + (n - 1) * K;
-        if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_bwd_batch<T, NV, R, K, true>(p, l, group, s0, c);
-        else gated_bwd_batch<T, NV, R, K, false>(p, l, group, s0, c);
+        if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_bwd_batch<T, NV, R, K, HASD, true>(p, l, group, s0, c);
+        else gated_bwd_batch<T, NV, R, K, HASD, false>(p, l, group, s0, c);
     }
-    if (p.d_initial && l.on && (!SPLIT || sp.index == p.blocks * kGatedSpans - 1))
+    if (p.d_initial && (!SPLIT || sp.index == p.blocks * kGatedSpans - 1))
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
@@ -510,11 +511,13 @@ static int gated_launch(const gsx_gated* s, const GatedPlan& g, bool backward, h
         if (grid > 0x7fffffffll) return GSX_E_RANGE;
         const dim3 dg((unsigned)grid), db(64 * kGatedSpans);
         if (backward) {
-            gated_fold_kernel<T, NV, R, true><<<dg, db, 0, stream>>>(p);
+            if (p.d_states) gated_fold_kernel<T, NV, R, true, true><<<dg, db, 0, stream>>>(p);
+            else gated_fold_kernel<T, NV, R, true, false><<<dg, db, 0, stream>>>(p);
             GSX_LAUNCH_CHECK();
-            gated_bwd_kernel<T, NV, R, true><<<dg, db, 0, stream>>>(p);
+            if (p.d_states) gated_bwd_kernel<T, NV, R, true, true><<<dg, db, 0, stream>>>(p);
+            else gated_bwd_kernel<T, NV, R, true, false><<<dg, db, 0, stream>>>(p);
         } else {
-            gated_fold_kernel<T, NV, R, false><<<dg, db, 0, stream>>>(p);
+            gated_fold_kernel<T, NV, R, false, true><<<dg, db, 0, stream>>>(p);
             GSX_LAUNCH_CHECK();
             gated_fwd_kernel<T, NV, R, true><<<dg, db, 0, stream>>>(p);
         }
@@ -522,7 +525,8 @@ static int gated_launch(const gsx_gated* s, const GatedPlan& g, bool backward, h
         const int64_t grid = ceil_div(p.groups, 64 * kGatedWaves);
         if (grid > 0x7fffffffll) return GSX_E_RANGE;
         const dim3 dg((unsigned)grid), db(64 * kGatedWaves);
-        if (backward) gated_bwd_kernel<T, NV, R, false><<<dg, db, 0, stream>>>(p);
+        if (backward && p.d_states) gated_bwd_kernel<T, NV, R, false, true><<<dg, db, 0, stream>>>(p);
+        else if (backward) gated_bwd_kernel<T, NV, R, false, false><<<dg, db, 0, stream>>>(p);
         else gated_fwd_kernel<T, NV, R, false><<<dg, db, 0, stream>>>(p);
     }
     GSX_LAUNCH_CHECK();
