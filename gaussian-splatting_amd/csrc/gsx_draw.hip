@@ -2,30 +2,49 @@
 // A row's weights are w_i = exp((l_i - top) / T) as shares of the largest.  The tokens ranked by (logit descending, index ascending),
 // the cuts keep a prefix of the ranking: the first k; of these the fewest whose mass reaches p of their mass; of these the ones with
 // w >= min_p.  A draw u is the lowest index whose inclusive mass over the kept tokens, in index order, exceeds u M.
-// Which index a u falls on is a comparison of sums of up to millions of terms: weights and sums are held in 64 bits (the card's
-// 64-bit vector FMA rate equals its 32-bit one, so a 64-bit exp per logit costs little beside reading the logits), and the masses of
-// the histogram that ranks are whole numbers in two 64-bit limbs, so that the order of its atomics cannot change a result.
+//
+// Which index a u falls on is a comparison of sums of up to millions of terms, and so is where the top p ends: weights and sums are held in
+// 64 bits (the card's 64-bit vector FMA rate equals its 32-bit one; the exp below is 17 of them), and the masses of histograms are whole
+// numbers in two limbs, so that the order of atomics cannot change a result.
+//
+// Three ways, by the length of a row:
+//   short  (V <= 512)      a few lanes to a row, its tokens in registers; the cuts by bisection of the key with ballots and masked sums.
+//   row    (one workgroup) the row read once per pass, from cache after the first: the top, a histogram, the tokens of the bin where a
+//                          cut falls, the masses, the draws -- one launch.
+//   parts  (a few long rows) the same passes as kernels, a row cut into parts over the card.
+// A histogram's 2048 bins are 1/64 of a unit of (top - l) / T wide: the tokens spread over hundreds of bins (few collisions in LDS), and the bin where
+// a cut falls holds few enough tokens to be ranked in LDS.  Where it does not (ties, extreme temperatures), narrower histograms of the 59-bit rank
+// (key, index) follow until it does: every row ends, whatever its values.
 #include "gsx_common.h"
 
 namespace gsx {
 
-constexpr int kDrawBlock = 1024;
-constexpr int kDrawBins = 256;
-constexpr int kDrawEach = 4;                        // consecutive tokens per thread and tile
-constexpr double kLimb = (double)(1ull << 36);      // a weight is hi 2^-36 + lo 2^-72; 2^27 weights fit a 64-bit sum of either
+constexpr int kDrawBins = 2048;                     // of the first histogram
+constexpr float kDrawBinsPerUnit = 64.0f;
+constexpr int kDrawFine = 512;                      // bins of the narrower ones
+constexpr int kDrawCand = 1024;                     // tokens that are ranked in LDS
+constexpr int kDrawSmall = 8192;                    // longest row that a quarter of a workgroup's threads takes
+constexpr int kDrawShort = 512;                     // longest row of the short way
+constexpr int kDrawWaveTiles = 4096;                // spans of 256 tokens whose masses are kept in LDS: rows of up to 1 M tokens
+constexpr int kDrawInRow = 64;                      // draws per row that its workgroup makes itself
+constexpr int kDrawIndexBits = 27;
+
+typedef unsigned long long u64;
 
 struct DrawArgs {
-    const void* logits; long long row_stride, V, S;
+    const void* logits; long long row_stride, R, V, S;
     const void* uniforms;
     float temperature, top_p, min_p; int top_k, uniforms_f64;
     const float* temperatures; const float* top_ps; const float* min_ps; const int32_t* top_ks;
     long long* indices; float* logprobs;
-    double* mass; double* total;                    // R x V inclusive masses, R totals (-1: the row has no valid settings)
-    float* tops;
-    uint32_t* keys; long long* bounds;              // per row: kept are the keys above, and of this key the indices below the bound
+    // workspace of rows whose draws are made by a kernel of their own
+    double* spans;                                  // [row][spans_row]: inclusive mass behind every 16 tokens
+    double* total; float* tops; u64* floors;        // per row: kept mass (-1: none), top, lowest kept rank
+    long long spans_row;
 };
 
-// logits as floats: NaN counts as -inf (a masked token), -0 as 0
+// ---- tokens ---------------------------------------------------------------------------------------------------------------
+// logits as floats: NaN counts as -inf (a masked token), -0 as 0.  A NaN float further on is "not a token" (a place outside the row).
 template <typename T>
 __device__ __forceinline__ float draw_logit(T v)
 {
@@ -33,21 +52,67 @@ __device__ __forceinline__ float draw_logit(T v)
     return f != f ? -__builtin_inff() : f + 0.0f;
 }
 
-// ascending unsigned order of the logits; never 0
-__device__ __forceinline__ uint32_t draw_key(float l)
+// ascending unsigned order of the logits
+__host__ __device__ __forceinline__ uint32_t draw_key(float l)
 {
     const uint32_t u = __builtin_bit_cast(uint32_t, l);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float draw_unkey(uint32_t k) { return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+// ascending order of (logit, -index): a cut keeps the tokens whose rank is at least some floor
+__device__ __forceinline__ u64 draw_rank(float l, long long i) { return (u64)draw_key(l) << kDrawIndexBits | (u64)(((1ll << kDrawIndexBits) - 1) - i); }
+
+// exp(x) for x <= 0: x = n ln 2 + r with ln 2 in two parts (the first of 32 bits: n times it is exact), |r| <= ln 2 / 2, the Taylor sum to
+// r^13 / 13! (what is left out is below 5e-18), times 2^n.
+__device__ __forceinline__ double draw_exp(double x)
+{
+    x = fmax(x, -760.0);                                             // 2^-1096: zero, and n stays an int
+    const double n = rint(x * 0x1.71547652b82fep+0);
+    double r = fma(n, -0x1.62e42ff000000p-1, x);
+    r = fma(n, 0x1.718432a1b0e26p-35, r);
+    double s = 1.0 / 6227020800.0;
+    s = fma(s, r, 1.0 / 479001600.0);
+    s = fma(s, r, 1.0 / 39916800.0);
+    s = fma(s, r, 1.0 / 3628800.0);
+    s = fma(s, r, 1.0 / 362880.0);
+    s = fma(s, r, 1.0 / 40320.0);
+    s = fma(s, r, 1.0 / 5040.0);
+    s = fma(s, r, 1.0 / 720.0);
+    s = fma(s, r, 1.0 / 120.0);
+    s = fma(s, r, 1.0 / 24.0);
+    s = fma(s, r, 1.0 / 6.0);
+    s = fma(s, r, 0.5);
+    s = fma(s, r, 1.0);
+    s = fma(s, r, 1.0);
+    return ldexp(s, (int)n);
 }
 
 __device__ __forceinline__ double draw_weight(float l, float top, double inv_t)
 {
     if (l == top) return 1.0;
-    if (l == -__builtin_inff() || top == __builtin_inff()) return 0.0;
-    return exp(((double)l - (double)top) * inv_t);
+    if (!(l > -__builtin_inff()) || top == __builtin_inff()) return 0.0;          // masked, not a token, or beside an infinite one
+    return draw_exp(((double)l - (double)top) * inv_t);
 }
 
-struct DrawRow { double inv_t, p, min_p; long long k; bool valid; };
+// bin of the first histogram: does not fall as l falls
+__device__ __forceinline__ int draw_bin(float l, float top, float scale)
+{
+    if (l == top) return 0;
+    const float t = (top - l) * scale;
+    return t < (float)(kDrawBins - 1) ? (int)t : kDrawBins - 1;
+}
+
+// a weight as whole numbers: w = hi 2^-31 + lo 2^-63, to the nearest; sums of 2^27 of either fit 64 bits
+__device__ __forceinline__ void draw_limbs(double w, uint32_t& hi, uint32_t& lo)
+{
+    const double t = w * 0x1p31;
+    hi = (uint32_t)t;
+    lo = (uint32_t)fmin((t - (double)hi) * 0x1p32 + 0.5, 4294967295.0);
+}
+__device__ __forceinline__ double limbs(u64 hi, u64 lo) { return (double)hi * 0x1p-31 + (double)lo * 0x1p-63; }
+
+struct DrawRow { double inv_t, p, min_p; long long k; float scale; bool valid; };
 
 __device__ __forceinline__ DrawRow draw_row(const DrawArgs& a, long long r)
 {
@@ -58,38 +123,62 @@ __device__ __forceinline__ DrawRow draw_row(const DrawArgs& a, long long r)
     const int k = a.top_ks ? a.top_ks[r] : a.top_k;
     s.valid = t >= 0.0f && p > 0.0f && m >= 0.0f && m <= 1.0f;
     s.inv_t = t > 0.0f ? 1.0 / (double)t : 1.0;
+    s.scale = (float)(s.inv_t * (double)kDrawBinsPerUnit);
     s.p = (double)p; s.min_p = (double)m;
     s.k = k > 0 && k < a.V ? k : a.V;
     if (t == 0.0f) { s.k = 1; s.p = 1.0; }           // the limit: the largest logit, its lowest index
     return s;
 }
 
-__device__ __forceinline__ double kept_weight(float l, long long i, uint32_t key, long long bound, float top, const DrawRow& set)
+__device__ __forceinline__ double draw_uniform(const DrawArgs& a, long long t)
 {
-    const uint32_t q = draw_key(l);
-    if (q < key || (q == key && i >= bound)) return 0.0;
+    const double u = a.uniforms_f64 ? ((const double*)a.uniforms)[t] : (double)((const float*)a.uniforms)[t];
+    return u >= 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;                     // NaN: 0
+}
+
+__device__ __forceinline__ double draw_kept(float l, long long i, u64 floor_rank, float top, const DrawRow& set)
+{
+    if (draw_rank(l, i) < floor_rank) return 0.0;
     const double w = draw_weight(l, top, set.inv_t);
     return w < set.min_p ? 0.0 : w;
 }
 
-template <typename T>
-__device__ __forceinline__ T block_reduce(T v, T* s_wave, T (*op)(T, T))
+__device__ __forceinline__ float draw_logprob(float l, float top, double inv_t, double total)
 {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = op(v, __shfl_xor(v, d, 64));
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) s_wave[wave] = v;
-    __syncthreads();
-    T r = s_wave[0];
-    for (int w = 1; w < kDrawBlock / 64; w++) r = op(r, s_wave[w]);
-    __syncthreads();
-    return r;
+    return (float)((l == top ? 0.0 : ((double)l - (double)top) * inv_t) - log(total));
 }
-__device__ __forceinline__ float op_maxf(float a, float b) { return fmaxf(a, b); }
 
-// exclusive sums over the block's threads; *sum = the block's
+// A row as groups of four tokens on a boundary of four: place 4 g + j is token 4 g + j - off.
 template <typename T>
-__device__ __forceinline__ T block_before(T v, T* s_wave, T* sum)
+struct Four { T v[4]; } __attribute__((aligned(4 * sizeof(T))));
+
+template <typename T>
+struct Places {
+    const T* base; long long V; int off;
+    __device__ __forceinline__ Places(const T* row, long long n) : V(n)
+    {
+        off = (int)(((uintptr_t)row / sizeof(T)) & 3);
+        base = row - off;
+    }
+    __device__ __forceinline__ long long groups() const { return (V + off + 3) >> 2; }
+    // places outside the row are NaN
+    __device__ __forceinline__ void load(long long g, float (&l)[4]) const
+    {
+        const long long i0 = 4 * g - off;
+        if (i0 >= 0 && i0 + 4 <= V) {
+            const Four<T> f = *(const Four<T>*)(base + 4 * g);
+#pragma unroll
+            for (int j = 0; j < 4; j++) l[j] = draw_logit(f.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) l[j] = i0 + j >= 0 && i0 + j < V ? draw_logit(base[4 * g + j]) : __builtin_nanf("");
+        }
+    }
+};
+
+// ---- workgroup helpers -------------------------------------------------------------------------------------------------------
+template <int NT, typename T>
+__device__ __forceinline__ T draw_before(T v, T* s_wave, T* sum)       // exclusive sums over the threads
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     T incl = v;
@@ -98,149 +187,347 @@ __device__ __forceinline__ T block_before(T v, T* s_wave, T* sum)
         const T o = __shfl_up(incl, d, 64);
         if (lane >= d) incl += o;
     }
+    __syncthreads();                                                 // s_wave may still be read from the call before
     if (lane == 63) s_wave[wave] = incl;
     __syncthreads();
     T base = 0, all = 0;
-    for (int w = 0; w < kDrawBlock / 64; w++) {
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) {
         if (w == wave) base = all;
         all += s_wave[w];
     }
     *sum = all;
-    __syncthreads();
-    T before = __shfl_up(incl, 1, 64);
+    const T before = __shfl_up(incl, 1, 64);
     return base + (lane ? before : (T)0);
 }
 
-struct DrawSel {                                    // LDS of the ranking
-    uint32_t count[kDrawBins];
-    unsigned long long hi[kDrawBins], lo[kDrawBins];
-    uint32_t prefix;                                // key bits settled so far
-    long long above_n; unsigned long long above_hi, above_lo;      // tokens in front of the settled bin, and their mass
-    double total;
-    uint32_t key; long long ties;                   // the last kept key, and how many of its tokens are kept
-    long long bound;                                // ... as an index: ties at an index below it are kept
+template <int NT>
+__device__ __forceinline__ float draw_max(float v, float* s_wave)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = s_wave[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; w++) r = fmaxf(r, s_wave[w]);
+    return r;
+}
+
+struct DrawHist { uint32_t count[kDrawBins]; u64 hi[kDrawBins], lo[kDrawBins]; };
+struct DrawFine { uint32_t count[kDrawFine]; u64 hi[kDrawFine], lo[kDrawFine]; };
+struct DrawCand { u64 rank[kDrawCand], ranked[kDrawCand]; double w[kDrawCand], ranked_w[kDrawCand]; };
+
+// What the threads of a workgroup share while a cut is found
+struct DrawCut {
+    long long above_n; u64 above_hi, above_lo;      // tokens in front of the bin, and their mass
+    int bin; uint32_t in_bin, slots; int last;
+    u64 lo, hi;                                     // ranks of the bin
+    u64 floor_rank; double mass;                    // the answer: the lowest kept rank, the mass kept
+    u64 wave_u[16]; uint32_t wave_n[16]; double wave_d[16]; float wave_f[16];
 };
 
-__device__ __forceinline__ double limbs(unsigned long long hi, unsigned long long lo) { return (double)hi * (1.0 / kLimb) + (double)lo * (1.0 / (kLimb * kLimb)); }
-
-// One level, 8 key bits, of the ranking by count (the first k) or by mass (the fewest that reach p of what the count cut left: keys above
-// floor_key, and of floor_key the indices below floor_bound).
-template <typename T>
-__device__ void draw_level(const T* row, long long V, float top, double inv_t, DrawSel& s, int shift, bool by_mass, uint32_t floor_key, long long floor_bound, long long k, double p)
+// The first of bins 0 .. last where what lies in and in front of it reaches k tokens or `want` mass, or else `last`; c.above_* move up to it (masses only with_mass).
+template <int NT>
+__device__ void draw_find(DrawCut& c, const uint32_t* count, const u64* hi, const u64* lo, int bins, int last, bool by_mass, bool with_mass, long long k, double want)
 {
-    for (int b = threadIdx.x; b < kDrawBins; b += kDrawBlock) { s.count[b] = 0; s.hi[b] = 0; s.lo[b] = 0; }
+    const int per = bins > NT ? bins / NT : 1, b0 = threadIdx.x * per;
+    uint32_t n = 0, all_n; u64 h = 0, l = 0, all;
+    const bool mine = b0 < bins;
+    if (mine)
+        for (int b = b0; b < b0 + per; b++) { n += count[b]; if (with_mass) { h += hi[b]; l += lo[b]; } }
+    const long long start_n = c.above_n; const u64 start_h = c.above_hi, start_l = c.above_lo;
+    long long at_n = start_n + draw_before<NT, uint32_t>(n, c.wave_n, &all_n);
+    u64 at_h = start_h, at_l = start_l;
+    if (with_mass) { at_h += draw_before<NT, u64>(h, c.wave_u, &all); at_l += draw_before<NT, u64>(l, c.wave_u, &all); }
     __syncthreads();
-    const uint32_t prefix = s.prefix;
-    for (long long i = threadIdx.x; i < V; i += kDrawBlock) {
-        const float l = draw_logit(row[i]);
-        const uint32_t key = draw_key(l);
-        if (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) continue;
-        if (by_mass && (key < floor_key || (key == floor_key && i >= floor_bound))) continue;
-        const int b = 255 - (int)((key >> shift) & 255);             // bin 0 holds the largest
-        atomicAdd(&s.count[b], 1u);
-        if (by_mass) {
-            const double w = draw_weight(l, top, inv_t) * kLimb;
-            const unsigned long long hi = (unsigned long long)w, lo = (unsigned long long)((w - (double)hi) * kLimb);
-            atomicAdd(&s.hi[b], hi);
-            atomicAdd(&s.lo[b], lo);
+    if (mine) {
+        bool before = by_mass ? b0 > 0 && limbs(at_h, at_l) >= want : at_n >= k;
+        for (int b = b0; b < b0 + per && b <= last && !before; b++) {
+            const long long next_n = at_n + count[b];
+            const u64 next_h = at_h + (with_mass ? hi[b] : 0), next_l = at_l + (with_mass ? lo[b] : 0);
+            const bool here = by_mass ? limbs(next_h, next_l) >= want : next_n >= k;
+            if (here || b == last) { c.bin = b; c.in_bin = count[b]; c.above_n = at_n; c.above_hi = at_h; c.above_lo = at_l; }
+            before = here;
+            at_n = next_n; at_h = next_h; at_l = next_l;
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        if (by_mass && shift == 24) {                                // the mass that p is a share of: all that the count cut left
-            unsigned long long hi = 0, lo = 0;
-            for (int b = 0; b < kDrawBins; b++) { hi += s.hi[b]; lo += s.lo[b]; }
-            s.total = limbs(hi, lo);
-        }
-        int b = 0;
-        for (; b < kDrawBins - 1; b++) {
-            if (by_mass ? limbs(s.above_hi + s.hi[b], s.above_lo + s.lo[b]) >= p * s.total : s.above_n + (long long)s.count[b] >= k) break;
-            s.above_n += s.count[b]; s.above_hi += s.hi[b]; s.above_lo += s.lo[b];
-        }
-        s.prefix = prefix | (uint32_t)(255 - b) << shift;
-        if (shift == 0) {
-            s.key = s.prefix;
-            const long long n = s.count[b];
-            if (!by_mass) s.ties = k - s.above_n < n ? k - s.above_n : n;
-            else {
-                const double left = p * s.total - limbs(s.above_hi, s.above_lo);
-                const double w = draw_weight(__builtin_bit_cast(float, s.key & 0x80000000u ? s.key & 0x7fffffffu : ~s.key), top, inv_t);
-                long long m = w > 0.0 ? (long long)ceil(left / w) : n;
-                s.ties = m < 1 ? 1 : m < n ? m : n;
+}
+
+// Finds where a cut ends among the tokens of bin c.bin (c.in_bin of them at most) whose rank is at least `floor_rank`.  each(f) calls f(l, rank)
+// for every token of the source, over all threads.
+template <int NT, typename Each>
+__device__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const Each& each, float top, double inv_t, float scale, u64 floor_rank, bool by_mass, bool with_mass, long long k, double want)
+{
+    const int bin = c.bin;
+    u64 lo = floor_rank, hi = ~0ull;
+    uint32_t n = c.in_bin;
+    const int most = NT < kDrawCand ? NT : kDrawCand;
+    bool narrowed = false;
+    while (n > (uint32_t)most) {
+        if (!narrowed) {                                             // the ranks of the bin: its keys are neighbours
+            if (threadIdx.x < 2) {
+                uint32_t a = draw_key(-__builtin_inff()), b = draw_key(__builtin_inff());
+                // the lowest key whose bin is at most `bin`; one below the lowest key whose bin is less than it
+                const int want_bin = threadIdx.x == 0 ? bin : bin - 1;
+                b += threadIdx.x;                                    // "none" for bin 0
+                while (a < b) {
+                    const uint32_t mid = a + (b - a) / 2;
+                    if (draw_bin(draw_unkey(mid), top, scale) <= want_bin) b = mid; else a = mid + 1;
+                }
+                if (threadIdx.x == 0) c.lo = (u64)a << kDrawIndexBits;
+                else c.hi = ((u64)a << kDrawIndexBits) - 1;
             }
+            __syncthreads();
+            lo = c.lo > lo ? c.lo : lo; hi = c.hi;
+            narrowed = true;
         }
+        int shift = 0;
+        while (((hi - lo) >> shift) >= (u64)kDrawFine) shift++;
+        for (int b = threadIdx.x; b < kDrawFine; b += NT) { fine.count[b] = 0; fine.hi[b] = 0; fine.lo[b] = 0; }
+        __syncthreads();
+        each([&](float l, u64 rank) {
+            if (rank < lo || rank > hi) return;
+            const int b = (int)((hi - rank) >> shift);
+            atomicAdd(&fine.count[b], 1u);
+            if (with_mass) {
+                uint32_t wh, wl;
+                draw_limbs(draw_weight(l, top, inv_t), wh, wl);
+                atomicAdd(&fine.hi[b], (u64)wh);
+                atomicAdd(&fine.lo[b], (u64)wl);
+            }
+        });
+        __syncthreads();
+        draw_find<NT>(c, fine.count, fine.hi, fine.lo, kDrawFine, (int)((hi - lo) >> shift), by_mass, with_mass, k, want);
+        hi -= (u64)c.bin << shift;
+        const u64 width = (1ull << shift) - 1;
+        lo = hi - lo > width ? hi - width : lo;
+        n = c.in_bin;
+        __syncthreads();
     }
+    if (threadIdx.x == 0) { c.slots = 0; c.last = 0; }
+    __syncthreads();
+    each([&](float l, u64 rank) {
+        if (rank < lo || rank > hi || (!narrowed && draw_bin(l, top, scale) != bin)) return;
+        const uint32_t slot = atomicAdd(&c.slots, 1u);
+        if (slot < (uint32_t)most) { cand.rank[slot] = rank; cand.w[slot] = draw_weight(l, top, inv_t); }
+    });
+    __syncthreads();
+    const int m = (int)(c.slots < (uint32_t)most ? c.slots : (uint32_t)most);
+    const int t = threadIdx.x;
+    if (t < m) {                                                     // its place among them: ranks are all different
+        const u64 mine = cand.rank[t];
+        int place = 0;
+        for (int j = 0; j < m; j++) place += cand.rank[j] > mine;
+        cand.ranked[place] = mine; cand.ranked_w[place] = cand.w[t];
+    }
+    __syncthreads();
+    double all;
+    const double w = t < m ? cand.ranked_w[t] : 0.0;
+    const double above = limbs(c.above_hi, c.above_lo);
+    const double before = draw_before<NT, double>(w, c.wave_d, &all);
+    const bool in = t < m && (t == 0 || (by_mass ? above + before < want : c.above_n + t < k));
+    if (in) atomicMax(&c.last, t);
+    __syncthreads();
+    if (t == c.last && m) { c.floor_rank = cand.ranked[t]; c.mass = above + before + w; }
+    if (t == 0 && !m) { c.floor_rank = lo; c.mass = above; }
     __syncthreads();
 }
 
-template <typename T>
-__device__ void draw_bound(const T* row, long long V, DrawSel& s, uint32_t* s_wave)
+__device__ __forceinline__ void draw_hist_add(DrawHist& h, float l, float top, double inv_t, float scale, bool by_mass)
 {
-    const uint32_t key = s.key; const long long ties = s.ties;
-    if (threadIdx.x == 0) s.bound = V;
-    long long seen = 0;
-    for (long long base = 0; base < V; base += kDrawBlock) {
-        const long long i = base + threadIdx.x;
-        const uint32_t is = i < V && draw_key(draw_logit(row[i])) == key;
-        uint32_t sum;
-        const uint32_t before = block_before<uint32_t>(is, s_wave, &sum);
-        if (is && seen + before == ties - 1) s.bound = i + 1;
-        seen += sum;
-        if (seen >= ties) break;                                     // the same for every thread
+    const int b = draw_bin(l, top, scale);
+    atomicAdd(&h.count[b], 1u);
+    if (by_mass) {
+        uint32_t wh, wl;
+        draw_limbs(draw_weight(l, top, inv_t), wh, wl);
+        if (wh) atomicAdd(&h.hi[b], (u64)wh);
+        if (wl) atomicAdd(&h.lo[b], (u64)wl);
     }
-    __syncthreads();
 }
 
-// one workgroup per row: top, cuts, inclusive masses
-template <typename T>
-__global__ __launch_bounds__(kDrawBlock) void draw_mass_kernel(DrawArgs a)
+// Both cuts from the first histogram; -> the lowest kept rank.
+template <int NT, typename Each>
+__device__ u64 draw_cuts(DrawCut& c, const DrawHist& hist, DrawFine& fine, DrawCand& cand, const Each& each, float top, const DrawRow& set, bool by_k, bool by_p)
 {
-    __shared__ DrawSel s;
-    __shared__ double s_d[kDrawBlock / 64];
-    __shared__ float s_f[kDrawBlock / 64];
-    __shared__ uint32_t s_u[kDrawBlock / 64];
-    const long long r = blockIdx.x, V = a.V;
-    const T* row = (const T*)a.logits + r * a.row_stride;
+    u64 floor_rank = 0;
+    int last = kDrawBins - 1;
+    double total = 0.0;
+    if (by_k) {
+        if (threadIdx.x == 0) { c.above_n = 0; c.above_hi = 0; c.above_lo = 0; }
+        __syncthreads();
+        draw_find<NT>(c, hist.count, hist.hi, hist.lo, kDrawBins, last, false, by_p, set.k, 0.0);
+        last = c.bin;
+        draw_resolve<NT>(c, fine, cand, each, top, set.inv_t, set.scale, 0, false, by_p, set.k, 0.0);
+        floor_rank = c.floor_rank;
+        total = c.mass;
+        __syncthreads();
+    }
+    if (by_p) {
+        if (!by_k) {
+            u64 h = 0, l = 0, all_h, all_l;
+            for (int b = threadIdx.x; b < kDrawBins; b += NT) { h += hist.hi[b]; l += hist.lo[b]; }
+            draw_before<NT, u64>(h, c.wave_u, &all_h);
+            draw_before<NT, u64>(l, c.wave_u, &all_l);
+            total = limbs(all_h, all_l);
+        }
+        if (threadIdx.x == 0) { c.above_n = 0; c.above_hi = 0; c.above_lo = 0; }
+        __syncthreads();
+        draw_find<NT>(c, hist.count, hist.hi, hist.lo, kDrawBins, last, true, true, 0, set.p * total);
+        draw_resolve<NT>(c, fine, cand, each, top, set.inv_t, set.scale, floor_rank, true, true, 0, set.p * total);
+        floor_rank = c.floor_rank > floor_rank ? c.floor_rank : floor_rank;
+    }
+    return floor_rank;
+}
+
+// ---- one workgroup per row -----------------------------------------------------------------------------------------------------
+template <typename T, int NT, bool PICK>
+__global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
+{
+    __shared__ union { struct { DrawHist hist; union { DrawFine fine; DrawCand cand; }; } s; double tile[kDrawWaveTiles]; } sh;
+    __shared__ DrawCut c;
+    constexpr int kWaves = NT / 64;
+    const long long r = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+    const long long groups = row.groups();
     const DrawRow set = draw_row(a, r);
     float top = -__builtin_inff();
-    for (long long i = threadIdx.x; i < V; i += kDrawBlock) top = fmaxf(top, draw_logit(row[i]));
-    top = block_reduce<float>(top, s_f, op_maxf);
+#pragma unroll 4
+    for (long long g = tid; g < groups; g += NT) {
+        float l[4];
+        row.load(g, l);
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = fmaxf(top, l[j]);
+    }
+    top = draw_max<NT>(top, c.wave_f);
     if (!set.valid || top == -__builtin_inff()) {
-        if (threadIdx.x == 0) { a.total[r] = -1.0; a.tops[r] = top; }
+        if (PICK) {
+            for (long long s = tid; s < a.S; s += NT) { a.indices[r * a.S + s] = -1; if (a.logprobs) a.logprobs[r * a.S + s] = -__builtin_inff(); }
+        } else if (tid == 0) a.total[r] = -1.0;
         return;
     }
-    uint32_t key = 0; long long bound = V;                           // keep keys above `key`, and of `key` the indices below `bound`
-    for (int cut = 0; cut < 2; cut++) {
-        if (cut == 0 ? set.k >= V : !(set.p < 1.0)) continue;
-        if (threadIdx.x == 0) { s.prefix = 0; s.above_n = 0; s.above_hi = 0; s.above_lo = 0; }
+    // f(l, i) for every token of the row, over all threads
+    auto tokens = [&](auto f) {
+#pragma unroll 2
+        for (long long g = tid; g < groups; g += NT) {
+            float l[4];
+            row.load(g, l);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (l[j] == l[j]) f(l[j], 4 * g + j - row.off);
+        }
+    };
+    const bool by_k = set.k < a.V, by_p = set.p < 1.0;
+    u64 floor_rank = 0;
+    if (by_k || by_p) {
+        for (int b = tid; b < kDrawBins; b += NT) { sh.s.hist.count[b] = 0; sh.s.hist.hi[b] = 0; sh.s.hist.lo[b] = 0; }
         __syncthreads();
-        for (int shift = 24; shift >= 0; shift -= 8) draw_level(row, V, top, set.inv_t, s, shift, cut == 1, key, bound, set.k, set.p);
-        draw_bound(row, V, s, s_u);
-        key = s.key; bound = s.bound;
+        tokens([&](float l, long long) { draw_hist_add(sh.s.hist, l, top, set.inv_t, set.scale, by_p); });
+        __syncthreads();
+        auto each = [&](auto f) { tokens([&](float l, long long i) { f(l, draw_rank(l, i)); }); };
+        floor_rank = draw_cuts<NT>(c, sh.s.hist, sh.s.fine, sh.s.cand, each, top, set, by_k, by_p);
         __syncthreads();
     }
-    if (threadIdx.x == 0) { a.keys[r] = key; a.bounds[r] = bound; }
-    double carry = 0.0;
-    double* mass = a.mass + r * V;
-    for (long long base = 0; base < V; base += kDrawBlock * kDrawEach) {
-        const long long i0 = base + threadIdx.x * kDrawEach;
-        double w[kDrawEach], sum = 0.0, all;
+    auto mass4 = [&](const float (&l)[4], long long g, double (&w)[4]) {
+        double sum = 0.0;
 #pragma unroll
-        for (int j = 0; j < kDrawEach; j++) {
-            w[j] = 0.0;
-            if (i0 + j < V) {
-                w[j] = kept_weight(draw_logit(row[i0 + j]), i0 + j, key, bound, top, set);
-            }
+        for (int j = 0; j < 4; j++) {
+            w[j] = l[j] == l[j] ? draw_kept(l[j], 4 * g + j - row.off, floor_rank, top, set) : 0.0;
             sum += w[j];
         }
-        double at = carry + block_before<double>(sum, s_d, &all);
+        return sum;
+    };
+    auto all_groups = [&](auto f) {                                  // every thread of a wave, also where the wave reaches beyond the row
+        for (long long g0 = 0; g0 < groups; g0 += NT) {
+            float l[4] = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            if (g0 + tid < groups) row.load(g0 + tid, l);
+            f(l, g0 + tid);
+        }
+    };
+    if (PICK) {
+        // masses of 256 tokens, one wave's groups, in LDS; then the inclusive sums of these
+        all_groups([&](const float (&l)[4], long long g) {
+            double w[4], sum = mass4(l, g, w);
 #pragma unroll
-        for (int j = 0; j < kDrawEach; j++) { at += w[j]; if (i0 + j < V) mass[i0 + j] = at; }
-        carry += all;
+            for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+            if (lane == 0) sh.tile[g >> 6] = sum;
+        });
+        __syncthreads();
+        const int tiles = (int)((groups + 63) >> 6), per = (tiles + NT - 1) / NT;
+        double sum = 0.0, total;
+        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) sum += sh.tile[q];
+        double at = draw_before<NT, double>(sum, c.wave_d, &total);
+        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) { at += sh.tile[q]; sh.tile[q] = at; }
+        __syncthreads();
+        for (long long s = wave; s < a.S; s += kWaves) {             // a wave per draw
+            const double want = draw_uniform(a, r * a.S + s) * total;
+            int lo = 0, hi = tiles - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (sh.tile[mid] > want) hi = mid; else lo = mid + 1;
+            }
+            // the first token in the tile that exceeds; where rounding leaves none, the last one with weight
+            for (int q = lo; q >= 0; q--) {
+                const long long g = (long long)q * 64 + lane;
+                float l[4] = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+                if (g < groups) row.load(g, l);
+                double w[4], mine = mass4(l, g, w), incl = mine;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const double o = __shfl_up(incl, d, 64);
+                    if (lane >= d) incl += o;
+                }
+                const double up = __shfl_up(incl, 1, 64);
+                double run = (q ? sh.tile[q - 1] : 0.0) + (lane ? up : 0.0);
+                int hit = -1, any = -1;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    run += w[j];
+                    if (w[j] > 0.0) { any = j; if (hit < 0 && run > want) hit = j; }
+                }
+                const u64 hits = __ballot(hit >= 0), some = __ballot(any >= 0);
+                if (!some) continue;
+                const int who = hits ? __ffsll((long long)hits) - 1 : 63 - __clzll((long long)some);
+                if (lane == who) {
+                    const int j = hits ? hit : any;
+                    float lj = l[0];
+#pragma unroll
+                    for (int e = 1; e < 4; e++) lj = e == j ? l[e] : lj;
+                    a.indices[r * a.S + s] = 4 * g + j - row.off;
+                    if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(lj, top, set.inv_t, total);
+                }
+                break;
+            }
+        }
+    } else {
+        // masses of 16 tokens, four neighbouring lanes', in the workspace; then the inclusive sums of these
+        double* spans = a.spans + r * a.spans_row;
+        const long long n = (groups + 3) >> 2;
+        all_groups([&](const float (&l)[4], long long g) {
+            double w[4], sum = mass4(l, g, w);
+            sum += __shfl_xor(sum, 1, 64);
+            sum += __shfl_xor(sum, 2, 64);
+            if ((lane & 3) == 0 && (g >> 2) < n) spans[g >> 2] = sum;
+        });
+        __syncthreads();
+        double carry = 0.0;
+        for (long long b = 0; b < n; b += 4 * NT) {
+            double v[4], sum = 0.0, all;
+#pragma unroll
+            for (int j = 0; j < 4; j++) { const long long q = b + 4 * tid + j; v[j] = q < n ? spans[q] : 0.0; sum += v[j]; }
+            double at = carry + draw_before<NT, double>(sum, c.wave_d, &all);
+#pragma unroll
+            for (int j = 0; j < 4; j++) { const long long q = b + 4 * tid + j; at += v[j]; if (q < n) spans[q] = at; }
+            carry += all;
+        }
+        if (tid == 0) { a.total[r] = carry; a.tops[r] = top; a.floors[r] = floor_rank; }
     }
-    if (threadIdx.x == 0) { a.total[r] = carry; a.tops[r] = top; }
 }
 
+// a thread per draw: the span of 16 tokens by bisection, then its tokens one after the other
 template <typename T>
 __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long n)
 {
@@ -249,24 +536,198 @@ __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long
     const long long r = t / a.S;
     const double total = a.total[r];
     if (!(total > 0.0)) { a.indices[t] = -1; if (a.logprobs) a.logprobs[t] = -__builtin_inff(); return; }
-    const double* mass = a.mass + r * a.V;
-    double u = a.uniforms_f64 ? ((const double*)a.uniforms)[t] : (double)((const float*)a.uniforms)[t];
-    u = u >= 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;                        // NaN: 0
-    const double want = u * mass[a.V - 1];
-    long long lo = 0, hi = a.V - 1;                                  // the lowest index with mass above `want`, or the last one
-    while (lo < hi) {
-        const long long mid = (lo + hi) >> 1;
-        if (mass[mid] > want) hi = mid; else lo = mid + 1;
-    }
-    // sums of neighbouring threads' spans may differ by a rounding from each other: never a token without weight, the last one with weight for u = 1
+    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
     const DrawRow set = draw_row(a, r);
     const float top = a.tops[r];
-    const T* row = (const T*)a.logits + r * a.row_stride;
-    while (lo > 0 && !(kept_weight(draw_logit(row[lo]), lo, a.keys[r], a.bounds[r], top, set) > 0.0)) lo--;
-    a.indices[t] = lo;
-    if (a.logprobs) {
-        const float l = draw_logit(row[lo]);
-        a.logprobs[t] = (float)((l == top ? 0.0 : ((double)l - (double)top) * set.inv_t) - log(total));
+    const u64 floor_rank = a.floors[r];
+    const double* spans = a.spans + r * a.spans_row;
+    const double want = draw_uniform(a, t) * total;
+    long long lo = 0, hi = ((row.groups() + 3) >> 2) - 1;
+    while (lo < hi) {
+        const long long mid = (lo + hi) >> 1;
+        if (spans[mid] > want) hi = mid; else lo = mid + 1;
+    }
+    // where rounding leaves no token that exceeds, the last one with weight
+    long long index = -1; float at_l = 0.0f; bool found = false;
+    for (long long q = lo; q >= 0 && index < 0; q--) {
+        double run = q ? spans[q - 1] : 0.0;
+        for (int e = 0; e < 4 && !found; e++) {
+            float l[4];
+            if (4 * q + e >= row.groups()) break;
+            row.load(4 * q + e, l);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const long long i = 4 * (4 * q + e) + j - row.off;
+                const double w = l[j] == l[j] && !found ? draw_kept(l[j], i, floor_rank, top, set) : 0.0;
+                run += w;
+                if (w > 0.0) { index = i; at_l = l[j]; found = run > want; }
+            }
+        }
+    }
+    a.indices[t] = index;
+    if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, total);
+}
+
+// ---- short rows: W lanes to a row, E tokens to a lane ----------------------------------------------------------------------------
+template <int W>
+__device__ __forceinline__ uint32_t draw_votes(bool b, int sub)       // lanes of the row that say yes
+{
+    const u64 v = __ballot(b);
+    return W == 64 ? __popcll(v) : __popcll((v >> (sub * W)) & ((1ull << (W & 63)) - 1));
+}
+template <int W>
+__device__ __forceinline__ double draw_lanes_sum(double v)
+{
+#pragma unroll
+    for (int d = W / 2; d; d >>= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+template <typename T, int W, int E>
+__global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
+{
+    constexpr int kRows = 64 / W;
+    __shared__ double s_mass[kBlock / 64][64 * E];
+    __shared__ float s_l[kBlock / 64][64 * E];
+    __shared__ double s_total[kBlock / 64][kRows], s_inv[kBlock / 64][kRows];
+    __shared__ float s_top[kBlock / 64][kRows];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / W, j0 = (lane % W) * E;
+    const long long r0 = ((long long)blockIdx.x * (kBlock / 64) + wave) * kRows, r = r0 + sub;
+    const int V = (int)a.V;
+    const bool on = r < a.R;
+    const DrawRow set = draw_row(a, on ? r : a.R - 1);
+    const T* row = (const T*)a.logits + (on ? r : a.R - 1) * a.row_stride;
+    float l[E];
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+        if (j0 + e + 4 <= V && ((uintptr_t)(row + j0 + e) & (4 * sizeof(T) - 1)) == 0) {
+            const Four<T> f = *(const Four<T>*)(row + j0 + e);
+#pragma unroll
+            for (int j = 0; j < 4; j++) l[e + j] = draw_logit(f.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) l[e + j] = j0 + e + j < V ? draw_logit(row[j0 + e + j]) : __builtin_nanf("");
+        }
+    }
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < E; e++) top = fmaxf(top, l[e]);
+#pragma unroll
+    for (int d = W / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const bool live = on && set.valid && top > -__builtin_inff();
+    double w[E];
+    uint32_t key[E];                                                 // 0: not a token, or cut
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        w[e] = draw_weight(l[e], top, set.inv_t);                    // 0 outside the row
+        key[e] = l[e] == l[e] ? draw_key(l[e]) : 0u;
+    }
+    // A cut at the highest key t for which the tokens of key >= t reach k, or `want`: found bit by bit; of the ones at t the first few in index order.
+#pragma unroll 1
+    for (int cut = 0; cut < 2; cut++) {
+        const bool mine = live && (cut == 0 ? set.k < a.V : set.p < 1.0);
+        if (!__any(mine)) continue;
+        double want = 0.0;
+        if (cut) {
+            double sum = 0.0;
+#pragma unroll
+            for (int e = 0; e < E; e++) sum += key[e] ? w[e] : 0.0;
+            want = set.p * draw_lanes_sum<W>(sum);
+        }
+        uint32_t t = 0;
+#pragma unroll 1
+        for (int b = 31; b >= 0; b--) {
+            const uint32_t up = t | 1u << b;
+            bool reached;
+            if (cut == 0) {
+                uint32_t n = 0;
+#pragma unroll
+                for (int e = 0; e < E; e++) n += draw_votes<W>(key[e] >= up, sub);
+                reached = (long long)n >= set.k;
+            } else {
+                double sum = 0.0;
+#pragma unroll
+                for (int e = 0; e < E; e++) sum += key[e] >= up ? w[e] : 0.0;
+                reached = draw_lanes_sum<W>(sum) >= want;
+            }
+            if (reached) t = up;
+        }
+        uint32_t ties = 0, above = 0, before = 0;
+        double mass = 0.0, tie_w = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            above += draw_votes<W>(key[e] > t, sub);
+            mass += key[e] > t ? w[e] : 0.0;
+            if (key[e] == t) { ties++; tie_w = w[e]; }
+        }
+        mass = draw_lanes_sum<W>(mass);
+        // ties in the lanes before this one, in all of them, and the weight that they share
+        uint32_t incl = ties;
+#pragma unroll
+        for (int d = 1; d < W; d <<= 1) {
+            const uint32_t o = __shfl_up(incl, d, W);
+            if (lane % W >= d) incl += o;
+        }
+        before = incl - ties;
+        const uint32_t all = __shfl(incl, W - 1, W);
+#pragma unroll
+        for (int d = W / 2; d; d >>= 1) tie_w = fmax(tie_w, __shfl_xor(tie_w, d, 64));
+        double m = cut == 0 ? (double)set.k - (double)above : tie_w > 0.0 ? ceil((want - mass) / tie_w) : (double)all;
+        const uint32_t kept = m < 1.0 ? 1u : m < (double)all ? (uint32_t)m : all;
+        if (mine)
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                if (key[e] == t && t) { if (before >= kept) key[e] = 0; before++; }
+                else if (key[e] < t) key[e] = 0;
+            }
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (!key[e] || w[e] < set.min_p) w[e] = 0.0;
+        sum += w[e];
+    }
+    double incl = sum;
+#pragma unroll
+    for (int d = 1; d < W; d <<= 1) {
+        const double o = __shfl_up(incl, d, W);
+        if (lane % W >= d) incl += o;
+    }
+    const double up = __shfl_up(incl, 1, W), total = __shfl(incl, W - 1, W);
+    double run = lane % W ? up : 0.0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        run += w[e];
+        // a token without weight is marked by its sign: sums of neighbouring lanes may differ by a rounding, and it is never drawn
+        s_mass[wave][lane * E + e] = w[e] > 0.0 ? run : -run;
+        s_l[wave][lane * E + e] = l[e];
+    }
+    if (lane % W == 0) { s_total[wave][sub] = live ? total : -1.0; s_inv[wave][sub] = set.inv_t; s_top[wave][sub] = top; }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");           // LDS of this wave's own lanes
+    __builtin_amdgcn_wave_barrier();
+    const int rows = a.R - r0 < kRows ? (int)(a.R - r0) : kRows;
+    if (rows <= 0) return;
+    for (long long q = lane; q < (long long)rows * a.S; q += 64) {
+        const int y = kRows == 1 ? 0 : (int)(q / a.S);
+        const double all = s_total[wave][y];
+        const double* mass = &s_mass[wave][y * W * E];
+        long long index = -1;
+        float lp = -__builtin_inff();
+        if (all > 0.0) {
+            const double want = draw_uniform(a, r0 * a.S + q) * all;
+            int lo = 0, hi = V - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (fabs(mass[mid]) > want) hi = mid; else lo = mid + 1;
+            }
+            int i = lo;
+            while (i > 0 && !(mass[i] > 0.0)) i--;
+            while (!(mass[i] > 0.0) && i < V - 1) i++;
+            index = i;
+            lp = draw_logprob(s_l[wave][y * W * E + i], s_top[wave][y], s_inv[wave][y], all);
+        }
+        a.indices[r0 * a.S + q] = index;
+        if (a.logprobs) a.logprobs[r0 * a.S + q] = lp;
     }
 }
 
@@ -282,28 +743,57 @@ static int draw_check(const gsx_draw* s)
     return GSX_OK;
 }
 
-struct DrawLayout { size_t mass, total, bounds, tops, keys, bytes; };
+struct DrawLayout { bool pick; long long spans_row; size_t spans, total, floors, tops, bytes; };
 
 static DrawLayout draw_layout(const gsx_draw* s)
 {
     DrawLayout l;
+    l.pick = s->V <= kDrawShort || (s->S <= kDrawInRow && s->V <= (int64_t)kDrawWaveTiles * 256 - 4);
+    l.spans_row = (s->V + 3 + 15) / 16;
+    l.spans = l.total = l.floors = l.tops = 0;
     size_t at = 0;
-    l.mass = at; at += align_up((size_t)s->R * (size_t)s->V * 8);
-    l.total = at; at += align_up((size_t)s->R * 8);
-    l.bounds = at; at += align_up((size_t)s->R * 8);
-    l.tops = at; at += align_up((size_t)s->R * 4);
-    l.keys = at; at += align_up((size_t)s->R * 4);
-    l.bytes = at;
+    if (!l.pick) {
+        l.spans = at; at += align_up((size_t)s->R * (size_t)l.spans_row * 8);
+        l.total = at; at += align_up((size_t)s->R * 8);
+        l.floors = at; at += align_up((size_t)s->R * 8);
+        l.tops = at; at += align_up((size_t)s->R * 4);
+    }
+    l.bytes = at ? at : 256;
     return l;
 }
 
-template <typename T>
-static int draw_run(const DrawArgs& a, int64_t R, hipStream_t stream)
+template <typename T, int W, int E>
+static void draw_short(const DrawArgs& a, hipStream_t stream)
 {
-    draw_mass_kernel<T><<<dim3((unsigned)R), dim3(kDrawBlock), 0, stream>>>(a);
-    GSX_LAUNCH_CHECK();
-    const int64_t n = R * a.S;
-    draw_pick_kernel<T><<<dim3((unsigned)ceil_div(n, kBlock)), dim3(kBlock), 0, stream>>>(a, n);
+    draw_short_kernel<T, W, E><<<dim3((unsigned)ceil_div(a.R, (kBlock / 64) * (64 / W))), dim3(kBlock), 0, stream>>>(a);
+}
+
+template <typename T>
+static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
+{
+    if (a.V <= kDrawShort) {
+        if (a.V <= 8) draw_short<T, 2, 4>(a, stream);
+        else if (a.V <= 16) draw_short<T, 4, 4>(a, stream);
+        else if (a.V <= 32) draw_short<T, 8, 4>(a, stream);
+        else if (a.V <= 64) draw_short<T, 16, 4>(a, stream);
+        else if (a.V <= 128) draw_short<T, 32, 4>(a, stream);
+        else if (a.V <= 256) draw_short<T, 64, 4>(a, stream);
+        else draw_short<T, 64, 8>(a, stream);
+        GSX_LAUNCH_CHECK();
+        return GSX_OK;
+    }
+    const dim3 grid((unsigned)a.R);
+    const bool small = a.V <= kDrawSmall && a.R > 256;           // there are rows to fill the card
+    if (l.pick) {
+        if (small) draw_row_kernel<T, 256, true><<<grid, dim3(256), 0, stream>>>(a);
+        else draw_row_kernel<T, 1024, true><<<grid, dim3(1024), 0, stream>>>(a);
+    } else {
+        if (small) draw_row_kernel<T, 256, false><<<grid, dim3(256), 0, stream>>>(a);
+        else draw_row_kernel<T, 1024, false><<<grid, dim3(1024), 0, stream>>>(a);
+        GSX_LAUNCH_CHECK();
+        const int64_t n = a.R * a.S;
+        draw_pick_kernel<T><<<dim3((unsigned)ceil_div(n, kBlock)), dim3(kBlock), 0, stream>>>(a, n);
+    }
     GSX_LAUNCH_CHECK();
     return GSX_OK;
 }
@@ -327,16 +817,16 @@ GSX_API int gsx_draw_indices(const gsx_draw* s, void* stream)
     if (s->ws_bytes < l.bytes) return GSX_E_CAPACITY;
     char* ws = (char*)s->ws;
     DrawArgs a;
-    a.logits = s->logits; a.row_stride = s->row_stride; a.V = s->V; a.S = s->S;
+    a.logits = s->logits; a.row_stride = s->row_stride; a.R = s->R; a.V = s->V; a.S = s->S;
     a.uniforms = s->uniforms; a.uniforms_f64 = s->uniforms_f64 != 0;
     a.temperature = s->temperature; a.top_p = s->top_p; a.min_p = s->min_p; a.top_k = s->top_k;
     a.temperatures = s->temperatures; a.top_ps = s->top_ps; a.min_ps = s->min_ps; a.top_ks = s->top_ks;
     a.indices = (long long*)s->indices; a.logprobs = s->logprobs;
-    a.mass = (double*)(ws + l.mass); a.total = (double*)(ws + l.total); a.tops = (float*)(ws + l.tops);
-    a.bounds = (long long*)(ws + l.bounds); a.keys = (uint32_t*)(ws + l.keys);
+    a.spans_row = l.spans_row;
+    a.spans = (double*)(ws + l.spans); a.total = (double*)(ws + l.total); a.floors = (u64*)(ws + l.floors); a.tops = (float*)(ws + l.tops);
     switch (s->dtype) {
-    case GSX_F32: return draw_run<float>(a, s->R, (hipStream_t)stream);
-    case GSX_BF16: return draw_run<__bf16>(a, s->R, (hipStream_t)stream);
-    default: return draw_run<_Float16>(a, s->R, (hipStream_t)stream);
+    case GSX_F32: return draw_run<float>(a, l, (hipStream_t)stream);
+    case GSX_BF16: return draw_run<__bf16>(a, l, (hipStream_t)stream);
+    default: return draw_run<_Float16>(a, l, (hipStream_t)stream);
     }
 }
