@@ -25,7 +25,7 @@ constexpr int kDrawFine = 512;                      // bins of the narrower ones
 constexpr int kDrawCand = 1024;                     // tokens that are ranked in LDS
 constexpr int kDrawSmall = 8192;                    // longest row that a quarter of a workgroup's threads takes
 constexpr int kDrawShort = 512;                     // longest row of the short way
-constexpr int kDrawWaveTiles = 4096;                // spans of 256 tokens whose masses are kept in LDS: rows of up to 1 M tokens
+constexpr int kDrawWaveTiles = 2048;                // spans of 256 tokens whose masses are kept in LDS: rows of up to 512 k tokens
 constexpr int kDrawInRow = 64;                      // draws per row that its workgroup makes itself
 constexpr int kDrawIndexBits = 27;
 
@@ -219,12 +219,16 @@ struct DrawHist { uint32_t count[kDrawBins]; u64 hi[kDrawBins], lo[kDrawBins]; }
 struct DrawFine { uint32_t count[kDrawFine]; u64 hi[kDrawFine], lo[kDrawFine]; };
 struct DrawCand { u64 rank[kDrawCand], ranked[kDrawCand]; double w[kDrawCand], ranked_w[kDrawCand]; };
 
+// The first try at the cuts of a row: where the histogram's bounds let them end.  Bins: k in bin bk, p in one of lo .. hi.
+struct DrawNear { int bk, lo, hi; long long above_k; int before_bk, upto_hi; bool sure; };
+
 // What the threads of a workgroup share while a cut is found
 struct DrawCut {
     long long above_n; u64 above_hi, above_lo;      // tokens in front of the bin, and their mass
     int bin; uint32_t in_bin, slots; int last;
     u64 lo, hi;                                     // ranks of the bin
     u64 floor_rank; double mass;                    // the answer: the lowest kept rank, the mass kept
+    DrawNear near;
     u64 wave_u[16]; uint32_t wave_n[16]; double wave_d[16]; float wave_f[16];
 };
 
@@ -382,11 +386,133 @@ __device__ u64 draw_cuts(DrawCut& c, const DrawHist& hist, DrawFine& fine, DrawC
     return floor_rank;
 }
 
+// The cuts in one pass over the row behind the histogram, where few enough tokens lie where they may end.
+// The histogram counts tokens and adds up 32-bit weights in units of 2^-31: near enough to say in which bins the top p may end (a bracket, usually
+// of one bin), not where.  One pass then adds up the 64-bit weights of the tokens in front of the bracket, which are kept whatever
+// happens, and collects the tokens inside it and in the bin where the top k end; these few are ranked and decided exactly.  `false`: too
+// many of them, or the sums do not bear the bracket out; the longer way has no such limits.
+// mass(q, w): adds a weight that is kept for certain to tile q (all lanes of the wave call it, once per group).
+template <int NT>
+__device__ __forceinline__ void draw_near_add(DrawHist& h, float l, float top, float scale, float units, bool by_k, bool by_p)
+{
+    const int b = draw_bin(l, top, scale);
+    if (by_k) atomicAdd(&h.count[b], 1u);
+    if (by_p) {
+        const float w = l == top ? 1.0f : __builtin_amdgcn_exp2f((l - top) * units);
+        const uint32_t m = (uint32_t)fminf(w * 0x1p31f + 0.5f, 2147483648.0f);
+        if (m) atomicAdd(&h.hi[b], (u64)m);
+    }
+}
+
+// where the cuts may end, from the histogram; c.near
+template <int NT>
+__device__ void draw_bracket(DrawCut& c, const DrawHist& h, const DrawRow& set, long long V, bool by_k, bool by_p)
+{
+    constexpr int per = kDrawBins / NT;
+    const int b0 = threadIdx.x * per;
+    if (threadIdx.x == 0) { c.near.bk = kDrawBins - 1; c.near.above_k = 0; c.near.lo = c.near.hi = kDrawBins - 1; }
+    uint32_t n = 0, all_n; u64 m = 0, all_m = 0, at_m = 0;
+#pragma unroll
+    for (int j = 0; j < per; j++) { if (by_k) n += h.count[b0 + j]; if (by_p) m += h.hi[b0 + j]; }
+    if (by_k) {
+        long long at = draw_before<NT, uint32_t>(n, c.wave_n, &all_n);
+#pragma unroll
+        for (int j = 0; j < per; j++) {
+            const long long next = at + h.count[b0 + j];
+            if (at < set.k && next >= set.k) { c.near.bk = b0 + j; c.near.above_k = at; }
+            at = next;
+        }
+    }
+    if (by_p) {
+        at_m = draw_before<NT, u64>(m, c.wave_u, &all_m);
+        __syncthreads();
+        // mass in front of bin bk and with it, and what the sums of 32-bit weights may be off: 2^-15 of them and half a unit per token
+        const int bk = c.near.bk;
+        double low = (double)all_m, high = low;
+        if (by_k) {
+            if (bk / per == (int)threadIdx.x) {
+                u64 a = at_m;
+#pragma unroll
+                for (int j = 0; j < per; j++) { if (b0 + j == bk) { c.lo = a; c.hi = a + h.hi[b0 + j]; } a += h.hi[b0 + j]; }
+            }
+            __syncthreads();
+            low = (double)c.lo; high = (double)c.hi;
+        }
+        const double off = (double)V * 0.5;
+        low = set.p * (low * (1.0 - 0x1p-15) - off); high = set.p * (high * (1.0 + 0x1p-15) + off);
+        const double want_lo = low * (1.0 - 0x1p-15) - off, want_hi = high * (1.0 + 0x1p-15) + off;
+        u64 at = at_m;
+#pragma unroll
+        for (int j = 0; j < per; j++) {
+            const u64 next = at + h.hi[b0 + j];
+            const int b = b0 + j;
+            if (b <= bk) {
+                if ((b == 0 || (double)at < want_lo) && ((double)next >= want_lo || b == bk)) c.near.lo = b;
+                if ((b == 0 || (double)at < want_hi) && ((double)next >= want_hi || b == bk)) c.near.hi = b;
+            }
+            at = next;
+        }
+    }
+    __syncthreads();
+}
+
+// The collected tokens (c.slots of them) ranked, and the cuts among them.  above: the 64-bit mass of all tokens in front of bin near.lo; total: of
+// all in front of bin near.bk (of all, without a top k).
+template <int NT>
+__device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, float top, bool by_k, bool by_p, double above, double total)
+{
+    const int most = NT < kDrawCand ? NT : kDrawCand, t = threadIdx.x;
+    if (c.slots > (uint32_t)most) return false;
+    const int m = (int)c.slots;
+    if (t < m) {
+        const u64 mine = cand.rank[t];
+        int place = 0;
+        for (int j = 0; j < m; j++) place += cand.rank[j] > mine;
+        cand.ranked[place] = mine; cand.ranked_w[place] = cand.w[t];
+    }
+    if (t == 0) { c.near.before_bk = 0; c.near.upto_hi = 0; c.near.sure = false; c.last = 0; }
+    __syncthreads();
+    const int bin = t < m ? draw_bin(draw_unkey((uint32_t)(cand.ranked[t] >> kDrawIndexBits)), top, set.scale) : kDrawBins;
+    const u64 front = __ballot(bin < c.near.bk), upto = __ballot(bin <= c.near.hi);
+    if ((t & 63) == 0) { atomicAdd(&c.near.before_bk, (int)__popcll(front)); atomicAdd(&c.near.upto_hi, (int)__popcll(upto)); }
+    __syncthreads();
+    int n = m;                                                       // candidates that the top k leaves
+    if (by_k) {
+        const long long left = (long long)c.near.before_bk + set.k - c.near.above_k;
+        n = left < m ? (int)left : m;
+    }
+    double all;
+    const double w = t < n ? cand.ranked_w[t] : 0.0;
+    const double before = draw_before<NT, double>(w, c.wave_d, &all);
+    if (!by_p) {
+        if (t == 0) c.floor_rank = cand.ranked[n - 1];
+        __syncthreads();
+        return true;
+    }
+    // the candidates of bin bk, where it lies behind the bracket, count for the total only
+    double tail = 0.0, none;
+    if (by_k) { none = draw_before<NT, double>(t >= c.near.before_bk ? w : 0.0, c.wave_d, &tail); (void)none; }
+    const double want = set.p * (total + tail);
+    const int upto_n = c.near.upto_hi < n ? c.near.upto_hi : n;
+    const bool in = t < upto_n && ((t == 0 && c.near.lo == 0) || above + before < want);
+    if (in) atomicMax(&c.last, t + 1);
+    // borne out: the first candidate is kept, and all of them reach the share, or nothing lies behind them
+    if (t == upto_n - 1) c.near.sure = above + before + w >= want || c.near.hi == c.near.bk;
+    __syncthreads();
+    const int last = c.last;
+    if (!c.near.sure || last == 0) return false;
+    if (t == 0) c.floor_rank = cand.ranked[last - 1];
+    __syncthreads();
+    return true;
+}
+
 // ---- one workgroup per row -----------------------------------------------------------------------------------------------------
 template <typename T, int NT, bool PICK>
 __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
 {
-    __shared__ union { struct { DrawHist hist; union { DrawFine fine; DrawCand cand; }; } s; double tile[kDrawWaveTiles]; } sh;
+    __shared__ DrawHist hist;                                        // its limbs take the candidates' masses by tile later on
+    __shared__ union { DrawFine fine; DrawCand cand; } sh;
+    __shared__ double tile[PICK ? kDrawWaveTiles : 1];
     __shared__ DrawCut c;
     constexpr int kWaves = NT / 64;
     const long long r = blockIdx.x;
@@ -420,15 +546,86 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
                 if (l[j] == l[j]) f(l[j], 4 * g + j - row.off);
         }
     };
+    auto all_groups = [&](auto f) {                                  // every thread of a wave, also where the wave reaches beyond the row
+        for (long long g0 = 0; g0 < groups; g0 += NT) {
+            float l[4] = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            if (g0 + tid < groups) row.load(g0 + tid, l);
+            f(l, g0 + tid);
+        }
+    };
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
     u64 floor_rank = 0;
+    bool tiled = false;                                              // the tiles' masses are there already
     if (by_k || by_p) {
-        for (int b = tid; b < kDrawBins; b += NT) { sh.s.hist.count[b] = 0; sh.s.hist.hi[b] = 0; sh.s.hist.lo[b] = 0; }
+        for (int b = tid; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; }
         __syncthreads();
-        tokens([&](float l, long long) { draw_hist_add(sh.s.hist, l, top, set.inv_t, set.scale, by_p); });
+        const float units = (float)(set.inv_t * 0x1.71547652b82fep+0);
+        tokens([&](float l, long long) { draw_near_add<NT>(hist, l, top, set.scale, units, by_k, by_p); });
         __syncthreads();
-        auto each = [&](auto f) { tokens([&](float l, long long i) { f(l, draw_rank(l, i)); }); };
-        floor_rank = draw_cuts<NT>(c, sh.s.hist, sh.s.fine, sh.s.cand, each, top, set, by_k, by_p);
+        draw_bracket<NT>(c, hist, set, a.V, by_k, by_p);
+        const int bk = c.near.bk, lo = by_p ? c.near.lo : bk, hi = by_p ? c.near.hi : bk;
+        if (tid == 0) c.slots = 0;
+        if (PICK) for (int q = tid; q < kDrawWaveTiles; q += NT) { hist.hi[q] = 0; hist.lo[q] = 0; tile[q] = 0.0; }
+        __syncthreads();
+        // 64-bit weights: of all tokens for the total of a top p, in front of the bracket for its sum and for the tiles
+        const int sums_to = by_p ? (by_k ? bk - 1 : kDrawBins - 1) : lo - 1;
+        double above = 0.0, total = 0.0;
+        auto pass = [&](const float (&l)[4], long long g) {
+            double sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int b = l[j] == l[j] ? draw_bin(l[j], top, set.scale) : kDrawBins;
+                const bool in = (b >= lo && b <= hi) || (by_k && b == bk);
+                double w = 0.0;
+                if (b <= sums_to || in) w = draw_weight(l[j], top, set.inv_t);
+                if (b <= sums_to) total += w;
+                if (b < lo) { above += w; sum += w < set.min_p ? 0.0 : w; }
+                if (in) {
+                    const uint32_t slot = atomicAdd(&c.slots, 1u);
+                    if (slot < (uint32_t)(NT < kDrawCand ? NT : kDrawCand)) { sh.cand.rank[slot] = draw_rank(l[j], 4 * g + j - row.off); sh.cand.w[slot] = w; }
+                }
+            }
+            if (PICK && lo > 0) {
+#pragma unroll
+                for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+                if (lane == 0) tile[g >> 6] = sum;
+            }
+        };
+        all_groups(pass);
+        __syncthreads();
+        double all_above, all_total;
+        draw_before<NT, double>(above, c.wave_d, &all_above);
+        draw_before<NT, double>(total, c.wave_d, &all_total);
+        __syncthreads();
+        if (draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, all_above, all_total)) {
+            floor_rank = c.floor_rank;
+            if (PICK) {
+                if (tid < (int)c.slots) {                            // the kept candidates' weights, as whole numbers: any order gives the same sums
+                    const u64 rank = sh.cand.rank[tid];
+                    const double w = sh.cand.w[tid];
+                    if (rank >= floor_rank && !(w < set.min_p)) {
+                        const long long i = ((1ll << kDrawIndexBits) - 1) - (long long)(rank & ((1ull << kDrawIndexBits) - 1));
+                        const int q = (int)((i + row.off) >> 8);
+                        uint32_t wh, wl;
+                        draw_limbs(w, wh, wl);
+                        atomicAdd(&hist.hi[q], (u64)wh);
+                        atomicAdd(&hist.lo[q], (u64)wl);
+                    }
+                }
+                __syncthreads();
+                const int tiles = (int)((groups + 63) >> 6);
+                for (int q = tid; q < tiles; q += NT) tile[q] += limbs(hist.hi[q], hist.lo[q]);
+                tiled = true;
+            }
+        } else {
+            __syncthreads();
+            for (int b = tid; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; hist.lo[b] = 0; }
+            __syncthreads();
+            tokens([&](float l, long long) { draw_hist_add(hist, l, top, set.inv_t, set.scale, by_p); });
+            __syncthreads();
+            auto each = [&](auto f) { tokens([&](float l, long long i) { f(l, draw_rank(l, i)); }); };
+            floor_rank = draw_cuts<NT>(c, hist, sh.fine, sh.cand, each, top, set, by_k, by_p);
+        }
         __syncthreads();
     }
     auto mass4 = [&](const float (&l)[4], long long g, double (&w)[4]) {
@@ -440,34 +637,28 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         }
         return sum;
     };
-    auto all_groups = [&](auto f) {                                  // every thread of a wave, also where the wave reaches beyond the row
-        for (long long g0 = 0; g0 < groups; g0 += NT) {
-            float l[4] = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-            if (g0 + tid < groups) row.load(g0 + tid, l);
-            f(l, g0 + tid);
-        }
-    };
     if (PICK) {
         // masses of 256 tokens, one wave's groups, in LDS; then the inclusive sums of these
-        all_groups([&](const float (&l)[4], long long g) {
-            double w[4], sum = mass4(l, g, w);
+        if (!tiled)
+            all_groups([&](const float (&l)[4], long long g) {
+                double w[4], sum = mass4(l, g, w);
 #pragma unroll
-            for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-            if (lane == 0) sh.tile[g >> 6] = sum;
-        });
+                for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+                if (lane == 0) tile[g >> 6] = sum;
+            });
         __syncthreads();
         const int tiles = (int)((groups + 63) >> 6), per = (tiles + NT - 1) / NT;
         double sum = 0.0, total;
-        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) sum += sh.tile[q];
+        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) sum += tile[q];
         double at = draw_before<NT, double>(sum, c.wave_d, &total);
-        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) { at += sh.tile[q]; sh.tile[q] = at; }
+        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) { at += tile[q]; tile[q] = at; }
         __syncthreads();
         for (long long s = wave; s < a.S; s += kWaves) {             // a wave per draw
             const double want = draw_uniform(a, r * a.S + s) * total;
             int lo = 0, hi = tiles - 1;
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
-                if (sh.tile[mid] > want) hi = mid; else lo = mid + 1;
+                if (tile[mid] > want) hi = mid; else lo = mid + 1;
             }
             // the first token in the tile that exceeds; where rounding leaves none, the last one with weight
             for (int q = lo; q >= 0; q--) {
@@ -481,7 +672,7 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
                     if (lane >= d) incl += o;
                 }
                 const double up = __shfl_up(incl, 1, 64);
-                double run = (q ? sh.tile[q - 1] : 0.0) + (lane ? up : 0.0);
+                double run = (q ? tile[q - 1] : 0.0) + (lane ? up : 0.0);
                 int hit = -1, any = -1;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
