@@ -27,6 +27,8 @@ constexpr int kDrawSmall = 8192;                    // longest row that a quarte
 constexpr int kDrawShort = 512;                     // longest row of the short way
 constexpr int kDrawWaveTiles = 2048;                // spans of 256 tokens whose masses are kept in LDS: rows of up to 512 k tokens
 constexpr int kDrawInRow = 64;                      // draws per row that its workgroup makes itself
+constexpr int64_t kDrawLong = 32768;                // rows longer than this are cut into parts ...
+constexpr int64_t kDrawFewRows = 128;               // ... where there are at most so many of them
 constexpr int kDrawIndexBits = 27;
 
 typedef unsigned long long u64;
@@ -41,6 +43,13 @@ struct DrawArgs {
     double* spans;                                  // [row][spans_row]: inclusive mass behind every 16 tokens
     double* total; float* tops; u64* floors;        // per row: kept mass (-1: none), top, lowest kept rank
     long long spans_row;
+    // rows in parts: `part` groups of four places each, `parts` to a row; `walkers` workgroups per row where a workgroup takes several parts
+    long long part; int parts, walkers, cuts;
+    float* part_top; double* part_mass;             // [row][part]
+    uint32_t* hist_n; u64* hist_m;                  // [row][walker][bin]
+    uint32_t* row_n; u64* row_m;                    // [row][bin]
+    double* sums;                                   // [row][walker][2]: 64-bit mass in front of the bracket, and the total's part
+    u64* list; uint32_t* list_n; long long list_most;        // [row]: ranks of the tokens where the cuts may end
 };
 
 // ---- tokens ---------------------------------------------------------------------------------------------------------------
@@ -224,7 +233,8 @@ struct DrawNear { int bk, lo, hi; long long above_k; int before_bk, upto_hi; boo
 
 // What the threads of a workgroup share while a cut is found
 struct DrawCut {
-    long long above_n; u64 above_hi, above_lo;      // tokens in front of the bin, and their mass
+    long long above_n; u64 above_hi, above_lo;      // tokens in front of the bin, and their mass: base and the limbs
+    double base;
     int bin; uint32_t in_bin, slots; int last;
     u64 lo, hi;                                     // ranks of the bin
     u64 floor_rank; double mass;                    // the answer: the lowest kept rank, the mass kept
@@ -238,6 +248,7 @@ __device__ void draw_find(DrawCut& c, const uint32_t* count, const u64* hi, cons
 {
     const int per = bins > NT ? bins / NT : 1, b0 = threadIdx.x * per;
     uint32_t n = 0, all_n; u64 h = 0, l = 0, all;
+    const double base = c.base;
     const bool mine = b0 < bins;
     if (mine)
         for (int b = b0; b < b0 + per; b++) { n += count[b]; if (with_mass) { h += hi[b]; l += lo[b]; } }
@@ -247,11 +258,11 @@ __device__ void draw_find(DrawCut& c, const uint32_t* count, const u64* hi, cons
     if (with_mass) { at_h += draw_before<NT, u64>(h, c.wave_u, &all); at_l += draw_before<NT, u64>(l, c.wave_u, &all); }
     __syncthreads();
     if (mine) {
-        bool before = by_mass ? b0 > 0 && limbs(at_h, at_l) >= want : at_n >= k;
+        bool before = by_mass ? b0 > 0 && base + limbs(at_h, at_l) >= want : at_n >= k;
         for (int b = b0; b < b0 + per && b <= last && !before; b++) {
             const long long next_n = at_n + count[b];
             const u64 next_h = at_h + (with_mass ? hi[b] : 0), next_l = at_l + (with_mass ? lo[b] : 0);
-            const bool here = by_mass ? limbs(next_h, next_l) >= want : next_n >= k;
+            const bool here = by_mass ? base + limbs(next_h, next_l) >= want : next_n >= k;
             if (here || b == last) { c.bin = b; c.in_bin = count[b]; c.above_n = at_n; c.above_hi = at_h; c.above_lo = at_l; }
             before = here;
             at_n = next_n; at_h = next_h; at_l = next_l;
@@ -260,12 +271,11 @@ __device__ void draw_find(DrawCut& c, const uint32_t* count, const u64* hi, cons
     __syncthreads();
 }
 
-// Finds where a cut ends among the tokens of bin c.bin (c.in_bin of them at most) whose rank is at least `floor_rank`.  each(f) calls f(l, rank)
+// Finds where a cut ends among the tokens of bins bin0 .. bin1 (c.in_bin of them at most) whose rank is at least `floor_rank`.  each(f) calls f(l, rank)
 // for every token of the source, over all threads.
 template <int NT, typename Each>
-__device__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const Each& each, float top, double inv_t, float scale, u64 floor_rank, bool by_mass, bool with_mass, long long k, double want)
+__device__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const Each& each, float top, double inv_t, float scale, int bin0, int bin1, u64 floor_rank, bool by_mass, bool with_mass, long long k, double want)
 {
-    const int bin = c.bin;
     u64 lo = floor_rank, hi = ~0ull;
     uint32_t n = c.in_bin;
     const int most = NT < kDrawCand ? NT : kDrawCand;
@@ -274,8 +284,8 @@ __device__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const E
         if (!narrowed) {                                             // the ranks of the bin: its keys are neighbours
             if (threadIdx.x < 2) {
                 uint32_t a = draw_key(-__builtin_inff()), b = draw_key(__builtin_inff());
-                // the lowest key whose bin is at most `bin`; one below the lowest key whose bin is less than it
-                const int want_bin = threadIdx.x == 0 ? bin : bin - 1;
+                // the lowest key whose bin is at most bin1; one below the lowest key whose bin is less than bin0
+                const int want_bin = threadIdx.x == 0 ? bin1 : bin0 - 1;
                 b += threadIdx.x;                                    // "none" for bin 0
                 while (a < b) {
                     const uint32_t mid = a + (b - a) / 2;
@@ -314,7 +324,8 @@ __device__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const E
     if (threadIdx.x == 0) { c.slots = 0; c.last = 0; }
     __syncthreads();
     each([&](float l, u64 rank) {
-        if (rank < lo || rank > hi || (!narrowed && draw_bin(l, top, scale) != bin)) return;
+        if (rank < lo || rank > hi) return;
+        if (!narrowed) { const int b = draw_bin(l, top, scale); if (b < bin0 || b > bin1) return; }
         const uint32_t slot = atomicAdd(&c.slots, 1u);
         if (slot < (uint32_t)most) { cand.rank[slot] = rank; cand.w[slot] = draw_weight(l, top, inv_t); }
     });
@@ -330,7 +341,7 @@ __device__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const E
     __syncthreads();
     double all;
     const double w = t < m ? cand.ranked_w[t] : 0.0;
-    const double above = limbs(c.above_hi, c.above_lo);
+    const double above = c.base + limbs(c.above_hi, c.above_lo);
     const double before = draw_before<NT, double>(w, c.wave_d, &all);
     const bool in = t < m && (t == 0 || (by_mass ? above + before < want : c.above_n + t < k));
     if (in) atomicMax(&c.last, t);
@@ -360,11 +371,11 @@ __device__ u64 draw_cuts(DrawCut& c, const DrawHist& hist, DrawFine& fine, DrawC
     int last = kDrawBins - 1;
     double total = 0.0;
     if (by_k) {
-        if (threadIdx.x == 0) { c.above_n = 0; c.above_hi = 0; c.above_lo = 0; }
+        if (threadIdx.x == 0) { c.above_n = 0; c.above_hi = 0; c.above_lo = 0; c.base = 0.0; }
         __syncthreads();
         draw_find<NT>(c, hist.count, hist.hi, hist.lo, kDrawBins, last, false, by_p, set.k, 0.0);
         last = c.bin;
-        draw_resolve<NT>(c, fine, cand, each, top, set.inv_t, set.scale, 0, false, by_p, set.k, 0.0);
+        draw_resolve<NT>(c, fine, cand, each, top, set.inv_t, set.scale, c.bin, c.bin, 0, false, by_p, set.k, 0.0);
         floor_rank = c.floor_rank;
         total = c.mass;
         __syncthreads();
@@ -377,10 +388,10 @@ __device__ u64 draw_cuts(DrawCut& c, const DrawHist& hist, DrawFine& fine, DrawC
             draw_before<NT, u64>(l, c.wave_u, &all_l);
             total = limbs(all_h, all_l);
         }
-        if (threadIdx.x == 0) { c.above_n = 0; c.above_hi = 0; c.above_lo = 0; }
+        if (threadIdx.x == 0) { c.above_n = 0; c.above_hi = 0; c.above_lo = 0; c.base = 0.0; }
         __syncthreads();
         draw_find<NT>(c, hist.count, hist.hi, hist.lo, kDrawBins, last, true, true, 0, set.p * total);
-        draw_resolve<NT>(c, fine, cand, each, top, set.inv_t, set.scale, floor_rank, true, true, 0, set.p * total);
+        draw_resolve<NT>(c, fine, cand, each, top, set.inv_t, set.scale, c.bin, c.bin, floor_rank, true, true, 0, set.p * total);
         floor_rank = c.floor_rank > floor_rank ? c.floor_rank : floor_rank;
     }
     return floor_rank;
@@ -759,6 +770,348 @@ __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long
     if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, total);
 }
 
+// ---- a few long rows, in parts over the card -------------------------------------------------------------------------------------
+constexpr int kDrawPart = 256;                      // threads of a part's workgroup, and spans of 16 tokens in a part times part / 1024
+constexpr int kDrawWalk = 512;                      // threads of a workgroup that walks several parts
+
+template <typename T>
+__global__ __launch_bounds__(kDrawPart) void draw_part_top_kernel(DrawArgs a)
+{
+    __shared__ float s_f[kDrawPart / 64];
+    const long long r = blockIdx.y;
+    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+    const long long groups = row.groups(), g0 = blockIdx.x * a.part, g1 = g0 + a.part < groups ? g0 + a.part : groups;
+    float top = -__builtin_inff();
+#pragma unroll 4
+    for (long long g = g0 + threadIdx.x; g < g1; g += kDrawPart) {
+        float l[4];
+        row.load(g, l);
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = fmaxf(top, l[j]);
+    }
+    top = draw_max<kDrawPart>(top, s_f);
+    if (threadIdx.x == 0) {
+        a.part_top[r * a.parts + blockIdx.x] = top;
+        if (blockIdx.x == 0 && a.cuts) a.list_n[r] = 0;
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ float draw_row_top(const DrawArgs& a, long long r, float* s_f)
+{
+    float top = -__builtin_inff();
+    for (int p = threadIdx.x; p < a.parts; p += NT) top = fmaxf(top, a.part_top[r * a.parts + p]);
+    return draw_max<NT>(top, s_f);
+}
+
+// f(l, g) for the groups of a walker's parts, every thread of a wave
+template <int NT, typename T, typename F>
+__device__ __forceinline__ void draw_walk(const DrawArgs& a, const Places<T>& row, F f)
+{
+    const long long groups = row.groups();
+    const long long each = ((groups + a.walkers - 1) / a.walkers + NT - 1) / NT * NT;
+    const long long g1 = (blockIdx.x + 1) * each < groups ? (blockIdx.x + 1) * each : groups;
+    for (long long g = blockIdx.x * each; g < g1; g += NT) {
+        float l[4] = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        if (g + threadIdx.x < g1) row.load(g + threadIdx.x, l);
+        f(l, g + threadIdx.x);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kDrawWalk) void draw_part_hist_kernel(DrawArgs a)
+{
+    __shared__ DrawHist hist;
+    __shared__ float s_f[kDrawWalk / 64];
+    const long long r = blockIdx.y;
+    const DrawRow set = draw_row(a, r);
+    const bool by_k = set.k < a.V, by_p = set.p < 1.0;
+    const float top = draw_row_top<kDrawWalk>(a, r, s_f);
+    if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) return;
+    for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) { hist.count[b] = 0; hist.hi[b] = 0; }
+    __syncthreads();
+    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+    const float units = (float)(set.inv_t * 0x1.71547652b82fep+0);
+    draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], long long) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (l[j] == l[j]) draw_near_add<kDrawWalk>(hist, l[j], top, set.scale, units, by_k, by_p);
+    });
+    __syncthreads();
+    const long long at = (r * a.walkers + blockIdx.x) * kDrawBins;
+    for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) { a.hist_n[at + b] = hist.count[b]; a.hist_m[at + b] = hist.hi[b]; }
+}
+
+// 64 bins to a workgroup, its waves share the walkers out
+__global__ __launch_bounds__(1024) void draw_sum_hist_kernel(DrawArgs a)
+{
+    __shared__ uint32_t s_n[16][64];
+    __shared__ u64 s_m[16][64];
+    const long long r = blockIdx.y;
+    const DrawRow set = draw_row(a, r);
+    if (!set.valid || (set.k >= a.V && !(set.p < 1.0))) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bin = blockIdx.x * 64 + lane;
+    uint32_t n = 0; u64 m = 0;
+#pragma unroll 8
+    for (int w = wave; w < a.walkers; w += 16) {
+        n += a.hist_n[(r * a.walkers + w) * kDrawBins + bin];
+        m += a.hist_m[(r * a.walkers + w) * kDrawBins + bin];
+    }
+    s_n[wave][lane] = n; s_m[wave][lane] = m;
+    __syncthreads();
+    if (wave == 0) {
+        for (int w = 1; w < 16; w++) { n += s_n[w][lane]; m += s_m[w][lane]; }
+        a.row_n[r * kDrawBins + bin] = n; a.row_m[r * kDrawBins + bin] = m;
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ void draw_load_hist(const DrawArgs& a, long long r, DrawHist& hist, DrawCut& c, const DrawRow& set, bool by_k, bool by_p)
+{
+    for (int b = threadIdx.x; b < kDrawBins; b += NT) { hist.count[b] = a.row_n[r * kDrawBins + b]; hist.hi[b] = a.row_m[r * kDrawBins + b]; }
+    __syncthreads();
+    draw_bracket<NT>(c, hist, set, a.V, by_k, by_p);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
+{
+    __shared__ DrawHist hist;
+    __shared__ DrawCut c;
+    const long long r = blockIdx.y;
+    const DrawRow set = draw_row(a, r);
+    const bool by_k = set.k < a.V, by_p = set.p < 1.0;
+    const float top = draw_row_top<kDrawWalk>(a, r, c.wave_f);
+    if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) return;
+    draw_load_hist<kDrawWalk>(a, r, hist, c, set, by_k, by_p);
+    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+    const int bk = c.near.bk, lo = by_p ? c.near.lo : bk, hi = by_p ? c.near.hi : bk;
+    const int sums_to = by_p ? (by_k ? bk - 1 : kDrawBins - 1) : -1;
+    double above = 0.0, total = 0.0;
+    const int lane = threadIdx.x & 63;
+    draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], long long g) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int b = l[j] == l[j] ? draw_bin(l[j], top, set.scale) : kDrawBins;
+            const bool in = (b >= lo && b <= hi) || (by_k && b == bk);
+            if (b <= sums_to) {
+                const double w = draw_weight(l[j], top, set.inv_t);
+                total += w;
+                if (b < lo) above += w;
+            }
+            const u64 who = __ballot(in);                            // one place in the list for a wave's tokens
+            if (who) {
+                uint32_t at = 0;
+                if (lane == __ffsll((long long)who) - 1) at = atomicAdd(&a.list_n[r], (uint32_t)__popcll(who));
+                at = __shfl(at, __ffsll((long long)who) - 1, 64) + (uint32_t)__popcll(who & ((1ull << lane) - 1));
+                if (in && at < (uint64_t)a.list_most) a.list[r * a.list_most + at] = draw_rank(l[j], 4 * g + j - row.off);
+            }
+        }
+    });
+    double all_above, all_total;
+    draw_before<kDrawWalk, double>(above, c.wave_d, &all_above);
+    draw_before<kDrawWalk, double>(total, c.wave_d, &all_total);
+    if (threadIdx.x == 0) {
+        a.sums[(r * a.walkers + blockIdx.x) * 2] = all_above;
+        a.sums[(r * a.walkers + blockIdx.x) * 2 + 1] = all_total;
+    }
+}
+
+// one workgroup per row: the cuts among the list's tokens, of any number; -> a.floors
+template <typename T>
+__global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
+{
+    constexpr int NT = 1024;
+    __shared__ DrawHist hist;
+    __shared__ union { DrawFine fine; DrawCand cand; } sh;
+    __shared__ DrawCut c;
+    const long long r = blockIdx.x;
+    const int tid = threadIdx.x;
+    const DrawRow set = draw_row(a, r);
+    const bool by_k = set.k < a.V, by_p = set.p < 1.0;
+    const float top = draw_row_top<NT>(a, r, c.wave_f);
+    if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) { if (tid == 0) a.floors[r] = 0; return; }
+    draw_load_hist<NT>(a, r, hist, c, set, by_k, by_p);
+    double above = 0.0, total = 0.0, v;
+    for (int w0 = 0; w0 < a.walkers; w0 += NT) {                     // a fixed order
+        const int w = w0 + tid;
+        draw_before<NT, double>(w < a.walkers ? a.sums[(r * a.walkers + w) * 2] : 0.0, c.wave_d, &v);
+        above += v;
+        draw_before<NT, double>(w < a.walkers ? a.sums[(r * a.walkers + w) * 2 + 1] : 0.0, c.wave_d, &v);
+        total += v;
+    }
+    const long long n = a.list_n[r];
+    const u64* list = a.list + r * a.list_most;
+    bool done = false;
+    if (n <= NT) {
+        if (tid < n) {
+            const u64 rank = list[tid];
+            sh.cand.rank[tid] = rank;
+            sh.cand.w[tid] = draw_weight(draw_unkey((uint32_t)(rank >> kDrawIndexBits)), top, set.inv_t);
+        }
+        if (tid == 0) c.slots = (uint32_t)n;
+        __syncthreads();
+        done = draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, above, total);
+    } else if (n <= a.list_most) {
+        auto each = [&](auto f) {
+            for (long long i = tid; i < n; i += NT) { const u64 rank = list[i]; f(draw_unkey((uint32_t)(rank >> kDrawIndexBits)), rank); }
+        };
+        const int bk = c.near.bk, lo = c.near.lo, hi = c.near.hi;
+        u64 floor_rank = 0;
+        __syncthreads();
+        if (by_k) {
+            if (tid == 0) { c.above_n = c.near.above_k; c.above_hi = 0; c.above_lo = 0; c.base = total; c.in_bin = (uint32_t)n; }
+            __syncthreads();
+            draw_resolve<NT>(c, sh.fine, sh.cand, each, top, set.inv_t, set.scale, bk, bk, 0, false, by_p, set.k, 0.0);
+            floor_rank = c.floor_rank; total = c.mass;
+            __syncthreads();
+        }
+        done = true;
+        if (by_p) {
+            const double want = set.p * total;
+            double mine = 0.0, in;
+            each([&](float l, u64 rank) { if (rank >= floor_rank && draw_bin(l, top, set.scale) <= hi) mine += draw_weight(l, top, set.inv_t); });
+            draw_before<NT, double>(mine, c.wave_d, &in);
+            done = (lo == 0 || above < want) && (hi == bk || above + in >= want);
+            if (done) {
+                if (tid == 0) { c.above_n = 0; c.above_hi = 0; c.above_lo = 0; c.base = above; c.in_bin = (uint32_t)n; }
+                __syncthreads();
+                draw_resolve<NT>(c, sh.fine, sh.cand, each, top, set.inv_t, set.scale, lo, hi, floor_rank, true, true, 0, want);
+                if (tid == 0 && c.floor_rank < floor_rank) c.floor_rank = floor_rank;
+                __syncthreads();
+            }
+        }
+    }
+    if (!done) {                                                     // over the whole row, exactly from the first histogram on
+        const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+        const long long groups = row.groups();
+        auto each = [&](auto f) {
+            for (long long g = tid; g < groups; g += NT) {
+                float l[4];
+                row.load(g, l);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (l[j] == l[j]) f(l[j], draw_rank(l[j], 4 * g + j - row.off));
+            }
+        };
+        __syncthreads();
+        for (int b = tid; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; hist.lo[b] = 0; }
+        __syncthreads();
+        each([&](float l, u64) { draw_hist_add(hist, l, top, set.inv_t, set.scale, by_p); });
+        __syncthreads();
+        const u64 floor_rank = draw_cuts<NT>(c, hist, sh.fine, sh.cand, each, top, set, by_k, by_p);
+        if (tid == 0) c.floor_rank = floor_rank;
+        __syncthreads();
+    }
+    if (tid == 0) a.floors[r] = c.floor_rank;
+}
+
+// the masses of a part: inclusive sums behind every 16 tokens, counted from the part's start
+template <typename T>
+__global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
+{
+    __shared__ double s_d[kDrawPart / 64];
+    __shared__ float s_f[kDrawPart / 64];
+    __shared__ double span[kDrawPart];
+    const long long r = blockIdx.y;
+    const int tid = threadIdx.x;
+    const DrawRow set = draw_row(a, r);
+    const float top = draw_row_top<kDrawPart>(a, r, s_f);
+    double carry = 0.0;
+    if (set.valid && top > -__builtin_inff()) {
+        const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+        const u64 floor_rank = a.cuts ? a.floors[r] : 0;
+        const long long groups = row.groups(), g0 = blockIdx.x * a.part;
+        double* spans = a.spans + r * a.spans_row + g0 / 4;
+        for (long long b = 0; b < a.part && g0 + b < groups; b += 4 * kDrawPart) {
+            float l[4][4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const long long g = g0 + b + q * kDrawPart + tid;
+                l[q][0] = l[q][1] = l[q][2] = l[q][3] = __builtin_nanf("");
+                if (g < groups) row.load(g, l[q]);
+            }
+            __syncthreads();                                         // span[] of the round before has been read
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                double sum = 0.0;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (l[q][j] == l[q][j]) sum += draw_kept(l[q][j], 4 * (g0 + b + q * kDrawPart + tid) + j - row.off, floor_rank, top, set);
+                sum += __shfl_xor(sum, 1, 64);
+                sum += __shfl_xor(sum, 2, 64);
+                if ((tid & 3) == 0) span[(q * kDrawPart + tid) >> 2] = sum;
+            }
+            __syncthreads();
+            double all;
+            const double mine = span[tid], before = draw_before<kDrawPart, double>(mine, s_d, &all);
+            if (4 * (b / 4 + tid) < groups - g0) spans[b / 4 + tid] = carry + before + mine;
+            carry += all;
+        }
+    }
+    if (tid == 0) a.part_mass[r * a.parts + blockIdx.x] = carry;
+}
+
+// draws of a row in parts: the part by bisection in LDS, the span of 16 in the workspace, then its tokens one after the other
+constexpr int kDrawMostParts = 2048;
+template <typename T>
+__global__ __launch_bounds__(kDrawPart) void draw_part_pick_kernel(DrawArgs a)
+{
+    __shared__ double s_part[kDrawMostParts];
+    __shared__ double s_d[kDrawPart / 64];
+    __shared__ float s_f[kDrawPart / 64];
+    const long long r = blockIdx.y;
+    const int tid = threadIdx.x;
+    const DrawRow set = draw_row(a, r);
+    const float top = draw_row_top<kDrawPart>(a, r, s_f);
+    const int per = (a.parts + kDrawPart - 1) / kDrawPart;
+    double sum = 0.0, total;
+    for (int p = tid * per; p < (tid + 1) * per && p < a.parts; p++) sum += a.part_mass[r * a.parts + p];
+    double at = draw_before<kDrawPart, double>(sum, s_d, &total);
+    for (int p = tid * per; p < (tid + 1) * per && p < a.parts; p++) { at += a.part_mass[r * a.parts + p]; s_part[p] = at; }
+    __syncthreads();
+    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+    const long long groups = row.groups(), part_spans = a.part / 4, row_spans = (groups + 3) / 4;
+    const double* spans = a.spans + r * a.spans_row;
+    const u64 floor_rank = a.cuts ? a.floors[r] : 0;
+    for (long long s = (long long)blockIdx.x * kDrawPart + tid; s < a.S; s += (long long)gridDim.x * kDrawPart) {
+        const long long t = r * a.S + s;
+        if (!(total > 0.0)) { a.indices[t] = -1; if (a.logprobs) a.logprobs[t] = -__builtin_inff(); continue; }
+        const double want = draw_uniform(a, t) * total;
+        int p = 0, p1 = a.parts - 1;
+        while (p < p1) {
+            const int mid = (p + p1) >> 1;
+            if (s_part[mid] > want) p1 = mid; else p = mid + 1;
+        }
+        const double base = p ? s_part[p - 1] : 0.0;
+        long long lo = p * part_spans, hi = lo + part_spans < row_spans ? lo + part_spans - 1 : row_spans - 1;
+        while (lo < hi) {
+            const long long mid = (lo + hi) >> 1;
+            if (base + spans[mid] > want) hi = mid; else lo = mid + 1;
+        }
+        // where rounding leaves no token that exceeds, the last one with weight
+        long long index = -1; float at_l = 0.0f; bool found = false;
+        for (long long q = lo; q >= 0 && index < 0; q--) {
+            const long long qp = q / part_spans;
+            double run = (qp ? s_part[qp - 1] : 0.0) + (q % part_spans ? spans[q - 1] : 0.0);
+            for (int e = 0; e < 4 && !found; e++) {
+                float l[4];
+                if (4 * q + e >= groups) break;
+                row.load(4 * q + e, l);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const long long i = 4 * (4 * q + e) + j - row.off;
+                    const double w = l[j] == l[j] && !found ? draw_kept(l[j], i, floor_rank, top, set) : 0.0;
+                    run += w;
+                    if (w > 0.0) { index = i; at_l = l[j]; found = run > want; }
+                }
+            }
+        }
+        a.indices[t] = index;
+        if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, total);
+    }
+}
+
 // ---- short rows: W lanes to a row, E tokens to a lane ----------------------------------------------------------------------------
 template <int W>
 __device__ __forceinline__ uint32_t draw_votes(bool b, int sub)       // lanes of the row that say yes
@@ -934,20 +1287,55 @@ static int draw_check(const gsx_draw* s)
     return GSX_OK;
 }
 
-struct DrawLayout { bool pick; long long spans_row; size_t spans, total, floors, tops, bytes; };
+struct DrawLayout {
+    enum Way { kShort, kRow, kRowSpans, kParts } way;
+    long long spans_row, part, list_most; int parts, walkers, cuts;
+    size_t spans, total, floors, tops, part_top, part_mass, hist_n, hist_m, row_n, row_m, sums, list, list_n, bytes;
+};
 
+// Which way, and its workspace.
 static DrawLayout draw_layout(const gsx_draw* s)
 {
-    DrawLayout l;
-    l.pick = s->V <= kDrawShort || (s->S <= kDrawInRow && s->V <= (int64_t)kDrawWaveTiles * 256 - 4);
-    l.spans_row = (s->V + 3 + 15) / 16;
-    l.spans = l.total = l.floors = l.tops = 0;
+    DrawLayout l = {};
     size_t at = 0;
-    if (!l.pick) {
-        l.spans = at; at += align_up((size_t)s->R * (size_t)l.spans_row * 8);
-        l.total = at; at += align_up((size_t)s->R * 8);
-        l.floors = at; at += align_up((size_t)s->R * 8);
-        l.tops = at; at += align_up((size_t)s->R * 4);
+    auto take = [&](size_t bytes) { const size_t here = at; at += align_up(bytes); return here; };
+    const size_t R = (size_t)s->R;
+    l.cuts = s->top_ks || s->top_ps || s->temperatures || s->temperature == 0.0f || (s->top_k > 0 && s->top_k < s->V) || s->top_p < 1.0f;
+    if (s->V <= kDrawShort) l.way = DrawLayout::kShort;
+    else if (s->V > kDrawLong && s->R <= kDrawFewRows) l.way = DrawLayout::kParts;
+    else if (s->S <= kDrawInRow && s->V <= (int64_t)kDrawWaveTiles * 256 - 4) l.way = DrawLayout::kRow;
+    else l.way = DrawLayout::kRowSpans;
+    if (l.way == DrawLayout::kRowSpans) {
+        l.spans_row = (s->V + 3 + 15) / 16;
+        l.spans = take(R * (size_t)l.spans_row * 8);
+        l.total = take(R * 8);
+        l.floors = take(R * 8);
+        l.tops = take(R * 4);
+    }
+    if (l.way == DrawLayout::kParts) {
+        const int64_t groups = (s->V + 3 + 3) / 4;
+        l.part = 4 * kDrawPart;
+        while (ceil_div(groups, l.part) > kDrawMostParts) l.part *= 2;
+        l.parts = (int)ceil_div(groups, l.part);
+        l.spans_row = (int64_t)l.parts * l.part / 4;
+        l.walkers = (int)(256 / s->R > 1 ? 256 / s->R : 1);
+        if (l.walkers > l.parts) l.walkers = l.parts;
+        l.spans = take(R * (size_t)l.spans_row * 8);
+        l.floors = take(R * 8);
+        l.part_top = take(R * l.parts * 4);
+        l.part_mass = take(R * l.parts * 8);
+        if (l.cuts) {
+            l.hist_n = take(R * l.walkers * kDrawBins * 4);
+            l.hist_m = take(R * l.walkers * kDrawBins * 8);
+            l.row_n = take(R * kDrawBins * 4);
+            l.row_m = take(R * kDrawBins * 8);
+            l.sums = take(R * l.walkers * 16);
+            // room for every token of a few rows, a quarter of a million at least of each of many; what does not fit goes the exact way
+            const int64_t most = (1ll << 24) / s->R;
+            l.list_most = s->V < most ? s->V : most;
+            l.list = take(R * (size_t)l.list_most * 8);
+            l.list_n = take(R * 4);
+        }
     }
     l.bytes = at ? at : 256;
     return l;
@@ -973,9 +1361,24 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
         GSX_LAUNCH_CHECK();
         return GSX_OK;
     }
+    if (l.way == DrawLayout::kParts) {
+        const dim3 parts((unsigned)l.parts, (unsigned)a.R), walkers((unsigned)l.walkers, (unsigned)a.R);
+        draw_part_top_kernel<T><<<parts, dim3(kDrawPart), 0, stream>>>(a);
+        if (l.cuts) {
+            draw_part_hist_kernel<T><<<walkers, dim3(kDrawWalk), 0, stream>>>(a);
+            draw_sum_hist_kernel<<<dim3(kDrawBins / 64, (unsigned)a.R), dim3(1024), 0, stream>>>(a);
+            draw_part_pass_kernel<T><<<walkers, dim3(kDrawWalk), 0, stream>>>(a);
+            draw_floor_kernel<T><<<dim3((unsigned)a.R), dim3(1024), 0, stream>>>(a);
+        }
+        draw_part_mass_kernel<T><<<parts, dim3(kDrawPart), 0, stream>>>(a);
+        const int64_t picks = ceil_div(a.S, kDrawPart);
+        draw_part_pick_kernel<T><<<dim3((unsigned)(picks < 1024 ? picks : 1024), (unsigned)a.R), dim3(kDrawPart), 0, stream>>>(a);
+        GSX_LAUNCH_CHECK();
+        return GSX_OK;
+    }
     const dim3 grid((unsigned)a.R);
-    const bool small = a.V <= kDrawSmall && a.R > 256;           // there are rows to fill the card
-    if (l.pick) {
+    const bool small = a.V <= kDrawSmall && a.R > 256;               // there are rows to fill the card
+    if (l.way == DrawLayout::kRow) {
         if (small) draw_row_kernel<T, 256, true><<<grid, dim3(256), 0, stream>>>(a);
         else draw_row_kernel<T, 1024, true><<<grid, dim3(1024), 0, stream>>>(a);
     } else {
@@ -1014,6 +1417,10 @@ GSX_API int gsx_draw_indices(const gsx_draw* s, void* stream)
     a.temperatures = s->temperatures; a.top_ps = s->top_ps; a.min_ps = s->min_ps; a.top_ks = s->top_ks;
     a.indices = (long long*)s->indices; a.logprobs = s->logprobs;
     a.spans_row = l.spans_row;
+    a.part = l.part; a.parts = l.parts; a.walkers = l.walkers; a.cuts = l.cuts; a.list_most = l.list_most;
+    a.part_top = (float*)(ws + l.part_top); a.part_mass = (double*)(ws + l.part_mass);
+    a.hist_n = (uint32_t*)(ws + l.hist_n); a.hist_m = (u64*)(ws + l.hist_m); a.row_n = (uint32_t*)(ws + l.row_n); a.row_m = (u64*)(ws + l.row_m);
+    a.sums = (double*)(ws + l.sums); a.list = (u64*)(ws + l.list); a.list_n = (uint32_t*)(ws + l.list_n);
     a.spans = (double*)(ws + l.spans); a.total = (double*)(ws + l.total); a.floors = (u64*)(ws + l.floors); a.tops = (float*)(ws + l.tops);
     switch (s->dtype) {
     case GSX_F32: return draw_run<float>(a, l, (hipStream_t)stream);

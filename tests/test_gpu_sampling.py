@@ -76,7 +76,7 @@ def test_rows(V, cut):
     check(logits, u, **cut)
 
 
-@pytest.mark.parametrize("R,V,S", [(1, 5, 1), (300, 3, 1), (1000, 40, 2), (7, 70001, 33), (2, 200003, 5), (1, 300000, 70000), (600, 1500, 1), (1, 1100003, 100)])
+@pytest.mark.parametrize("R,V,S", [(1, 5, 1), (300, 3, 1), (1000, 40, 2), (7, 70001, 33), (2, 200003, 5), (1, 300000, 70000), (600, 1500, 1), (1, 1100003, 100), (130, 40001, 2), (129, 33000, 70), (3, 40000, 300)])
 @pytest.mark.parametrize("cut", [dict(), dict(p=0.8), dict(k=300, p=0.95, m=0.001, T=0.9)], ids=str)
 def test_sizes(R, V, S, cut):
     logits, u = rand(R + V, R, V, S, sigma=1.5, f64=V > 100000)
@@ -96,6 +96,14 @@ def test_equal_logits_and_borders(V):
         check(logits, u)
         for cut in (dict(k=max(1, V // 3)), dict(p=0.5), dict(p=0.25, k=max(1, V // 2)), dict(m=1.0), dict(T=0.0), dict(p=0.5, m=0.5)):
             check(logits, u, **cut)
+
+
+def test_more_ties_than_any_list_holds():
+    logits = torch.zeros(128, 140000, device="cuda")
+    logits[:, ::2] = 1.0
+    u = torch.rand(128, 3, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2), dtype=torch.float64)
+    check(logits, u, k=100001)
+    check(logits[:40], u[:40], p=0.9)
 
 
 def test_ties_at_the_cut():
