@@ -152,9 +152,9 @@ __device__ __forceinline__ double draw_kept(float l, long long i, u64 floor_rank
     return w < set.min_p ? 0.0 : w;
 }
 
-__device__ __forceinline__ float draw_logprob(float l, float top, double inv_t, double total)
+__device__ __forceinline__ float draw_logprob(float l, float top, double inv_t, double log_total)
 {
-    return (float)((l == top ? 0.0 : ((double)l - (double)top) * inv_t) - log(total));
+    return (float)((l == top ? 0.0 : ((double)l - (double)top) * inv_t) - log_total);
 }
 
 // A row as groups of four tokens on a boundary of four: place 4 g + j is token 4 g + j - off.
@@ -185,17 +185,41 @@ struct Places {
     }
 };
 
-// ---- workgroup helpers -------------------------------------------------------------------------------------------------------
+// ---- wave and workgroup helpers --------------------------------------------------------------------------------------------------
+// Values moved between lanes by DPP: register moves of a few cycles, where a shuffle is a round trip through the LDS unit that the histograms' atomics
+// keep busy.  Lanes without a source get zero.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T draw_dpp(T v)
+{
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    } else {
+        const u64 u = __builtin_bit_cast(u64, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, (u64)hi << 32 | lo);
+    }
+}
+// inclusive sums over the wave: within rows of 16 lanes, then the rows' last lanes onto the rows behind them
+template <typename T>
+__device__ __forceinline__ T draw_wave_scan(T v)
+{
+    v += draw_dpp<0x111, 0xf>(v);     // row_shr:1
+    v += draw_dpp<0x112, 0xf>(v);
+    v += draw_dpp<0x114, 0xf>(v);
+    v += draw_dpp<0x118, 0xf>(v);
+    v += draw_dpp<0x142, 0xa>(v);     // row_bcast:15 onto rows 1 and 3
+    v += draw_dpp<0x143, 0xc>(v);     // row_bcast:31 onto rows 2 and 3
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T draw_wave_shift(T v) { return draw_dpp<0x138, 0xf>(v); }       // from the lane before; zero into lane 0
+
 template <int NT, typename T>
 __device__ __forceinline__ T draw_before(T v, T* s_wave, T* sum)       // exclusive sums over the threads
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    T incl = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T o = __shfl_up(incl, d, 64);
-        if (lane >= d) incl += o;
-    }
+    const T incl = draw_wave_scan(v);
     __syncthreads();                                                 // s_wave may still be read from the call before
     if (lane == 63) s_wave[wave] = incl;
     __syncthreads();
@@ -206,8 +230,7 @@ __device__ __forceinline__ T draw_before(T v, T* s_wave, T* sum)       // exclus
         all += s_wave[w];
     }
     *sum = all;
-    const T before = __shfl_up(incl, 1, 64);
-    return base + (lane ? before : (T)0);
+    return base + draw_wave_shift(incl);
 }
 
 template <int NT>
@@ -226,7 +249,7 @@ __device__ __forceinline__ float draw_max(float v, float* s_wave)
 
 struct DrawHist { uint32_t count[kDrawBins]; u64 hi[kDrawBins], lo[kDrawBins]; };
 struct DrawFine { uint32_t count[kDrawFine]; u64 hi[kDrawFine], lo[kDrawFine]; };
-struct DrawCand { u64 rank[kDrawCand], ranked[kDrawCand]; double w[kDrawCand], ranked_w[kDrawCand]; };
+struct DrawCand { u64 rank[kDrawCand], ranked[kDrawCand]; };
 
 // The first try at the cuts of a row: where the histogram's bounds let them end.  Bins: k in bin bk, p in one of lo .. hi.
 struct DrawNear { int bk, lo, hi; long long above_k; int before_bk, upto_hi; bool sure; };
@@ -241,6 +264,40 @@ struct DrawCut {
     DrawNear near;
     u64 wave_u[16]; uint32_t wave_n[16]; double wave_d[16]; float wave_f[16];
 };
+
+// One rank per thread, sorted descending over the workgroup (a bitonic network; partners within a wave by shuffles, further apart through LDS).
+template <int NT>
+__device__ __forceinline__ u64 draw_sort(u64 v, u64* lds)
+{
+    const int t = threadIdx.x;
+#pragma unroll 1
+    for (int size = 2; size <= NT; size <<= 1) {
+#pragma unroll 1
+        for (int d = size >> 1; d; d >>= 1) {
+            u64 o;
+            if (d >= 64) {
+                __syncthreads();
+                lds[t] = v;
+                __syncthreads();
+                o = lds[t ^ d];
+            } else o = __shfl_xor(v, d, 64);
+            const bool larger = ((t & d) == 0) == ((t & size) == 0);     // this thread keeps the larger one
+            v = (larger ? o > v : o < v) ? o : v;
+        }
+    }
+    __syncthreads();
+    return v;
+}
+
+// Ranks cand.rank[0 .. m) sorted into cand.ranked (m at most NT)
+template <int NT>
+__device__ __forceinline__ void draw_rank_cand(DrawCand& cand, int m)
+{
+    const int t = threadIdx.x;
+    const u64 v = draw_sort<NT>(t < m ? cand.rank[t] : 0, cand.ranked);
+    cand.ranked[t] = v;
+    __syncthreads();
+}
 
 // The first of bins 0 .. last where what lies in and in front of it reaches k tokens or `want` mass, or else `last`; c.above_* move up to it (masses only with_mass).
 template <int NT>
@@ -327,20 +384,14 @@ __device__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const E
         if (rank < lo || rank > hi) return;
         if (!narrowed) { const int b = draw_bin(l, top, scale); if (b < bin0 || b > bin1) return; }
         const uint32_t slot = atomicAdd(&c.slots, 1u);
-        if (slot < (uint32_t)most) { cand.rank[slot] = rank; cand.w[slot] = draw_weight(l, top, inv_t); }
+        if (slot < (uint32_t)most) cand.rank[slot] = rank;
     });
     __syncthreads();
     const int m = (int)(c.slots < (uint32_t)most ? c.slots : (uint32_t)most);
     const int t = threadIdx.x;
-    if (t < m) {                                                     // its place among them: ranks are all different
-        const u64 mine = cand.rank[t];
-        int place = 0;
-        for (int j = 0; j < m; j++) place += cand.rank[j] > mine;
-        cand.ranked[place] = mine; cand.ranked_w[place] = cand.w[t];
-    }
-    __syncthreads();
+    draw_rank_cand<NT>(cand, m);
     double all;
-    const double w = t < m ? cand.ranked_w[t] : 0.0;
+    const double w = t < m ? draw_weight(draw_unkey((uint32_t)(cand.ranked[t] >> kDrawIndexBits)), top, inv_t) : 0.0;
     const double above = c.base + limbs(c.above_hi, c.above_lo);
     const double before = draw_before<NT, double>(w, c.wave_d, &all);
     const bool in = t < m && (t == 0 || (by_mass ? above + before < want : c.above_n + t < k));
@@ -475,15 +526,11 @@ __device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, floa
     const int most = NT < kDrawCand ? NT : kDrawCand, t = threadIdx.x;
     if (c.slots > (uint32_t)most) return false;
     const int m = (int)c.slots;
-    if (t < m) {
-        const u64 mine = cand.rank[t];
-        int place = 0;
-        for (int j = 0; j < m; j++) place += cand.rank[j] > mine;
-        cand.ranked[place] = mine; cand.ranked_w[place] = cand.w[t];
-    }
+    draw_rank_cand<NT>(cand, m);
     if (t == 0) { c.near.before_bk = 0; c.near.upto_hi = 0; c.near.sure = false; c.last = 0; }
     __syncthreads();
-    const int bin = t < m ? draw_bin(draw_unkey((uint32_t)(cand.ranked[t] >> kDrawIndexBits)), top, set.scale) : kDrawBins;
+    const float l = draw_unkey((uint32_t)(cand.ranked[t] >> kDrawIndexBits));
+    const int bin = t < m ? draw_bin(l, top, set.scale) : kDrawBins;
     const u64 front = __ballot(bin < c.near.bk), upto = __ballot(bin <= c.near.hi);
     if ((t & 63) == 0) { atomicAdd(&c.near.before_bk, (int)__popcll(front)); atomicAdd(&c.near.upto_hi, (int)__popcll(upto)); }
     __syncthreads();
@@ -493,7 +540,7 @@ __device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, floa
         n = left < m ? (int)left : m;
     }
     double all;
-    const double w = t < n ? cand.ranked_w[t] : 0.0;
+    const double w = t < n ? draw_weight(l, top, set.inv_t) : 0.0;
     const double before = draw_before<NT, double>(w, c.wave_d, &all);
     if (!by_p) {
         if (t == 0) c.floor_rank = cand.ranked[n - 1];
@@ -587,19 +634,19 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
             for (int j = 0; j < 4; j++) {
                 const int b = l[j] == l[j] ? draw_bin(l[j], top, set.scale) : kDrawBins;
                 const bool in = (b >= lo && b <= hi) || (by_k && b == bk);
-                double w = 0.0;
-                if (b <= sums_to || in) w = draw_weight(l[j], top, set.inv_t);
-                if (b <= sums_to) total += w;
-                if (b < lo) { above += w; sum += w < set.min_p ? 0.0 : w; }
+                if (b <= sums_to) {
+                    const double w = draw_weight(l[j], top, set.inv_t);
+                    total += w;
+                    if (b < lo) { above += w; sum += w < set.min_p ? 0.0 : w; }
+                }
                 if (in) {
                     const uint32_t slot = atomicAdd(&c.slots, 1u);
-                    if (slot < (uint32_t)(NT < kDrawCand ? NT : kDrawCand)) { sh.cand.rank[slot] = draw_rank(l[j], 4 * g + j - row.off); sh.cand.w[slot] = w; }
+                    if (slot < (uint32_t)(NT < kDrawCand ? NT : kDrawCand)) sh.cand.rank[slot] = draw_rank(l[j], 4 * g + j - row.off);
                 }
             }
             if (PICK && lo > 0) {
-#pragma unroll
-                for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-                if (lane == 0) tile[g >> 6] = sum;
+                sum = draw_wave_scan(sum);
+                if (lane == 63) tile[g >> 6] = sum;
             }
         };
         all_groups(pass);
@@ -613,7 +660,7 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
             if (PICK) {
                 if (tid < (int)c.slots) {                            // the kept candidates' weights, as whole numbers: any order gives the same sums
                     const u64 rank = sh.cand.rank[tid];
-                    const double w = sh.cand.w[tid];
+                    const double w = draw_weight(draw_unkey((uint32_t)(rank >> kDrawIndexBits)), top, set.inv_t);
                     if (rank >= floor_rank && !(w < set.min_p)) {
                         const long long i = ((1ll << kDrawIndexBits) - 1) - (long long)(rank & ((1ull << kDrawIndexBits) - 1));
                         const int q = (int)((i + row.off) >> 8);
@@ -653,9 +700,8 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         if (!tiled)
             all_groups([&](const float (&l)[4], long long g) {
                 double w[4], sum = mass4(l, g, w);
-#pragma unroll
-                for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-                if (lane == 0) tile[g >> 6] = sum;
+                sum = draw_wave_scan(sum);
+                if (lane == 63) tile[g >> 6] = sum;
             });
         __syncthreads();
         const int tiles = (int)((groups + 63) >> 6), per = (tiles + NT - 1) / NT;
@@ -664,6 +710,7 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         double at = draw_before<NT, double>(sum, c.wave_d, &total);
         for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) { at += tile[q]; tile[q] = at; }
         __syncthreads();
+        const double log_total = log(total);
         for (long long s = wave; s < a.S; s += kWaves) {             // a wave per draw
             const double want = draw_uniform(a, r * a.S + s) * total;
             int lo = 0, hi = tiles - 1;
@@ -676,14 +723,8 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
                 const long long g = (long long)q * 64 + lane;
                 float l[4] = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
                 if (g < groups) row.load(g, l);
-                double w[4], mine = mass4(l, g, w), incl = mine;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const double o = __shfl_up(incl, d, 64);
-                    if (lane >= d) incl += o;
-                }
-                const double up = __shfl_up(incl, 1, 64);
-                double run = (q ? tile[q - 1] : 0.0) + (lane ? up : 0.0);
+                double w[4], incl = draw_wave_scan(mass4(l, g, w));
+                double run = (q ? tile[q - 1] : 0.0) + draw_wave_shift(incl);
                 int hit = -1, any = -1;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -699,7 +740,7 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
 #pragma unroll
                     for (int e = 1; e < 4; e++) lj = e == j ? l[e] : lj;
                     a.indices[r * a.S + s] = 4 * g + j - row.off;
-                    if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(lj, top, set.inv_t, total);
+                    if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(lj, top, set.inv_t, log_total);
                 }
                 break;
             }
@@ -767,7 +808,7 @@ __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long
         }
     }
     a.indices[t] = index;
-    if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, total);
+    if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, log(total));
 }
 
 // ---- a few long rows, in parts over the card -------------------------------------------------------------------------------------
@@ -878,6 +919,8 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
 {
     __shared__ DrawHist hist;
     __shared__ DrawCut c;
+    constexpr uint32_t kStash = 8 * kDrawWalk;
+    __shared__ u64 s_list[kStash];
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
@@ -888,7 +931,19 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
     const int bk = c.near.bk, lo = by_p ? c.near.lo : bk, hi = by_p ? c.near.hi : bk;
     const int sums_to = by_p ? (by_k ? bk - 1 : kDrawBins - 1) : -1;
     double above = 0.0, total = 0.0;
-    const int lane = threadIdx.x & 63;
+    if (threadIdx.x == 0) c.slots = 0;
+    __syncthreads();
+    auto flush = [&]() {
+        const uint32_t n = c.slots;
+        if (threadIdx.x == 0) c.in_bin = atomicAdd(&a.list_n[r], n);
+        __syncthreads();
+        const uint32_t at = c.in_bin;
+        for (uint32_t q = threadIdx.x; q < n; q += kDrawWalk)
+            if ((long long)at + q < a.list_most) a.list[r * a.list_most + at + q] = s_list[q];
+        __syncthreads();
+        if (threadIdx.x == 0) c.slots = 0;
+        __syncthreads();
+    };
     draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], long long g) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -899,15 +954,17 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
                 total += w;
                 if (b < lo) above += w;
             }
-            const u64 who = __ballot(in);                            // one place in the list for a wave's tokens
-            if (who) {
-                uint32_t at = 0;
-                if (lane == __ffsll((long long)who) - 1) at = atomicAdd(&a.list_n[r], (uint32_t)__popcll(who));
-                at = __shfl(at, __ffsll((long long)who) - 1, 64) + (uint32_t)__popcll(who & ((1ull << lane) - 1));
-                if (in && at < (uint64_t)a.list_most) a.list[r * a.list_most + at] = draw_rank(l[j], 4 * g + j - row.off);
+            if (in) {
+                const uint32_t slot = atomicAdd(&c.slots, 1u);
+                s_list[slot] = draw_rank(l[j], 4 * g + j - row.off);
             }
         }
+        // the collected tokens to the row's list before the next round could overflow: one global atomic for many of them
+        __syncthreads();
+        if (c.slots > kStash - 4 * kDrawWalk) flush();
+        __syncthreads();
     });
+    flush();
     double all_above, all_total;
     draw_before<kDrawWalk, double>(above, c.wave_d, &all_above);
     draw_before<kDrawWalk, double>(total, c.wave_d, &all_total);
@@ -944,11 +1001,7 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
     const u64* list = a.list + r * a.list_most;
     bool done = false;
     if (n <= NT) {
-        if (tid < n) {
-            const u64 rank = list[tid];
-            sh.cand.rank[tid] = rank;
-            sh.cand.w[tid] = draw_weight(draw_unkey((uint32_t)(rank >> kDrawIndexBits)), top, set.inv_t);
-        }
+        if (tid < n) sh.cand.rank[tid] = list[tid];
         if (tid == 0) c.slots = (uint32_t)n;
         __syncthreads();
         done = draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, above, total);
@@ -1074,6 +1127,7 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_pick_kernel(DrawArgs a)
     const long long groups = row.groups(), part_spans = a.part / 4, row_spans = (groups + 3) / 4;
     const double* spans = a.spans + r * a.spans_row;
     const u64 floor_rank = a.cuts ? a.floors[r] : 0;
+    const double log_total = log(total);
     for (long long s = (long long)blockIdx.x * kDrawPart + tid; s < a.S; s += (long long)gridDim.x * kDrawPart) {
         const long long t = r * a.S + s;
         if (!(total > 0.0)) { a.indices[t] = -1; if (a.logprobs) a.logprobs[t] = -__builtin_inff(); continue; }
@@ -1108,7 +1162,7 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_pick_kernel(DrawArgs a)
             }
         }
         a.indices[t] = index;
-        if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, total);
+        if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, log_total);
     }
 }
 
@@ -1133,7 +1187,7 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
     constexpr int kRows = 64 / W;
     __shared__ double s_mass[kBlock / 64][64 * E];
     __shared__ float s_l[kBlock / 64][64 * E];
-    __shared__ double s_total[kBlock / 64][kRows], s_inv[kBlock / 64][kRows];
+    __shared__ double s_total[kBlock / 64][kRows], s_log[kBlock / 64][kRows], s_inv[kBlock / 64][kRows];
     __shared__ float s_top[kBlock / 64][kRows];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / W, j0 = (lane % W) * E;
     const long long r0 = ((long long)blockIdx.x * (kBlock / 64) + wave) * kRows, r = r0 + sub;
@@ -1246,7 +1300,7 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
         s_mass[wave][lane * E + e] = w[e] > 0.0 ? run : -run;
         s_l[wave][lane * E + e] = l[e];
     }
-    if (lane % W == 0) { s_total[wave][sub] = live ? total : -1.0; s_inv[wave][sub] = set.inv_t; s_top[wave][sub] = top; }
+    if (lane % W == 0) { s_total[wave][sub] = live ? total : -1.0; s_log[wave][sub] = log(total); s_inv[wave][sub] = set.inv_t; s_top[wave][sub] = top; }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");           // LDS of this wave's own lanes
     __builtin_amdgcn_wave_barrier();
     const int rows = a.R - r0 < kRows ? (int)(a.R - r0) : kRows;
@@ -1268,7 +1322,7 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
             while (i > 0 && !(mass[i] > 0.0)) i--;
             while (!(mass[i] > 0.0) && i < V - 1) i++;
             index = i;
-            lp = draw_logprob(s_l[wave][y * W * E + i], s_top[wave][y], s_inv[wave][y], all);
+            lp = draw_logprob(s_l[wave][y * W * E + i], s_top[wave][y], s_inv[wave][y], s_log[wave][y]);
         }
         a.indices[r0 * a.S + q] = index;
         if (a.logprobs) a.logprobs[r0 * a.S + q] = lp;
