@@ -40,44 +40,54 @@ struct DrawArgs {
     const float* temperatures; const float* top_ps; const float* min_ps; const int32_t* top_ks;
     long long* indices; float* logprobs;
     // workspace of rows whose draws are made by a kernel of their own
-    double* spans;                                  // [row][spans_row]: inclusive mass behind every 16 tokens
+    double* spans;                                  // [row][spans_row]: inclusive mass behind every 8 tokens
     double* total; float* tops; u64* floors;        // per row: kept mass (-1: none), top, lowest kept rank
     long long spans_row;
     // rows in parts: `part` groups of four places each, `parts` to a row; `walkers` workgroups per row where a workgroup takes several parts
-    long long part; int parts, walkers, cuts;
+    int part, parts, walkers, cuts;
     float* part_top; double* part_mass;             // [row][part]
-    uint32_t* hist_n; u64* hist_m;                  // [row][walker][bin]
+    uint32_t* hist_n; float* hist_m;                // [row][walker][bin]
     uint32_t* row_n; u64* row_m;                    // [row][bin]
     double* sums;                                   // [row][walker][2]: 64-bit mass in front of the bracket, and the total's part
     u64* list; uint32_t* list_n; long long list_most;        // [row]: ranks of the tokens where the cuts may end
 };
 
 // ---- tokens ---------------------------------------------------------------------------------------------------------------
-// logits as floats: NaN counts as -inf (a masked token), -0 as 0.  A NaN float further on is "not a token" (a place outside the row).
+// logits as floats: NaN counts as -inf (a masked token).  A NaN float further on is "not a token" (a place outside the row).
 template <typename T>
 __device__ __forceinline__ float draw_logit(T v)
 {
     const float f = (float)v;
-    return f != f ? -__builtin_inff() : f + 0.0f;
+    return f != f ? -__builtin_inff() : f;
 }
 
-// ascending unsigned order of the logits
-__host__ __device__ __forceinline__ uint32_t draw_key(float l)
+// ascending unsigned order of the logits, -0 as 0
+__device__ __forceinline__ uint32_t draw_key(float l)
 {
-    const uint32_t u = __builtin_bit_cast(uint32_t, l);
+    const uint32_t u = __builtin_bit_cast(uint32_t, l + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float draw_unkey(uint32_t k) { return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 // ascending order of (logit, -index): a cut keeps the tokens whose rank is at least some floor
-__device__ __forceinline__ u64 draw_rank(float l, long long i) { return (u64)draw_key(l) << kDrawIndexBits | (u64)(((1ll << kDrawIndexBits) - 1) - i); }
+constexpr u64 kDrawIndexMask = (1ull << kDrawIndexBits) - 1;
+__device__ __forceinline__ u64 draw_rank(float l, int i) { return (u64)draw_key(l) << kDrawIndexBits | (kDrawIndexMask - (u64)i); }
+__device__ __forceinline__ float draw_rank_logit(u64 rank) { return draw_unkey((uint32_t)(rank >> kDrawIndexBits)); }
+__device__ __forceinline__ int draw_rank_index(u64 rank) { return (int)(kDrawIndexMask - (rank & kDrawIndexMask)); }
 
-// exp(x) for x <= 0: x = n ln 2 + r with ln 2 in two parts (the first of 32 bits: n times it is exact), |r| <= ln 2 / 2, the Taylor sum to
-// r^13 / 13! (what is left out is below 5e-18), times 2^n.
+// A floor as the token that it is: kept are larger logits, and equal ones up to its index.  Rank 0: everything is kept.
+struct DrawFloor {
+    float l; int i;
+    __device__ __forceinline__ DrawFloor(u64 rank) : l(rank ? draw_rank_logit(rank) : -__builtin_inff()), i(rank ? draw_rank_index(rank) : 0x7fffffff) {}
+    __device__ __forceinline__ bool keeps(float v, int at) const { return v > l || (v == l && at <= i); }
+};
+
+// exp(x) for x <= 0; 0 below -708, for -inf and for NaN.  x = n ln 2 + r with ln 2 in two parts (the first of 32 bits: n times it is exact),
+// |r| <= ln 2 / 2, the Taylor sum to r^13 / 13! (what is left out is below 5e-18), times 2^n by the exponent's bits.  n comes from an addition
+// that leaves it in the low bits: conversions and roundings of 64-bit numbers run at a quarter of the rate of the FMA.
 __device__ __forceinline__ double draw_exp(double x)
 {
-    x = fmax(x, -760.0);                                             // 2^-1096: zero, and n stays an int
-    const double n = rint(x * 0x1.71547652b82fep+0);
+    const double t = fma(x, 0x1.71547652b82fep+0, 0x1.8p52), n = t - 0x1.8p52;
     double r = fma(n, -0x1.62e42ff000000p-1, x);
     r = fma(n, 0x1.718432a1b0e26p-35, r);
     double s = 1.0 / 6227020800.0;
@@ -94,22 +104,20 @@ __device__ __forceinline__ double draw_exp(double x)
     s = fma(s, r, 0.5);
     s = fma(s, r, 1.0);
     s = fma(s, r, 1.0);
-    return ldexp(s, (int)n);
+    const u64 bits = __builtin_bit_cast(u64, s);
+    const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(u64, t) << 20);
+    const double v = __builtin_bit_cast(double, (u64)hi << 32 | (uint32_t)bits);
+    return x >= -708.0 ? v : 0.0;
 }
 
-__device__ __forceinline__ double draw_weight(float l, float top, double inv_t)
-{
-    if (l == top) return 1.0;
-    if (!(l > -__builtin_inff()) || top == __builtin_inff()) return 0.0;          // masked, not a token, or beside an infinite one
-    return draw_exp(((double)l - (double)top) * inv_t);
-}
+// 1 at the top, 0 where masked and outside the row; the top is finite (Places)
+__device__ __forceinline__ double draw_weight(float l, float top, double inv_t) { return draw_exp(((double)l - (double)top) * inv_t); }
 
 // bin of the first histogram: does not fall as l falls
 __device__ __forceinline__ int draw_bin(float l, float top, float scale)
 {
-    if (l == top) return 0;
     const float t = (top - l) * scale;
-    return t < (float)(kDrawBins - 1) ? (int)t : kDrawBins - 1;
+    return t < (float)(kDrawBins - 1) ? (int)t : kDrawBins - 1;      // NaN (-inf at an endless temperature): the last
 }
 
 // a weight as whole numbers: w = hi 2^-31 + lo 2^-63, to the nearest; sums of 2^27 of either fit 64 bits
@@ -145,43 +153,54 @@ __device__ __forceinline__ double draw_uniform(const DrawArgs& a, long long t)
     return u >= 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;                     // NaN: 0
 }
 
-__device__ __forceinline__ double draw_kept(float l, long long i, u64 floor_rank, float top, const DrawRow& set)
+__device__ __forceinline__ double draw_kept(float l, int i, const DrawFloor& floor, float top, const DrawRow& set)
 {
-    if (draw_rank(l, i) < floor_rank) return 0.0;
+    if (!__any(floor.keeps(l, i))) return 0.0;                       // most waves beyond a cut keep nothing
     const double w = draw_weight(l, top, set.inv_t);
-    return w < set.min_p ? 0.0 : w;
+    return floor.keeps(l, i) && w >= set.min_p ? w : 0.0;
 }
 
 __device__ __forceinline__ float draw_logprob(float l, float top, double inv_t, double log_total)
 {
-    return (float)((l == top ? 0.0 : ((double)l - (double)top) * inv_t) - log_total);
+    return (float)(((double)l - (double)top) * inv_t - log_total);
 }
 
 // A row as groups of four tokens on a boundary of four: place 4 g + j is token 4 g + j - off.
 template <typename T>
 struct Four { T v[4]; } __attribute__((aligned(4 * sizeof(T))));
 
+// Where a row's top is +inf, such tokens share all mass: they are taken as 0 and all others as -inf.
 template <typename T>
 struct Places {
-    const T* base; long long V; int off;
-    __device__ __forceinline__ Places(const T* row, long long n) : V(n)
+    const T* base; int V, off; bool infinite;
+    __device__ __forceinline__ Places(const DrawArgs& a, long long r) : V((int)a.V), infinite(false)
     {
+        const T* row = (const T*)a.logits + r * a.row_stride;
         off = (int)(((uintptr_t)row / sizeof(T)) & 3);
         base = row - off;
     }
-    __device__ __forceinline__ long long groups() const { return (V + off + 3) >> 2; }
+    __device__ __forceinline__ float finite_top(float top) { infinite = top == __builtin_inff(); return infinite ? 0.0f : top; }
+    __device__ __forceinline__ int groups() const { return (V + off + 3) >> 2; }
     // places outside the row are NaN
-    __device__ __forceinline__ void load(long long g, float (&l)[4]) const
+    __device__ __forceinline__ void load(int g, float (&l)[4]) const
     {
-        const long long i0 = 4 * g - off;
+        const int i0 = 4 * g - off;
         if (i0 >= 0 && i0 + 4 <= V) {
-            const Four<T> f = *(const Four<T>*)(base + 4 * g);
+            const Four<T> f = *(const Four<T>*)(base + 4ll * g);
 #pragma unroll
             for (int j = 0; j < 4; j++) l[j] = draw_logit(f.v[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) l[j] = i0 + j >= 0 && i0 + j < V ? draw_logit(base[4 * g + j]) : __builtin_nanf("");
+            for (int j = 0; j < 4; j++) l[j] = i0 + j >= 0 && i0 + j < V ? draw_logit(base[4ll * g + j]) : __builtin_nanf("");
         }
+        if (infinite)
+#pragma unroll
+            for (int j = 0; j < 4; j++) l[j] = l[j] != l[j] ? l[j] : l[j] == __builtin_inff() ? 0.0f : -__builtin_inff();
+    }
+    __device__ __forceinline__ void load_or_none(int g, int end, float (&l)[4]) const
+    {
+        l[0] = l[1] = l[2] = l[3] = __builtin_nanf("");
+        if (g < end) load(g, l);
     }
 };
 
@@ -233,13 +252,37 @@ __device__ __forceinline__ T draw_before(T v, T* s_wave, T* sum)       // exclus
     return base + draw_wave_shift(incl);
 }
 
+template <int CTRL, int ROWS>                       // lanes without a source keep their own
+__device__ __forceinline__ float draw_dpp_or(float v)
+{
+    const int u = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(u, u, CTRL, ROWS, 0xf, false));
+}
+
+// sums of two values over the workgroup
+template <int NT>
+__device__ __forceinline__ void draw_sums(double& x, double& y, double (*s_wave)[2])
+{
+    x = draw_wave_scan(x); y = draw_wave_scan(y);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) { s_wave[threadIdx.x >> 6][0] = x; s_wave[threadIdx.x >> 6][1] = y; }
+    __syncthreads();
+    x = s_wave[0][0]; y = s_wave[0][1];
+#pragma unroll
+    for (int w = 1; w < NT / 64; w++) { x += s_wave[w][0]; y += s_wave[w][1]; }
+}
+
 template <int NT>
 __device__ __forceinline__ float draw_max(float v, float* s_wave)
 {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+    v = fmaxf(v, draw_dpp_or<0x111, 0xf>(v));
+    v = fmaxf(v, draw_dpp_or<0x112, 0xf>(v));
+    v = fmaxf(v, draw_dpp_or<0x114, 0xf>(v));
+    v = fmaxf(v, draw_dpp_or<0x118, 0xf>(v));
+    v = fmaxf(v, draw_dpp_or<0x142, 0xa>(v));
+    v = fmaxf(v, draw_dpp_or<0x143, 0xc>(v));
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) s_wave[threadIdx.x >> 6] = v;
     __syncthreads();
     float r = s_wave[0];
 #pragma unroll
@@ -262,39 +305,41 @@ struct DrawCut {
     u64 lo, hi;                                     // ranks of the bin
     u64 floor_rank; double mass;                    // the answer: the lowest kept rank, the mass kept
     DrawNear near;
-    u64 wave_u[16]; uint32_t wave_n[16]; double wave_d[16]; float wave_f[16];
+    u64 wave_u[16]; uint32_t wave_n[16]; double wave_d[16], wave_2[16][2]; float wave_f[16];
 };
 
-// One rank per thread, sorted descending over the workgroup (a bitonic network; partners within a wave by shuffles, further apart through LDS).
+// Ranks cand.rank[0 .. m), all different, sorted descending into cand.ranked (m at most NT).  A few by counting the larger ones (m broadcast reads
+// a thread); more by a bitonic network over the next power of two, a rank per thread, partners within a wave by shuffles: its 55
+// steps at 1024 take 8 us, the counting 12; at 200 the counting is the quicker.
 template <int NT>
-__device__ __forceinline__ u64 draw_sort(u64 v, u64* lds)
+__device__ __forceinline__ void draw_rank_cand(DrawCand& cand, int m)
 {
     const int t = threadIdx.x;
-#pragma unroll 1
-    for (int size = 2; size <= NT; size <<= 1) {
-#pragma unroll 1
+    if (m <= 256) {
+        if (t < m) {
+            const u64 mine = cand.rank[t];
+            int place = 0;
+            for (int j = 0; j < m; j++) place += cand.rank[j] > mine;
+            cand.ranked[place] = mine;
+        }
+        __syncthreads();
+        return;
+    }
+    u64 v = t < m ? cand.rank[t] : 0;
+    for (int size = 2; size < 2 * m; size <<= 1) {
         for (int d = size >> 1; d; d >>= 1) {
             u64 o;
             if (d >= 64) {
                 __syncthreads();
-                lds[t] = v;
+                cand.ranked[t] = v;
                 __syncthreads();
-                o = lds[t ^ d];
+                o = cand.ranked[t ^ d];
             } else o = __shfl_xor(v, d, 64);
             const bool larger = ((t & d) == 0) == ((t & size) == 0);     // this thread keeps the larger one
             v = (larger ? o > v : o < v) ? o : v;
         }
     }
     __syncthreads();
-    return v;
-}
-
-// Ranks cand.rank[0 .. m) sorted into cand.ranked (m at most NT)
-template <int NT>
-__device__ __forceinline__ void draw_rank_cand(DrawCand& cand, int m)
-{
-    const int t = threadIdx.x;
-    const u64 v = draw_sort<NT>(t < m ? cand.rank[t] : 0, cand.ranked);
     cand.ranked[t] = v;
     __syncthreads();
 }
@@ -391,7 +436,7 @@ __device__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const E
     const int t = threadIdx.x;
     draw_rank_cand<NT>(cand, m);
     double all;
-    const double w = t < m ? draw_weight(draw_unkey((uint32_t)(cand.ranked[t] >> kDrawIndexBits)), top, inv_t) : 0.0;
+    const double w = t < m ? draw_weight(draw_rank_logit(cand.ranked[t]), top, inv_t) : 0.0;
     const double above = c.base + limbs(c.above_hi, c.above_lo);
     const double before = draw_before<NT, double>(w, c.wave_d, &all);
     const bool in = t < m && (t == 0 || (by_mass ? above + before < want : c.above_n + t < k));
@@ -460,8 +505,7 @@ __device__ __forceinline__ void draw_near_add(DrawHist& h, float l, float top, f
     const int b = draw_bin(l, top, scale);
     if (by_k) atomicAdd(&h.count[b], 1u);
     if (by_p) {
-        const float w = l == top ? 1.0f : __builtin_amdgcn_exp2f((l - top) * units);
-        const uint32_t m = (uint32_t)fminf(w * 0x1p31f + 0.5f, 2147483648.0f);
+        const uint32_t m = (uint32_t)fmaf(__builtin_amdgcn_exp2f((l - top) * units), 0x1p31f, 0.5f);      // NaN: 0
         if (m) atomicAdd(&h.hi[b], (u64)m);
     }
 }
@@ -529,7 +573,7 @@ __device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, floa
     draw_rank_cand<NT>(cand, m);
     if (t == 0) { c.near.before_bk = 0; c.near.upto_hi = 0; c.near.sure = false; c.last = 0; }
     __syncthreads();
-    const float l = draw_unkey((uint32_t)(cand.ranked[t] >> kDrawIndexBits));
+    const float l = draw_rank_logit(cand.ranked[t]);
     const int bin = t < m ? draw_bin(l, top, set.scale) : kDrawBins;
     const u64 front = __ballot(bin < c.near.bk), upto = __ballot(bin <= c.near.hi);
     if ((t & 63) == 0) { atomicAdd(&c.near.before_bk, (int)__popcll(front)); atomicAdd(&c.near.upto_hi, (int)__popcll(upto)); }
@@ -548,8 +592,8 @@ __device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, floa
         return true;
     }
     // the candidates of bin bk, where it lies behind the bracket, count for the total only
-    double tail = 0.0, none;
-    if (by_k) { none = draw_before<NT, double>(t >= c.near.before_bk ? w : 0.0, c.wave_d, &tail); (void)none; }
+    double tail = 0.0, none = 0.0;
+    if (by_k) { tail = t >= c.near.before_bk ? w : 0.0; draw_sums<NT>(tail, none, c.wave_2); }
     const double want = set.p * (total + tail);
     const int upto_n = c.near.upto_hi < n ? c.near.upto_hi : n;
     const bool in = t < upto_n && ((t == 0 && c.near.lo == 0) || above + before < want);
@@ -575,12 +619,12 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
     constexpr int kWaves = NT / 64;
     const long long r = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
-    const long long groups = row.groups();
+    Places<T> row(a, r);
+    const int groups = row.groups();
     const DrawRow set = draw_row(a, r);
     float top = -__builtin_inff();
 #pragma unroll 4
-    for (long long g = tid; g < groups; g += NT) {
+    for (int g = tid; g < groups; g += NT) {
         float l[4];
         row.load(g, l);
 #pragma unroll
@@ -593,22 +637,29 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         } else if (tid == 0) a.total[r] = -1.0;
         return;
     }
+    const float raw_top = top;
+    top = row.finite_top(top);
     // f(l, i) for every token of the row, over all threads
     auto tokens = [&](auto f) {
-#pragma unroll 2
-        for (long long g = tid; g < groups; g += NT) {
-            float l[4];
-            row.load(g, l);
+        for (int g0 = 0; g0 < groups; g0 += 2 * NT) {                // two groups' loads in flight
+            float l[2][4];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (l[j] == l[j]) f(l[j], 4 * g + j - row.off);
+            for (int q = 0; q < 2; q++) row.load_or_none(g0 + q * NT + tid, groups, l[q]);
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (l[q][j] == l[q][j]) f(l[q][j], 4 * (g0 + q * NT + tid) + j - row.off);
         }
     };
     auto all_groups = [&](auto f) {                                  // every thread of a wave, also where the wave reaches beyond the row
-        for (long long g0 = 0; g0 < groups; g0 += NT) {
-            float l[4] = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-            if (g0 + tid < groups) row.load(g0 + tid, l);
-            f(l, g0 + tid);
+        for (int g0 = 0; g0 < groups; g0 += 2 * NT) {
+            float l[2][4];
+#pragma unroll
+            for (int q = 0; q < 2; q++) row.load_or_none(g0 + q * NT + tid, groups, l[q]);
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+                if (g0 + q * NT < groups) f(l[q], g0 + q * NT + tid);
         }
     };
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
@@ -618,7 +669,7 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         for (int b = tid; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; }
         __syncthreads();
         const float units = (float)(set.inv_t * 0x1.71547652b82fep+0);
-        tokens([&](float l, long long) { draw_near_add<NT>(hist, l, top, set.scale, units, by_k, by_p); });
+        tokens([&](float l, int) { draw_near_add<NT>(hist, l, top, set.scale, units, by_k, by_p); });
         __syncthreads();
         draw_bracket<NT>(c, hist, set, a.V, by_k, by_p);
         const int bk = c.near.bk, lo = by_p ? c.near.lo : bk, hi = by_p ? c.near.hi : bk;
@@ -628,21 +679,28 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         // 64-bit weights: of all tokens for the total of a top p, in front of the bracket for its sum and for the tiles
         const int sums_to = by_p ? (by_k ? bk - 1 : kDrawBins - 1) : lo - 1;
         double above = 0.0, total = 0.0;
-        auto pass = [&](const float (&l)[4], long long g) {
-            double sum = 0.0;
+        auto pass = [&](const float (&l)[4], int g) {
+            int b[4];
+            bool in[4], sums = false;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int b = l[j] == l[j] ? draw_bin(l[j], top, set.scale) : kDrawBins;
-                const bool in = (b >= lo && b <= hi) || (by_k && b == bk);
-                if (b <= sums_to) {
-                    const double w = draw_weight(l[j], top, set.inv_t);
-                    total += w;
-                    if (b < lo) { above += w; sum += w < set.min_p ? 0.0 : w; }
-                }
-                if (in) {
+                b[j] = l[j] == l[j] ? draw_bin(l[j], top, set.scale) : kDrawBins;
+                in[j] = (b[j] >= lo && b[j] <= hi) || (by_k && b[j] == bk);
+                sums |= b[j] <= sums_to;
+                if (in[j]) {
                     const uint32_t slot = atomicAdd(&c.slots, 1u);
                     if (slot < (uint32_t)(NT < kDrawCand ? NT : kDrawCand)) sh.cand.rank[slot] = draw_rank(l[j], 4 * g + j - row.off);
                 }
+            }
+            if (!__any(sums)) return;                                // its tile has been cleared
+            double sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const double w = draw_weight(l[j], top, set.inv_t);
+                total += b[j] <= sums_to ? w : 0.0;
+                const double front = b[j] <= sums_to && b[j] < lo ? w : 0.0;
+                above += front;
+                sum += front >= set.min_p ? front : 0.0;
             }
             if (PICK && lo > 0) {
                 sum = draw_wave_scan(sum);
@@ -651,19 +709,16 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         };
         all_groups(pass);
         __syncthreads();
-        double all_above, all_total;
-        draw_before<NT, double>(above, c.wave_d, &all_above);
-        draw_before<NT, double>(total, c.wave_d, &all_total);
+        if (by_p) draw_sums<NT>(above, total, c.wave_2);
         __syncthreads();
-        if (draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, all_above, all_total)) {
+        if (draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, above, total)) {
             floor_rank = c.floor_rank;
             if (PICK) {
                 if (tid < (int)c.slots) {                            // the kept candidates' weights, as whole numbers: any order gives the same sums
                     const u64 rank = sh.cand.rank[tid];
-                    const double w = draw_weight(draw_unkey((uint32_t)(rank >> kDrawIndexBits)), top, set.inv_t);
+                    const double w = draw_weight(draw_rank_logit(rank), top, set.inv_t);
                     if (rank >= floor_rank && !(w < set.min_p)) {
-                        const long long i = ((1ll << kDrawIndexBits) - 1) - (long long)(rank & ((1ull << kDrawIndexBits) - 1));
-                        const int q = (int)((i + row.off) >> 8);
+                        const int q = (draw_rank_index(rank) + row.off) >> 8;
                         uint32_t wh, wl;
                         draw_limbs(w, wh, wl);
                         atomicAdd(&hist.hi[q], (u64)wh);
@@ -679,18 +734,19 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
             __syncthreads();
             for (int b = tid; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; hist.lo[b] = 0; }
             __syncthreads();
-            tokens([&](float l, long long) { draw_hist_add(hist, l, top, set.inv_t, set.scale, by_p); });
+            tokens([&](float l, int) { draw_hist_add(hist, l, top, set.inv_t, set.scale, by_p); });
             __syncthreads();
-            auto each = [&](auto f) { tokens([&](float l, long long i) { f(l, draw_rank(l, i)); }); };
+            auto each = [&](auto f) { tokens([&](float l, int i) { f(l, draw_rank(l, i)); }); };
             floor_rank = draw_cuts<NT>(c, hist, sh.fine, sh.cand, each, top, set, by_k, by_p);
         }
         __syncthreads();
     }
-    auto mass4 = [&](const float (&l)[4], long long g, double (&w)[4]) {
+    const DrawFloor floor(floor_rank);
+    auto mass4 = [&](const float (&l)[4], int g, double (&w)[4]) {
         double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            w[j] = l[j] == l[j] ? draw_kept(l[j], 4 * g + j - row.off, floor_rank, top, set) : 0.0;
+            w[j] = draw_kept(l[j], 4 * g + j - row.off, floor, top, set);
             sum += w[j];
         }
         return sum;
@@ -698,7 +754,7 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
     if (PICK) {
         // masses of 256 tokens, one wave's groups, in LDS; then the inclusive sums of these
         if (!tiled)
-            all_groups([&](const float (&l)[4], long long g) {
+            all_groups([&](const float (&l)[4], int g) {
                 double w[4], sum = mass4(l, g, w);
                 sum = draw_wave_scan(sum);
                 if (lane == 63) tile[g >> 6] = sum;
@@ -720,9 +776,9 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
             }
             // the first token in the tile that exceeds; where rounding leaves none, the last one with weight
             for (int q = lo; q >= 0; q--) {
-                const long long g = (long long)q * 64 + lane;
-                float l[4] = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-                if (g < groups) row.load(g, l);
+                const int g = q * 64 + lane;
+                float l[4];
+                row.load_or_none(g, groups, l);
                 double w[4], incl = draw_wave_scan(mass4(l, g, w));
                 double run = (q ? tile[q - 1] : 0.0) + draw_wave_shift(incl);
                 int hit = -1, any = -1;
@@ -746,31 +802,51 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
             }
         }
     } else {
-        // masses of 16 tokens, four neighbouring lanes', in the workspace; then the inclusive sums of these
+        // masses of 8 tokens, two neighbouring lanes', in the workspace; then the inclusive sums of these
         double* spans = a.spans + r * a.spans_row;
-        const long long n = (groups + 3) >> 2;
-        all_groups([&](const float (&l)[4], long long g) {
+        const int n = (groups + 1) >> 1;
+        all_groups([&](const float (&l)[4], int g) {
             double w[4], sum = mass4(l, g, w);
-            sum += __shfl_xor(sum, 1, 64);
-            sum += __shfl_xor(sum, 2, 64);
-            if ((lane & 3) == 0 && (g >> 2) < n) spans[g >> 2] = sum;
+            sum += draw_dpp<0xB1, 0xf>(sum);
+            if ((lane & 1) == 0 && (g >> 1) < n) spans[g >> 1] = sum;
         });
         __syncthreads();
         double carry = 0.0;
-        for (long long b = 0; b < n; b += 4 * NT) {
+        for (int b = 0; b < n; b += 4 * NT) {
             double v[4], sum = 0.0, all;
 #pragma unroll
-            for (int j = 0; j < 4; j++) { const long long q = b + 4 * tid + j; v[j] = q < n ? spans[q] : 0.0; sum += v[j]; }
+            for (int j = 0; j < 4; j++) { const int q = b + 4 * tid + j; v[j] = q < n ? spans[q] : 0.0; sum += v[j]; }
             double at = carry + draw_before<NT, double>(sum, c.wave_d, &all);
 #pragma unroll
-            for (int j = 0; j < 4; j++) { const long long q = b + 4 * tid + j; at += v[j]; if (q < n) spans[q] = at; }
+            for (int j = 0; j < 4; j++) { const int q = b + 4 * tid + j; at += v[j]; if (q < n) spans[q] = at; }
             carry += all;
         }
-        if (tid == 0) { a.total[r] = carry; a.tops[r] = top; a.floors[r] = floor_rank; }
+        if (tid == 0) { a.total[r] = carry; a.tops[r] = raw_top; a.floors[r] = floor_rank; }
     }
 }
 
-// a thread per draw: the span of 16 tokens by bisection, then its tokens one after the other
+// The draw within a span of 8 tokens whose masses begin at `run`: the first token that exceeds, or where rounding leaves none the last one with weight;
+// -1: none has any.
+template <typename T>
+__device__ __forceinline__ int draw_in_span(const Places<T>& row, int span, double run, double want, const DrawFloor& floor, float top, const DrawRow& set, float& at_l)
+{
+    int index = -1; bool found = false;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        float l[4];
+        row.load_or_none(2 * span + e, row.groups(), l);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int i = 4 * (2 * span + e) + j - row.off;
+            const double w = draw_kept(l[j], i, floor, top, set);
+            run += w;
+            if (!found && w > 0.0) { index = i; at_l = l[j]; found = run > want; }
+        }
+    }
+    return index;
+}
+
+// a thread per draw: the span by bisection, then its tokens one after the other
 template <typename T>
 __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long n)
 {
@@ -779,40 +855,25 @@ __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long
     const long long r = t / a.S;
     const double total = a.total[r];
     if (!(total > 0.0)) { a.indices[t] = -1; if (a.logprobs) a.logprobs[t] = -__builtin_inff(); return; }
-    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+    Places<T> row(a, r);
     const DrawRow set = draw_row(a, r);
-    const float top = a.tops[r];
-    const u64 floor_rank = a.floors[r];
+    const float top = row.finite_top(a.tops[r]);
+    const DrawFloor floor(a.floors[r]);
     const double* spans = a.spans + r * a.spans_row;
     const double want = draw_uniform(a, t) * total;
-    long long lo = 0, hi = ((row.groups() + 3) >> 2) - 1;
+    int lo = 0, hi = ((row.groups() + 1) >> 1) - 1;
     while (lo < hi) {
-        const long long mid = (lo + hi) >> 1;
+        const int mid = (lo + hi) >> 1;
         if (spans[mid] > want) hi = mid; else lo = mid + 1;
     }
-    // where rounding leaves no token that exceeds, the last one with weight
-    long long index = -1; float at_l = 0.0f; bool found = false;
-    for (long long q = lo; q >= 0 && index < 0; q--) {
-        double run = q ? spans[q - 1] : 0.0;
-        for (int e = 0; e < 4 && !found; e++) {
-            float l[4];
-            if (4 * q + e >= row.groups()) break;
-            row.load(4 * q + e, l);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const long long i = 4 * (4 * q + e) + j - row.off;
-                const double w = l[j] == l[j] && !found ? draw_kept(l[j], i, floor_rank, top, set) : 0.0;
-                run += w;
-                if (w > 0.0) { index = i; at_l = l[j]; found = run > want; }
-            }
-        }
-    }
+    int index = -1; float at_l = 0.0f;
+    for (int q = lo; q >= 0 && index < 0; q--) index = draw_in_span(row, q, q ? spans[q - 1] : 0.0, want, floor, top, set, at_l);
     a.indices[t] = index;
     if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, log(total));
 }
 
 // ---- a few long rows, in parts over the card -------------------------------------------------------------------------------------
-constexpr int kDrawPart = 256;                      // threads of a part's workgroup, and spans of 16 tokens in a part times part / 1024
+constexpr int kDrawPart = 256;                      // threads of a part's workgroup
 constexpr int kDrawWalk = 512;                      // threads of a workgroup that walks several parts
 
 template <typename T>
@@ -820,15 +881,17 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_top_kernel(DrawArgs a)
 {
     __shared__ float s_f[kDrawPart / 64];
     const long long r = blockIdx.y;
-    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
-    const long long groups = row.groups(), g0 = blockIdx.x * a.part, g1 = g0 + a.part < groups ? g0 + a.part : groups;
+    Places<T> row(a, r);
+    const int groups = row.groups(), g0 = blockIdx.x * a.part, g1 = g0 + a.part < groups ? g0 + a.part : groups;
     float top = -__builtin_inff();
-#pragma unroll 4
-    for (long long g = g0 + threadIdx.x; g < g1; g += kDrawPart) {
-        float l[4];
-        row.load(g, l);
+    for (int g = g0 + threadIdx.x; g < g1; g += 4 * kDrawPart) {
+        float l[4][4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) top = fmaxf(top, l[j]);
+        for (int q = 0; q < 4; q++) row.load_or_none(g + q * kDrawPart, g1, l[q]);
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) top = fmaxf(top, l[q][j]);
     }
     top = draw_max<kDrawPart>(top, s_f);
     if (threadIdx.x == 0) {
@@ -845,17 +908,20 @@ __device__ __forceinline__ float draw_row_top(const DrawArgs& a, long long r, fl
     return draw_max<NT>(top, s_f);
 }
 
-// f(l, g) for the groups of a walker's parts, every thread of a wave
+// f(l, g) for a walker's share of the row's groups, every thread of a wave; four groups' loads in flight
 template <int NT, typename T, typename F>
 __device__ __forceinline__ void draw_walk(const DrawArgs& a, const Places<T>& row, F f)
 {
-    const long long groups = row.groups();
-    const long long each = ((groups + a.walkers - 1) / a.walkers + NT - 1) / NT * NT;
-    const long long g1 = (blockIdx.x + 1) * each < groups ? (blockIdx.x + 1) * each : groups;
-    for (long long g = blockIdx.x * each; g < g1; g += NT) {
-        float l[4] = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-        if (g + threadIdx.x < g1) row.load(g + threadIdx.x, l);
-        f(l, g + threadIdx.x);
+    const int groups = row.groups();
+    const int each = ((groups + a.walkers - 1) / a.walkers + 63) & ~63;
+    const int g0 = (int)blockIdx.x * each, g1 = g0 + each < groups ? g0 + each : groups;
+    for (int g = g0; g < g1; g += 4 * NT) {
+        float l[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) row.load_or_none(g + q * NT + threadIdx.x, g1, l[q]);
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            if (g + q * NT < g1) f(l[q], g + q * NT + (int)threadIdx.x);
     }
 }
 
@@ -867,42 +933,43 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_hist_kernel(DrawArgs a)
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
-    const float top = draw_row_top<kDrawWalk>(a, r, s_f);
+    float top = draw_row_top<kDrawWalk>(a, r, s_f);
     if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) return;
     for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) { hist.count[b] = 0; hist.hi[b] = 0; }
     __syncthreads();
-    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+    Places<T> row(a, r);
+    top = row.finite_top(top);
     const float units = (float)(set.inv_t * 0x1.71547652b82fep+0);
-    draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], long long) {
+    draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], int) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
             if (l[j] == l[j]) draw_near_add<kDrawWalk>(hist, l[j], top, set.scale, units, by_k, by_p);
     });
     __syncthreads();
     const long long at = (r * a.walkers + blockIdx.x) * kDrawBins;
-    for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) { a.hist_n[at + b] = hist.count[b]; a.hist_m[at + b] = hist.hi[b]; }
+    for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) { a.hist_n[at + b] = hist.count[b]; a.hist_m[at + b] = (float)hist.hi[b]; }
 }
 
 // 64 bins to a workgroup, its waves share the walkers out
 __global__ __launch_bounds__(1024) void draw_sum_hist_kernel(DrawArgs a)
 {
     __shared__ uint32_t s_n[16][64];
-    __shared__ u64 s_m[16][64];
+    __shared__ double s_m[16][64];
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
     if (!set.valid || (set.k >= a.V && !(set.p < 1.0))) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bin = blockIdx.x * 64 + lane;
-    uint32_t n = 0; u64 m = 0;
+    uint32_t n = 0; double m = 0.0;
 #pragma unroll 8
     for (int w = wave; w < a.walkers; w += 16) {
         n += a.hist_n[(r * a.walkers + w) * kDrawBins + bin];
-        m += a.hist_m[(r * a.walkers + w) * kDrawBins + bin];
+        m += (double)a.hist_m[(r * a.walkers + w) * kDrawBins + bin];
     }
     s_n[wave][lane] = n; s_m[wave][lane] = m;
     __syncthreads();
     if (wave == 0) {
         for (int w = 1; w < 16; w++) { n += s_n[w][lane]; m += s_m[w][lane]; }
-        a.row_n[r * kDrawBins + bin] = n; a.row_m[r * kDrawBins + bin] = m;
+        a.row_n[r * kDrawBins + bin] = n; a.row_m[r * kDrawBins + bin] = (u64)m;
     }
 }
 
@@ -919,58 +986,64 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
 {
     __shared__ DrawHist hist;
     __shared__ DrawCut c;
-    constexpr uint32_t kStash = 8 * kDrawWalk;
-    __shared__ u64 s_list[kStash];
+    constexpr int kStash = 512;                                      // ranks that a wave holds back for one atomic on the row's list
+    __shared__ u64 s_list[kDrawWalk / 64][kStash];
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
-    const float top = draw_row_top<kDrawWalk>(a, r, c.wave_f);
+    float top = draw_row_top<kDrawWalk>(a, r, c.wave_f);
     if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) return;
     draw_load_hist<kDrawWalk>(a, r, hist, c, set, by_k, by_p);
-    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
+    Places<T> row(a, r);
+    top = row.finite_top(top);
     const int bk = c.near.bk, lo = by_p ? c.near.lo : bk, hi = by_p ? c.near.hi : bk;
     const int sums_to = by_p ? (by_k ? bk - 1 : kDrawBins - 1) : -1;
+    const int lane = threadIdx.x & 63;
+    u64* stash = s_list[threadIdx.x >> 6];
     double above = 0.0, total = 0.0;
-    if (threadIdx.x == 0) c.slots = 0;
-    __syncthreads();
+    int held = 0;                                                    // the same in every lane
     auto flush = [&]() {
-        const uint32_t n = c.slots;
-        if (threadIdx.x == 0) c.in_bin = atomicAdd(&a.list_n[r], n);
-        __syncthreads();
-        const uint32_t at = c.in_bin;
-        for (uint32_t q = threadIdx.x; q < n; q += kDrawWalk)
-            if ((long long)at + q < a.list_most) a.list[r * a.list_most + at + q] = s_list[q];
-        __syncthreads();
-        if (threadIdx.x == 0) c.slots = 0;
-        __syncthreads();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&a.list_n[r], (uint32_t)held);
+        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+        for (int q = lane; q < held; q += 64)
+            if ((long long)at + q < a.list_most) a.list[r * a.list_most + at + q] = stash[q];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        held = 0;
     };
-    draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], long long g) {
+    draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], int g) {
+        int b[4];
+        bool in[4], sums = false, some = false;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int b = l[j] == l[j] ? draw_bin(l[j], top, set.scale) : kDrawBins;
-            const bool in = (b >= lo && b <= hi) || (by_k && b == bk);
-            if (b <= sums_to) {
-                const double w = draw_weight(l[j], top, set.inv_t);
-                total += w;
-                if (b < lo) above += w;
-            }
-            if (in) {
-                const uint32_t slot = atomicAdd(&c.slots, 1u);
-                s_list[slot] = draw_rank(l[j], 4 * g + j - row.off);
-            }
+            b[j] = l[j] == l[j] ? draw_bin(l[j], top, set.scale) : kDrawBins;
+            in[j] = (b[j] >= lo && b[j] <= hi) || (by_k && b[j] == bk);
+            sums |= b[j] <= sums_to;
+            some |= in[j];
         }
-        // the collected tokens to the row's list before the next round could overflow: one global atomic for many of them
-        __syncthreads();
-        if (c.slots > kStash - 4 * kDrawWalk) flush();
-        __syncthreads();
+        if (__any(sums))
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const double w = draw_weight(l[j], top, set.inv_t);
+                total += b[j] <= sums_to ? w : 0.0;
+                above += b[j] <= sums_to && b[j] < lo ? w : 0.0;
+            }
+        if (__any(some)) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const u64 who = __ballot(in[j]);
+                if (in[j]) stash[held + __popcll(who & ((1ull << lane) - 1))] = draw_rank(l[j], 4 * g + j - row.off);
+                held += __popcll(who);
+            }
+            if (held > kStash - 256) flush();
+        }
     });
-    flush();
-    double all_above, all_total;
-    draw_before<kDrawWalk, double>(above, c.wave_d, &all_above);
-    draw_before<kDrawWalk, double>(total, c.wave_d, &all_total);
+    if (held) flush();
+    draw_sums<kDrawWalk>(above, total, c.wave_2);
     if (threadIdx.x == 0) {
-        a.sums[(r * a.walkers + blockIdx.x) * 2] = all_above;
-        a.sums[(r * a.walkers + blockIdx.x) * 2 + 1] = all_total;
+        a.sums[(r * a.walkers + blockIdx.x) * 2] = above;
+        a.sums[(r * a.walkers + blockIdx.x) * 2 + 1] = total;
     }
 }
 
@@ -986,17 +1059,14 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
     const int tid = threadIdx.x;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
-    const float top = draw_row_top<NT>(a, r, c.wave_f);
+    float top = draw_row_top<NT>(a, r, c.wave_f);
     if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) { if (tid == 0) a.floors[r] = 0; return; }
+    Places<T> row(a, r);
+    top = row.finite_top(top);
     draw_load_hist<NT>(a, r, hist, c, set, by_k, by_p);
-    double above = 0.0, total = 0.0, v;
-    for (int w0 = 0; w0 < a.walkers; w0 += NT) {                     // a fixed order
-        const int w = w0 + tid;
-        draw_before<NT, double>(w < a.walkers ? a.sums[(r * a.walkers + w) * 2] : 0.0, c.wave_d, &v);
-        above += v;
-        draw_before<NT, double>(w < a.walkers ? a.sums[(r * a.walkers + w) * 2 + 1] : 0.0, c.wave_d, &v);
-        total += v;
-    }
+    // at most 256 walkers
+    double above = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2] : 0.0, total = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2 + 1] : 0.0;
+    draw_sums<NT>(above, total, c.wave_2);
     const long long n = a.list_n[r];
     const u64* list = a.list + r * a.list_most;
     bool done = false;
@@ -1007,7 +1077,7 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
         done = draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, above, total);
     } else if (n <= a.list_most) {
         auto each = [&](auto f) {
-            for (long long i = tid; i < n; i += NT) { const u64 rank = list[i]; f(draw_unkey((uint32_t)(rank >> kDrawIndexBits)), rank); }
+            for (long long i = tid; i < n; i += NT) { const u64 rank = list[i]; f(draw_rank_logit(rank), rank); }
         };
         const int bk = c.near.bk, lo = c.near.lo, hi = c.near.hi;
         u64 floor_rank = 0;
@@ -1022,24 +1092,20 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
         done = true;
         if (by_p) {
             const double want = set.p * total;
-            double mine = 0.0, in;
-            each([&](float l, u64 rank) { if (rank >= floor_rank && draw_bin(l, top, set.scale) <= hi) mine += draw_weight(l, top, set.inv_t); });
-            draw_before<NT, double>(mine, c.wave_d, &in);
-            done = (lo == 0 || above < want) && (hi == bk || above + in >= want);
-            if (done) {
+            if (lo == 0 || above < want) {
                 if (tid == 0) { c.above_n = 0; c.above_hi = 0; c.above_lo = 0; c.base = above; c.in_bin = (uint32_t)n; }
                 __syncthreads();
                 draw_resolve<NT>(c, sh.fine, sh.cand, each, top, set.inv_t, set.scale, lo, hi, floor_rank, true, true, 0, want);
+                done = hi == bk || c.mass >= want;                   // or else the bracket was too short
                 if (tid == 0 && c.floor_rank < floor_rank) c.floor_rank = floor_rank;
                 __syncthreads();
-            }
+            } else done = false;
         }
     }
     if (!done) {                                                     // over the whole row, exactly from the first histogram on
-        const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
-        const long long groups = row.groups();
+        const int groups = row.groups();
         auto each = [&](auto f) {
-            for (long long g = tid; g < groups; g += NT) {
+            for (int g = tid; g < groups; g += NT) {
                 float l[4];
                 row.load(g, l);
 #pragma unroll
@@ -1059,76 +1125,75 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
     if (tid == 0) a.floors[r] = c.floor_rank;
 }
 
-// the masses of a part: inclusive sums behind every 16 tokens, counted from the part's start
+// the masses of a part: inclusive sums behind every 8 tokens, counted from the part's start
 template <typename T>
 __global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
 {
     __shared__ double s_d[kDrawPart / 64];
     __shared__ float s_f[kDrawPart / 64];
-    __shared__ double span[kDrawPart];
+    __shared__ double span[2 * kDrawPart];
     const long long r = blockIdx.y;
     const int tid = threadIdx.x;
     const DrawRow set = draw_row(a, r);
-    const float top = draw_row_top<kDrawPart>(a, r, s_f);
+    float top = draw_row_top<kDrawPart>(a, r, s_f);
     double carry = 0.0;
     if (set.valid && top > -__builtin_inff()) {
-        const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
-        const u64 floor_rank = a.cuts ? a.floors[r] : 0;
-        const long long groups = row.groups(), g0 = blockIdx.x * a.part;
-        double* spans = a.spans + r * a.spans_row + g0 / 4;
-        for (long long b = 0; b < a.part && g0 + b < groups; b += 4 * kDrawPart) {
+        Places<T> row(a, r);
+        top = row.finite_top(top);
+        const DrawFloor floor(a.cuts ? a.floors[r] : 0);
+        const int groups = row.groups(), g0 = blockIdx.x * a.part;
+        double* spans = a.spans + r * a.spans_row + g0 / 2;
+        for (int b = 0; b < a.part && g0 + b < groups; b += 4 * kDrawPart) {
             float l[4][4];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const long long g = g0 + b + q * kDrawPart + tid;
-                l[q][0] = l[q][1] = l[q][2] = l[q][3] = __builtin_nanf("");
-                if (g < groups) row.load(g, l[q]);
-            }
+            for (int q = 0; q < 4; q++) row.load_or_none(g0 + b + q * kDrawPart + tid, groups, l[q]);
             __syncthreads();                                         // span[] of the round before has been read
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 double sum = 0.0;
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (l[q][j] == l[q][j]) sum += draw_kept(l[q][j], 4 * (g0 + b + q * kDrawPart + tid) + j - row.off, floor_rank, top, set);
-                sum += __shfl_xor(sum, 1, 64);
-                sum += __shfl_xor(sum, 2, 64);
-                if ((tid & 3) == 0) span[(q * kDrawPart + tid) >> 2] = sum;
+                for (int j = 0; j < 4; j++) sum += draw_kept(l[q][j], 4 * (g0 + b + q * kDrawPart + tid) + j - row.off, floor, top, set);
+                sum += draw_dpp<0xB1, 0xf>(sum);
+                if ((tid & 1) == 0) span[(q * kDrawPart + tid) >> 1] = sum;
             }
             __syncthreads();
             double all;
-            const double mine = span[tid], before = draw_before<kDrawPart, double>(mine, s_d, &all);
-            if (4 * (b / 4 + tid) < groups - g0) spans[b / 4 + tid] = carry + before + mine;
+            const double w0 = span[2 * tid], w1 = span[2 * tid + 1];
+            const double at = carry + draw_before<kDrawPart, double>(w0 + w1, s_d, &all) + w0;
+            const int q = b / 2 + 2 * tid;
+            if (2 * q < groups - g0) spans[q] = at;
+            if (2 * (q + 1) < groups - g0) spans[q + 1] = at + w1;
             carry += all;
         }
     }
     if (tid == 0) a.part_mass[r * a.parts + blockIdx.x] = carry;
 }
 
-// draws of a row in parts: the part by bisection in LDS, the span of 16 in the workspace, then its tokens one after the other
+// draws of a row in parts: the part by bisection in LDS, the span in the workspace, then its tokens one after the other
 constexpr int kDrawMostParts = 2048;
+constexpr int kDrawPickers = 512;
 template <typename T>
-__global__ __launch_bounds__(kDrawPart) void draw_part_pick_kernel(DrawArgs a)
+__global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a)
 {
     __shared__ double s_part[kDrawMostParts];
-    __shared__ double s_d[kDrawPart / 64];
-    __shared__ float s_f[kDrawPart / 64];
+    __shared__ double s_d[kDrawPickers / 64];
+    __shared__ float s_f[kDrawPickers / 64];
     const long long r = blockIdx.y;
     const int tid = threadIdx.x;
     const DrawRow set = draw_row(a, r);
-    const float top = draw_row_top<kDrawPart>(a, r, s_f);
-    const int per = (a.parts + kDrawPart - 1) / kDrawPart;
+    Places<T> row(a, r);
+    const float top = row.finite_top(draw_row_top<kDrawPickers>(a, r, s_f));
+    const int per = (a.parts + kDrawPickers - 1) / kDrawPickers;
     double sum = 0.0, total;
     for (int p = tid * per; p < (tid + 1) * per && p < a.parts; p++) sum += a.part_mass[r * a.parts + p];
-    double at = draw_before<kDrawPart, double>(sum, s_d, &total);
+    double at = draw_before<kDrawPickers, double>(sum, s_d, &total);
     for (int p = tid * per; p < (tid + 1) * per && p < a.parts; p++) { at += a.part_mass[r * a.parts + p]; s_part[p] = at; }
     __syncthreads();
-    const Places<T> row((const T*)a.logits + r * a.row_stride, a.V);
-    const long long groups = row.groups(), part_spans = a.part / 4, row_spans = (groups + 3) / 4;
+    const int part_spans = (int)(a.part / 2), row_spans = (row.groups() + 1) / 2;
     const double* spans = a.spans + r * a.spans_row;
-    const u64 floor_rank = a.cuts ? a.floors[r] : 0;
+    const DrawFloor floor(a.cuts ? a.floors[r] : 0);
     const double log_total = log(total);
-    for (long long s = (long long)blockIdx.x * kDrawPart + tid; s < a.S; s += (long long)gridDim.x * kDrawPart) {
+    for (long long s = (long long)blockIdx.x * kDrawPickers + tid; s < a.S; s += (long long)gridDim.x * kDrawPickers) {
         const long long t = r * a.S + s;
         if (!(total > 0.0)) { a.indices[t] = -1; if (a.logprobs) a.logprobs[t] = -__builtin_inff(); continue; }
         const double want = draw_uniform(a, t) * total;
@@ -1138,28 +1203,16 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_pick_kernel(DrawArgs a)
             if (s_part[mid] > want) p1 = mid; else p = mid + 1;
         }
         const double base = p ? s_part[p - 1] : 0.0;
-        long long lo = p * part_spans, hi = lo + part_spans < row_spans ? lo + part_spans - 1 : row_spans - 1;
+        int lo = p * part_spans, hi = lo + part_spans < row_spans ? lo + part_spans - 1 : row_spans - 1;
+        if (lo > hi) lo = hi;                                        // rounding beyond the last part with tokens
         while (lo < hi) {
-            const long long mid = (lo + hi) >> 1;
+            const int mid = (lo + hi) >> 1;
             if (base + spans[mid] > want) hi = mid; else lo = mid + 1;
         }
-        // where rounding leaves no token that exceeds, the last one with weight
-        long long index = -1; float at_l = 0.0f; bool found = false;
-        for (long long q = lo; q >= 0 && index < 0; q--) {
-            const long long qp = q / part_spans;
-            double run = (qp ? s_part[qp - 1] : 0.0) + (q % part_spans ? spans[q - 1] : 0.0);
-            for (int e = 0; e < 4 && !found; e++) {
-                float l[4];
-                if (4 * q + e >= groups) break;
-                row.load(4 * q + e, l);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const long long i = 4 * (4 * q + e) + j - row.off;
-                    const double w = l[j] == l[j] && !found ? draw_kept(l[j], i, floor_rank, top, set) : 0.0;
-                    run += w;
-                    if (w > 0.0) { index = i; at_l = l[j]; found = run > want; }
-                }
-            }
+        int index = -1; float at_l = 0.0f;
+        for (int q = lo; q >= 0 && index < 0; q--) {
+            const int qp = q / part_spans;
+            index = draw_in_span(row, q, (qp ? s_part[qp - 1] : 0.0) + (q % part_spans ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
         }
         a.indices[t] = index;
         if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, log_total);
@@ -1213,6 +1266,12 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
 #pragma unroll
     for (int d = W / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
     const bool live = on && set.valid && top > -__builtin_inff();
+    if (__any(top == __builtin_inff())) {                            // as Places has it
+        const bool infinite = top == __builtin_inff();
+#pragma unroll
+        for (int e = 0; e < E; e++) l[e] = !infinite || l[e] != l[e] ? l[e] : l[e] == __builtin_inff() ? 0.0f : -__builtin_inff();
+        top = infinite ? 0.0f : top;
+    }
     double w[E];
     uint32_t key[E];                                                 // 0: not a token, or cut
 #pragma unroll
@@ -1360,7 +1419,7 @@ static DrawLayout draw_layout(const gsx_draw* s)
     else if (s->S <= kDrawInRow && s->V <= (int64_t)kDrawWaveTiles * 256 - 4) l.way = DrawLayout::kRow;
     else l.way = DrawLayout::kRowSpans;
     if (l.way == DrawLayout::kRowSpans) {
-        l.spans_row = (s->V + 3 + 15) / 16;
+        l.spans_row = (s->V + 3 + 7) / 8;
         l.spans = take(R * (size_t)l.spans_row * 8);
         l.total = take(R * 8);
         l.floors = take(R * 8);
@@ -1371,8 +1430,8 @@ static DrawLayout draw_layout(const gsx_draw* s)
         l.part = 4 * kDrawPart;
         while (ceil_div(groups, l.part) > kDrawMostParts) l.part *= 2;
         l.parts = (int)ceil_div(groups, l.part);
-        l.spans_row = (int64_t)l.parts * l.part / 4;
-        l.walkers = (int)(256 / s->R > 1 ? 256 / s->R : 1);
+        l.spans_row = (int64_t)l.parts * l.part / 2;
+        l.walkers = (int)(1024 / s->R > 256 ? 256 : 1024 / s->R > 1 ? 1024 / s->R : 1);
         if (l.walkers > l.parts) l.walkers = l.parts;
         l.spans = take(R * (size_t)l.spans_row * 8);
         l.floors = take(R * 8);
@@ -1380,7 +1439,7 @@ static DrawLayout draw_layout(const gsx_draw* s)
         l.part_mass = take(R * l.parts * 8);
         if (l.cuts) {
             l.hist_n = take(R * l.walkers * kDrawBins * 4);
-            l.hist_m = take(R * l.walkers * kDrawBins * 8);
+            l.hist_m = take(R * l.walkers * kDrawBins * 4);
             l.row_n = take(R * kDrawBins * 4);
             l.row_m = take(R * kDrawBins * 8);
             l.sums = take(R * l.walkers * 16);
@@ -1425,8 +1484,8 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
             draw_floor_kernel<T><<<dim3((unsigned)a.R), dim3(1024), 0, stream>>>(a);
         }
         draw_part_mass_kernel<T><<<parts, dim3(kDrawPart), 0, stream>>>(a);
-        const int64_t picks = ceil_div(a.S, kDrawPart);
-        draw_part_pick_kernel<T><<<dim3((unsigned)(picks < 1024 ? picks : 1024), (unsigned)a.R), dim3(kDrawPart), 0, stream>>>(a);
+        const int64_t picks = ceil_div(a.S, kDrawPickers);
+        draw_part_pick_kernel<T><<<dim3((unsigned)(picks < 1024 ? picks : 1024), (unsigned)a.R), dim3(kDrawPickers), 0, stream>>>(a);
         GSX_LAUNCH_CHECK();
         return GSX_OK;
     }
@@ -1471,9 +1530,9 @@ GSX_API int gsx_draw_indices(const gsx_draw* s, void* stream)
     a.temperatures = s->temperatures; a.top_ps = s->top_ps; a.min_ps = s->min_ps; a.top_ks = s->top_ks;
     a.indices = (long long*)s->indices; a.logprobs = s->logprobs;
     a.spans_row = l.spans_row;
-    a.part = l.part; a.parts = l.parts; a.walkers = l.walkers; a.cuts = l.cuts; a.list_most = l.list_most;
+    a.part = (int)l.part; a.parts = l.parts; a.walkers = l.walkers; a.cuts = l.cuts; a.list_most = l.list_most;
     a.part_top = (float*)(ws + l.part_top); a.part_mass = (double*)(ws + l.part_mass);
-    a.hist_n = (uint32_t*)(ws + l.hist_n); a.hist_m = (u64*)(ws + l.hist_m); a.row_n = (uint32_t*)(ws + l.row_n); a.row_m = (u64*)(ws + l.row_m);
+    a.hist_n = (uint32_t*)(ws + l.hist_n); a.hist_m = (float*)(ws + l.hist_m); a.row_n = (uint32_t*)(ws + l.row_n); a.row_m = (u64*)(ws + l.row_m);
     a.sums = (double*)(ws + l.sums); a.list = (u64*)(ws + l.list); a.list_n = (uint32_t*)(ws + l.list_n);
     a.spans = (double*)(ws + l.spans); a.total = (double*)(ws + l.total); a.floors = (u64*)(ws + l.floors); a.tops = (float*)(ws + l.tops);
     switch (s->dtype) {
