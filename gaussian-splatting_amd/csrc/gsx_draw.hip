@@ -37,6 +37,7 @@ struct DrawArgs {
     const void* logits; long long row_stride, R, V, S;
     const void* uniforms;
     float temperature, top_p, min_p; int top_k, uniforms_f64;
+    double inv_t;                                   // of `temperature`: a 64-bit division per row would cost as much as an exp
     const float* temperatures; const float* top_ps; const float* min_ps; const int32_t* top_ks;
     long long* indices; float* logprobs;
     // workspace of rows whose draws are made by a kernel of their own
@@ -44,10 +45,11 @@ struct DrawArgs {
     double* total; float* tops; u64* floors;        // per row: kept mass (-1: none), top, lowest kept rank
     long long spans_row;
     // rows in parts: `part` groups of four places each, `parts` to a row; `walkers` workgroups per row where a workgroup takes several parts
-    int part, parts, walkers, cuts;
+    int part, parts, nodes, walkers, cuts;
     float* part_top; double* part_mass;             // [row][part]
     uint32_t* hist_n; float* hist_m;                // [row][walker][bin]
-    uint32_t* row_n; u64* row_m;                    // [row][bin]
+    uint32_t* row_n; double* row_m;                 // [row][bin]
+    struct DrawNear* near;                          // [row]
     double* sums;                                   // [row][walker][2]: 64-bit mass in front of the bracket, and the total's part
     u64* list; uint32_t* list_n; long long list_most;        // [row]: ranks of the tokens where the cuts may end
 };
@@ -139,7 +141,8 @@ __device__ __forceinline__ DrawRow draw_row(const DrawArgs& a, long long r)
     const float m = a.min_ps ? a.min_ps[r] : a.min_p;
     const int k = a.top_ks ? a.top_ks[r] : a.top_k;
     s.valid = t >= 0.0f && p > 0.0f && m >= 0.0f && m <= 1.0f;
-    s.inv_t = t > 0.0f ? 1.0 / (double)t : 1.0;
+    s.inv_t = a.inv_t;
+    if (a.temperatures) s.inv_t = t > 0.0f ? 1.0 / (double)t : 1.0;
     s.scale = (float)(s.inv_t * (double)kDrawBinsPerUnit);
     s.p = (double)p; s.min_p = (double)m;
     s.k = k > 0 && k < a.V ? k : a.V;
@@ -158,6 +161,13 @@ __device__ __forceinline__ double draw_kept(float l, int i, const DrawFloor& flo
     if (!__any(floor.keeps(l, i))) return 0.0;                       // most waves beyond a cut keep nothing
     const double w = draw_weight(l, top, set.inv_t);
     return floor.keeps(l, i) && w >= set.min_p ? w : 0.0;
+}
+
+// log(x) for x >= 1 (a row's top weighs 1): the 32-bit one and a Newton step, y + x e^-y - 1, which squares its error of 1e-6
+__device__ __forceinline__ double draw_log(double x)
+{
+    const double y = (double)(__builtin_amdgcn_logf((float)x) * 0.693147181f);
+    return y + (x * draw_exp(-y) - 1.0);
 }
 
 __device__ __forceinline__ float draw_logprob(float l, float top, double inv_t, double log_total)
@@ -291,6 +301,7 @@ __device__ __forceinline__ float draw_max(float v, float* s_wave)
 }
 
 struct DrawHist { uint32_t count[kDrawBins]; u64 hi[kDrawBins], lo[kDrawBins]; };
+struct DrawNearHist { uint32_t count[kDrawBins]; u64 hi[kDrawBins]; };       // without the second limb
 struct DrawFine { uint32_t count[kDrawFine]; u64 hi[kDrawFine], lo[kDrawFine]; };
 struct DrawCand { u64 rank[kDrawCand], ranked[kDrawCand]; };
 
@@ -499,8 +510,8 @@ __device__ u64 draw_cuts(DrawCut& c, const DrawHist& hist, DrawFine& fine, DrawC
 // happens, and collects the tokens inside it and in the bin where the top k end; these few are ranked and decided exactly.  `false`: too
 // many of them, or the sums do not bear the bracket out; the longer way has no such limits.
 // mass(q, w): adds a weight that is kept for certain to tile q (all lanes of the wave call it, once per group).
-template <int NT>
-__device__ __forceinline__ void draw_near_add(DrawHist& h, float l, float top, float scale, float units, bool by_k, bool by_p)
+template <typename Hist>
+__device__ __forceinline__ void draw_near_add(Hist& h, float l, float top, float scale, float units, bool by_k, bool by_p)
 {
     const int b = draw_bin(l, top, scale);
     if (by_k) atomicAdd(&h.count[b], 1u);
@@ -511,8 +522,8 @@ __device__ __forceinline__ void draw_near_add(DrawHist& h, float l, float top, f
 }
 
 // where the cuts may end, from the histogram; c.near
-template <int NT>
-__device__ void draw_bracket(DrawCut& c, const DrawHist& h, const DrawRow& set, long long V, bool by_k, bool by_p)
+template <int NT, typename Hist>
+__device__ void draw_bracket(DrawCut& c, const Hist& h, const DrawRow& set, long long V, bool by_k, bool by_p)
 {
     constexpr int per = kDrawBins / NT;
     const int b0 = threadIdx.x * per;
@@ -669,7 +680,7 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         for (int b = tid; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; }
         __syncthreads();
         const float units = (float)(set.inv_t * 0x1.71547652b82fep+0);
-        tokens([&](float l, int) { draw_near_add<NT>(hist, l, top, set.scale, units, by_k, by_p); });
+        tokens([&](float l, int) { draw_near_add(hist, l, top, set.scale, units, by_k, by_p); });
         __syncthreads();
         draw_bracket<NT>(c, hist, set, a.V, by_k, by_p);
         const int bk = c.near.bk, lo = by_p ? c.near.lo : bk, hi = by_p ? c.near.hi : bk;
@@ -766,7 +777,7 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         double at = draw_before<NT, double>(sum, c.wave_d, &total);
         for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) { at += tile[q]; tile[q] = at; }
         __syncthreads();
-        const double log_total = log(total);
+        const double log_total = draw_log(total);
         for (long long s = wave; s < a.S; s += kWaves) {             // a wave per draw
             const double want = draw_uniform(a, r * a.S + s) * total;
             int lo = 0, hi = tiles - 1;
@@ -869,11 +880,12 @@ __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long
     int index = -1; float at_l = 0.0f;
     for (int q = lo; q >= 0 && index < 0; q--) index = draw_in_span(row, q, q ? spans[q - 1] : 0.0, want, floor, top, set, at_l);
     a.indices[t] = index;
-    if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, log(total));
+    if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, draw_log(total));
 }
 
 // ---- a few long rows, in parts over the card -------------------------------------------------------------------------------------
 constexpr int kDrawPart = 256;                      // threads of a part's workgroup
+constexpr int kDrawFewWalkers = 32;
 constexpr int kDrawWalk = 512;                      // threads of a workgroup that walks several parts
 
 template <typename T>
@@ -928,7 +940,7 @@ __device__ __forceinline__ void draw_walk(const DrawArgs& a, const Places<T>& ro
 template <typename T>
 __global__ __launch_bounds__(kDrawWalk) void draw_part_hist_kernel(DrawArgs a)
 {
-    __shared__ DrawHist hist;
+    __shared__ DrawNearHist hist;
     __shared__ float s_f[kDrawWalk / 64];
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
@@ -943,7 +955,7 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_hist_kernel(DrawArgs a)
     draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], int) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (l[j] == l[j]) draw_near_add<kDrawWalk>(hist, l[j], top, set.scale, units, by_k, by_p);
+            if (l[j] == l[j]) draw_near_add(hist, l[j], top, set.scale, units, by_k, by_p);
     });
     __syncthreads();
     const long long at = (r * a.walkers + blockIdx.x) * kDrawBins;
@@ -969,48 +981,69 @@ __global__ __launch_bounds__(1024) void draw_sum_hist_kernel(DrawArgs a)
     __syncthreads();
     if (wave == 0) {
         for (int w = 1; w < 16; w++) { n += s_n[w][lane]; m += s_m[w][lane]; }
-        a.row_n[r * kDrawBins + bin] = n; a.row_m[r * kDrawBins + bin] = (u64)m;
+        a.row_n[r * kDrawBins + bin] = n; a.row_m[r * kDrawBins + bin] = m;
     }
 }
 
-template <int NT>
-__device__ __forceinline__ void draw_load_hist(const DrawArgs& a, long long r, DrawHist& hist, DrawCut& c, const DrawRow& set, bool by_k, bool by_p)
+// one workgroup per row: the bracket, from the walkers' histograms where they are few, else from their sum
+__global__ __launch_bounds__(1024) void draw_near_kernel(DrawArgs a)
 {
-    for (int b = threadIdx.x; b < kDrawBins; b += NT) { hist.count[b] = a.row_n[r * kDrawBins + b]; hist.hi[b] = a.row_m[r * kDrawBins + b]; }
+    constexpr int NT = 1024;
+    __shared__ DrawNearHist hist;
+    __shared__ DrawCut c;
+    const long long r = blockIdx.x;
+    const DrawRow set = draw_row(a, r);
+    const bool by_k = set.k < a.V, by_p = set.p < 1.0;
+    if (!set.valid || (!by_k && !by_p)) return;
+    for (int b = threadIdx.x; b < kDrawBins; b += NT) {
+        uint32_t n = 0; double m = 0.0;
+        if (a.walkers <= kDrawFewWalkers) {
+#pragma unroll 4
+            for (int w = 0; w < a.walkers; w++) {
+                n += a.hist_n[(r * a.walkers + w) * kDrawBins + b];
+                m += (double)a.hist_m[(r * a.walkers + w) * kDrawBins + b];
+            }
+        } else { n = a.row_n[r * kDrawBins + b]; m = a.row_m[r * kDrawBins + b]; }
+        hist.count[b] = n; hist.hi[b] = (u64)m;
+    }
     __syncthreads();
     draw_bracket<NT>(c, hist, set, a.V, by_k, by_p);
+    if (threadIdx.x == 0) a.near[r] = c.near;
 }
 
 template <typename T>
 __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
 {
-    __shared__ DrawHist hist;
-    __shared__ DrawCut c;
-    constexpr int kStash = 512;                                      // ranks that a wave holds back for one atomic on the row's list
-    __shared__ u64 s_list[kDrawWalk / 64][kStash];
+    constexpr int kStash = 512, kWaves = kDrawWalk / 64;             // ranks that a wave holds back for one atomic on the row's list
+    __shared__ u64 s_list[kWaves][kStash];
+    __shared__ uint32_t s_held[kWaves + 1];
+    __shared__ double s_2[kWaves][2];
+    __shared__ float s_f[kWaves];
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
-    float top = draw_row_top<kDrawWalk>(a, r, c.wave_f);
+    float top = draw_row_top<kDrawWalk>(a, r, s_f);
     if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) return;
-    draw_load_hist<kDrawWalk>(a, r, hist, c, set, by_k, by_p);
+    const DrawNear near = a.near[r];
     Places<T> row(a, r);
     top = row.finite_top(top);
-    const int bk = c.near.bk, lo = by_p ? c.near.lo : bk, hi = by_p ? c.near.hi : bk;
+    const int bk = near.bk, lo = by_p ? near.lo : bk, hi = by_p ? near.hi : bk;
     const int sums_to = by_p ? (by_k ? bk - 1 : kDrawBins - 1) : -1;
     const int lane = threadIdx.x & 63;
     u64* stash = s_list[threadIdx.x >> 6];
     double above = 0.0, total = 0.0;
     int held = 0;                                                    // the same in every lane
-    auto flush = [&]() {
+    auto flush_to = [&](uint32_t at) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        uint32_t at = 0;
-        if (lane == 0) at = atomicAdd(&a.list_n[r], (uint32_t)held);
-        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
         for (int q = lane; q < held; q += 64)
             if ((long long)at + q < a.list_most) a.list[r * a.list_most + at + q] = stash[q];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         held = 0;
+    };
+    auto flush = [&]() {
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&a.list_n[r], (uint32_t)held);
+        flush_to((uint32_t)__builtin_amdgcn_readfirstlane((int)at));
     };
     draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], int g) {
         int b[4];
@@ -1039,8 +1072,16 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
             if (held > kStash - 256) flush();
         }
     });
-    if (held) flush();
-    draw_sums<kDrawWalk>(above, total, c.wave_2);
+    // what is left, with one atomic for the workgroup: atomics on one address take some 10 ns each
+    if (lane == 0) s_held[threadIdx.x >> 6] = (uint32_t)held;
+    __syncthreads();
+    uint32_t front = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) { if (w == (int)(threadIdx.x >> 6)) front = all; all += s_held[w]; }
+    if (threadIdx.x == 0) s_held[kWaves] = all ? atomicAdd(&a.list_n[r], all) : 0;
+    __syncthreads();
+    flush_to(s_held[kWaves] + front);
+    draw_sums<kDrawWalk>(above, total, s_2);
     if (threadIdx.x == 0) {
         a.sums[(r * a.walkers + blockIdx.x) * 2] = above;
         a.sums[(r * a.walkers + blockIdx.x) * 2 + 1] = total;
@@ -1063,7 +1104,8 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
     if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) { if (tid == 0) a.floors[r] = 0; return; }
     Places<T> row(a, r);
     top = row.finite_top(top);
-    draw_load_hist<NT>(a, r, hist, c, set, by_k, by_p);
+    if (tid == 0) c.near = a.near[r];
+    __syncthreads();
     // at most 256 walkers
     double above = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2] : 0.0, total = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2 + 1] : 0.0;
     draw_sums<NT>(above, total, c.wave_2);
@@ -1169,13 +1211,16 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
     if (tid == 0) a.part_mass[r * a.parts + blockIdx.x] = carry;
 }
 
-// draws of a row in parts: the part by bisection in LDS, the span in the workspace, then its tokens one after the other
+// Draws of a row in parts.  For many draws what bounds them is the lines that a bisection touches (at 1 M tokens and draws: 7 lines of 128 B through each CU's 64 B a
+// cycle, 80 us); so the sums behind every 1 / nodes of a part lie in LDS, down to 16 spans, a line: a draw then reads one line of spans and one of tokens.
 constexpr int kDrawMostParts = 2048;
-constexpr int kDrawPickers = 512;
+constexpr int kDrawMostNodes = 16384;
+constexpr int64_t kDrawManyDraws = 1 << 15;         // from here on the nodes' 128 KB are worth their loading
+constexpr int kDrawPickers = 1024;
 template <typename T>
 __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a)
 {
-    __shared__ double s_part[kDrawMostParts];
+    extern __shared__ double s_sum[];                                // masses in front of each part, then behind each node
     __shared__ double s_d[kDrawPickers / 64];
     __shared__ float s_f[kDrawPickers / 64];
     const long long r = blockIdx.y;
@@ -1183,37 +1228,43 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
     const DrawRow set = draw_row(a, r);
     Places<T> row(a, r);
     const float top = row.finite_top(draw_row_top<kDrawPickers>(a, r, s_f));
+    double* s_part = s_sum;
+    double* s_node = s_sum + a.parts;
+    const int part_spans = a.part / 2, row_spans = (row.groups() + 1) / 2, step = part_spans / a.nodes;
+    const double* spans = a.spans + r * a.spans_row;
     const int per = (a.parts + kDrawPickers - 1) / kDrawPickers;
     double sum = 0.0, total;
     for (int p = tid * per; p < (tid + 1) * per && p < a.parts; p++) sum += a.part_mass[r * a.parts + p];
     double at = draw_before<kDrawPickers, double>(sum, s_d, &total);
-    for (int p = tid * per; p < (tid + 1) * per && p < a.parts; p++) { at += a.part_mass[r * a.parts + p]; s_part[p] = at; }
+    for (int p = tid * per; p < (tid + 1) * per && p < a.parts; p++) { s_part[p] = at; at += a.part_mass[r * a.parts + p]; }
     __syncthreads();
-    const int part_spans = (int)(a.part / 2), row_spans = (row.groups() + 1) / 2;
-    const double* spans = a.spans + r * a.spans_row;
+    const int nodes = a.parts * a.nodes;
+    for (int q = tid; q < nodes; q += kDrawPickers) {
+        const int p = q / a.nodes, last = (q + 1) * step - 1;        // the node's last span
+        s_node[q] = s_part[p] + (last < row_spans && (q + 1) % a.nodes ? spans[last] : a.part_mass[r * a.parts + p]);
+    }
+    __syncthreads();
     const DrawFloor floor(a.cuts ? a.floors[r] : 0);
-    const double log_total = log(total);
+    const double log_total = draw_log(total);
     for (long long s = (long long)blockIdx.x * kDrawPickers + tid; s < a.S; s += (long long)gridDim.x * kDrawPickers) {
         const long long t = r * a.S + s;
         if (!(total > 0.0)) { a.indices[t] = -1; if (a.logprobs) a.logprobs[t] = -__builtin_inff(); continue; }
         const double want = draw_uniform(a, t) * total;
-        int p = 0, p1 = a.parts - 1;
-        while (p < p1) {
-            const int mid = (p + p1) >> 1;
-            if (s_part[mid] > want) p1 = mid; else p = mid + 1;
+        int n = 0, n1 = nodes - 1;
+        while (n < n1) {
+            const int mid = (n + n1) >> 1;
+            if (s_node[mid] > want) n1 = mid; else n = mid + 1;
         }
-        const double base = p ? s_part[p - 1] : 0.0;
-        int lo = p * part_spans, hi = lo + part_spans < row_spans ? lo + part_spans - 1 : row_spans - 1;
-        if (lo > hi) lo = hi;                                        // rounding beyond the last part with tokens
+        int lo = n * step, hi = lo + step < row_spans ? lo + step - 1 : row_spans - 1;
+        if (lo > hi) lo = hi;                                        // rounding beyond the last node with tokens
+        const double base = s_part[lo / part_spans];
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (base + spans[mid] > want) hi = mid; else lo = mid + 1;
         }
         int index = -1; float at_l = 0.0f;
-        for (int q = lo; q >= 0 && index < 0; q--) {
-            const int qp = q / part_spans;
-            index = draw_in_span(row, q, (qp ? s_part[qp - 1] : 0.0) + (q % part_spans ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
-        }
+        for (int q = lo; q >= 0 && index < 0; q--)
+            index = draw_in_span(row, q, s_part[q / part_spans] + (q % part_spans ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
         a.indices[t] = index;
         if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, log_total);
     }
@@ -1226,11 +1277,32 @@ __device__ __forceinline__ uint32_t draw_votes(bool b, int sub)       // lanes o
     const u64 v = __ballot(b);
     return W == 64 ? __popcll(v) : __popcll((v >> (sub * W)) & ((1ull << (W & 63)) - 1));
 }
-template <int W>
-__device__ __forceinline__ double draw_lanes_sum(double v)
+// all W lanes of a row get op over them: within 16 lanes by DPP (mirrors reach the other half once a half is equal)
+template <int W, typename T, typename Op>
+__device__ __forceinline__ T draw_lanes_all(T v, Op op)
 {
-#pragma unroll
-    for (int d = W / 2; d; d >>= 1) v += __shfl_xor(v, d, 64);
+    if (W >= 2) v = op(v, draw_dpp<0xB1, 0xf>(v));
+    if (W >= 4) v = op(v, draw_dpp<0x4E, 0xf>(v));
+    if (W >= 8) v = op(v, draw_dpp<0x141, 0xf>(v));
+    if (W >= 16) v = op(v, draw_dpp<0x140, 0xf>(v));
+    if (W >= 32) v = op(v, __shfl_xor(v, 16, 64));
+    if (W >= 64) v = op(v, __shfl_xor(v, 32, 64));
+    return v;
+}
+template <int W>
+__device__ __forceinline__ double draw_lanes_sum(double v) { return draw_lanes_all<W>(v, [](double x, double y) { return x + y; }); }
+// inclusive sums over the row's lanes
+template <int W, typename T>
+__device__ __forceinline__ T draw_lanes_scan(T v)
+{
+    const int at = threadIdx.x % W;
+    if (W >= 2) { const T o = draw_dpp<0x111, 0xf>(v); v += at >= 1 ? o : (T)0; }
+    if (W >= 4) { const T o = draw_dpp<0x112, 0xf>(v); v += at >= 2 ? o : (T)0; }
+    if (W >= 8) { const T o = draw_dpp<0x114, 0xf>(v); v += at >= 4 ? o : (T)0; }
+    if (W >= 16) { const T o = draw_dpp<0x118, 0xf>(v); v += at >= 8 ? o : (T)0; }
+    // DPP stays within 16 lanes: from there on the last lane of the lower half is added to the upper one
+    if (W >= 32) { const T o = __shfl(v, 15, 32); v += (at & 16) ? o : (T)0; }
+    if (W >= 64) { const T o = __shfl(v, 31, 64); v += at >= 32 ? o : (T)0; }
     return v;
 }
 
@@ -1263,8 +1335,7 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
     float top = -__builtin_inff();
 #pragma unroll
     for (int e = 0; e < E; e++) top = fmaxf(top, l[e]);
-#pragma unroll
-    for (int d = W / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    top = draw_lanes_all<W>(top, [](float x, float y) { return fmaxf(x, y); });
     const bool live = on && set.valid && top > -__builtin_inff();
     if (__any(top == __builtin_inff())) {                            // as Places has it
         const bool infinite = top == __builtin_inff();
@@ -1274,14 +1345,16 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
     }
     double w[E];
     uint32_t key[E];                                                 // 0: not a token, or cut
+    const bool cuts = __any(live && (set.k < a.V || set.p < 1.0));
 #pragma unroll
     for (int e = 0; e < E; e++) {
         w[e] = draw_weight(l[e], top, set.inv_t);                    // 0 outside the row
-        key[e] = l[e] == l[e] ? draw_key(l[e]) : 0u;
+        key[e] = 1u;
+        if (cuts) key[e] = l[e] == l[e] ? draw_key(l[e]) : 0u;
     }
     // A cut at the highest key t for which the tokens of key >= t reach k, or `want`: found bit by bit; of the ones at t the first few in index order.
 #pragma unroll 1
-    for (int cut = 0; cut < 2; cut++) {
+    for (int cut = 0; cuts && cut < 2; cut++) {
         const bool mine = live && (cut == 0 ? set.k < a.V : set.p < 1.0);
         if (!__any(mine)) continue;
         double want = 0.0;
@@ -1319,16 +1392,10 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
         }
         mass = draw_lanes_sum<W>(mass);
         // ties in the lanes before this one, in all of them, and the weight that they share
-        uint32_t incl = ties;
-#pragma unroll
-        for (int d = 1; d < W; d <<= 1) {
-            const uint32_t o = __shfl_up(incl, d, W);
-            if (lane % W >= d) incl += o;
-        }
+        const uint32_t incl = draw_lanes_scan<W>(ties);
         before = incl - ties;
         const uint32_t all = __shfl(incl, W - 1, W);
-#pragma unroll
-        for (int d = W / 2; d; d >>= 1) tie_w = fmax(tie_w, __shfl_xor(tie_w, d, 64));
+        tie_w = draw_lanes_all<W>(tie_w, [](double x, double y) { return fmax(x, y); });
         double m = cut == 0 ? (double)set.k - (double)above : tie_w > 0.0 ? ceil((want - mass) / tie_w) : (double)all;
         const uint32_t kept = m < 1.0 ? 1u : m < (double)all ? (uint32_t)m : all;
         if (mine)
@@ -1344,13 +1411,7 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
         if (!key[e] || w[e] < set.min_p) w[e] = 0.0;
         sum += w[e];
     }
-    double incl = sum;
-#pragma unroll
-    for (int d = 1; d < W; d <<= 1) {
-        const double o = __shfl_up(incl, d, W);
-        if (lane % W >= d) incl += o;
-    }
-    const double up = __shfl_up(incl, 1, W), total = __shfl(incl, W - 1, W);
+    const double incl = draw_lanes_scan<W>(sum), up = draw_wave_shift(incl), total = __shfl(incl, W - 1, W);
     double run = lane % W ? up : 0.0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
@@ -1359,7 +1420,7 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
         s_mass[wave][lane * E + e] = w[e] > 0.0 ? run : -run;
         s_l[wave][lane * E + e] = l[e];
     }
-    if (lane % W == 0) { s_total[wave][sub] = live ? total : -1.0; s_log[wave][sub] = log(total); s_inv[wave][sub] = set.inv_t; s_top[wave][sub] = top; }
+    if (lane % W == 0) { s_total[wave][sub] = live ? total : -1.0; s_log[wave][sub] = draw_log(total); s_inv[wave][sub] = set.inv_t; s_top[wave][sub] = top; }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");           // LDS of this wave's own lanes
     __builtin_amdgcn_wave_barrier();
     const int rows = a.R - r0 < kRows ? (int)(a.R - r0) : kRows;
@@ -1402,8 +1463,8 @@ static int draw_check(const gsx_draw* s)
 
 struct DrawLayout {
     enum Way { kShort, kRow, kRowSpans, kParts } way;
-    long long spans_row, part, list_most; int parts, walkers, cuts;
-    size_t spans, total, floors, tops, part_top, part_mass, hist_n, hist_m, row_n, row_m, sums, list, list_n, bytes;
+    long long spans_row, part, list_most; int parts, nodes, walkers, cuts;
+    size_t spans, total, floors, tops, part_top, part_mass, hist_n, hist_m, row_n, row_m, near, sums, list, list_n, bytes;
 };
 
 // Which way, and its workspace.
@@ -1431,7 +1492,10 @@ static DrawLayout draw_layout(const gsx_draw* s)
         while (ceil_div(groups, l.part) > kDrawMostParts) l.part *= 2;
         l.parts = (int)ceil_div(groups, l.part);
         l.spans_row = (int64_t)l.parts * l.part / 2;
-        l.walkers = (int)(1024 / s->R > 256 ? 256 : 1024 / s->R > 1 ? 1024 / s->R : 1);
+        l.nodes = 1;
+        if (s->S >= kDrawManyDraws)
+            while (l.nodes < l.part / 32 && (int64_t)l.parts * l.nodes * 2 <= kDrawMostNodes) l.nodes *= 2;
+        l.walkers = (int)(512 / s->R > 256 ? 256 : 512 / s->R > 1 ? 512 / s->R : 1);
         if (l.walkers > l.parts) l.walkers = l.parts;
         l.spans = take(R * (size_t)l.spans_row * 8);
         l.floors = take(R * 8);
@@ -1440,8 +1504,8 @@ static DrawLayout draw_layout(const gsx_draw* s)
         if (l.cuts) {
             l.hist_n = take(R * l.walkers * kDrawBins * 4);
             l.hist_m = take(R * l.walkers * kDrawBins * 4);
-            l.row_n = take(R * kDrawBins * 4);
-            l.row_m = take(R * kDrawBins * 8);
+            if (l.walkers > kDrawFewWalkers) { l.row_n = take(R * kDrawBins * 4); l.row_m = take(R * kDrawBins * 8); }
+            l.near = take(R * sizeof(DrawNear));
             l.sums = take(R * l.walkers * 16);
             // room for every token of a few rows, a quarter of a million at least of each of many; what does not fit goes the exact way
             const int64_t most = (1ll << 24) / s->R;
@@ -1479,13 +1543,16 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
         draw_part_top_kernel<T><<<parts, dim3(kDrawPart), 0, stream>>>(a);
         if (l.cuts) {
             draw_part_hist_kernel<T><<<walkers, dim3(kDrawWalk), 0, stream>>>(a);
-            draw_sum_hist_kernel<<<dim3(kDrawBins / 64, (unsigned)a.R), dim3(1024), 0, stream>>>(a);
+            if (l.walkers > kDrawFewWalkers) draw_sum_hist_kernel<<<dim3(kDrawBins / 64, (unsigned)a.R), dim3(1024), 0, stream>>>(a);
+            draw_near_kernel<<<dim3((unsigned)a.R), dim3(1024), 0, stream>>>(a);
             draw_part_pass_kernel<T><<<walkers, dim3(kDrawWalk), 0, stream>>>(a);
             draw_floor_kernel<T><<<dim3((unsigned)a.R), dim3(1024), 0, stream>>>(a);
         }
         draw_part_mass_kernel<T><<<parts, dim3(kDrawPart), 0, stream>>>(a);
         const int64_t picks = ceil_div(a.S, kDrawPickers);
-        draw_part_pick_kernel<T><<<dim3((unsigned)(picks < 1024 ? picks : 1024), (unsigned)a.R), dim3(kDrawPickers), 0, stream>>>(a);
+        const size_t lds = ((size_t)l.parts * l.nodes + l.parts) * 8;
+        GSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(draw_part_pick_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, (kDrawMostNodes + kDrawMostParts) * 8));
+        draw_part_pick_kernel<T><<<dim3((unsigned)(picks < 512 ? picks : 512), (unsigned)a.R), dim3(kDrawPickers), lds, stream>>>(a);
         GSX_LAUNCH_CHECK();
         return GSX_OK;
     }
@@ -1527,12 +1594,13 @@ GSX_API int gsx_draw_indices(const gsx_draw* s, void* stream)
     a.logits = s->logits; a.row_stride = s->row_stride; a.R = s->R; a.V = s->V; a.S = s->S;
     a.uniforms = s->uniforms; a.uniforms_f64 = s->uniforms_f64 != 0;
     a.temperature = s->temperature; a.top_p = s->top_p; a.min_p = s->min_p; a.top_k = s->top_k;
+    a.inv_t = s->temperature > 0.0f ? 1.0 / (double)s->temperature : 1.0;
     a.temperatures = s->temperatures; a.top_ps = s->top_ps; a.min_ps = s->min_ps; a.top_ks = s->top_ks;
     a.indices = (long long*)s->indices; a.logprobs = s->logprobs;
     a.spans_row = l.spans_row;
-    a.part = (int)l.part; a.parts = l.parts; a.walkers = l.walkers; a.cuts = l.cuts; a.list_most = l.list_most;
+    a.part = (int)l.part; a.parts = l.parts; a.nodes = l.nodes; a.walkers = l.walkers; a.cuts = l.cuts; a.list_most = l.list_most;
     a.part_top = (float*)(ws + l.part_top); a.part_mass = (double*)(ws + l.part_mass);
-    a.hist_n = (uint32_t*)(ws + l.hist_n); a.hist_m = (float*)(ws + l.hist_m); a.row_n = (uint32_t*)(ws + l.row_n); a.row_m = (u64*)(ws + l.row_m);
+    a.hist_n = (uint32_t*)(ws + l.hist_n); a.hist_m = (float*)(ws + l.hist_m); a.row_n = (uint32_t*)(ws + l.row_n); a.row_m = (double*)(ws + l.row_m); a.near = (DrawNear*)(ws + l.near);
     a.sums = (double*)(ws + l.sums); a.list = (u64*)(ws + l.list); a.list_n = (uint32_t*)(ws + l.list_n);
     a.spans = (double*)(ws + l.spans); a.total = (double*)(ws + l.total); a.floors = (u64*)(ws + l.floors); a.tops = (float*)(ws + l.tops);
     switch (s->dtype) {
