@@ -44,11 +44,12 @@ struct DrawArgs {
     double* spans;                                  // [row][spans_row]: inclusive mass behind every 8 tokens
     double* total; float* tops; u64* floors;        // per row: kept mass (-1: none), top, lowest kept rank
     long long spans_row;
+    double* lines;                                  // every 16th of the spans again, side by side (rows in parts)
     // rows in parts: `part` groups of four places each, `parts` to a row; `walkers` workgroups per row where a workgroup takes several parts
-    int part, parts, nodes, walkers, cuts;
+    int part, parts, nodes, nodes_log, walkers, cuts;
     float* part_top; double* part_mass;             // [row][part]
-    uint32_t* hist_n; float* hist_m;                // [row][walker][bin]
-    uint32_t* row_n; double* row_m;                 // [row][bin]
+    u64* hist;                                      // [row][walker][bin]
+    uint32_t* row_n; u64* row_m;                    // [row][bin]
     struct DrawNear* near;                          // [row]
     double* sums;                                   // [row][walker][2]: 64-bit mass in front of the bracket, and the total's part
     u64* list; uint32_t* list_n; long long list_most;        // [row]: ranks of the tokens where the cuts may end
@@ -301,12 +302,11 @@ __device__ __forceinline__ float draw_max(float v, float* s_wave)
 }
 
 struct DrawHist { uint32_t count[kDrawBins]; u64 hi[kDrawBins], lo[kDrawBins]; };
-struct DrawNearHist { uint32_t count[kDrawBins]; u64 hi[kDrawBins]; };       // without the second limb
 struct DrawFine { uint32_t count[kDrawFine]; u64 hi[kDrawFine], lo[kDrawFine]; };
 struct DrawCand { u64 rank[kDrawCand], ranked[kDrawCand]; };
 
 // The first try at the cuts of a row: where the histogram's bounds let them end.  Bins: k in bin bk, p in one of lo .. hi.
-struct DrawNear { int bk, lo, hi; long long above_k; int before_bk, upto_hi; bool sure; };
+struct DrawNear { int bk, lo, hi; long long above_k, to_bk; int before_bk, upto_hi; bool sure; };       // above_k, to_bk: tokens in front of bin bk, and with it
 
 // What the threads of a workgroup share while a cut is found
 struct DrawCut {
@@ -505,38 +505,38 @@ __device__ u64 draw_cuts(DrawCut& c, const DrawHist& hist, DrawFine& fine, DrawC
 }
 
 // The cuts in one pass over the row behind the histogram, where few enough tokens lie where they may end.
-// The histogram counts tokens and adds up 32-bit weights in units of 2^-31: near enough to say in which bins the top p may end (a bracket, usually
+// The histogram counts tokens and adds up 32-bit weights: near enough to say in which bins the top p may end (a bracket, usually
 // of one bin), not where.  One pass then adds up the 64-bit weights of the tokens in front of the bracket, which are kept whatever
 // happens, and collects the tokens inside it and in the bin where the top k end; these few are ranked and decided exactly.  `false`: too
 // many of them, or the sums do not bear the bracket out; the longer way has no such limits.
 // mass(q, w): adds a weight that is kept for certain to tile q (all lanes of the wave call it, once per group).
-template <typename Hist>
-__device__ __forceinline__ void draw_near_add(Hist& h, float l, float top, float scale, float units, bool by_k, bool by_p)
+// A bin is one 64-bit word, one atomic per token: its tokens from bit 45 on, below the 32-bit weights in units of 2^-26 (2^19 tokens fit both).
+constexpr int kDrawCountBit = 45;
+constexpr int64_t kDrawMostInHist = 1 << 19;
+__device__ __forceinline__ void draw_near_add(u64* bins, float l, float top, float scale, float units)
 {
-    const int b = draw_bin(l, top, scale);
-    if (by_k) atomicAdd(&h.count[b], 1u);
-    if (by_p) {
-        const uint32_t m = (uint32_t)fmaf(__builtin_amdgcn_exp2f((l - top) * units), 0x1p31f, 0.5f);      // NaN: 0
-        if (m) atomicAdd(&h.hi[b], (u64)m);
-    }
+    const uint32_t m = (uint32_t)fmaf(__builtin_amdgcn_exp2f((l - top) * units), 0x1p26f, 0.5f);      // NaN: 0
+    atomicAdd(&bins[draw_bin(l, top, scale)], (1ull << kDrawCountBit) + m);
 }
+__device__ __forceinline__ uint32_t draw_near_count(u64 v) { return (uint32_t)(v >> kDrawCountBit); }
+__device__ __forceinline__ u64 draw_near_mass(u64 v) { return v & ((1ull << kDrawCountBit) - 1); }
 
 // where the cuts may end, from the histogram; c.near
-template <int NT, typename Hist>
-__device__ void draw_bracket(DrawCut& c, const Hist& h, const DrawRow& set, long long V, bool by_k, bool by_p)
+template <int NT, typename Count, typename Mass>
+__device__ void draw_bracket(DrawCut& c, const Count& count, const Mass& mass, const DrawRow& set, long long V, bool by_k, bool by_p)
 {
     constexpr int per = kDrawBins / NT;
     const int b0 = threadIdx.x * per;
-    if (threadIdx.x == 0) { c.near.bk = kDrawBins - 1; c.near.above_k = 0; c.near.lo = c.near.hi = kDrawBins - 1; }
+    if (threadIdx.x == 0) { c.near.bk = kDrawBins - 1; c.near.above_k = c.near.to_bk = 0; c.near.lo = c.near.hi = kDrawBins - 1; }
     uint32_t n = 0, all_n; u64 m = 0, all_m = 0, at_m = 0;
 #pragma unroll
-    for (int j = 0; j < per; j++) { if (by_k) n += h.count[b0 + j]; if (by_p) m += h.hi[b0 + j]; }
+    for (int j = 0; j < per; j++) { if (by_k) n += count(b0 + j); if (by_p) m += mass(b0 + j); }
     if (by_k) {
         long long at = draw_before<NT, uint32_t>(n, c.wave_n, &all_n);
 #pragma unroll
         for (int j = 0; j < per; j++) {
-            const long long next = at + h.count[b0 + j];
-            if (at < set.k && next >= set.k) { c.near.bk = b0 + j; c.near.above_k = at; }
+            const long long next = at + count(b0 + j);
+            if (at < set.k && next >= set.k) { c.near.bk = b0 + j; c.near.above_k = at; c.near.to_bk = next; }
             at = next;
         }
     }
@@ -550,7 +550,7 @@ __device__ void draw_bracket(DrawCut& c, const Hist& h, const DrawRow& set, long
             if (bk / per == (int)threadIdx.x) {
                 u64 a = at_m;
 #pragma unroll
-                for (int j = 0; j < per; j++) { if (b0 + j == bk) { c.lo = a; c.hi = a + h.hi[b0 + j]; } a += h.hi[b0 + j]; }
+                for (int j = 0; j < per; j++) { if (b0 + j == bk) { c.lo = a; c.hi = a + mass(b0 + j); } a += mass(b0 + j); }
             }
             __syncthreads();
             low = (double)c.lo; high = (double)c.hi;
@@ -561,7 +561,7 @@ __device__ void draw_bracket(DrawCut& c, const Hist& h, const DrawRow& set, long
         u64 at = at_m;
 #pragma unroll
         for (int j = 0; j < per; j++) {
-            const u64 next = at + h.hi[b0 + j];
+            const u64 next = at + mass(b0 + j);
             const int b = b0 + j;
             if (b <= bk) {
                 if ((b == 0 || (double)at < want_lo) && ((double)next >= want_lo || b == bk)) c.near.lo = b;
@@ -576,7 +576,7 @@ __device__ void draw_bracket(DrawCut& c, const Hist& h, const DrawRow& set, long
 // The collected tokens (c.slots of them) ranked, and the cuts among them.  above: the 64-bit mass of all tokens in front of bin near.lo; total: of
 // all in front of bin near.bk (of all, without a top k).
 template <int NT>
-__device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, float top, bool by_k, bool by_p, double above, double total)
+__device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, float top, bool by_k, bool by_p, double above, double total, bool all_listed = false)
 {
     const int most = NT < kDrawCand ? NT : kDrawCand, t = threadIdx.x;
     if (c.slots > (uint32_t)most) return false;
@@ -591,7 +591,7 @@ __device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, floa
     __syncthreads();
     int n = m;                                                       // candidates that the top k leaves
     if (by_k) {
-        const long long left = (long long)c.near.before_bk + set.k - c.near.above_k;
+        const long long left = all_listed ? set.k : (long long)c.near.before_bk + set.k - c.near.above_k;
         n = left < m ? (int)left : m;
     }
     double all;
@@ -604,7 +604,7 @@ __device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, floa
     }
     // the candidates of bin bk, where it lies behind the bracket, count for the total only
     double tail = 0.0, none = 0.0;
-    if (by_k) { tail = t >= c.near.before_bk ? w : 0.0; draw_sums<NT>(tail, none, c.wave_2); }
+    if (by_k) { tail = all_listed || t >= c.near.before_bk ? w : 0.0; draw_sums<NT>(tail, none, c.wave_2); }
     const double want = set.p * (total + tail);
     const int upto_n = c.near.upto_hi < n ? c.near.upto_hi : n;
     const bool in = t < upto_n && ((t == 0 && c.near.lo == 0) || above + before < want);
@@ -677,12 +677,12 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
     u64 floor_rank = 0;
     bool tiled = false;                                              // the tiles' masses are there already
     if (by_k || by_p) {
-        for (int b = tid; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; }
+        for (int b = tid; b < kDrawBins; b += NT) hist.hi[b] = 0;
         __syncthreads();
         const float units = (float)(set.inv_t * 0x1.71547652b82fep+0);
-        tokens([&](float l, int) { draw_near_add(hist, l, top, set.scale, units, by_k, by_p); });
+        tokens([&](float l, int) { draw_near_add(hist.hi, l, top, set.scale, units); });
         __syncthreads();
-        draw_bracket<NT>(c, hist, set, a.V, by_k, by_p);
+        draw_bracket<NT>(c, [&](int b) { return draw_near_count(hist.hi[b]); }, [&](int b) { return draw_near_mass(hist.hi[b]); }, set, a.V, by_k, by_p);
         const int bk = c.near.bk, lo = by_p ? c.near.lo : bk, hi = by_p ? c.near.hi : bk;
         if (tid == 0) c.slots = 0;
         if (PICK) for (int q = tid; q < kDrawWaveTiles; q += NT) { hist.hi[q] = 0; hist.lo[q] = 0; tile[q] = 0.0; }
@@ -940,14 +940,14 @@ __device__ __forceinline__ void draw_walk(const DrawArgs& a, const Places<T>& ro
 template <typename T>
 __global__ __launch_bounds__(kDrawWalk) void draw_part_hist_kernel(DrawArgs a)
 {
-    __shared__ DrawNearHist hist;
+    __shared__ u64 bins[kDrawBins];
     __shared__ float s_f[kDrawWalk / 64];
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
     float top = draw_row_top<kDrawWalk>(a, r, s_f);
     if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) return;
-    for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) { hist.count[b] = 0; hist.hi[b] = 0; }
+    for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) bins[b] = 0;
     __syncthreads();
     Places<T> row(a, r);
     top = row.finite_top(top);
@@ -955,27 +955,27 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_hist_kernel(DrawArgs a)
     draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], int) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (l[j] == l[j]) draw_near_add(hist, l[j], top, set.scale, units, by_k, by_p);
+            if (l[j] == l[j]) draw_near_add(bins, l[j], top, set.scale, units);
     });
     __syncthreads();
     const long long at = (r * a.walkers + blockIdx.x) * kDrawBins;
-    for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) { a.hist_n[at + b] = hist.count[b]; a.hist_m[at + b] = (float)hist.hi[b]; }
+    for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) a.hist[at + b] = bins[b];
 }
 
 // 64 bins to a workgroup, its waves share the walkers out
 __global__ __launch_bounds__(1024) void draw_sum_hist_kernel(DrawArgs a)
 {
     __shared__ uint32_t s_n[16][64];
-    __shared__ double s_m[16][64];
+    __shared__ u64 s_m[16][64];
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
     if (!set.valid || (set.k >= a.V && !(set.p < 1.0))) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bin = blockIdx.x * 64 + lane;
-    uint32_t n = 0; double m = 0.0;
+    uint32_t n = 0; u64 m = 0;
 #pragma unroll 8
     for (int w = wave; w < a.walkers; w += 16) {
-        n += a.hist_n[(r * a.walkers + w) * kDrawBins + bin];
-        m += (double)a.hist_m[(r * a.walkers + w) * kDrawBins + bin];
+        const u64 v = a.hist[(r * a.walkers + w) * kDrawBins + bin];
+        n += draw_near_count(v); m += draw_near_mass(v);
     }
     s_n[wave][lane] = n; s_m[wave][lane] = m;
     __syncthreads();
@@ -989,27 +989,30 @@ __global__ __launch_bounds__(1024) void draw_sum_hist_kernel(DrawArgs a)
 __global__ __launch_bounds__(1024) void draw_near_kernel(DrawArgs a)
 {
     constexpr int NT = 1024;
-    __shared__ DrawNearHist hist;
+    __shared__ uint32_t count[kDrawBins];
+    __shared__ u64 mass[kDrawBins];
     __shared__ DrawCut c;
     const long long r = blockIdx.x;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
     if (!set.valid || (!by_k && !by_p)) return;
     for (int b = threadIdx.x; b < kDrawBins; b += NT) {
-        uint32_t n = 0; double m = 0.0;
+        uint32_t n = 0; u64 m = 0;
         if (a.walkers <= kDrawFewWalkers) {
 #pragma unroll 4
             for (int w = 0; w < a.walkers; w++) {
-                n += a.hist_n[(r * a.walkers + w) * kDrawBins + b];
-                m += (double)a.hist_m[(r * a.walkers + w) * kDrawBins + b];
+                const u64 v = a.hist[(r * a.walkers + w) * kDrawBins + b];
+                n += draw_near_count(v); m += draw_near_mass(v);
             }
         } else { n = a.row_n[r * kDrawBins + b]; m = a.row_m[r * kDrawBins + b]; }
-        hist.count[b] = n; hist.hi[b] = (u64)m;
+        count[b] = n; mass[b] = m;
     }
     __syncthreads();
-    draw_bracket<NT>(c, hist, set, a.V, by_k, by_p);
+    draw_bracket<NT>(c, [&](int b) { return count[b]; }, [&](int b) { return mass[b]; }, set, a.V, by_k, by_p);
     if (threadIdx.x == 0) a.near[r] = c.near;
 }
+
+__device__ __forceinline__ bool draw_all_listed(const DrawNear& near, bool by_k) { return by_k && near.to_bk <= 1024; }
 
 template <typename T>
 __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
@@ -1027,8 +1030,10 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
     const DrawNear near = a.near[r];
     Places<T> row(a, r);
     top = row.finite_top(top);
-    const int bk = near.bk, lo = by_p ? near.lo : bk, hi = by_p ? near.hi : bk;
-    const int sums_to = by_p ? (by_k ? bk - 1 : kDrawBins - 1) : -1;
+    // a short list takes everything up to bin bk: the row ends in draw_floor_kernel then
+    const bool listed = draw_all_listed(near, by_k);
+    const int bk = near.bk, lo = listed ? 0 : by_p ? near.lo : bk, hi = listed ? bk : by_p ? near.hi : bk;
+    const int sums_to = listed || !by_p ? -1 : by_k ? bk - 1 : kDrawBins - 1;
     const int lane = threadIdx.x & 63;
     u64* stash = s_list[threadIdx.x >> 6];
     double above = 0.0, total = 0.0;
@@ -1106,17 +1111,59 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
     top = row.finite_top(top);
     if (tid == 0) c.near = a.near[r];
     __syncthreads();
-    // at most 256 walkers
+    // at most 512 walkers
     double above = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2] : 0.0, total = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2 + 1] : 0.0;
     draw_sums<NT>(above, total, c.wave_2);
     const long long n = a.list_n[r];
     const u64* list = a.list + r * a.list_most;
     bool done = false;
+    const bool all_listed = draw_all_listed(c.near, by_k);
+    if (all_listed) {                                                // the row's first to_bk tokens, of which the first k count
+        if (tid == 0) { c.near.lo = 0; c.near.hi = c.near.bk; }
+        above = total = 0.0;
+        __syncthreads();
+    }
     if (n <= NT) {
         if (tid < n) sh.cand.rank[tid] = list[tid];
         if (tid == 0) c.slots = (uint32_t)n;
         __syncthreads();
-        done = draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, above, total);
+        done = draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, above, total, all_listed);
+        if (all_listed) {                                            // and its draws, from the kept ones in index order
+            const u64 rank = tid < n ? sh.cand.rank[tid] : 0;
+            const float l = draw_rank_logit(rank);
+            const double lw = tid < n && rank >= c.floor_rank ? draw_weight(l, top, set.inv_t) : 0.0;
+            const bool in = lw > 0.0 && lw >= set.min_p;
+            const int i = draw_rank_index(rank);
+            __syncthreads();
+            if (tid == 0) c.slots = 0;
+            __syncthreads();
+            if (in) sh.cand.rank[atomicAdd(&c.slots, 1u)] = (u64)(0x7fffffff - i) << 32 | __builtin_bit_cast(uint32_t, l);
+            __syncthreads();
+            const int m = (int)c.slots;
+            draw_rank_cand<NT>(sh.cand, m);
+            const u64 mine = tid < m ? sh.cand.ranked[tid] : 0;
+            const float ml = __builtin_bit_cast(float, (uint32_t)mine);
+            double mass = 0.0;
+            const double w = tid < m ? draw_weight(ml, top, set.inv_t) : 0.0, at = draw_before<NT, double>(w, c.wave_d, &mass) + w;
+            double* upto = reinterpret_cast<double*>(sh.cand.rank);
+            __syncthreads();
+            if (tid < m) upto[tid] = at;
+            __syncthreads();
+            const double log_mass = draw_log(mass);
+            for (long long s = tid; s < a.S; s += NT) {
+                const double want = draw_uniform(a, r * a.S + s) * mass;
+                int lo = 0, hi = m - 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (upto[mid] > want) hi = mid; else lo = mid + 1;
+                }
+                const u64 v = sh.cand.ranked[lo];
+                a.indices[r * a.S + s] = 0x7fffffff - (int)(v >> 32);
+                if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(__builtin_bit_cast(float, (uint32_t)v), top, set.inv_t, log_mass);
+            }
+            if (tid == 0) a.floors[r] = ~0ull;                       // done
+            return;
+        }
     } else if (n <= a.list_most) {
         auto each = [&](auto f) {
             for (long long i = tid; i < n; i += NT) { const u64 rank = list[i]; f(draw_rank_logit(rank), rank); }
@@ -1177,6 +1224,7 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
     const long long r = blockIdx.y;
     const int tid = threadIdx.x;
     const DrawRow set = draw_row(a, r);
+    if (a.cuts && a.floors[r] == ~0ull) return;                      // the row has its draws already
     float top = draw_row_top<kDrawPart>(a, r, s_f);
     double carry = 0.0;
     if (set.valid && top > -__builtin_inff()) {
@@ -1205,6 +1253,7 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
             const int q = b / 2 + 2 * tid;
             if (2 * q < groups - g0) spans[q] = at;
             if (2 * (q + 1) < groups - g0) spans[q + 1] = at + w1;
+            if ((tid & 7) == 7) a.lines[(r * a.spans_row + g0 / 2 + q) / 16] = at + w1;
             carry += all;
         }
     }
@@ -1226,6 +1275,7 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
     const long long r = blockIdx.y;
     const int tid = threadIdx.x;
     const DrawRow set = draw_row(a, r);
+    if (a.cuts && a.floors[r] == ~0ull) return;
     Places<T> row(a, r);
     const float top = row.finite_top(draw_row_top<kDrawPickers>(a, r, s_f));
     double* s_part = s_sum;
@@ -1240,8 +1290,8 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
     __syncthreads();
     const int nodes = a.parts * a.nodes;
     for (int q = tid; q < nodes; q += kDrawPickers) {
-        const int p = q / a.nodes, last = (q + 1) * step - 1;        // the node's last span
-        s_node[q] = s_part[p] + (last < row_spans && (q + 1) % a.nodes ? spans[last] : a.part_mass[r * a.parts + p]);
+        const int p = q >> a.nodes_log, last = (q + 1) * step - 1;   // the node's last span
+        s_node[q] = s_part[p] + (a.nodes > 1 && last < row_spans && ((q + 1) & (a.nodes - 1)) ? a.lines[(r * a.spans_row + last) / 16] : a.part_mass[r * a.parts + p]);
     }
     __syncthreads();
     const DrawFloor floor(a.cuts ? a.floors[r] : 0);
@@ -1457,14 +1507,14 @@ static int draw_check(const gsx_draw* s)
     if (!s->top_ps && !(s->top_p > 0.0f)) return GSX_E_INVALID;
     if (!s->min_ps && !(s->min_p >= 0.0f && s->min_p <= 1.0f)) return GSX_E_INVALID;
     if (!s->top_ks && s->top_k < 0) return GSX_E_INVALID;
-    if (s->V > GSX_DRAW_MAX_V || s->R > 0x7fffffffll || s->S > (1ll << 38) || (s->R && s->S > (1ll << 38) / s->R)) return GSX_E_RANGE;
+    if (s->V > GSX_DRAW_MAX_V || s->R > 0x7fffffffll || (s->R > GSX_DRAW_MAX_LONG_ROWS && s->V > (int64_t)kDrawWaveTiles * 256 - 4) || s->S > (1ll << 38) || (s->R && s->S > (1ll << 38) / s->R)) return GSX_E_RANGE;
     return GSX_OK;
 }
 
 struct DrawLayout {
     enum Way { kShort, kRow, kRowSpans, kParts } way;
     long long spans_row, part, list_most; int parts, nodes, walkers, cuts;
-    size_t spans, total, floors, tops, part_top, part_mass, hist_n, hist_m, row_n, row_m, near, sums, list, list_n, bytes;
+    size_t spans, lines, total, floors, tops, part_top, part_mass, hist, row_n, row_m, near, sums, list, list_n, bytes;
 };
 
 // Which way, and its workspace.
@@ -1476,7 +1526,7 @@ static DrawLayout draw_layout(const gsx_draw* s)
     const size_t R = (size_t)s->R;
     l.cuts = s->top_ks || s->top_ps || s->temperatures || s->temperature == 0.0f || (s->top_k > 0 && s->top_k < s->V) || s->top_p < 1.0f;
     if (s->V <= kDrawShort) l.way = DrawLayout::kShort;
-    else if (s->V > kDrawLong && s->R <= kDrawFewRows) l.way = DrawLayout::kParts;
+    else if (s->V > kDrawLong && (s->R <= kDrawFewRows || s->V > (int64_t)kDrawWaveTiles * 256 - 4)) l.way = DrawLayout::kParts;
     else if (s->S <= kDrawInRow && s->V <= (int64_t)kDrawWaveTiles * 256 - 4) l.way = DrawLayout::kRow;
     else l.way = DrawLayout::kRowSpans;
     if (l.way == DrawLayout::kRowSpans) {
@@ -1496,19 +1546,21 @@ static DrawLayout draw_layout(const gsx_draw* s)
         if (s->S >= kDrawManyDraws)
             while (l.nodes < l.part / 32 && (int64_t)l.parts * l.nodes * 2 <= kDrawMostNodes) l.nodes *= 2;
         l.walkers = (int)(512 / s->R > 256 ? 256 : 512 / s->R > 1 ? 512 / s->R : 1);
+        if (l.walkers < ceil_div(s->V, kDrawMostInHist / 2)) l.walkers = (int)ceil_div(s->V, kDrawMostInHist / 2);
         if (l.walkers > l.parts) l.walkers = l.parts;
         l.spans = take(R * (size_t)l.spans_row * 8);
+        l.lines = take(R * (size_t)l.spans_row / 16 * 8);
         l.floors = take(R * 8);
         l.part_top = take(R * l.parts * 4);
         l.part_mass = take(R * l.parts * 8);
         if (l.cuts) {
-            l.hist_n = take(R * l.walkers * kDrawBins * 4);
-            l.hist_m = take(R * l.walkers * kDrawBins * 4);
+            l.hist = take(R * l.walkers * kDrawBins * 8);
             if (l.walkers > kDrawFewWalkers) { l.row_n = take(R * kDrawBins * 4); l.row_m = take(R * kDrawBins * 8); }
             l.near = take(R * sizeof(DrawNear));
             l.sums = take(R * l.walkers * 16);
             // room for every token of a few rows, a quarter of a million at least of each of many; what does not fit goes the exact way
-            const int64_t most = (1ll << 24) / s->R;
+            int64_t most = (1ll << 24) / s->R;
+            if (most < 4096) most = 4096;
             l.list_most = s->V < most ? s->V : most;
             l.list = take(R * (size_t)l.list_most * 8);
             l.list_n = take(R * 4);
@@ -1552,7 +1604,7 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
         const int64_t picks = ceil_div(a.S, kDrawPickers);
         const size_t lds = ((size_t)l.parts * l.nodes + l.parts) * 8;
         GSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(draw_part_pick_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, (kDrawMostNodes + kDrawMostParts) * 8));
-        draw_part_pick_kernel<T><<<dim3((unsigned)(picks < 512 ? picks : 512), (unsigned)a.R), dim3(kDrawPickers), lds, stream>>>(a);
+        draw_part_pick_kernel<T><<<dim3((unsigned)(picks < 256 ? picks : 256), (unsigned)a.R), dim3(kDrawPickers), lds, stream>>>(a);
         GSX_LAUNCH_CHECK();
         return GSX_OK;
     }
@@ -1598,9 +1650,9 @@ GSX_API int gsx_draw_indices(const gsx_draw* s, void* stream)
     a.temperatures = s->temperatures; a.top_ps = s->top_ps; a.min_ps = s->min_ps; a.top_ks = s->top_ks;
     a.indices = (long long*)s->indices; a.logprobs = s->logprobs;
     a.spans_row = l.spans_row;
-    a.part = (int)l.part; a.parts = l.parts; a.nodes = l.nodes; a.walkers = l.walkers; a.cuts = l.cuts; a.list_most = l.list_most;
+    a.part = (int)l.part; a.parts = l.parts; a.nodes = l.nodes; a.nodes_log = __builtin_ctz(l.nodes ? l.nodes : 1); a.lines = (double*)(ws + l.lines); a.walkers = l.walkers; a.cuts = l.cuts; a.list_most = l.list_most;
     a.part_top = (float*)(ws + l.part_top); a.part_mass = (double*)(ws + l.part_mass);
-    a.hist_n = (uint32_t*)(ws + l.hist_n); a.hist_m = (float*)(ws + l.hist_m); a.row_n = (uint32_t*)(ws + l.row_n); a.row_m = (double*)(ws + l.row_m); a.near = (DrawNear*)(ws + l.near);
+    a.hist = (u64*)(ws + l.hist); a.row_n = (uint32_t*)(ws + l.row_n); a.row_m = (u64*)(ws + l.row_m); a.near = (DrawNear*)(ws + l.near);
     a.sums = (double*)(ws + l.sums); a.list = (u64*)(ws + l.list); a.list_n = (uint32_t*)(ws + l.list_n);
     a.spans = (double*)(ws + l.spans); a.total = (double*)(ws + l.total); a.floors = (u64*)(ws + l.floors); a.tops = (float*)(ws + l.tops);
     switch (s->dtype) {

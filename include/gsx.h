@@ -467,8 +467,10 @@ int gsx_gated_step(int32_t dtype, int32_t form, int64_t n, float* state, const v
  * doubles where V is large.  indices[r][s] = the lowest index whose inclusive mass over the kept tokens, in index order, exceeds
  * u * (all kept mass); logprobs (nullable) = the log of its share of the kept mass.  A row with nothing left, or with settings of its own
  * out of range, gets -1 and -inf.  Masses are summed in 64 bits in a fixed order: the same bits every time.
- * ws: gsx_draw_workspace_bytes (0: the arguments are refused), 256-byte aligned. */
+ * ws: gsx_draw_workspace_bytes (0: the arguments are refused), 256-byte aligned.
+ * GSX_E_RANGE: more than GSX_DRAW_MAX_V tokens, or more than GSX_DRAW_MAX_LONG_ROWS rows of more than 524284. */
 #define GSX_DRAW_MAX_V (1ll << 27)
+#define GSX_DRAW_MAX_LONG_ROWS 65535
 typedef struct gsx_draw {
     int32_t dtype, uniforms_f64;
     int64_t R, V, S;
