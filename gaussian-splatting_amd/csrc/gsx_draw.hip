@@ -29,6 +29,7 @@ constexpr int kDrawWaveTiles = 2048;                // spans of 256 tokens whose
 constexpr int kDrawInRow = 64;                      // draws per row that its workgroup makes itself
 constexpr int64_t kDrawLong = 32768;                // rows longer than this are cut into parts ...
 constexpr int64_t kDrawFewRows = 128;               // ... where there are at most so many of them
+constexpr int kDrawExact = 512;                     // threads where a cut is searched for: all of the registers that it needs
 constexpr int kDrawIndexBits = 27;
 
 typedef unsigned long long u64;
@@ -43,11 +44,13 @@ struct DrawArgs {
     // workspace of rows whose draws are made by a kernel of their own
     double* spans;                                  // [row][spans_row]: inclusive mass behind every 8 tokens
     double* total; float* tops; u64* floors;        // per row: kept mass (-1: none), top, lowest kept rank
+    uint32_t* left;                                 // per row: its cuts are left to the exact way
     long long spans_row;
-    double* lines;                                  // every 16th of the spans again, side by side (rows in parts)
+    double* lines;                                  // every 8th of the spans again, side by side (rows in parts)
     // rows in parts: `part` groups of four places each, `parts` to a row; `walkers` workgroups per row where a workgroup takes several parts
     int part, parts, nodes, nodes_log, walkers, cuts;
-    float* part_top; double* part_mass;             // [row][part]
+    float* walk_top;                                // [row][walker]
+    double* part_mass;                              // [row][part]
     u64* hist;                                      // [row][walker][bin]
     uint32_t* row_n; u64* row_m;                    // [row][bin]
     struct DrawNear* near;                          // [row]
@@ -192,26 +195,37 @@ struct Places {
     }
     __device__ __forceinline__ float finite_top(float top) { infinite = top == __builtin_inff(); return infinite ? 0.0f : top; }
     __device__ __forceinline__ int groups() const { return (V + off + 3) >> 2; }
-    // places outside the row are NaN
-    __device__ __forceinline__ void load(int g, float (&l)[4]) const
+    // A group's load and what follows on it are apart, so that several loads are in flight: any use of one waits for it.  fetch() reads the nearest
+    // group that lies in the row whole (rows here have more than 512 tokens); finish() reads the two at the ends token by token.
+    __device__ __forceinline__ Four<T> fetch(int g) const
+    {
+        const int first = off ? 1 : 0, last = ((V + off) >> 2) - 1;
+        g = g < first ? first : g > last ? last : g;
+        return *(const Four<T>*)(base + 4ll * g);
+    }
+    // places outside the row, and groups from `end` on, are NaN
+    __device__ __forceinline__ void finish(int g, int end, const Four<T>& f, float (&l)[4]) const
     {
         const int i0 = 4 * g - off;
-        if (i0 >= 0 && i0 + 4 <= V) {
-            const Four<T> f = *(const Four<T>*)(base + 4ll * g);
 #pragma unroll
-            for (int j = 0; j < 4; j++) l[j] = draw_logit(f.v[j]);
-        } else {
+        for (int j = 0; j < 4; j++) l[j] = draw_logit(f.v[j]);
+        if (i0 < 0 || i0 + 4 > V || g >= end)
 #pragma unroll
-            for (int j = 0; j < 4; j++) l[j] = i0 + j >= 0 && i0 + j < V ? draw_logit(base[4ll * g + j]) : __builtin_nanf("");
-        }
+            for (int j = 0; j < 4; j++) l[j] = g < end && i0 + j >= 0 && i0 + j < V ? draw_logit(base[4ll * g + j]) : __builtin_nanf("");
         if (infinite)
 #pragma unroll
             for (int j = 0; j < 4; j++) l[j] = l[j] != l[j] ? l[j] : l[j] == __builtin_inff() ? 0.0f : -__builtin_inff();
     }
-    __device__ __forceinline__ void load_or_none(int g, int end, float (&l)[4]) const
+    __device__ __forceinline__ void load(int g, int end, float (&l)[4]) const { finish(g, end, fetch(g), l); }
+    // N groups, `step` apart
+    template <int N>
+    __device__ __forceinline__ void load_many(int g, int step, int end, float (&l)[N][4]) const
     {
-        l[0] = l[1] = l[2] = l[3] = __builtin_nanf("");
-        if (g < end) load(g, l);
+        Four<T> f[N];
+#pragma unroll
+        for (int q = 0; q < N; q++) f[q] = fetch(g + q * step);
+#pragma unroll
+        for (int q = 0; q < N; q++) finish(g + q * step, end, f[q], l[q]);
     }
 };
 
@@ -303,7 +317,7 @@ __device__ __forceinline__ float draw_max(float v, float* s_wave)
 
 struct DrawHist { uint32_t count[kDrawBins]; u64 hi[kDrawBins], lo[kDrawBins]; };
 struct DrawFine { uint32_t count[kDrawFine]; u64 hi[kDrawFine], lo[kDrawFine]; };
-struct DrawCand { u64 rank[kDrawCand], ranked[kDrawCand]; };
+struct alignas(16) DrawCand { u64 rank[kDrawCand + 2], ranked[kDrawCand]; };
 
 // The first try at the cuts of a row: where the histogram's bounds let them end.  Bins: k in bin bk, p in one of lo .. hi.
 struct DrawNear { int bk, lo, hi; long long above_k, to_bk; int before_bk, upto_hi; bool sure; };       // above_k, to_bk: tokens in front of bin bk, and with it
@@ -319,20 +333,32 @@ struct DrawCut {
     u64 wave_u[16]; uint32_t wave_n[16]; double wave_d[16], wave_2[16][2]; float wave_f[16];
 };
 
-// Ranks cand.rank[0 .. m), all different, sorted descending into cand.ranked (m at most NT).  A few by counting the larger ones (m broadcast reads
-// a thread); more by a bitonic network over the next power of two, a rank per thread, partners within a wave by shuffles: its 55
-// steps at 1024 take 8 us, the counting 12; at 200 the counting is the quicker.
+// Ranks cand.rank[0 .. m), all different, sorted descending into cand.ranked (m at most NT; cand.rank[m] is overwritten).  Up to half a workgroup of them by
+// counting the larger ones, several threads to a rank; more by a bitonic network over the next power of two, a rank per thread, partners within a
+// wave by shuffles.  The counting costs m^2 / 128 LDS reads of 16 bytes (512: 3 us), the network 55 steps at 1024 (8 us).
 template <int NT>
 __device__ __forceinline__ void draw_rank_cand(DrawCand& cand, int m)
 {
     const int t = threadIdx.x;
-    if (m <= 256) {
-        if (t < m) {
-            const u64 mine = cand.rank[t];
-            int place = 0;
-            for (int j = 0; j < m; j++) place += cand.rank[j] > mine;
-            cand.ranked[place] = mine;
+    if (2 * m <= NT) {
+        int share = 1;                                               // log2 of the threads per rank
+        while (share < 4 && m << (share + 1) <= NT) share++;
+        if (t == 0) cand.rank[m] = 0;                                // pairs are read
+        __syncthreads();
+        const int e = t >> share;
+        int place = 0;
+        const u64 mine = e < m ? cand.rank[e] : ~0ull;
+        const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(cand.rank);
+#pragma unroll 4
+        for (int j = t & ((1 << share) - 1); 2 * j < m; j += 1 << share) {
+            const ulonglong2 v = pairs[j];
+            place += (v.x > mine) + (v.y > mine);
         }
+        place += __builtin_bit_cast(int, draw_dpp<0xB1, 0xf>(__builtin_bit_cast(float, place)));
+        if (share > 1) place += __builtin_bit_cast(int, draw_dpp<0x4E, 0xf>(__builtin_bit_cast(float, place)));
+        if (share > 2) place += __builtin_bit_cast(int, draw_dpp<0x141, 0xf>(__builtin_bit_cast(float, place)));
+        if (share > 3) place += __builtin_bit_cast(int, draw_dpp<0x140, 0xf>(__builtin_bit_cast(float, place)));
+        if (e < m && (t & ((1 << share) - 1)) == 0) cand.ranked[place] = mine;
         __syncthreads();
         return;
     }
@@ -619,27 +645,152 @@ __device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, floa
     return true;
 }
 
+// The cuts of a row exactly from the first histogram on: for rows that the quicker way cannot decide (ties, brackets of too many tokens), in kernels
+// of their own, whose registers would cost the others.
+template <typename T, int NT>
+__device__ __forceinline__ u64 draw_exact_floor(const DrawArgs& a, const Places<T>& row, const DrawRow& set, float top, DrawCut& c, DrawHist& hist, DrawFine& fine, DrawCand& cand)
+{
+    const int groups = row.groups();
+    auto each = [&](auto f) {
+        for (int g = threadIdx.x; g < groups; g += NT) {
+            float l[4];
+            row.load(g, groups, l);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (l[j] == l[j]) f(l[j], draw_rank(l[j], 4 * g + j - row.off));
+        }
+    };
+    const bool by_k = set.k < a.V, by_p = set.p < 1.0;
+    for (int b = threadIdx.x; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; hist.lo[b] = 0; }
+    __syncthreads();
+    each([&](float l, u64) { draw_hist_add(hist, l, top, set.inv_t, set.scale, by_p); });
+    __syncthreads();
+    const u64 floor_rank = draw_cuts<NT>(c, hist, fine, cand, each, top, set, by_k, by_p);
+    __syncthreads();
+    return floor_rank;
+}
+
 // ---- one workgroup per row -----------------------------------------------------------------------------------------------------
+// Masses and draws of a row whose lowest kept rank is known; `tiled`: the tiles' masses lie in `tile` already.
+template <typename T, int NT, bool PICK>
+__device__ __forceinline__ void draw_row_draws(const DrawArgs& a, long long r, const Places<T>& row, const DrawRow& set, float raw_top, float top, u64 floor_rank, bool tiled, double* tile, double* s_wave)
+{
+    constexpr int kWaves = NT / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = row.groups();
+    auto all_groups = [&](auto f) {                                  // every thread of a wave, also where the wave reaches beyond the row
+        for (int g0 = 0; g0 < groups; g0 += 4 * NT) {
+            float l[4][4];
+            row.load_many(g0 + tid, NT, groups, l);
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                if (g0 + q * NT < groups) f(l[q], g0 + q * NT + tid);
+        }
+    };
+    const DrawFloor floor(floor_rank);
+    auto mass4 = [&](const float (&l)[4], int g, double (&w)[4]) {
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            w[j] = draw_kept(l[j], 4 * g + j - row.off, floor, top, set);
+            sum += w[j];
+        }
+        return sum;
+    };
+    if (PICK) {
+        // masses of 256 tokens, one wave's groups, in LDS; then the inclusive sums of these
+        if (!tiled)
+            all_groups([&](const float (&l)[4], int g) {
+                double w[4], sum = mass4(l, g, w);
+                sum = draw_wave_scan(sum);
+                if (lane == 63) tile[g >> 6] = sum;
+            });
+        __syncthreads();
+        const int tiles = (int)((groups + 63) >> 6), per = (tiles + NT - 1) / NT;
+        double sum = 0.0, total;
+        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) sum += tile[q];
+        double at = draw_before<NT, double>(sum, s_wave, &total);
+        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) { at += tile[q]; tile[q] = at; }
+        __syncthreads();
+        const double log_total = draw_log(total);
+        for (long long s = wave; s < a.S; s += kWaves) {             // a wave per draw
+            const double want = draw_uniform(a, r * a.S + s) * total;
+            int lo = 0, hi = tiles - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (tile[mid] > want) hi = mid; else lo = mid + 1;
+            }
+            // the first token in the tile that exceeds; where rounding leaves none, the last one with weight
+            for (int q = lo; q >= 0; q--) {
+                const int g = q * 64 + lane;
+                float l[4];
+                row.load(g, groups, l);
+                double w[4], incl = draw_wave_scan(mass4(l, g, w));
+                double run = (q ? tile[q - 1] : 0.0) + draw_wave_shift(incl);
+                int hit = -1, any = -1;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    run += w[j];
+                    if (w[j] > 0.0) { any = j; if (hit < 0 && run > want) hit = j; }
+                }
+                const u64 hits = __ballot(hit >= 0), some = __ballot(any >= 0);
+                if (!some) continue;
+                const int who = hits ? __ffsll((long long)hits) - 1 : 63 - __clzll((long long)some);
+                if (lane == who) {
+                    const int j = hits ? hit : any;
+                    float lj = l[0];
+#pragma unroll
+                    for (int e = 1; e < 4; e++) lj = e == j ? l[e] : lj;
+                    a.indices[r * a.S + s] = 4 * g + j - row.off;
+                    if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(lj, top, set.inv_t, log_total);
+                }
+                break;
+            }
+        }
+    } else {
+        // masses of 8 tokens, two neighbouring lanes', in the workspace; then the inclusive sums of these
+        double* spans = a.spans + r * a.spans_row;
+        const int n = (groups + 1) >> 1;
+        all_groups([&](const float (&l)[4], int g) {
+            double w[4], sum = mass4(l, g, w);
+            sum += draw_dpp<0xB1, 0xf>(sum);
+            if ((lane & 1) == 0 && (g >> 1) < n) spans[g >> 1] = sum;
+        });
+        __syncthreads();
+        double carry = 0.0;
+        for (int b = 0; b < n; b += 4 * NT) {
+            double v[4], sum = 0.0, all;
+#pragma unroll
+            for (int j = 0; j < 4; j++) { const int q = b + 4 * tid + j; v[j] = q < n ? spans[q] : 0.0; sum += v[j]; }
+            double at = carry + draw_before<NT, double>(sum, s_wave, &all);
+#pragma unroll
+            for (int j = 0; j < 4; j++) { const int q = b + 4 * tid + j; at += v[j]; if (q < n) spans[q] = at; }
+            carry += all;
+        }
+        if (tid == 0) { a.total[r] = carry; a.tops[r] = raw_top; a.floors[r] = floor_rank; }
+    }
+}
+
 template <typename T, int NT, bool PICK>
 __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
 {
-    __shared__ DrawHist hist;                                        // its limbs take the candidates' masses by tile later on
-    __shared__ union { DrawFine fine; DrawCand cand; } sh;
+    __shared__ struct { u64 hi[kDrawBins], lo[kDrawBins]; } hist;    // the bins, then the candidates' masses by tile
+    __shared__ struct { DrawCand cand; } sh;
     __shared__ double tile[PICK ? kDrawWaveTiles : 1];
     __shared__ DrawCut c;
-    constexpr int kWaves = NT / 64;
     const long long r = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (a.cuts && tid == 0) a.left[r] = 0;
     Places<T> row(a, r);
     const int groups = row.groups();
     const DrawRow set = draw_row(a, r);
     float top = -__builtin_inff();
-#pragma unroll 4
-    for (int g = tid; g < groups; g += NT) {
-        float l[4];
-        row.load(g, l);
+    for (int g = tid; g < groups; g += 4 * NT) {
+        float l[4][4];
+        row.load_many(g, NT, groups, l);
 #pragma unroll
-        for (int j = 0; j < 4; j++) top = fmaxf(top, l[j]);
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) top = fmaxf(top, l[q][j]);
     }
     top = draw_max<NT>(top, c.wave_f);
     if (!set.valid || top == -__builtin_inff()) {
@@ -652,24 +803,22 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
     top = row.finite_top(top);
     // f(l, i) for every token of the row, over all threads
     auto tokens = [&](auto f) {
-        for (int g0 = 0; g0 < groups; g0 += 2 * NT) {                // two groups' loads in flight
-            float l[2][4];
+        for (int g0 = 0; g0 < groups; g0 += 4 * NT) {
+            float l[4][4];
+            row.load_many(g0 + tid, NT, groups, l);
 #pragma unroll
-            for (int q = 0; q < 2; q++) row.load_or_none(g0 + q * NT + tid, groups, l[q]);
-#pragma unroll
-            for (int q = 0; q < 2; q++)
+            for (int q = 0; q < 4; q++)
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (l[q][j] == l[q][j]) f(l[q][j], 4 * (g0 + q * NT + tid) + j - row.off);
         }
     };
     auto all_groups = [&](auto f) {                                  // every thread of a wave, also where the wave reaches beyond the row
-        for (int g0 = 0; g0 < groups; g0 += 2 * NT) {
-            float l[2][4];
+        for (int g0 = 0; g0 < groups; g0 += 4 * NT) {
+            float l[4][4];
+            row.load_many(g0 + tid, NT, groups, l);
 #pragma unroll
-            for (int q = 0; q < 2; q++) row.load_or_none(g0 + q * NT + tid, groups, l[q]);
-#pragma unroll
-            for (int q = 0; q < 2; q++)
+            for (int q = 0; q < 4; q++)
                 if (g0 + q * NT < groups) f(l[q], g0 + q * NT + tid);
         }
     };
@@ -741,99 +890,31 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
                 for (int q = tid; q < tiles; q += NT) tile[q] += limbs(hist.hi[q], hist.lo[q]);
                 tiled = true;
             }
-        } else {
-            __syncthreads();
-            for (int b = tid; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; hist.lo[b] = 0; }
-            __syncthreads();
-            tokens([&](float l, int) { draw_hist_add(hist, l, top, set.inv_t, set.scale, by_p); });
-            __syncthreads();
-            auto each = [&](auto f) { tokens([&](float l, int i) { f(l, draw_rank(l, i)); }); };
-            floor_rank = draw_cuts<NT>(c, hist, sh.fine, sh.cand, each, top, set, by_k, by_p);
+        } else {                                                     // left to draw_exact_kernel
+            if (tid == 0) { a.left[r] = 1; a.tops[r] = raw_top; }
+            return;
         }
         __syncthreads();
     }
-    const DrawFloor floor(floor_rank);
-    auto mass4 = [&](const float (&l)[4], int g, double (&w)[4]) {
-        double sum = 0.0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            w[j] = draw_kept(l[j], 4 * g + j - row.off, floor, top, set);
-            sum += w[j];
-        }
-        return sum;
-    };
-    if (PICK) {
-        // masses of 256 tokens, one wave's groups, in LDS; then the inclusive sums of these
-        if (!tiled)
-            all_groups([&](const float (&l)[4], int g) {
-                double w[4], sum = mass4(l, g, w);
-                sum = draw_wave_scan(sum);
-                if (lane == 63) tile[g >> 6] = sum;
-            });
-        __syncthreads();
-        const int tiles = (int)((groups + 63) >> 6), per = (tiles + NT - 1) / NT;
-        double sum = 0.0, total;
-        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) sum += tile[q];
-        double at = draw_before<NT, double>(sum, c.wave_d, &total);
-        for (int q = tid * per; q < (tid + 1) * per && q < tiles; q++) { at += tile[q]; tile[q] = at; }
-        __syncthreads();
-        const double log_total = draw_log(total);
-        for (long long s = wave; s < a.S; s += kWaves) {             // a wave per draw
-            const double want = draw_uniform(a, r * a.S + s) * total;
-            int lo = 0, hi = tiles - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (tile[mid] > want) hi = mid; else lo = mid + 1;
-            }
-            // the first token in the tile that exceeds; where rounding leaves none, the last one with weight
-            for (int q = lo; q >= 0; q--) {
-                const int g = q * 64 + lane;
-                float l[4];
-                row.load_or_none(g, groups, l);
-                double w[4], incl = draw_wave_scan(mass4(l, g, w));
-                double run = (q ? tile[q - 1] : 0.0) + draw_wave_shift(incl);
-                int hit = -1, any = -1;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    run += w[j];
-                    if (w[j] > 0.0) { any = j; if (hit < 0 && run > want) hit = j; }
-                }
-                const u64 hits = __ballot(hit >= 0), some = __ballot(any >= 0);
-                if (!some) continue;
-                const int who = hits ? __ffsll((long long)hits) - 1 : 63 - __clzll((long long)some);
-                if (lane == who) {
-                    const int j = hits ? hit : any;
-                    float lj = l[0];
-#pragma unroll
-                    for (int e = 1; e < 4; e++) lj = e == j ? l[e] : lj;
-                    a.indices[r * a.S + s] = 4 * g + j - row.off;
-                    if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(lj, top, set.inv_t, log_total);
-                }
-                break;
-            }
-        }
-    } else {
-        // masses of 8 tokens, two neighbouring lanes', in the workspace; then the inclusive sums of these
-        double* spans = a.spans + r * a.spans_row;
-        const int n = (groups + 1) >> 1;
-        all_groups([&](const float (&l)[4], int g) {
-            double w[4], sum = mass4(l, g, w);
-            sum += draw_dpp<0xB1, 0xf>(sum);
-            if ((lane & 1) == 0 && (g >> 1) < n) spans[g >> 1] = sum;
-        });
-        __syncthreads();
-        double carry = 0.0;
-        for (int b = 0; b < n; b += 4 * NT) {
-            double v[4], sum = 0.0, all;
-#pragma unroll
-            for (int j = 0; j < 4; j++) { const int q = b + 4 * tid + j; v[j] = q < n ? spans[q] : 0.0; sum += v[j]; }
-            double at = carry + draw_before<NT, double>(sum, c.wave_d, &all);
-#pragma unroll
-            for (int j = 0; j < 4; j++) { const int q = b + 4 * tid + j; at += v[j]; if (q < n) spans[q] = at; }
-            carry += all;
-        }
-        if (tid == 0) { a.total[r] = carry; a.tops[r] = raw_top; a.floors[r] = floor_rank; }
-    }
+    draw_row_draws<T, NT, PICK>(a, r, row, set, raw_top, top, floor_rank, tiled, tile, c.wave_d);
+}
+
+// the rows that the kernel before left: their cuts exactly, from the first histogram on, then their draws
+template <typename T, bool PICK>
+__global__ __launch_bounds__(kDrawExact) void draw_exact_kernel(DrawArgs a)
+{
+    constexpr int NT = kDrawExact;
+    __shared__ DrawHist hist;
+    __shared__ union { DrawFine fine; DrawCand cand; } sh;
+    __shared__ double tile[PICK ? kDrawWaveTiles : 1];
+    __shared__ DrawCut c;
+    const long long r = blockIdx.x;
+    if (!a.left[r]) return;
+    Places<T> row(a, r);
+    const DrawRow set = draw_row(a, r);
+    const float raw_top = a.tops[r], top = row.finite_top(raw_top);
+    const u64 floor_rank = draw_exact_floor<T, NT>(a, row, set, top, c, hist, sh.fine, sh.cand);
+    draw_row_draws<T, NT, PICK>(a, r, row, set, raw_top, top, floor_rank, false, tile, c.wave_d);
 }
 
 // The draw within a span of 8 tokens whose masses begin at `run`: the first token that exceeds, or where rounding leaves none the last one with weight;
@@ -842,10 +923,12 @@ template <typename T>
 __device__ __forceinline__ int draw_in_span(const Places<T>& row, int span, double run, double want, const DrawFloor& floor, float top, const DrawRow& set, float& at_l)
 {
     int index = -1; bool found = false;
+    Four<T> f[2];
+    f[0] = row.fetch(2 * span); f[1] = row.fetch(2 * span + 1);
 #pragma unroll
     for (int e = 0; e < 2; e++) {
         float l[4];
-        row.load_or_none(2 * span + e, row.groups(), l);
+        row.finish(2 * span + e, row.groups(), f[e], l);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int i = 4 * (2 * span + e) + j - row.off;
@@ -888,35 +971,11 @@ constexpr int kDrawPart = 256;                      // threads of a part's workg
 constexpr int kDrawFewWalkers = 32;
 constexpr int kDrawWalk = 512;                      // threads of a workgroup that walks several parts
 
-template <typename T>
-__global__ __launch_bounds__(kDrawPart) void draw_part_top_kernel(DrawArgs a)
-{
-    __shared__ float s_f[kDrawPart / 64];
-    const long long r = blockIdx.y;
-    Places<T> row(a, r);
-    const int groups = row.groups(), g0 = blockIdx.x * a.part, g1 = g0 + a.part < groups ? g0 + a.part : groups;
-    float top = -__builtin_inff();
-    for (int g = g0 + threadIdx.x; g < g1; g += 4 * kDrawPart) {
-        float l[4][4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) row.load_or_none(g + q * kDrawPart, g1, l[q]);
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) top = fmaxf(top, l[q][j]);
-    }
-    top = draw_max<kDrawPart>(top, s_f);
-    if (threadIdx.x == 0) {
-        a.part_top[r * a.parts + blockIdx.x] = top;
-        if (blockIdx.x == 0 && a.cuts) a.list_n[r] = 0;
-    }
-}
-
 template <int NT>
 __device__ __forceinline__ float draw_row_top(const DrawArgs& a, long long r, float* s_f)
 {
     float top = -__builtin_inff();
-    for (int p = threadIdx.x; p < a.parts; p += NT) top = fmaxf(top, a.part_top[r * a.parts + p]);
+    for (int w = threadIdx.x; w < a.walkers; w += NT) top = fmaxf(top, a.walk_top[r * a.walkers + w]);
     return draw_max<NT>(top, s_f);
 }
 
@@ -929,11 +988,28 @@ __device__ __forceinline__ void draw_walk(const DrawArgs& a, const Places<T>& ro
     const int g0 = (int)blockIdx.x * each, g1 = g0 + each < groups ? g0 + each : groups;
     for (int g = g0; g < g1; g += 4 * NT) {
         float l[4][4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) row.load_or_none(g + q * NT + threadIdx.x, g1, l[q]);
+        row.load_many(g + (int)threadIdx.x, NT, g1, l);
 #pragma unroll
         for (int q = 0; q < 4; q++)
             if (g + q * NT < g1) f(l[q], g + q * NT + (int)threadIdx.x);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kDrawWalk) void draw_part_top_kernel(DrawArgs a)
+{
+    __shared__ float s_f[kDrawWalk / 64];
+    const long long r = blockIdx.y;
+    Places<T> row(a, r);
+    float top = -__builtin_inff();
+    draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = fmaxf(top, l[j]);
+    });
+    top = draw_max<kDrawWalk>(top, s_f);
+    if (threadIdx.x == 0) {
+        a.walk_top[r * a.walkers + blockIdx.x] = top;
+        if (blockIdx.x == 0 && a.cuts) a.list_n[r] = 0;
     }
 }
 
@@ -1012,7 +1088,7 @@ __global__ __launch_bounds__(1024) void draw_near_kernel(DrawArgs a)
     if (threadIdx.x == 0) a.near[r] = c.near;
 }
 
-__device__ __forceinline__ bool draw_all_listed(const DrawNear& near, bool by_k) { return by_k && near.to_bk <= 1024; }
+__device__ __forceinline__ bool draw_all_listed(const DrawNear& near, bool by_k) { return by_k && near.to_bk <= kDrawExact; }
 
 template <typename T>
 __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
@@ -1095,10 +1171,9 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
 
 // one workgroup per row: the cuts among the list's tokens, of any number; -> a.floors
 template <typename T>
-__global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
+__global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
 {
-    constexpr int NT = 1024;
-    __shared__ DrawHist hist;
+    constexpr int NT = kDrawExact;
     __shared__ union { DrawFine fine; DrawCand cand; } sh;
     __shared__ DrawCut c;
     const long long r = blockIdx.x;
@@ -1106,9 +1181,9 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
     float top = draw_row_top<NT>(a, r, c.wave_f);
-    if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) { if (tid == 0) a.floors[r] = 0; return; }
-    Places<T> row(a, r);
-    top = row.finite_top(top);
+    if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) { if (tid == 0) { a.floors[r] = 0; a.left[r] = 0; } return; }
+    const float raw_top = top;
+    top = top == __builtin_inff() ? 0.0f : top;                      // as Places has it
     if (tid == 0) c.near = a.near[r];
     __syncthreads();
     // at most 512 walkers
@@ -1161,7 +1236,7 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
                 a.indices[r * a.S + s] = 0x7fffffff - (int)(v >> 32);
                 if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(__builtin_bit_cast(float, (uint32_t)v), top, set.inv_t, log_mass);
             }
-            if (tid == 0) a.floors[r] = ~0ull;                       // done
+            if (tid == 0) { a.floors[r] = ~0ull; a.left[r] = 0; }    // done
             return;
         }
     } else if (n <= a.list_most) {
@@ -1191,27 +1266,23 @@ __global__ __launch_bounds__(1024) void draw_floor_kernel(DrawArgs a)
             } else done = false;
         }
     }
-    if (!done) {                                                     // over the whole row, exactly from the first histogram on
-        const int groups = row.groups();
-        auto each = [&](auto f) {
-            for (int g = tid; g < groups; g += NT) {
-                float l[4];
-                row.load(g, l);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (l[j] == l[j]) f(l[j], draw_rank(l[j], 4 * g + j - row.off));
-            }
-        };
-        __syncthreads();
-        for (int b = tid; b < kDrawBins; b += NT) { hist.count[b] = 0; hist.hi[b] = 0; hist.lo[b] = 0; }
-        __syncthreads();
-        each([&](float l, u64) { draw_hist_add(hist, l, top, set.inv_t, set.scale, by_p); });
-        __syncthreads();
-        const u64 floor_rank = draw_cuts<NT>(c, hist, sh.fine, sh.cand, each, top, set, by_k, by_p);
-        if (tid == 0) c.floor_rank = floor_rank;
-        __syncthreads();
-    }
-    if (tid == 0) a.floors[r] = c.floor_rank;
+    if (tid == 0) { a.floors[r] = c.floor_rank; a.left[r] = !done; a.tops[r] = raw_top; }
+}
+
+// the rows that the kernel before left
+template <typename T>
+__global__ __launch_bounds__(kDrawExact) void draw_exact_floor_kernel(DrawArgs a)
+{
+    __shared__ DrawHist hist;
+    __shared__ union { DrawFine fine; DrawCand cand; } sh;
+    __shared__ DrawCut c;
+    const long long r = blockIdx.x;
+    if (!a.left[r]) return;
+    Places<T> row(a, r);
+    const DrawRow set = draw_row(a, r);
+    const float top = row.finite_top(a.tops[r]);
+    const u64 floor_rank = draw_exact_floor<T, kDrawExact>(a, row, set, top, c, hist, sh.fine, sh.cand);
+    if (threadIdx.x == 0) a.floors[r] = floor_rank;
 }
 
 // the masses of a part: inclusive sums behind every 8 tokens, counted from the part's start
@@ -1235,8 +1306,7 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
         double* spans = a.spans + r * a.spans_row + g0 / 2;
         for (int b = 0; b < a.part && g0 + b < groups; b += 4 * kDrawPart) {
             float l[4][4];
-#pragma unroll
-            for (int q = 0; q < 4; q++) row.load_or_none(g0 + b + q * kDrawPart + tid, groups, l[q]);
+            row.load_many(g0 + b + tid, kDrawPart, groups, l);
             __syncthreads();                                         // span[] of the round before has been read
 #pragma unroll
             for (int q = 0; q < 4; q++) {
@@ -1253,7 +1323,7 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
             const int q = b / 2 + 2 * tid;
             if (2 * q < groups - g0) spans[q] = at;
             if (2 * (q + 1) < groups - g0) spans[q + 1] = at + w1;
-            if ((tid & 7) == 7) a.lines[(r * a.spans_row + g0 / 2 + q) / 16] = at + w1;
+            if ((tid & 3) == 3) a.lines[(r * a.spans_row + g0 / 2 + q) / 8] = at + w1;
             carry += all;
         }
     }
@@ -1261,7 +1331,7 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
 }
 
 // Draws of a row in parts.  For many draws what bounds them is the lines that a bisection touches (at 1 M tokens and draws: 7 lines of 128 B through each CU's 64 B a
-// cycle, 80 us); so the sums behind every 1 / nodes of a part lie in LDS, down to 16 spans, a line: a draw then reads one line of spans and one of tokens.
+// cycle, 80 us); so the sums behind every 1 / nodes of a part lie in LDS, down to 8 spans: a draw then reads one line of spans and one of tokens.
 constexpr int kDrawMostParts = 2048;
 constexpr int kDrawMostNodes = 16384;
 constexpr int64_t kDrawManyDraws = 1 << 15;         // from here on the nodes' 128 KB are worth their loading
@@ -1291,7 +1361,7 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
     const int nodes = a.parts * a.nodes;
     for (int q = tid; q < nodes; q += kDrawPickers) {
         const int p = q >> a.nodes_log, last = (q + 1) * step - 1;   // the node's last span
-        s_node[q] = s_part[p] + (a.nodes > 1 && last < row_spans && ((q + 1) & (a.nodes - 1)) ? a.lines[(r * a.spans_row + last) / 16] : a.part_mass[r * a.parts + p]);
+        s_node[q] = s_part[p] + (a.nodes > 1 && last < row_spans && ((q + 1) & (a.nodes - 1)) ? a.lines[(r * a.spans_row + last) / 8] : a.part_mass[r * a.parts + p]);
     }
     __syncthreads();
     const DrawFloor floor(a.cuts ? a.floors[r] : 0);
@@ -1307,13 +1377,17 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
         }
         int lo = n * step, hi = lo + step < row_spans ? lo + step - 1 : row_spans - 1;
         if (lo > hi) lo = hi;                                        // rounding beyond the last node with tokens
-        const double base = s_part[lo / part_spans];
+        const int p = lo / part_spans;
+        const double base = s_part[p];
+        double run = lo == p * part_spans ? 0.0 : lo & 7 ? spans[lo - 1] : a.lines[(r * a.spans_row + lo - 1) / 8];       // in front of span lo
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (base + spans[mid] > want) hi = mid; else lo = mid + 1;
+            const double v = spans[mid];
+            if (base + v > want) hi = mid; else { lo = mid + 1; run = v; }
         }
-        int index = -1; float at_l = 0.0f;
-        for (int q = lo; q >= 0 && index < 0; q--)
+        float at_l = 0.0f;
+        int index = draw_in_span(row, lo, base + run, want, floor, top, set, at_l);
+        for (int q = lo - 1; q >= 0 && index < 0; q--)                // nothing there: rounding; the last one in front with weight
             index = draw_in_span(row, q, s_part[q / part_spans] + (q % part_spans ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
         a.indices[t] = index;
         if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, log_total);
@@ -1514,7 +1588,7 @@ static int draw_check(const gsx_draw* s)
 struct DrawLayout {
     enum Way { kShort, kRow, kRowSpans, kParts } way;
     long long spans_row, part, list_most; int parts, nodes, walkers, cuts;
-    size_t spans, lines, total, floors, tops, part_top, part_mass, hist, row_n, row_m, near, sums, list, list_n, bytes;
+    size_t spans, lines, total, floors, tops, left, walk_top, part_mass, hist, row_n, row_m, near, sums, list, list_n, bytes;
 };
 
 // Which way, and its workspace.
@@ -1529,12 +1603,12 @@ static DrawLayout draw_layout(const gsx_draw* s)
     else if (s->V > kDrawLong && (s->R <= kDrawFewRows || s->V > (int64_t)kDrawWaveTiles * 256 - 4)) l.way = DrawLayout::kParts;
     else if (s->S <= kDrawInRow && s->V <= (int64_t)kDrawWaveTiles * 256 - 4) l.way = DrawLayout::kRow;
     else l.way = DrawLayout::kRowSpans;
+    if (l.way != DrawLayout::kShort) { l.tops = take(R * 4); l.left = take(R * 4); }
     if (l.way == DrawLayout::kRowSpans) {
         l.spans_row = (s->V + 3 + 7) / 8;
         l.spans = take(R * (size_t)l.spans_row * 8);
         l.total = take(R * 8);
         l.floors = take(R * 8);
-        l.tops = take(R * 4);
     }
     if (l.way == DrawLayout::kParts) {
         const int64_t groups = (s->V + 3 + 3) / 4;
@@ -1544,14 +1618,14 @@ static DrawLayout draw_layout(const gsx_draw* s)
         l.spans_row = (int64_t)l.parts * l.part / 2;
         l.nodes = 1;
         if (s->S >= kDrawManyDraws)
-            while (l.nodes < l.part / 32 && (int64_t)l.parts * l.nodes * 2 <= kDrawMostNodes) l.nodes *= 2;
+            while (l.nodes < l.part / 16 && (int64_t)l.parts * l.nodes * 2 <= kDrawMostNodes) l.nodes *= 2;
         l.walkers = (int)(512 / s->R > 256 ? 256 : 512 / s->R > 1 ? 512 / s->R : 1);
         if (l.walkers < ceil_div(s->V, kDrawMostInHist / 2)) l.walkers = (int)ceil_div(s->V, kDrawMostInHist / 2);
         if (l.walkers > l.parts) l.walkers = l.parts;
         l.spans = take(R * (size_t)l.spans_row * 8);
-        l.lines = take(R * (size_t)l.spans_row / 16 * 8);
+        l.lines = take(R * (size_t)l.spans_row / 8 * 8);
         l.floors = take(R * 8);
-        l.part_top = take(R * l.parts * 4);
+        l.walk_top = take(R * l.walkers * 4);
         l.part_mass = take(R * l.parts * 8);
         if (l.cuts) {
             l.hist = take(R * l.walkers * kDrawBins * 8);
@@ -1592,13 +1666,14 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
     }
     if (l.way == DrawLayout::kParts) {
         const dim3 parts((unsigned)l.parts, (unsigned)a.R), walkers((unsigned)l.walkers, (unsigned)a.R);
-        draw_part_top_kernel<T><<<parts, dim3(kDrawPart), 0, stream>>>(a);
+        draw_part_top_kernel<T><<<walkers, dim3(kDrawWalk), 0, stream>>>(a);
         if (l.cuts) {
             draw_part_hist_kernel<T><<<walkers, dim3(kDrawWalk), 0, stream>>>(a);
             if (l.walkers > kDrawFewWalkers) draw_sum_hist_kernel<<<dim3(kDrawBins / 64, (unsigned)a.R), dim3(1024), 0, stream>>>(a);
             draw_near_kernel<<<dim3((unsigned)a.R), dim3(1024), 0, stream>>>(a);
             draw_part_pass_kernel<T><<<walkers, dim3(kDrawWalk), 0, stream>>>(a);
-            draw_floor_kernel<T><<<dim3((unsigned)a.R), dim3(1024), 0, stream>>>(a);
+            draw_floor_kernel<T><<<dim3((unsigned)a.R), dim3(kDrawExact), 0, stream>>>(a);
+            draw_exact_floor_kernel<T><<<dim3((unsigned)a.R), dim3(kDrawExact), 0, stream>>>(a);
         }
         draw_part_mass_kernel<T><<<parts, dim3(kDrawPart), 0, stream>>>(a);
         const int64_t picks = ceil_div(a.S, kDrawPickers);
@@ -1613,10 +1688,11 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
     if (l.way == DrawLayout::kRow) {
         if (small) draw_row_kernel<T, 256, true><<<grid, dim3(256), 0, stream>>>(a);
         else draw_row_kernel<T, 1024, true><<<grid, dim3(1024), 0, stream>>>(a);
+        if (l.cuts) draw_exact_kernel<T, true><<<grid, dim3(kDrawExact), 0, stream>>>(a);
     } else {
         if (small) draw_row_kernel<T, 256, false><<<grid, dim3(256), 0, stream>>>(a);
         else draw_row_kernel<T, 1024, false><<<grid, dim3(1024), 0, stream>>>(a);
-        GSX_LAUNCH_CHECK();
+        if (l.cuts) draw_exact_kernel<T, false><<<grid, dim3(kDrawExact), 0, stream>>>(a);
         const int64_t n = a.R * a.S;
         draw_pick_kernel<T><<<dim3((unsigned)ceil_div(n, kBlock)), dim3(kBlock), 0, stream>>>(a, n);
     }
@@ -1651,10 +1727,10 @@ GSX_API int gsx_draw_indices(const gsx_draw* s, void* stream)
     a.indices = (long long*)s->indices; a.logprobs = s->logprobs;
     a.spans_row = l.spans_row;
     a.part = (int)l.part; a.parts = l.parts; a.nodes = l.nodes; a.nodes_log = __builtin_ctz(l.nodes ? l.nodes : 1); a.lines = (double*)(ws + l.lines); a.walkers = l.walkers; a.cuts = l.cuts; a.list_most = l.list_most;
-    a.part_top = (float*)(ws + l.part_top); a.part_mass = (double*)(ws + l.part_mass);
+    a.walk_top = (float*)(ws + l.walk_top); a.part_mass = (double*)(ws + l.part_mass);
     a.hist = (u64*)(ws + l.hist); a.row_n = (uint32_t*)(ws + l.row_n); a.row_m = (u64*)(ws + l.row_m); a.near = (DrawNear*)(ws + l.near);
     a.sums = (double*)(ws + l.sums); a.list = (u64*)(ws + l.list); a.list_n = (uint32_t*)(ws + l.list_n);
-    a.spans = (double*)(ws + l.spans); a.total = (double*)(ws + l.total); a.floors = (u64*)(ws + l.floors); a.tops = (float*)(ws + l.tops);
+    a.spans = (double*)(ws + l.spans); a.total = (double*)(ws + l.total); a.floors = (u64*)(ws + l.floors); a.tops = (float*)(ws + l.tops); a.left = (uint32_t*)(ws + l.left);
     switch (s->dtype) {
     case GSX_F32: return draw_run<float>(a, l, (hipStream_t)stream);
     case GSX_BF16: return draw_run<__bf16>(a, l, (hipStream_t)stream);
