@@ -15,6 +15,7 @@
 // A histogram's 2048 bins are 1/64 of a unit of (top - l) / T wide: the tokens spread over hundreds of bins (few collisions in LDS), and the bin where
 // a cut falls holds few enough tokens to be ranked in LDS.  Where it does not (ties, extreme temperatures), narrower histograms of the 59-bit rank
 // (key, index) follow until it does: every row ends, whatever its values.
+#include <type_traits>
 #include "gsx_common.h"
 
 namespace gsx {
@@ -23,7 +24,7 @@ constexpr int kDrawBins = 2048;                     // of the first histogram
 constexpr float kDrawBinsPerUnit = 64.0f;
 constexpr int kDrawFine = 512;                      // bins of the narrower ones
 constexpr int kDrawCand = 1024;                     // tokens that are ranked in LDS
-constexpr int kDrawSmall = 8192;                    // longest row that a quarter of a workgroup's threads takes
+constexpr int kDrawSmall = 16384;                   // longest row whose workgroup is of 512 threads and decides by itself in every case
 constexpr int kDrawShort = 512;                     // longest row of the short way
 constexpr int kDrawWaveTiles = 2048;                // spans of 256 tokens whose masses are kept in LDS: rows of up to 512 k tokens
 constexpr int kDrawInRow = 64;                      // draws per row that its workgroup makes itself
@@ -383,7 +384,7 @@ __device__ __forceinline__ void draw_rank_cand(DrawCand& cand, int m)
 
 // The first of bins 0 .. last where what lies in and in front of it reaches k tokens or `want` mass, or else `last`; c.above_* move up to it (masses only with_mass).
 template <int NT>
-__device__ void draw_find(DrawCut& c, const uint32_t* count, const u64* hi, const u64* lo, int bins, int last, bool by_mass, bool with_mass, long long k, double want)
+__device__ __forceinline__ void draw_find(DrawCut& c, const uint32_t* count, const u64* hi, const u64* lo, int bins, int last, bool by_mass, bool with_mass, long long k, double want)
 {
     const int per = bins > NT ? bins / NT : 1, b0 = threadIdx.x * per;
     uint32_t n = 0, all_n; u64 h = 0, l = 0, all;
@@ -413,7 +414,7 @@ __device__ void draw_find(DrawCut& c, const uint32_t* count, const u64* hi, cons
 // Finds where a cut ends among the tokens of bins bin0 .. bin1 (c.in_bin of them at most) whose rank is at least `floor_rank`.  each(f) calls f(l, rank)
 // for every token of the source, over all threads.
 template <int NT, typename Each>
-__device__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const Each& each, float top, double inv_t, float scale, int bin0, int bin1, u64 floor_rank, bool by_mass, bool with_mass, long long k, double want)
+__device__ __forceinline__ void draw_resolve(DrawCut& c, DrawFine& fine, DrawCand& cand, const Each& each, float top, double inv_t, float scale, int bin0, int bin1, u64 floor_rank, bool by_mass, bool with_mass, long long k, double want)
 {
     u64 lo = floor_rank, hi = ~0ull;
     uint32_t n = c.in_bin;
@@ -498,7 +499,7 @@ __device__ __forceinline__ void draw_hist_add(DrawHist& h, float l, float top, d
 
 // Both cuts from the first histogram; -> the lowest kept rank.
 template <int NT, typename Each>
-__device__ u64 draw_cuts(DrawCut& c, const DrawHist& hist, DrawFine& fine, DrawCand& cand, const Each& each, float top, const DrawRow& set, bool by_k, bool by_p)
+__device__ __forceinline__ u64 draw_cuts(DrawCut& c, const DrawHist& hist, DrawFine& fine, DrawCand& cand, const Each& each, float top, const DrawRow& set, bool by_k, bool by_p)
 {
     u64 floor_rank = 0;
     int last = kDrawBins - 1;
@@ -549,7 +550,7 @@ __device__ __forceinline__ u64 draw_near_mass(u64 v) { return v & ((1ull << kDra
 
 // where the cuts may end, from the histogram; c.near
 template <int NT, typename Count, typename Mass>
-__device__ void draw_bracket(DrawCut& c, const Count& count, const Mass& mass, const DrawRow& set, long long V, bool by_k, bool by_p)
+__device__ __forceinline__ void draw_bracket(DrawCut& c, const Count& count, const Mass& mass, const DrawRow& set, long long V, bool by_k, bool by_p)
 {
     constexpr int per = kDrawBins / NT;
     const int b0 = threadIdx.x * per;
@@ -602,7 +603,7 @@ __device__ void draw_bracket(DrawCut& c, const Count& count, const Mass& mass, c
 // The collected tokens (c.slots of them) ranked, and the cuts among them.  above: the 64-bit mass of all tokens in front of bin near.lo; total: of
 // all in front of bin near.bk (of all, without a top k).
 template <int NT>
-__device__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, float top, bool by_k, bool by_p, double above, double total, bool all_listed = false)
+__device__ __forceinline__ bool draw_decide(DrawCut& c, DrawCand& cand, const DrawRow& set, float top, bool by_k, bool by_p, double above, double total, bool all_listed = false)
 {
     const int most = NT < kDrawCand ? NT : kDrawCand, t = threadIdx.x;
     if (c.slots > (uint32_t)most) return false;
@@ -770,16 +771,19 @@ __device__ __forceinline__ void draw_row_draws(const DrawArgs& a, long long r, c
     }
 }
 
-template <typename T, int NT, bool PICK>
+template <typename T, int NT, bool PICK, bool EXACT>
 __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
 {
-    __shared__ struct { u64 hi[kDrawBins], lo[kDrawBins]; } hist;    // the bins, then the candidates' masses by tile
-    __shared__ struct { DrawCand cand; } sh;
+    struct Tiles { u64 hi[kDrawBins], lo[kDrawBins]; };
+    struct Cand { DrawCand cand; };
+    union Fine { DrawFine fine; DrawCand cand; };
+    __shared__ std::conditional_t<EXACT, DrawHist, Tiles> hist;      // the bins, then the candidates' masses by tile
+    __shared__ std::conditional_t<EXACT, Fine, Cand> sh;
     __shared__ double tile[PICK ? kDrawWaveTiles : 1];
     __shared__ DrawCut c;
     const long long r = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
-    if (a.cuts && tid == 0) a.left[r] = 0;
+    if (!EXACT && a.cuts && tid == 0) a.left[r] = 0;
     Places<T> row(a, r);
     const int groups = row.groups();
     const DrawRow set = draw_row(a, r);
@@ -890,6 +894,9 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
                 for (int q = tid; q < tiles; q += NT) tile[q] += limbs(hist.hi[q], hist.lo[q]);
                 tiled = true;
             }
+        } else if constexpr (EXACT) {
+            __syncthreads();
+            floor_rank = draw_exact_floor<T, NT>(a, row, set, top, c, hist, sh.fine, sh.cand);
         } else {                                                     // left to draw_exact_kernel
             if (tid == 0) { a.left[r] = 1; a.tops[r] = raw_top; }
             return;
@@ -1379,14 +1386,14 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
         if (lo > hi) lo = hi;                                        // rounding beyond the last node with tokens
         const int p = lo / part_spans;
         const double base = s_part[p];
-        double run = lo == p * part_spans ? 0.0 : lo & 7 ? spans[lo - 1] : a.lines[(r * a.spans_row + lo - 1) / 8];       // in front of span lo
+        double run = lo == p * part_spans ? base : lo == n * step ? s_node[n - 1] : base + spans[lo - 1];       // in front of span lo
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            const double v = spans[mid];
-            if (base + v > want) hi = mid; else { lo = mid + 1; run = v; }
+            const double v = base + spans[mid];
+            if (v > want) hi = mid; else { lo = mid + 1; run = v; }
         }
         float at_l = 0.0f;
-        int index = draw_in_span(row, lo, base + run, want, floor, top, set, at_l);
+        int index = draw_in_span(row, lo, run, want, floor, top, set, at_l);
         for (int q = lo - 1; q >= 0 && index < 0; q--)                // nothing there: rounding; the last one in front with weight
             index = draw_in_span(row, q, s_part[q / part_spans] + (q % part_spans ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
         a.indices[t] = index;
@@ -1684,15 +1691,16 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
         return GSX_OK;
     }
     const dim3 grid((unsigned)a.R);
-    const bool small = a.V <= kDrawSmall && a.R > 256;               // there are rows to fill the card
+    const bool small = a.V <= kDrawSmall;
     if (l.way == DrawLayout::kRow) {
-        if (small) draw_row_kernel<T, 256, true><<<grid, dim3(256), 0, stream>>>(a);
-        else draw_row_kernel<T, 1024, true><<<grid, dim3(1024), 0, stream>>>(a);
-        if (l.cuts) draw_exact_kernel<T, true><<<grid, dim3(kDrawExact), 0, stream>>>(a);
+        if (small) draw_row_kernel<T, kDrawExact, true, true><<<grid, dim3(kDrawExact), 0, stream>>>(a);
+        else draw_row_kernel<T, 1024, true, false><<<grid, dim3(1024), 0, stream>>>(a);
+        if (!small && l.cuts) draw_exact_kernel<T, true><<<grid, dim3(kDrawExact), 0, stream>>>(a);
     } else {
-        if (small) draw_row_kernel<T, 256, false><<<grid, dim3(256), 0, stream>>>(a);
-        else draw_row_kernel<T, 1024, false><<<grid, dim3(1024), 0, stream>>>(a);
-        if (l.cuts) draw_exact_kernel<T, false><<<grid, dim3(kDrawExact), 0, stream>>>(a);
+        if (small) draw_row_kernel<T, kDrawExact, false, true><<<grid, dim3(kDrawExact), 0, stream>>>(a);
+        else draw_row_kernel<T, 1024, false, false><<<grid, dim3(1024), 0, stream>>>(a);
+        if (!small && l.cuts) draw_exact_kernel<T, false><<<grid, dim3(kDrawExact), 0, stream>>>(a);
+        GSX_LAUNCH_CHECK();
         const int64_t n = a.R * a.S;
         draw_pick_kernel<T><<<dim3((unsigned)ceil_div(n, kBlock)), dim3(kBlock), 0, stream>>>(a, n);
     }
