@@ -43,11 +43,11 @@ struct DrawArgs {
     const float* temperatures; const float* top_ps; const float* min_ps; const int32_t* top_ks;
     long long* indices; float* logprobs;
     // workspace of rows whose draws are made by a kernel of their own
-    double* spans;                                  // [row][spans_row]: inclusive mass behind every 8 tokens
+    double* spans;                                  // [row][spans_row]: inclusive mass behind every group of four tokens
     double* total; float* tops; u64* floors;        // per row: kept mass (-1: none), top, lowest kept rank
     uint32_t* left;                                 // per row: its cuts are left to the exact way
     long long spans_row;
-    double* lines;                                  // every 8th of the spans again, side by side (rows in parts)
+    double* lines;                                  // every 16th of them again, side by side (rows in parts)
     // rows in parts: `part` groups of four places each, `parts` to a row; `walkers` workgroups per row where a workgroup takes several parts
     int part, parts, nodes, nodes_log, walkers, cuts;
     float* walk_top;                                // [row][walker]
@@ -748,13 +748,13 @@ __device__ __forceinline__ void draw_row_draws(const DrawArgs& a, long long r, c
             }
         }
     } else {
-        // masses of 8 tokens, two neighbouring lanes', in the workspace; then the inclusive sums of these
+        // the groups' masses in the workspace; then the inclusive sums of these
         double* spans = a.spans + r * a.spans_row;
-        const int n = (groups + 1) >> 1;
+        const int n = groups;
         all_groups([&](const float (&l)[4], int g) {
-            double w[4], sum = mass4(l, g, w);
-            sum += draw_dpp<0xB1, 0xf>(sum);
-            if ((lane & 1) == 0 && (g >> 1) < n) spans[g >> 1] = sum;
+            double w[4];
+            const double sum = mass4(l, g, w);
+            if (g < n) spans[g] = sum;
         });
         __syncthreads();
         double carry = 0.0;
@@ -924,30 +924,25 @@ __global__ __launch_bounds__(kDrawExact) void draw_exact_kernel(DrawArgs a)
     draw_row_draws<T, NT, PICK>(a, r, row, set, raw_top, top, floor_rank, false, tile, c.wave_d);
 }
 
-// The draw within a span of 8 tokens whose masses begin at `run`: the first token that exceeds, or where rounding leaves none the last one with weight;
-// -1: none has any.
+// The draw within a group whose masses begin at `run`: the first token that exceeds, or where rounding leaves none the last one with weight; -1: none
+// has any.
 template <typename T>
-__device__ __forceinline__ int draw_in_span(const Places<T>& row, int span, double run, double want, const DrawFloor& floor, float top, const DrawRow& set, float& at_l)
+__device__ __forceinline__ int draw_in_group(const Places<T>& row, int g, double run, double want, const DrawFloor& floor, float top, const DrawRow& set, float& at_l)
 {
     int index = -1; bool found = false;
-    Four<T> f[2];
-    f[0] = row.fetch(2 * span); f[1] = row.fetch(2 * span + 1);
+    float l[4];
+    row.load(g, row.groups(), l);
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-        float l[4];
-        row.finish(2 * span + e, row.groups(), f[e], l);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int i = 4 * (2 * span + e) + j - row.off;
-            const double w = draw_kept(l[j], i, floor, top, set);
-            run += w;
-            if (!found && w > 0.0) { index = i; at_l = l[j]; found = run > want; }
-        }
+    for (int j = 0; j < 4; j++) {
+        const int i = 4 * g + j - row.off;
+        const double w = draw_kept(l[j], i, floor, top, set);
+        run += w;
+        if (!found && w > 0.0) { index = i; at_l = l[j]; found = run > want; }
     }
     return index;
 }
 
-// a thread per draw: the span by bisection, then its tokens one after the other
+// a thread per draw: the group by bisection, then its tokens one after the other
 template <typename T>
 __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long n)
 {
@@ -962,13 +957,13 @@ __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long
     const DrawFloor floor(a.floors[r]);
     const double* spans = a.spans + r * a.spans_row;
     const double want = draw_uniform(a, t) * total;
-    int lo = 0, hi = ((row.groups() + 1) >> 1) - 1;
+    int lo = 0, hi = row.groups() - 1;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (spans[mid] > want) hi = mid; else lo = mid + 1;
     }
     int index = -1; float at_l = 0.0f;
-    for (int q = lo; q >= 0 && index < 0; q--) index = draw_in_span(row, q, q ? spans[q - 1] : 0.0, want, floor, top, set, at_l);
+    for (int q = lo; q >= 0 && index < 0; q--) index = draw_in_group(row, q, q ? spans[q - 1] : 0.0, want, floor, top, set, at_l);
     a.indices[t] = index;
     if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, draw_log(total));
 }
@@ -978,9 +973,11 @@ constexpr int kDrawPart = 256;                      // threads of a part's workg
 constexpr int kDrawFewWalkers = 32;
 constexpr int kDrawWalk = 512;                      // threads of a workgroup that walks several parts
 
+// the walkers' tops together; where a row may be cut, draw_near_kernel has left the result
 template <int NT>
-__device__ __forceinline__ float draw_row_top(const DrawArgs& a, long long r, float* s_f)
+__device__ __forceinline__ float draw_row_top(const DrawArgs& a, long long r, float* s_f, bool known)
 {
+    if (known) return a.tops[r];
     float top = -__builtin_inff();
     for (int w = threadIdx.x; w < a.walkers; w += NT) top = fmaxf(top, a.walk_top[r * a.walkers + w]);
     return draw_max<NT>(top, s_f);
@@ -1028,7 +1025,7 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_hist_kernel(DrawArgs a)
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
-    float top = draw_row_top<kDrawWalk>(a, r, s_f);
+    float top = draw_row_top<kDrawWalk>(a, r, s_f, false);
     if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) return;
     for (int b = threadIdx.x; b < kDrawBins; b += kDrawWalk) bins[b] = 0;
     __syncthreads();
@@ -1068,7 +1065,7 @@ __global__ __launch_bounds__(1024) void draw_sum_hist_kernel(DrawArgs a)
     }
 }
 
-// one workgroup per row: the bracket, from the walkers' histograms where they are few, else from their sum
+// one workgroup per row: its top, and the bracket from the walkers' histograms where they are few, else from their sum
 __global__ __launch_bounds__(1024) void draw_near_kernel(DrawArgs a)
 {
     constexpr int NT = 1024;
@@ -1078,6 +1075,8 @@ __global__ __launch_bounds__(1024) void draw_near_kernel(DrawArgs a)
     const long long r = blockIdx.x;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
+    const float top = draw_row_top<NT>(a, r, c.wave_f, false);
+    if (threadIdx.x == 0) a.tops[r] = top;
     if (!set.valid || (!by_k && !by_p)) return;
     for (int b = threadIdx.x; b < kDrawBins; b += NT) {
         uint32_t n = 0; u64 m = 0;
@@ -1108,7 +1107,7 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
     const long long r = blockIdx.y;
     const DrawRow set = draw_row(a, r);
     const bool by_k = set.k < a.V, by_p = set.p < 1.0;
-    float top = draw_row_top<kDrawWalk>(a, r, s_f);
+    float top = draw_row_top<kDrawWalk>(a, r, s_f, true);
     if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) return;
     const DrawNear near = a.near[r];
     Places<T> row(a, r);
@@ -1181,22 +1180,25 @@ template <typename T>
 __global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
 {
     constexpr int NT = kDrawExact;
+    __shared__ DrawHist hist;
     __shared__ union { DrawFine fine; DrawCand cand; } sh;
     __shared__ DrawCut c;
     const long long r = blockIdx.x;
     const int tid = threadIdx.x;
+    // all loads first: each is a round trip through the caches
     const DrawRow set = draw_row(a, r);
-    const bool by_k = set.k < a.V, by_p = set.p < 1.0;
-    float top = draw_row_top<NT>(a, r, c.wave_f);
-    if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) { if (tid == 0) { a.floors[r] = 0; a.left[r] = 0; } return; }
-    const float raw_top = top;
-    top = top == __builtin_inff() ? 0.0f : top;                      // as Places has it
-    if (tid == 0) c.near = a.near[r];
-    __syncthreads();
-    // at most 512 walkers
-    double above = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2] : 0.0, total = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2 + 1] : 0.0;
-    draw_sums<NT>(above, total, c.wave_2);
+    const DrawNear near = a.near[r];
+    float top = a.tops[r];
     const long long n = a.list_n[r];
+    const u64 first_rank = a.list[r * a.list_most + tid];            // list_most is 4096 at least
+    const double first_u = tid < a.S ? draw_uniform(a, r * a.S + tid) : 0.0;
+    double above = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2] : 0.0, total = tid < a.walkers ? a.sums[(r * a.walkers + tid) * 2 + 1] : 0.0;       // at most 512
+    const bool by_k = set.k < a.V, by_p = set.p < 1.0;
+    if (!set.valid || top == -__builtin_inff() || (!by_k && !by_p)) { if (tid == 0) a.floors[r] = 0; return; }
+    Places<T> row(a, r);
+    top = row.finite_top(top);
+    if (tid == 0) c.near = near;
+    draw_sums<NT>(above, total, c.wave_2);
     const u64* list = a.list + r * a.list_most;
     bool done = false;
     const bool all_listed = draw_all_listed(c.near, by_k);
@@ -1206,7 +1208,7 @@ __global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
         __syncthreads();
     }
     if (n <= NT) {
-        if (tid < n) sh.cand.rank[tid] = list[tid];
+        if (tid < n) sh.cand.rank[tid] = first_rank;
         if (tid == 0) c.slots = (uint32_t)n;
         __syncthreads();
         done = draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, above, total, all_listed);
@@ -1233,7 +1235,7 @@ __global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
             __syncthreads();
             const double log_mass = draw_log(mass);
             for (long long s = tid; s < a.S; s += NT) {
-                const double want = draw_uniform(a, r * a.S + s) * mass;
+                const double want = (s == tid ? first_u : draw_uniform(a, r * a.S + s)) * mass;
                 int lo = 0, hi = m - 1;
                 while (lo < hi) {
                     const int mid = (lo + hi) >> 1;
@@ -1243,7 +1245,7 @@ __global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
                 a.indices[r * a.S + s] = 0x7fffffff - (int)(v >> 32);
                 if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(__builtin_bit_cast(float, (uint32_t)v), top, set.inv_t, log_mass);
             }
-            if (tid == 0) { a.floors[r] = ~0ull; a.left[r] = 0; }    // done
+            if (tid == 0) a.floors[r] = ~0ull;                       // done
             return;
         }
     } else if (n <= a.list_most) {
@@ -1273,44 +1275,33 @@ __global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
             } else done = false;
         }
     }
-    if (tid == 0) { a.floors[r] = c.floor_rank; a.left[r] = !done; a.tops[r] = raw_top; }
+    u64 floor_rank = c.floor_rank;
+    if (!done) {
+        __syncthreads();
+        floor_rank = draw_exact_floor<T, NT>(a, row, set, top, c, hist, sh.fine, sh.cand);
+    }
+    if (tid == 0) a.floors[r] = floor_rank;
 }
 
-// the rows that the kernel before left
+// the masses of a part: inclusive sums behind every group, counted from the part's start
 template <typename T>
-__global__ __launch_bounds__(kDrawExact) void draw_exact_floor_kernel(DrawArgs a)
-{
-    __shared__ DrawHist hist;
-    __shared__ union { DrawFine fine; DrawCand cand; } sh;
-    __shared__ DrawCut c;
-    const long long r = blockIdx.x;
-    if (!a.left[r]) return;
-    Places<T> row(a, r);
-    const DrawRow set = draw_row(a, r);
-    const float top = row.finite_top(a.tops[r]);
-    const u64 floor_rank = draw_exact_floor<T, kDrawExact>(a, row, set, top, c, hist, sh.fine, sh.cand);
-    if (threadIdx.x == 0) a.floors[r] = floor_rank;
-}
-
-// the masses of a part: inclusive sums behind every 8 tokens, counted from the part's start
-template <typename T>
-__global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
+__global__ __launch_bounds__(kDrawPart, 6) void draw_part_mass_kernel(DrawArgs a)
 {
     __shared__ double s_d[kDrawPart / 64];
     __shared__ float s_f[kDrawPart / 64];
-    __shared__ double span[2 * kDrawPart];
+    __shared__ double span[4 * kDrawPart];
     const long long r = blockIdx.y;
     const int tid = threadIdx.x;
     const DrawRow set = draw_row(a, r);
     if (a.cuts && a.floors[r] == ~0ull) return;                      // the row has its draws already
-    float top = draw_row_top<kDrawPart>(a, r, s_f);
+    float top = draw_row_top<kDrawPart>(a, r, s_f, a.cuts);
     double carry = 0.0;
     if (set.valid && top > -__builtin_inff()) {
         Places<T> row(a, r);
         top = row.finite_top(top);
         const DrawFloor floor(a.cuts ? a.floors[r] : 0);
         const int groups = row.groups(), g0 = blockIdx.x * a.part;
-        double* spans = a.spans + r * a.spans_row + g0 / 2;
+        double* spans = a.spans + r * a.spans_row + g0;
         for (int b = 0; b < a.part && g0 + b < groups; b += 4 * kDrawPart) {
             float l[4][4];
             row.load_many(g0 + b + tid, kDrawPart, groups, l);
@@ -1320,17 +1311,19 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
                 double sum = 0.0;
 #pragma unroll
                 for (int j = 0; j < 4; j++) sum += draw_kept(l[q][j], 4 * (g0 + b + q * kDrawPart + tid) + j - row.off, floor, top, set);
-                sum += draw_dpp<0xB1, 0xf>(sum);
-                if ((tid & 1) == 0) span[(q * kDrawPart + tid) >> 1] = sum;
+                span[q * kDrawPart + tid] = sum;
+                __builtin_amdgcn_sched_barrier(0);                   // one group's exps at a time: 80 registers, six waves a SIMD
             }
             __syncthreads();
-            double all;
-            const double w0 = span[2 * tid], w1 = span[2 * tid + 1];
-            const double at = carry + draw_before<kDrawPart, double>(w0 + w1, s_d, &all) + w0;
-            const int q = b / 2 + 2 * tid;
-            if (2 * q < groups - g0) spans[q] = at;
-            if (2 * (q + 1) < groups - g0) spans[q + 1] = at + w1;
-            if ((tid & 3) == 3) a.lines[(r * a.spans_row + g0 / 2 + q) / 8] = at + w1;
+            double w[4], all;
+#pragma unroll
+            for (int q = 0; q < 4; q++) w[q] = span[4 * tid + q];
+            w[1] += w[0]; w[2] += w[1]; w[3] += w[2];
+            const double at = carry + draw_before<kDrawPart, double>(w[3], s_d, &all);
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                if (b + 4 * tid + q < groups - g0) spans[b + 4 * tid + q] = at + w[q];
+            if ((tid & 3) == 3) a.lines[(r * a.spans_row + g0 + b) / 16 + tid / 4] = at + w[3];
             carry += all;
         }
     }
@@ -1338,7 +1331,7 @@ __global__ __launch_bounds__(kDrawPart) void draw_part_mass_kernel(DrawArgs a)
 }
 
 // Draws of a row in parts.  For many draws what bounds them is the lines that a bisection touches (at 1 M tokens and draws: 7 lines of 128 B through each CU's 64 B a
-// cycle, 80 us); so the sums behind every 1 / nodes of a part lie in LDS, down to 8 spans: a draw then reads one line of spans and one of tokens.
+// cycle, 80 us); so the sums behind every 1 / nodes of a part lie in LDS, down to 16 groups: a draw then reads one line of sums and one of tokens.
 constexpr int kDrawMostParts = 2048;
 constexpr int kDrawMostNodes = 16384;
 constexpr int64_t kDrawManyDraws = 1 << 15;         // from here on the nodes' 128 KB are worth their loading
@@ -1354,10 +1347,10 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
     const DrawRow set = draw_row(a, r);
     if (a.cuts && a.floors[r] == ~0ull) return;
     Places<T> row(a, r);
-    const float top = row.finite_top(draw_row_top<kDrawPickers>(a, r, s_f));
+    const float top = row.finite_top(draw_row_top<kDrawPickers>(a, r, s_f, a.cuts));
     double* s_part = s_sum;
     double* s_node = s_sum + a.parts;
-    const int part_spans = a.part / 2, row_spans = (row.groups() + 1) / 2, step = part_spans / a.nodes;
+    const int part_log = __builtin_ctz(a.part), groups = row.groups(), step = a.part >> a.nodes_log;
     const double* spans = a.spans + r * a.spans_row;
     const int per = (a.parts + kDrawPickers - 1) / kDrawPickers;
     double sum = 0.0, total;
@@ -1367,8 +1360,8 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
     __syncthreads();
     const int nodes = a.parts * a.nodes;
     for (int q = tid; q < nodes; q += kDrawPickers) {
-        const int p = q >> a.nodes_log, last = (q + 1) * step - 1;   // the node's last span
-        s_node[q] = s_part[p] + (a.nodes > 1 && last < row_spans && ((q + 1) & (a.nodes - 1)) ? a.lines[(r * a.spans_row + last) / 8] : a.part_mass[r * a.parts + p]);
+        const int p = q >> a.nodes_log, last = (q + 1) * step - 1;   // the node's last group
+        s_node[q] = s_part[p] + (last < groups && ((q + 1) & (a.nodes - 1)) ? a.lines[(r * a.spans_row + last) / 16] : a.part_mass[r * a.parts + p]);
     }
     __syncthreads();
     const DrawFloor floor(a.cuts ? a.floors[r] : 0);
@@ -1382,20 +1375,20 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
             const int mid = (n + n1) >> 1;
             if (s_node[mid] > want) n1 = mid; else n = mid + 1;
         }
-        int lo = n * step, hi = lo + step < row_spans ? lo + step - 1 : row_spans - 1;
+        int lo = n * step, hi = lo + step < groups ? lo + step - 1 : groups - 1;
         if (lo > hi) lo = hi;                                        // rounding beyond the last node with tokens
-        const int p = lo / part_spans;
+        const int p = lo >> part_log;
         const double base = s_part[p];
-        double run = lo == p * part_spans ? base : lo == n * step ? s_node[n - 1] : base + spans[lo - 1];       // in front of span lo
+        double run = lo == p << part_log ? base : lo == n * step ? s_node[n - 1] : base + spans[lo - 1];       // in front of group lo
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             const double v = base + spans[mid];
             if (v > want) hi = mid; else { lo = mid + 1; run = v; }
         }
         float at_l = 0.0f;
-        int index = draw_in_span(row, lo, run, want, floor, top, set, at_l);
-        for (int q = lo - 1; q >= 0 && index < 0; q--)                // nothing there: rounding; the last one in front with weight
-            index = draw_in_span(row, q, s_part[q / part_spans] + (q % part_spans ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
+        int index = draw_in_group(row, lo, run, want, floor, top, set, at_l);
+        for (int q = lo - 1; q >= 0 && index < 0; q--)               // nothing there: rounding; the last one in front with weight
+            index = draw_in_group(row, q, s_part[q >> part_log] + (q & (a.part - 1) ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
         a.indices[t] = index;
         if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, log_total);
     }
@@ -1556,8 +1549,16 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
     __builtin_amdgcn_wave_barrier();
     const int rows = a.R - r0 < kRows ? (int)(a.R - r0) : kRows;
     if (rows <= 0) return;
+    const float per_row = 1.0f / (float)a.S;
     for (long long q = lane; q < (long long)rows * a.S; q += 64) {
-        const int y = kRows == 1 ? 0 : (int)(q / a.S);
+        int y = 0;                                                   // q / S: a 64-bit division would cost as much as four exps
+        if (kRows > 1) {
+            if (a.S < (1 << 18)) {
+                y = (int)((float)(int)q * per_row);
+                const int left = (int)q - y * (int)a.S;
+                y += left < 0 ? -1 : left >= (int)a.S ? 1 : 0;
+            } else y = (int)(q / a.S);
+        }
         const double all = s_total[wave][y];
         const double* mass = &s_mass[wave][y * W * E];
         long long index = -1;
@@ -1610,9 +1611,9 @@ static DrawLayout draw_layout(const gsx_draw* s)
     else if (s->V > kDrawLong && (s->R <= kDrawFewRows || s->V > (int64_t)kDrawWaveTiles * 256 - 4)) l.way = DrawLayout::kParts;
     else if (s->S <= kDrawInRow && s->V <= (int64_t)kDrawWaveTiles * 256 - 4) l.way = DrawLayout::kRow;
     else l.way = DrawLayout::kRowSpans;
-    if (l.way != DrawLayout::kShort) { l.tops = take(R * 4); l.left = take(R * 4); }
+    if (l.way != DrawLayout::kShort) { l.tops = take(R * 4); l.left = take(R * 4); }       // left: one launch's word to the next
     if (l.way == DrawLayout::kRowSpans) {
-        l.spans_row = (s->V + 3 + 7) / 8;
+        l.spans_row = (s->V + 3 + 3) / 4;
         l.spans = take(R * (size_t)l.spans_row * 8);
         l.total = take(R * 8);
         l.floors = take(R * 8);
@@ -1622,15 +1623,15 @@ static DrawLayout draw_layout(const gsx_draw* s)
         l.part = 4 * kDrawPart;
         while (ceil_div(groups, l.part) > kDrawMostParts) l.part *= 2;
         l.parts = (int)ceil_div(groups, l.part);
-        l.spans_row = (int64_t)l.parts * l.part / 2;
+        l.spans_row = (int64_t)l.parts * l.part;
         l.nodes = 1;
         if (s->S >= kDrawManyDraws)
             while (l.nodes < l.part / 16 && (int64_t)l.parts * l.nodes * 2 <= kDrawMostNodes) l.nodes *= 2;
-        l.walkers = (int)(512 / s->R > 256 ? 256 : 512 / s->R > 1 ? 512 / s->R : 1);
+        l.walkers = (int)(512 / s->R > 1 ? 512 / s->R : 1);
         if (l.walkers < ceil_div(s->V, kDrawMostInHist / 2)) l.walkers = (int)ceil_div(s->V, kDrawMostInHist / 2);
         if (l.walkers > l.parts) l.walkers = l.parts;
         l.spans = take(R * (size_t)l.spans_row * 8);
-        l.lines = take(R * (size_t)l.spans_row / 8 * 8);
+        l.lines = take(R * (size_t)l.spans_row / 16 * 8);
         l.floors = take(R * 8);
         l.walk_top = take(R * l.walkers * 4);
         l.part_mass = take(R * l.parts * 8);
@@ -1680,7 +1681,6 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
             draw_near_kernel<<<dim3((unsigned)a.R), dim3(1024), 0, stream>>>(a);
             draw_part_pass_kernel<T><<<walkers, dim3(kDrawWalk), 0, stream>>>(a);
             draw_floor_kernel<T><<<dim3((unsigned)a.R), dim3(kDrawExact), 0, stream>>>(a);
-            draw_exact_floor_kernel<T><<<dim3((unsigned)a.R), dim3(kDrawExact), 0, stream>>>(a);
         }
         draw_part_mass_kernel<T><<<parts, dim3(kDrawPart), 0, stream>>>(a);
         const int64_t picks = ceil_div(a.S, kDrawPickers);
