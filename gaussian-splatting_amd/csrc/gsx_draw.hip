@@ -318,7 +318,7 @@ __device__ __forceinline__ float draw_max(float v, float* s_wave)
 
 struct DrawHist { uint32_t count[kDrawBins]; u64 hi[kDrawBins], lo[kDrawBins]; };
 struct DrawFine { uint32_t count[kDrawFine]; u64 hi[kDrawFine], lo[kDrawFine]; };
-struct alignas(16) DrawCand { u64 rank[kDrawCand + 2], ranked[kDrawCand]; };
+struct DrawCand { u64 rank[kDrawCand], ranked[kDrawCand]; };
 
 // The first try at the cuts of a row: where the histogram's bounds let them end.  Bins: k in bin bk, p in one of lo .. hi.
 struct DrawNear { int bk, lo, hi; long long above_k, to_bk; int before_bk, upto_hi; bool sure; };       // above_k, to_bk: tokens in front of bin bk, and with it
@@ -334,51 +334,67 @@ struct DrawCut {
     u64 wave_u[16]; uint32_t wave_n[16]; double wave_d[16], wave_2[16][2]; float wave_f[16];
 };
 
-// Ranks cand.rank[0 .. m), all different, sorted descending into cand.ranked (m at most NT; cand.rank[m] is overwritten).  Up to half a workgroup of them by
-// counting the larger ones, several threads to a rank; more by a bitonic network over the next power of two, a rank per thread, partners within a
-// wave by shuffles.  The counting costs m^2 / 128 LDS reads of 16 bytes (512: 3 us), the network 55 steps at 1024 (8 us).
+// the value of the lane whose number differs in bit D
+template <int D>
+__device__ __forceinline__ u64 draw_lane_xor(u64 v)
+{
+    if constexpr (D == 1) return draw_dpp<0xB1, 0xf>(v);
+    else if constexpr (D == 2) return draw_dpp<0x4E, 0xf>(v);
+    else if constexpr (D == 4) return draw_dpp<0x1B, 0xf>(draw_dpp<0x141, 0xf>(v));      // the half row mirrored, then each quad
+    else if constexpr (D == 8) return draw_dpp<0x141, 0xf>(draw_dpp<0x140, 0xf>(v));     // the row mirrored, then each half
+    else return __shfl_xor(v, D, 64);
+}
+template <int SIZE, int D>
+__device__ __forceinline__ u64 draw_sort_step(u64 v, int lane)
+{
+    const u64 o = draw_lane_xor<D>(v);
+    const bool larger = ((lane & D) == 0) == ((lane & SIZE) == 0);   // this lane keeps the larger one
+    v = (o > v) == larger ? o : v;
+    if constexpr (D > 1) return draw_sort_step<SIZE, D / 2>(v, lane);
+    else return v;
+}
+// descending over the wave: a bitonic network of 21 steps
+__device__ __forceinline__ u64 draw_sort_wave(u64 v, int lane)
+{
+    v = draw_sort_step<2, 1>(v, lane);
+    v = draw_sort_step<4, 2>(v, lane);
+    v = draw_sort_step<8, 4>(v, lane);
+    v = draw_sort_step<16, 8>(v, lane);
+    v = draw_sort_step<32, 16>(v, lane);
+    return draw_sort_step<64, 32>(v, lane);
+}
+
+// Ranks cand.rank[0 .. m), all different, sorted descending into cand.ranked (m at most NT): each wave sorts its 64 in registers, then every one looks its
+// place up in the other waves' by bisection.  (Counting the larger ones costs m^2 / 128 LDS reads, a network over the workgroup 55
+// steps with barriers: 10 and 8 us at 400; this 2.)
 template <int NT>
 __device__ __forceinline__ void draw_rank_cand(DrawCand& cand, int m)
 {
-    const int t = threadIdx.x;
-    if (2 * m <= NT) {
-        int share = 1;                                               // log2 of the threads per rank
-        while (share < 4 && m << (share + 1) <= NT) share++;
-        if (t == 0) cand.rank[m] = 0;                                // pairs are read
-        __syncthreads();
-        const int e = t >> share;
-        int place = 0;
-        const u64 mine = e < m ? cand.rank[e] : ~0ull;
-        const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(cand.rank);
-#pragma unroll 4
-        for (int j = t & ((1 << share) - 1); 2 * j < m; j += 1 << share) {
-            const ulonglong2 v = pairs[j];
-            place += (v.x > mine) + (v.y > mine);
-        }
-        place += __builtin_bit_cast(int, draw_dpp<0xB1, 0xf>(__builtin_bit_cast(float, place)));
-        if (share > 1) place += __builtin_bit_cast(int, draw_dpp<0x4E, 0xf>(__builtin_bit_cast(float, place)));
-        if (share > 2) place += __builtin_bit_cast(int, draw_dpp<0x141, 0xf>(__builtin_bit_cast(float, place)));
-        if (share > 3) place += __builtin_bit_cast(int, draw_dpp<0x140, 0xf>(__builtin_bit_cast(float, place)));
-        if (e < m && (t & ((1 << share) - 1)) == 0) cand.ranked[place] = mine;
-        __syncthreads();
-        return;
-    }
-    u64 v = t < m ? cand.rank[t] : 0;
-    for (int size = 2; size < 2 * m; size <<= 1) {
-        for (int d = size >> 1; d; d >>= 1) {
-            u64 o;
-            if (d >= 64) {
-                __syncthreads();
-                cand.ranked[t] = v;
-                __syncthreads();
-                o = cand.ranked[t ^ d];
-            } else o = __shfl_xor(v, d, 64);
-            const bool larger = ((t & d) == 0) == ((t & size) == 0);     // this thread keeps the larger one
-            v = (larger ? o > v : o < v) ? o : v;
-        }
-    }
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, runs = (m + 63) >> 6;
+    const u64 mine = wave < runs ? draw_sort_wave(t < m ? cand.rank[t] : 0, lane) : 0;
     __syncthreads();
-    cand.ranked[t] = v;
+    u64* run = cand.rank;                                            // they stay the first m, in another order
+    if (wave < runs) run[t] = mine;
+    __syncthreads();
+    if (wave < runs) {
+        int place = lane;
+        for (int w0 = 0; w0 < runs; w0 += 4) {                       // four bisections at a time
+            int at[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int step = 32; step; step >>= 1)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int w = w0 + q < runs ? w0 + q : runs - 1;
+                    if (run[w * 64 + at[q] + step - 1] > mine) at[q] += step;
+                }
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int w = w0 + q;
+                if (w < runs && w != wave) place += at[q] + (run[w * 64 + at[q]] > mine ? 1 : 0);
+            }
+        }
+        if (mine) cand.ranked[place] = mine;                         // no rank is 0
+    }
     __syncthreads();
 }
 
