@@ -5,6 +5,8 @@ which depth-ordered splats are composited (/root/reference/model/gaussian_splatt
     linear   h_t = z_t h_(t-1) + x_t
     blend    h_t = (1 - z_t) h_(t-1) + z_t x_t          (straight colours over each other, z = alpha)
     over     h_t = (1 - z_t) h_(t-1) + x_t              (premultiplied colours)"""
+import ctypes as C
+import struct
 import torch
 from . import _lib as L
 
@@ -22,74 +24,85 @@ def _channels(t):
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _shape(gate, x, lengths, form, reverse):
-    s = L.GsxGated()
-    s.dtype = DTYPES[x.dtype]; s.form = FORMS[form]; s.reverse = int(reverse)
-    s.B, s.T, s.D = gate.shape
-    s.planes = x.shape[2] if x.dim() == 4 else 1
-    s.gate = _ptr(gate); s.gate_stride[:] = [gate.stride(0), gate.stride(1)]
-    s.x = _ptr(x); s.x_stride[:] = [x.stride(0), x.stride(1), x.stride(2) if x.dim() == 4 else 0]
-    s.lengths = _ptr(lengths)
-    return s
+# struct gsx_gated as bytes: filling the ctypes structure field by field takes several times as long
+_PACK = struct.Struct("4i3qQ2qQ3q5QQ3q4QQQ").pack
+_entry = {}
 
 
-def _workspace(lib, s, backward, dev):
-    n = lib.gsx_gated_workspace_bytes(s, backward)
-    if not n:
-        return None
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    s.ws = _ptr(ws); s.ws_bytes = n
-    return ws
+def _entries():
+    """(workspace, forward, backward) that take the packed struct"""
+    if not _entry:
+        lib = L.lib()
+        for name, argtypes, restype in (("gsx_gated_workspace_bytes", [C.c_char_p, C.c_int32], C.c_size_t),
+                                        ("gsx_gated_scan_fwd", [C.c_char_p, C.c_void_p], C.c_int), ("gsx_gated_scan_bwd", [C.c_char_p, C.c_void_p], C.c_int)):
+            fn = lib[name]                                       # a function object of its own: the binding's keeps its types
+            fn.argtypes, fn.restype = argtypes, restype
+            _entry[name] = fn
+    return _entry
+
+
+def _call(name, backward, head, tail, dev):
+    e = _entries()
+    packed = _PACK(*head, *tail, 0, 0)
+    n = e["gsx_gated_workspace_bytes"](packed, backward)
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        packed = _PACK(*head, *tail, ws.data_ptr(), n)
+    with L.on_device(dev):
+        L.check(e[name](packed, L.stream_ptr(dev)), name)
+
+
+def _head(gate, x, initial, lengths, form, reverse):
+    gs, xs = gate.stride(), x.stride()
+    B, T, D = gate.shape
+    four = x.dim() == 4
+    return (DTYPES[x.dtype], FORMS[form], reverse, x.shape[2] if four else 1, B, T, D, gate.data_ptr(), gs[0], gs[1],
+            x.data_ptr(), xs[0], xs[1], xs[2] if four else 0, initial.data_ptr() if initial is not None else 0, lengths.data_ptr() if lengths is not None else 0)
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, initial, lengths, form, reverse, want_states, want_grad):
-        lib = L.lib()
-        gate, x = _channels(gate.detach()), _channels(x.detach())
+        gate, x = _channels(gate), _channels(x)
         dev = x.device
         state_shape = x.shape[:1] + x.shape[2:]
-        h0 = initial.detach().to(torch.float32).contiguous() if initial is not None else None
+        h0 = initial.to(torch.float32).contiguous() if initial is not None else None
         states = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_states else None
         last = torch.empty(state_shape, dtype=torch.float32, device=dev)
-        s = _shape(gate, x, lengths, form, reverse)
+        head = _head(gate, x, h0, lengths, form, reverse)
         marks = None
         if want_grad:
-            marks = torch.empty(lib.gsx_gated_marks_floats(s.B, s.T, s.planes, s.D), dtype=torch.float32, device=dev)
-        s.initial = _ptr(h0); s.states = _ptr(states); s.last = _ptr(last); s.marks = _ptr(marks)
-        ws = _workspace(lib, s, 0, dev)
-        with L.on_device(dev):
-            L.check(lib.gsx_gated_scan_fwd(s, L.stream_ptr(dev)), "gsx_gated_scan_fwd")
-        if marks is not None:
+            marks = torch.empty(L.lib().gsx_gated_marks_floats(head[4], head[5], head[3], head[6]), dtype=torch.float32, device=dev)
+        _call("gsx_gated_scan_fwd", 0, head, (states.data_ptr() if want_states else 0, last.data_ptr(), marks.data_ptr() if want_grad else 0,
+                                              0, 0, 0, 0, 0, 0, 0, 0), dev)
+        if want_grad:
             ctx.save_for_backward(gate, x, marks, lengths)
             ctx.how = (form, reverse, initial.dtype if initial is not None else None)
         ctx.set_materialize_grads(False)
         return states, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_states, d_last):
+        if torch.is_grad_enabled():                              # create_graph: the gradients' own gradients are not here
+            raise RuntimeError("gated_scan is differentiable once only")
         gate, x, marks, lengths = ctx.saved_tensors
         form, reverse, initial_dtype = ctx.how
-        lib = L.lib()
+        need = ctx.needs_input_grad
         dev = x.device
-        s = _shape(gate, x, lengths, form, reverse)
-        s.marks = _ptr(marks)
+        ds = (0, 0, 0)
         if d_states is not None:
             d_states = _channels(d_states)
-            s.d_states = _ptr(d_states)
-            s.d_states_stride[:] = [d_states.stride(0), d_states.stride(1), d_states.stride(2) if x.dim() == 4 else 0]
+            st = d_states.stride()
+            ds = (st[0], st[1], st[2] if x.dim() == 4 else 0)
         if d_last is not None:
             d_last = d_last.contiguous()
-            s.d_last = _ptr(d_last)
-        d_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        d_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[1] else None
-        d_initial = torch.empty(x.shape[:1] + x.shape[2:], dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
-        s.d_gate = _ptr(d_gate); s.d_x = _ptr(d_x); s.d_initial = _ptr(d_initial)
-        ws = _workspace(lib, s, 1, dev)
-        with L.on_device(dev):
-            L.check(lib.gsx_gated_scan_bwd(s, L.stream_ptr(dev)), "gsx_gated_scan_bwd")
-        if d_initial is not None:
+        d_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[0] else None
+        d_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[1] else None
+        d_initial = torch.empty(x.shape[:1] + x.shape[2:], dtype=torch.float32, device=dev) if need[2] else None
+        at = lambda t: t.data_ptr() if t is not None else 0  # noqa: E731
+        _call("gsx_gated_scan_bwd", 1, _head(gate, x, None, lengths, form, reverse),
+              (0, 0, marks.data_ptr(), at(d_states), *ds, at(d_last), at(d_gate), at(d_x), at(d_initial)), dev)
+        if d_initial is not None and initial_dtype != torch.float32:
             d_initial = d_initial.to(initial_dtype)
         return d_gate, d_x, d_initial, None, None, None, None, None
 
@@ -132,18 +145,21 @@ def gated_scan(gate, x, initial=None, lengths=None, form="linear", reverse=False
     return _GatedScan.apply(gate, x, initial, lengths, form, bool(reverse), bool(return_states), want_grad)
 
 
-@torch.no_grad()
 def gated_step(state, gate, x, form="linear"):
-    """One step in place on a 32-bit state that lives between calls (a served stream): state, gate, x of one shape, contiguous.  -> state."""
+    """One step in place on a 32-bit state that lives between calls (a served stream): state, gate, x of one shape, contiguous.  -> state.
+    Not differentiable (gated_scan with one step is)."""
     _check_pair(gate, x, form)
-    if state.dtype != torch.float32 or state.shape != x.shape or gate.shape != x.shape or state.device != x.device:
+    shape = state.shape
+    if state.dtype != torch.float32 or shape != x.shape or gate.shape != shape or state.device != x.device:
         raise ValueError(f"state (float32), gate and x must share a shape and a device, got {tuple(state.shape)} {state.dtype}, {tuple(gate.shape)}, {tuple(x.shape)}")
     if not state.is_contiguous():
         raise ValueError("gated_step writes the state in place: it must be contiguous")
     _refuse_host(x, "recurrence")
+    if state.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("gated_step writes the state in place and leaves no graph: the state must not require a gradient")
     gate, x = gate.contiguous(), x.contiguous()
     dev = x.device
     with L.on_device(dev):
         L.check(L.lib().gsx_gated_step(DTYPES[x.dtype], FORMS[form], x.numel(), state.data_ptr(), gate.data_ptr(), x.data_ptr(), L.stream_ptr(dev)), "gsx_gated_step")
-    torch.autograd.graph.increment_version(state)                # written through a raw pointer: autograd must see it
+    torch._C._increment_version((state,))                        # written through a raw pointer: autograd must see it
     return state
