@@ -136,6 +136,22 @@ __device__ __forceinline__ void draw_limbs(double w, uint32_t& hi, uint32_t& lo)
 }
 __device__ __forceinline__ double limbs(u64 hi, u64 lo) { return (double)hi * 0x1p-31 + (double)lo * 0x1p-63; }
 
+// the largest power of two up to n
+__device__ __forceinline__ int draw_power(int n) { return 1 << (31 - __builtin_clz(n)); }
+
+// How many of the n ascending numbers at(0) .. at(n - 1) lie at or below `want`, n - 1 at most: the place of a draw.  Steps of falling powers of two, no branches; `top` is the
+// largest power of two below 2 n.
+template <typename At>
+__device__ __forceinline__ int draw_place(const At& at, int n, int top, double want)
+{
+    int place = 0;
+    for (int step = top; step; step >>= 1) {
+        const int i = place + step - 1;
+        place = i < n - 1 && at(i < n ? i : n - 1) <= want ? place + step : place;
+    }
+    return place;
+}
+
 struct DrawRow { double inv_t, p, min_p; long long k; float scale; bool valid; };
 
 __device__ __forceinline__ DrawRow draw_row(const DrawArgs& a, long long r)
@@ -232,16 +248,16 @@ struct Places {
 
 // ---- wave and workgroup helpers --------------------------------------------------------------------------------------------------
 // Values moved between lanes by DPP: register moves of a few cycles, where a shuffle is a round trip through the LDS unit that the histograms' atomics
-// keep busy.  Lanes without a source get zero.
+// keep busy.  Lanes without a source get zero (with all rows enabled by the instruction's own bound control, without a move).
 template <int CTRL, int ROWS, typename T>
 __device__ __forceinline__ T draw_dpp(T v)
 {
     if constexpr (sizeof(T) == 4) {
-        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, ROWS == 0xf));
     } else {
         const u64 u = __builtin_bit_cast(u64, v);
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
-        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, ROWS == 0xf);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, ROWS == 0xf);
         return __builtin_bit_cast(T, (u64)hi << 32 | lo);
     }
 }
@@ -731,11 +747,7 @@ __device__ __forceinline__ void draw_row_draws(const DrawArgs& a, long long r, c
         const double log_total = draw_log(total);
         for (long long s = wave; s < a.S; s += kWaves) {             // a wave per draw
             const double want = draw_uniform(a, r * a.S + s) * total;
-            int lo = 0, hi = tiles - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (tile[mid] > want) hi = mid; else lo = mid + 1;
-            }
+            const int lo = draw_place([&](int i) { return tile[i]; }, tiles, draw_power(tiles), want);
             // the first token in the tile that exceeds; where rounding leaves none, the last one with weight
             for (int q = lo; q >= 0; q--) {
                 const int g = q * 64 + lane;
@@ -943,11 +955,9 @@ __global__ __launch_bounds__(kDrawExact) void draw_exact_kernel(DrawArgs a)
 // The draw within a group whose masses begin at `run`: the first token that exceeds, or where rounding leaves none the last one with weight; -1: none
 // has any.
 template <typename T>
-__device__ __forceinline__ int draw_in_group(const Places<T>& row, int g, double run, double want, const DrawFloor& floor, float top, const DrawRow& set, float& at_l)
+__device__ __forceinline__ int draw_in_group(const Places<T>& row, int g, const float (&l)[4], double run, double want, const DrawFloor& floor, float top, const DrawRow& set, float& at_l)
 {
     int index = -1; bool found = false;
-    float l[4];
-    row.load(g, row.groups(), l);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int i = 4 * g + j - row.off;
@@ -973,13 +983,13 @@ __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long
     const DrawFloor floor(a.floors[r]);
     const double* spans = a.spans + r * a.spans_row;
     const double want = draw_uniform(a, t) * total;
-    int lo = 0, hi = row.groups() - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (spans[mid] > want) hi = mid; else lo = mid + 1;
-    }
+    const int lo = draw_place([&](int i) { return spans[i]; }, row.groups(), draw_power(row.groups()), want);
     int index = -1; float at_l = 0.0f;
-    for (int q = lo; q >= 0 && index < 0; q--) index = draw_in_group(row, q, q ? spans[q - 1] : 0.0, want, floor, top, set, at_l);
+    for (int q = lo; q >= 0 && index < 0; q--) {
+        float l[4];
+        row.load(q, row.groups(), l);
+        index = draw_in_group(row, q, l, q ? spans[q - 1] : 0.0, want, floor, top, set, at_l);
+    }
     a.indices[t] = index;
     if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, draw_log(total));
 }
@@ -1252,11 +1262,7 @@ __global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
             const double log_mass = draw_log(mass);
             for (long long s = tid; s < a.S; s += NT) {
                 const double want = (s == tid ? first_u : draw_uniform(a, r * a.S + s)) * mass;
-                int lo = 0, hi = m - 1;
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (upto[mid] > want) hi = mid; else lo = mid + 1;
-                }
+                const int lo = draw_place([&](int i) { return upto[i]; }, m, draw_power(m), want);
                 const u64 v = sh.cand.ranked[lo];
                 a.indices[r * a.S + s] = 0x7fffffff - (int)(v >> 32);
                 if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(__builtin_bit_cast(float, (uint32_t)v), top, set.inv_t, log_mass);
@@ -1346,8 +1352,10 @@ __global__ __launch_bounds__(kDrawPart, 6) void draw_part_mass_kernel(DrawArgs a
     if (tid == 0) a.part_mass[r * a.parts + blockIdx.x] = carry;
 }
 
-// Draws of a row in parts.  For many draws what bounds them is the lines that a bisection touches (at 1 M tokens and draws: 7 lines of 128 B through each CU's 64 B a
-// cycle, 80 us); so the sums behind every 1 / nodes of a part lie in LDS, down to 16 groups: a draw then reads one line of sums and one of tokens.
+// Draws of a row in parts.  What bounds many of them is the chain of loads that wait for each other and the lines that these touch; so the sums behind every 1 / nodes of a
+// part lie in LDS, down to 16 groups where they fit, the sums behind every 16 groups lie side by side, and a draw reads one line of each kind of sums and one of tokens.
+// Measured: 1 M tokens and draws 35 us, 6 M tokens and 1 M draws 75 us (88 with the steps down to 16 groups in the sums behind each group); two draws of a thread side by
+// side 38 and 85, four 41 and 91: with 16 waves a CU the loads of one draw hide behind those of others, and the registers of more cost waves.
 constexpr int kDrawMostParts = 2048;
 constexpr int kDrawMostNodes = 16384;
 constexpr int64_t kDrawManyDraws = 1 << 15;         // from here on the nodes' 128 KB are worth their loading
@@ -1365,9 +1373,9 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
     Places<T> row(a, r);
     const float top = row.finite_top(draw_row_top<kDrawPickers>(a, r, s_f, a.cuts));
     double* s_part = s_sum;
-    double* s_node = s_sum + a.parts;
+    double* s_node = s_sum + a.parts;                                // a gap after every 32: steps of powers of two would meet in one bank
     const int part_log = __builtin_ctz(a.part), groups = row.groups(), step = a.part >> a.nodes_log;
-    const double* spans = a.spans + r * a.spans_row;
+    const double *spans = a.spans + r * a.spans_row, *lines = a.lines + r * a.spans_row / 16;       // lines: what stands behind every 16th group, side by side
     const int per = (a.parts + kDrawPickers - 1) / kDrawPickers;
     double sum = 0.0, total;
     for (int p = tid * per; p < (tid + 1) * per && p < a.parts; p++) sum += a.part_mass[r * a.parts + p];
@@ -1375,38 +1383,75 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
     for (int p = tid * per; p < (tid + 1) * per && p < a.parts; p++) { s_part[p] = at; at += a.part_mass[r * a.parts + p]; }
     __syncthreads();
     const int nodes = a.parts * a.nodes;
-    for (int q = tid; q < nodes; q += kDrawPickers) {
-        const int p = q >> a.nodes_log, last = (q + 1) * step - 1;   // the node's last group
-        s_node[q] = s_part[p] + (last < groups && ((q + 1) & (a.nodes - 1)) ? a.lines[(r * a.spans_row + last) / 16] : a.part_mass[r * a.parts + p]);
+    for (int q0 = tid; q0 < nodes; q0 += 8 * kDrawPickers) {         // eight loads in flight: 16 k nodes one by one would be 16 trips
+        double v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int q = q0 + j * kDrawPickers < nodes ? q0 + j * kDrawPickers : nodes - 1, last = (q + 1) * step - 1;       // the node's last group
+            const bool whole = last < groups && ((q + 1) & (a.nodes - 1));
+            const double* at = whole ? lines + last / 16 : a.part_mass + r * a.parts + (q >> a.nodes_log);
+            v[j] = *at;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int q = q0 + j * kDrawPickers;
+            if (q < nodes) s_node[q + (q >> 5)] = s_part[q >> a.nodes_log] + v[j];
+        }
     }
     __syncthreads();
     const DrawFloor floor(a.cuts ? a.floors[r] : 0);
+    if (!(total > 0.0)) {
+        for (long long s = (long long)blockIdx.x * kDrawPickers + tid; s < a.S; s += (long long)gridDim.x * kDrawPickers) {
+            a.indices[r * a.S + s] = -1;
+            if (a.logprobs) a.logprobs[r * a.S + s] = -__builtin_inff();
+        }
+        return;
+    }
+    const int top_node = draw_power(nodes);
     const double log_total = draw_log(total);
     for (long long s = (long long)blockIdx.x * kDrawPickers + tid; s < a.S; s += (long long)gridDim.x * kDrawPickers) {
-        const long long t = r * a.S + s;
-        if (!(total > 0.0)) { a.indices[t] = -1; if (a.logprobs) a.logprobs[t] = -__builtin_inff(); continue; }
-        const double want = draw_uniform(a, t) * total;
-        int n = 0, n1 = nodes - 1;
-        while (n < n1) {
-            const int mid = (n + n1) >> 1;
-            if (s_node[mid] > want) n1 = mid; else n = mid + 1;
+        const double want = draw_uniform(a, r * a.S + s) * total;
+        int n = 0;
+        for (int by = top_node; by; by >>= 1) {                      // as draw_place
+            const int i = n + by - 1, j = i < nodes ? i : nodes - 1;
+            n = i < nodes - 1 && s_node[j + (j >> 5)] <= want ? n + by : n;
         }
-        int lo = n * step, hi = lo + step < groups ? lo + step - 1 : groups - 1;
-        if (lo > hi) lo = hi;                                        // rounding beyond the last node with tokens
-        const int p = lo >> part_log;
-        const double base = s_part[p];
-        double run = lo == p << part_log ? base : lo == n * step ? s_node[n - 1] : base + spans[lo - 1];       // in front of group lo
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            const double v = base + spans[mid];
-            if (v > want) hi = mid; else { lo = mid + 1; run = v; }
+        int lo = n * step;
+        const int hi = lo + step < groups ? lo + step - 1 : groups - 1;
+        const bool beyond = lo > hi;                                 // rounding beyond the last node with tokens
+        lo = beyond ? hi : lo;
+        const double base = s_part[lo >> part_log];
+        double run = (lo & (a.part - 1)) == 0 ? base : beyond ? base + spans[lo - 1] : s_node[n - 1 + ((n - 1) >> 5)];        // in front of group lo
+        for (int by = step >> 1; by >= 16; by >>= 1) {
+            const int i = lo + by - 1;
+            const double v = base + lines[(i < hi ? i : hi) >> 4];
+            const bool on = i < hi && v <= want;
+            lo = on ? lo + by : lo;
+            run = on ? v : run;
         }
-        float at_l = 0.0f;
-        int index = draw_in_group(row, lo, run, want, floor, top, set, at_l);
-        for (int q = lo - 1; q >= 0 && index < 0; q--)               // nothing there: rounding; the last one in front with weight
-            index = draw_in_group(row, q, s_part[q >> part_log] + (q & (a.part - 1) ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
-        a.indices[t] = index;
-        if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, log_total);
+        // the line of 16 sums that is left, in two steps of four ways: each way's load would be one more trip
+#pragma unroll
+        for (int by = 4; by > 0; by -= 3) {
+            const int from = lo;
+            double v[3];
+#pragma unroll
+            for (int j = 0; j < 3; j++) { const int i = from + (j + 1) * by - 1; v[j] = base + spans[i < hi ? i : hi]; }
+#pragma unroll
+            for (int j = 0; j < 3; j++) {
+                const bool on = from + (j + 1) * by - 1 < hi && v[j] <= want;
+                lo = on ? from + (j + 1) * by : lo;
+                run = on ? v[j] : run;
+            }
+        }
+        float l[4], at_l = 0.0f;
+        row.load(lo, groups, l);
+        int index = draw_in_group(row, lo, l, run, want, floor, top, set, at_l);
+        for (int q = lo - 1; q >= 0 && index < 0; q--) {             // nothing there: rounding; the last one in front with weight
+            row.load(q, groups, l);
+            index = draw_in_group(row, q, l, s_part[q >> part_log] + (q & (a.part - 1) ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
+        }
+        a.indices[r * a.S + s] = index;
+        if (a.logprobs) a.logprobs[r * a.S + s] = draw_logprob(at_l, top, set.inv_t, log_total);
     }
 }
 
@@ -1565,7 +1610,7 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
     __builtin_amdgcn_wave_barrier();
     const int rows = a.R - r0 < kRows ? (int)(a.R - r0) : kRows;
     if (rows <= 0) return;
-    const float per_row = 1.0f / (float)a.S;
+    const float per_row = __builtin_amdgcn_rcpf((float)a.S);
     for (long long q = lane; q < (long long)rows * a.S; q += 64) {
         int y = 0;                                                   // q / S: a 64-bit division would cost as much as four exps
         if (kRows > 1) {
@@ -1581,12 +1626,9 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
         float lp = -__builtin_inff();
         if (all > 0.0) {
             const double want = draw_uniform(a, r0 * a.S + q) * all;
-            int lo = 0, hi = V - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (fabs(mass[mid]) > want) hi = mid; else lo = mid + 1;
-            }
-            int i = lo;
+            int i = 0;                                               // places behind the row hold its total
+#pragma unroll
+            for (int step = W * E / 2; step; step >>= 1) i += fabs(mass[i + step - 1]) <= want ? step : 0;
             while (i > 0 && !(mass[i] > 0.0)) i--;
             while (!(mass[i] > 0.0) && i < V - 1) i++;
             index = i;
@@ -1700,8 +1742,9 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
         }
         draw_part_mass_kernel<T><<<parts, dim3(kDrawPart), 0, stream>>>(a);
         const int64_t picks = ceil_div(a.S, kDrawPickers);
-        const size_t lds = ((size_t)l.parts * l.nodes + l.parts) * 8;
-        GSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(draw_part_pick_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, (kDrawMostNodes + kDrawMostParts) * 8));
+        const size_t lds = ((size_t)l.parts * l.nodes + l.parts * l.nodes / 32 + 1 + l.parts) * 8;
+        GSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(draw_part_pick_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    (kDrawMostNodes + kDrawMostNodes / 32 + 1 + kDrawMostParts) * 8));
         draw_part_pick_kernel<T><<<dim3((unsigned)(picks < 256 ? picks : 256), (unsigned)a.R), dim3(kDrawPickers), lds, stream>>>(a);
         GSX_LAUNCH_CHECK();
         return GSX_OK;
