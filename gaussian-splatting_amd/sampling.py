@@ -13,7 +13,12 @@ def _setting(v, name, R, device, dtype, ok, where):
     if torch.is_tensor(v):
         if v.shape != (R,) or v.device != device:
             raise ValueError(f"{name} must be a number or ({R},) on {device}, got {tuple(v.shape)} on {v.device}")
-        return 0, v.detach().to(dtype).contiguous()
+        if dtype == torch.int32 and (v.is_floating_point() or v.is_complex()):
+            raise TypeError(f"{name} by row must be whole numbers, got {v.dtype}")
+        v = v.detach()
+        if v.dtype == torch.int64 and dtype == torch.int32:
+            v = v.clamp(-1, MAX_V)                               # all tokens and more, where a cast alone would wrap
+        return 0, v.to(dtype).contiguous()
     if not ok(v):
         raise ValueError(f"{name} must be {where}, got {v}")
     return v, None

@@ -373,3 +373,45 @@ def test_a_trace_over_views_picks_the_points():
     c = torch.cumsum(lw, 0)
     idx = kept[torch.searchsorted(c, u * c[-1], right=True)]
     assert torch.equal(pts, torch.cat([m.positions[idx], m.features[idx]], 1))
+
+
+def test_offsets_beyond_32_bits():
+    """more than 2^31 elements: the last channels to the last steps, forward and backward; the others are zero"""
+    from gaussian_splatting_amd import gated_scan
+    T, D, n = 2100, 1050000, 64
+    gate, x = (torch.zeros(1, T, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    few_gate, few_x, _, _, d, dl = make(1, T, 1, n, torch.bfloat16, "linear", 40)
+    gate[..., -n:], x[..., -n:] = few_gate, few_x
+    want = walk("linear", few_gate.double(), few_x.double()[:, :, None], torch.zeros(1, 1, n, dtype=torch.float64, device="cuda"), None, False, d.double()[:, :, None], dl.double()[:, None])
+    want = {k: v if k == "d_gate" else tuple(e.squeeze(-2) for e in v) for k, v in want.items()}
+    states, last = gated_scan(gate.requires_grad_(True), x.requires_grad_(True))
+    close(last[:, -n:], want["last"], torch.float32, "last")
+    close(states[..., -n:], want["states"], torch.bfloat16, "states")
+    assert not bool(last[:, :-n].any()) and not bool(states[:, -1, :-n].any())
+    ds, dls = torch.zeros_like(states), torch.zeros_like(last)
+    ds[..., -n:], dls[:, -n:] = d, dl
+    got = torch.autograd.grad((states, last), (gate, x), (ds, dls))
+    close(got[0][..., -n:], want["d_gate"], torch.bfloat16, "d_gate")
+    close(got[1][..., -n:], want["d_x"], torch.bfloat16, "d_x")
+
+
+def test_two_streams_at_once():
+    from gaussian_splatting_amd import gated_scan
+    sets = [make(2, 3000, 1, 70, torch.bfloat16, "linear", 6), make(1, 40, 3, 5000, torch.float32, "blend", 7)]
+    def once(s, form):
+        leaves = [v.detach().requires_grad_(True) for v in s[:3]]
+        st, l = gated_scan(*leaves, form=form)
+        return (st, l) + torch.autograd.grad((st, l), leaves, (s[4], s[5]))
+    forms = ("linear", "blend")
+    alone = [once(s, f) for s, f in zip(sets, forms)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    outs = [[] for _ in sets]
+    for _ in range(5):
+        for st, s, f, o in zip(streams, sets, forms, outs):
+            with torch.cuda.stream(st):
+                o.append(once(s, f))
+    torch.cuda.synchronize()
+    for a, out in zip(alone, outs):
+        for o in out:
+            assert all(torch.equal(p, q) for p, q in zip(a, o))

@@ -248,3 +248,83 @@ def test_dense_points():
         m.opacity.fill_(math.nan)
     with pytest.raises(ValueError, match="no Gaussian is left"):
         m.get_dense_points(10, top_k=5)
+
+
+def test_ranks_by_row_beyond_32_bits():
+    logits, u = rand(11, 4, 700, 6)
+    k = torch.tensor([2 ** 33, 2 ** 32 + 5, 3, -(2 ** 40)], device="cuda")
+    check(logits, u, k=k)
+
+
+@pytest.mark.parametrize("R,V,S,t", [(3, 600001, 40, "bf16"), (2, 90000, 40000, "f16"), (5, 70000, 9, "bf16"), (1, 9000011, 40000, "f32")])
+def test_rows_in_parts_with_settings_by_row(R, V, S, t):
+    """more than one part, walker and node, every type, many draws of several rows"""
+    logits, u = rand(R + S, R, V, S, DT[t], f64=True)
+    check(logits, u)
+    dev = logits.device
+    by_row = dict(T=torch.linspace(0.5, 1.1, R, device=dev), k=torch.arange(R, device=dev) * 700, p=torch.linspace(0.99, 0.4, R, device=dev), m=torch.linspace(0, 0.001, R, device=dev))
+    check(logits, u, **by_row)
+    if R > 1:
+        logits[0, ::3], logits[1, : V - 1] = math.inf, -math.inf
+        check(logits, u, p=0.5)
+
+
+@pytest.mark.parametrize("R,V", [(11000, 200000), (4000, 600000)])
+def test_offsets_beyond_32_bits(R, V):
+    """rows that begin behind 2^31 elements: the same draws as the rows by themselves"""
+    from gaussian_splatting_amd import sample
+    logits = torch.empty(R, V, dtype=torch.bfloat16, device="cuda")
+    logits[: R - 3] = 0
+    logits[R - 3:], u = rand(12, 3, V, 4, torch.bfloat16, f64=True)
+    us = torch.zeros(R, 4, dtype=torch.float64, device="cuda")
+    us[R - 3:] = u
+    for cut in (dict(), dict(k=500, p=0.9)):
+        got = sample(logits, us, top_k=cut.get("k", 0), top_p=cut.get("p", 1.0))
+        assert bool((got[: R - 3] == 0).all())
+        check(logits[R - 3:], u, **cut)
+        assert torch.equal(got[R - 3:], sample(logits[R - 3:], u, top_k=cut.get("k", 0), top_p=cut.get("p", 1.0)))
+
+
+def test_two_streams_at_once():
+    from gaussian_splatting_amd import sample
+    sets = [rand(20 + n, R, V, S, f64=True) for n, (R, V, S) in enumerate([(2, 300000, 50), (200, 9000, 3), (2000, 40, 2)])]
+    alone = [sample(l, u, top_p=0.9) for l, u in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    outs = [[] for _ in sets]
+    for _ in range(5):
+        for s, (l, u), o in zip(streams, sets, outs):
+            with torch.cuda.stream(s):
+                o.append(sample(l, u, top_p=0.9))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, o) for a, out in zip(alone, outs) for o in out)
+
+
+def test_in_inference_mode():
+    from gaussian_splatting_amd import sample, gated_scan, gated_step
+    with torch.inference_mode():
+        logits, u = rand(30, 3, 1000, 5)
+        check(logits, u, k=20)
+        state, z, x = torch.zeros(3, 1000, device="cuda"), torch.rand(3, 1000, device="cuda"), torch.randn(3, 1000, device="cuda")
+        _, last = gated_scan(z[:, None], x[:, None])
+        assert torch.equal(gated_step(state, z, x), last)
+
+
+def test_the_longest_row():
+    from gaussian_splatting_amd import sample
+    from gaussian_splatting_amd.sampling import MAX_V
+    u = torch.rand(1, 300, device="cuda", dtype=torch.float64, generator=torch.Generator(device="cuda").manual_seed(41))
+    logits = torch.zeros(1, MAX_V, device="cuda")
+    assert torch.equal(sample(logits, u), torch.floor(u * MAX_V).long())                 # whole numbers: exact
+    assert torch.equal(sample(logits, u, top_k=MAX_V // 2), torch.floor(u * (MAX_V // 2)).long())
+    logits.normal_(generator=torch.Generator(device="cuda").manual_seed(42))
+    w = torch.exp(logits[0].double() - logits.max().double())
+    rank = torch.sort(logits[0], descending=True, stable=True).indices
+    run = torch.cumsum(w[rank], 0)
+    keep = 1 + int((run < float(np.float32(0.7)) * run[-1]).sum())
+    kept = torch.zeros_like(w)
+    kept[rank[:keep]] = w[rank[:keep]]
+    c = torch.cumsum(kept, 0)
+    assert torch.equal(sample(logits, u, top_p=0.7)[0], torch.searchsorted(c, u[0] * c[-1], right=True))
+    with pytest.raises(ValueError, match="tokens"):
+        sample(torch.zeros(1, 1, device="cuda").expand(1, MAX_V + 1), u)

@@ -80,6 +80,12 @@ def test_draw_refusals():
         m.get_dense_points(5, logits=z(4))
 
 
+def test_ranks_by_row_are_whole_numbers():
+    from gaussian_splatting_amd import sample
+    with pytest.raises(TypeError, match="whole numbers"):
+        sample(torch.zeros(3, 5), torch.zeros(3, 2), top_k=torch.full((3,), 2.5))
+
+
 def test_c_entry_points_refuse_before_the_device():
     lib = L.lib()
     ok = dict(dtype=0, form=0, planes=1, B=1, T=2, D=3)
