@@ -24,12 +24,19 @@ constexpr int kDrawBins = 2048;                     // of the first histogram
 constexpr float kDrawBinsPerUnit = 64.0f;
 constexpr int kDrawFine = 512;                      // bins of the narrower ones
 constexpr int kDrawCand = 1024;                     // tokens that are ranked in LDS
-constexpr int kDrawSmall = 16384;                   // longest row whose workgroup is of 512 threads and decides by itself in every case
-constexpr int kDrawShort = 512;                     // longest row of the short way
+// Which way, thread count and kernels a call takes; us a call, by length, rows and draws, of N(0, 2) logits in 32 bits cut to k = 50, p = 0.9:
+// Longest row of the short way.  100000 rows of 500: 532, with a workgroup each 2866; one row of 500: 19 against 15.
+constexpr int kDrawShort = 512;
+// Longest row whose workgroup is of 512 threads and decides by itself in every case; 1024 threads read a longer one sooner while it has a CU to itself, and of more rows
+// than CUs two of 512 share one.  1 x 32000: 30.4 with 512 threads, 29.7 with 1024; 1000 x 32000: 90, 117; 256 x 60000: 57, 50; 300 x 60000: 68, 83; 512 x 131072: 136, 149.
+constexpr int64_t kDrawSmall = 16384, kDrawSmallOfMany = 65536, kDrawCus = 256;
 constexpr int kDrawWaveTiles = 2048;                // spans of 256 tokens whose masses are kept in LDS: rows of up to 512 k tokens
-constexpr int kDrawInRow = 64;                      // draws per row that its workgroup makes itself
-constexpr int64_t kDrawLong = 32768;                // rows longer than this are cut into parts ...
-constexpr int64_t kDrawFewRows = 128;               // ... where there are at most so many of them
+// Draws per row that its workgroup makes itself, a wave to a draw; of more a kernel with a thread to each.  1000 x 2000: 16 draws 41.8 in the row's workgroup, 42.9 in a
+// kernel; 32: 52, 43; 64: 71, 44.  10 x 20000: 32 draws 33, 40; 64: 38, 40.
+constexpr int64_t kDrawInRow = 64, kDrawInRowOfMany = 16;
+// Longer rows are cut into parts, where there are at most kDrawFewRows of them.  1 x 48000: 32.4 in parts, 34.8 by a workgroup; 32 x 48000: 39, 36; 32 x 64000: 43, 41;
+// 64 x 131072: 46, 61; 128 x 40000: 43, 36; 128 x 131072: 65, 67; 192 x 131072: 87, 72.
+constexpr int64_t kDrawLong = 49152, kDrawFewRows = 128;
 constexpr int kDrawExact = 512;                     // threads where a cut is searched for: all of the registers that it needs
 constexpr int kDrawIndexBits = 27;
 
@@ -1358,7 +1365,7 @@ __global__ __launch_bounds__(kDrawPart, 6) void draw_part_mass_kernel(DrawArgs a
 // side 38 and 85, four 41 and 91: with 16 waves a CU the loads of one draw hide behind those of others, and the registers of more cost waves.
 constexpr int kDrawMostParts = 2048;
 constexpr int kDrawMostNodes = 16384;
-constexpr int64_t kDrawManyDraws = 1 << 15;         // from here on the nodes' 128 KB are worth their loading
+constexpr int64_t kDrawManyDraws = 1 << 15;         // from here on the nodes' 128 KB are worth their loading (1 M tokens: 64 draws 20.7 us with them, 19.0 without; 32768: 25.6, 26.4)
 constexpr int kDrawPickers = 1024;
 template <typename T>
 __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a)
@@ -1667,7 +1674,7 @@ static DrawLayout draw_layout(const gsx_draw* s)
     l.cuts = s->top_ks || s->top_ps || s->temperatures || s->temperature == 0.0f || (s->top_k > 0 && s->top_k < s->V) || s->top_p < 1.0f;
     if (s->V <= kDrawShort) l.way = DrawLayout::kShort;
     else if (s->V > kDrawLong && (s->R <= kDrawFewRows || s->V > (int64_t)kDrawWaveTiles * 256 - 4)) l.way = DrawLayout::kParts;
-    else if (s->S <= kDrawInRow && s->V <= (int64_t)kDrawWaveTiles * 256 - 4) l.way = DrawLayout::kRow;
+    else if (s->S <= (s->R <= kDrawCus ? kDrawInRow : kDrawInRowOfMany) && s->V <= (int64_t)kDrawWaveTiles * 256 - 4) l.way = DrawLayout::kRow;
     else l.way = DrawLayout::kRowSpans;
     if (l.way != DrawLayout::kShort) { l.tops = take(R * 4); l.left = take(R * 4); }       // left: one launch's word to the next
     if (l.way == DrawLayout::kRowSpans) {
@@ -1750,7 +1757,7 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
         return GSX_OK;
     }
     const dim3 grid((unsigned)a.R);
-    const bool small = a.V <= kDrawSmall;
+    const bool small = a.V <= (a.R <= kDrawCus ? kDrawSmall : kDrawSmallOfMany);
     if (l.way == DrawLayout::kRow) {
         if (small) draw_row_kernel<T, kDrawExact, true, true><<<grid, dim3(kDrawExact), 0, stream>>>(a);
         else draw_row_kernel<T, 1024, true, false><<<grid, dim3(1024), 0, stream>>>(a);

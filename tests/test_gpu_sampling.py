@@ -328,3 +328,16 @@ def test_the_longest_row():
     assert torch.equal(sample(logits, u, top_p=0.7)[0], torch.searchsorted(c, u[0] * c[-1], right=True))
     with pytest.raises(ValueError, match="tokens"):
         sample(torch.zeros(1, 1, device="cuda").expand(1, MAX_V + 1), u)
+
+
+@pytest.mark.parametrize("R,V,S", [(300, 20001, 2), (260, 65536, 17), (260, 66000, 3), (300, 17000, 30), (3, 49152, 65), (2, 49153, 20), (257, 600, 16)])
+@pytest.mark.parametrize("cut", [dict(), dict(k=300, p=0.95, T=0.9), dict(p=0.7, T=30.0)], ids=str)
+def test_more_rows_than_compute_units(R, V, S, cut):
+    """both sides of the choices by the number of rows; the high temperature leaves more tokens in a bin than are ranked at once"""
+    from gaussian_splatting_amd import sample
+    logits, u = rand(R + V + S, R, V, S, f64=True)
+    rows = [0, 1, R // 2, R - 1]
+    got = sample(logits, u, temperature=cut.get("T", 1.0), top_k=cut.get("k", 0), top_p=cut.get("p", 1.0)).cpu().numpy()
+    for r in rows:
+        want, _ = oracle_row(logits[r].double().cpu().numpy(), u[r].cpu().numpy(), float(np.float32(cut.get("T", 1.0))), cut.get("k", 0), float(np.float32(cut.get("p", 1.0))), 0.0)
+        assert np.array_equal(got[r], want), (r, got[r], want)
