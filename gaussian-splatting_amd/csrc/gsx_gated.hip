@@ -10,6 +10,7 @@
 // the states' gradient, once each -- as much as a backward that reads `states` instead of x, and `states` need not exist.
 // Few channels and many steps: the steps are split into spans, one per wave.  A first kernel folds every span to the (A, H) of
 // h -> A h + H, and every workgroup's spans to one; the second begins each span from what the spans in front of it come to.
+#include <type_traits>
 #include "gsx_common.h"
 
 namespace gsx {
@@ -37,14 +38,41 @@ struct GatedArgs {
 template <typename T, int NV>
 struct alignas(sizeof(T) * NV) Pack { T v[NV]; };
 
+// Packs read or written past the caches (LAST).  A walk of whole columns reads what nothing will read soon and more than the caches hold: 1 M channels x 60 steps 142 us
+// through them, 118 past them; 32 layers of 800 x 800 forward 92, 70.  Its backward reads what the forward has left there and writes its gradients past it: 131, 114.
+// States are written through (118, past 131), and a split walk reads again what its fold has read.
+template <bool LAST, typename P>
+__device__ __forceinline__ P pack_load(const void* at)
+{
+    using W = std::conditional_t<sizeof(P) == 2, uint16_t, std::conditional_t<sizeof(P) == 4, uint32_t, unsigned long long>>;
+    return __builtin_bit_cast(P, LAST ? __builtin_nontemporal_load((const W*)at) : *(const W*)at);
+}
+template <bool LAST, typename P>
+__device__ __forceinline__ void pack_store(void* at, const P& p)
+{
+    using W = std::conditional_t<sizeof(P) == 2, uint16_t, std::conditional_t<sizeof(P) == 4, uint32_t, unsigned long long>>;
+    const W w = __builtin_bit_cast(W, p);
+    if (LAST) __builtin_nontemporal_store(w, (W*)at); else *(W*)at = w;
+}
+
 template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }         // round to nearest even
 
 // coefficients of one step: a, and m of b = m x
-__device__ __forceinline__ void gated_am(int form, float z, float& a, float& m)
+template <int FORM>
+__device__ __forceinline__ void gated_am(float z, float& a, float& m)
 {
-    a = form == GSX_GATED_LINEAR ? z : 1.0f - z;
-    m = form == GSX_GATED_BLEND ? z : 1.0f;
+    a = FORM == GSX_GATED_LINEAR ? z : 1.0f - z;
+    m = FORM == GSX_GATED_BLEND ? z : 1.0f;
+}
+
+// f(form) with the form known to the compiler: decided once per kernel, where a choice per element costs as much as the element
+template <typename F>
+__device__ __forceinline__ void gated_formed(int form, F f)
+{
+    if (form == GSX_GATED_LINEAR) f(std::integral_constant<int, GSX_GATED_LINEAR>{});
+    else if (form == GSX_GATED_BLEND) f(std::integral_constant<int, GSX_GATED_BLEND>{});
+    else f(std::integral_constant<int, GSX_GATED_OVER>{});
 }
 
 // A lane's place: which sequence and channels, and where its steps lie.  Scan position s is memory step s, or T - 1 - s in reverse;
@@ -73,8 +101,8 @@ __device__ __forceinline__ Lane lane_of(const GatedArgs& p, long long group)
     return l;
 }
 
-template <typename T, int NV, int R, int K, bool WHOLE>
-__device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& l, long long s0, float (&h)[R][NV])
+template <typename T, int FORM, int NV, int R, int K, bool SPLIT, bool WHOLE>
+__device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& l, long long group, long long s0, float (&h)[R][NV])
 {
     using P = Pack<T, NV>;
     P z[K], x[K][R];
@@ -83,12 +111,25 @@ __device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& 
     const T* xp = (const T*)p.x + l.b * p.x_b + m0 * p.x_t + l.d;
 #pragma unroll
     for (int k = 0; k < K; k++)
+    {
         if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
-            z[k] = *(const P*)(gp + dir * k * p.gate_t);
+            z[k] = pack_load<!SPLIT, P>(gp);
 #pragma unroll
-            for (int r = 0; r < R; r++) x[k][r] = *(const P*)(xp + dir * k * p.x_t + r * p.x_r);
+            for (int r = 0; r < R; r++) x[k][r] = pack_load<!SPLIT, P>(xp + r * p.x_r);
         }
-    T* sp = p.states ? (T*)p.states + ((l.b * p.T + m0) * R) * p.D + l.d : nullptr;
+        gp += dir * p.gate_t; xp += dir * p.x_t;                             // one step on: the multiples of a step would fill the scalar registers
+    }
+    if (p.marks) {                                                           // behind the loads: a wait for these is none for the stores
+        float* mk = p.marks + (s0 / K) * R * p.groups * NV + group * NV;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            Pack<float, NV> o;
+#pragma unroll
+            for (int i = 0; i < NV; i++) o.v[i] = h[r][i];
+            *(Pack<float, NV>*)(mk + r * p.groups * NV) = o;
+        }
+    }
+    T* sp = (T*)p.states + ((l.b * p.T + m0) * R) * p.D + l.d;              // no states: not written
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const bool in = WHOLE || (s0 + k >= l.lo && s0 + k < l.hi);
@@ -96,29 +137,31 @@ __device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& 
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 float a, m;
-                gated_am(p.form, to_f(z[k].v[i]), a, m);
+                gated_am<FORM>(to_f(z[k].v[i]), a, m);
 #pragma unroll
                 for (int r = 0; r < R; r++) h[r][i] = __builtin_fmaf(a, h[r][i], m * to_f(x[k][r].v[i]));
             }
         }
-        if (sp && (WHOLE || s0 + k < p.T)) {
+        if (p.states && (WHOLE || s0 + k < p.T)) {
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 P o;
 #pragma unroll
                 for (int i = 0; i < NV; i++) o.v[i] = in ? from_f<T>(h[r][i]) : from_f<T>(0.0f);
-                *(P*)(sp + (dir * k * R + r) * p.D) = o;
+                *(P*)(sp + r * p.D) = o;
             }
         }
+        sp += dir * R * p.D;
     }
 }
 
-// A product of gates in 64 bits that stays finite: times a zero state it is a zero, times any other one it leaves 32 bits, as the walk would
-__device__ __forceinline__ double gated_times(double A, double a) { return fmin(fmax(A * a, -1e300), 1e300); }
+// A product of gates in 64 bits that stays finite: times a zero state it is a zero, times any other one it leaves 32 bits, as the walk would.  Four more gates of up to 2^128
+// reach 2^1012 at most, two products 2^1000.
+__device__ __forceinline__ double gated_bound(double A) { return fmin(fmax(A, -0x1p500), 0x1p500); }
 
 // Folds steps [s0, s0 + K) to h -> A h + H, in 64 bits: H and A h may be far larger than the state that they add up to, and a 32-bit H would
 // then be less exact than the walk itself (its 64-bit FMA is as fast on this card as the 32-bit one).  Backward: c -> A c + H of c_t = a_t (d_t + c_(t+1)), from the last step to the first.
-template <typename T, int NV, int R, int K, bool BACK, bool HASV, bool WHOLE>
+template <typename T, int FORM, int NV, int R, int K, bool BACK, bool HASV, bool WHOLE>
 __device__ __forceinline__ void gated_fold_batch(const GatedArgs& p, const Lane& l, long long s0, double (&A)[NV], double (&H)[R][NV])
 {
     using P = Pack<T, NV>;
@@ -129,24 +172,27 @@ __device__ __forceinline__ void gated_fold_batch(const GatedArgs& p, const Lane&
     const long long v_t = BACK ? p.ds_t : p.x_t, v_r = BACK ? p.ds_r : p.x_r;
 #pragma unroll
     for (int k = 0; k < K; k++)
+    {
         if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
-            z[k] = *(const P*)(gp + dir * k * p.gate_t);
+            z[k] = *(const P*)gp;
             if (HASV)
 #pragma unroll
-                for (int r = 0; r < R; r++) v[k][r] = *(const P*)(vp + dir * k * v_t + r * v_r);
+                for (int r = 0; r < R; r++) v[k][r] = *(const P*)(vp + r * v_r);
         }
+        gp += dir * p.gate_t; vp += dir * v_t;
+    }
 #pragma unroll
     for (int q = 0; q < K; q++) {
         const int k = BACK ? K - 1 - q : q;
         if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi))
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                const double zd = (double)to_f(z[k].v[i]), a = p.form == GSX_GATED_LINEAR ? zd : 1.0 - zd;
-                A[i] = gated_times(A[i], a);
+                const double zd = (double)to_f(z[k].v[i]), a = FORM == GSX_GATED_LINEAR ? zd : 1.0 - zd;
+                A[i] = (q & 3) == 3 ? gated_bound(A[i] * a) : A[i] * a;
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     const double vd = HASV ? (double)to_f(v[k][r].v[i]) : 0.0;
-                    H[r][i] = BACK ? a * (H[r][i] + vd) : fma(a, H[r][i], p.form == GSX_GATED_BLEND ? zd * vd : vd);
+                    H[r][i] = BACK ? a * (H[r][i] + vd) : fma(a, H[r][i], FORM == GSX_GATED_BLEND ? zd * vd : vd);
                 }
             }
     }
@@ -185,12 +231,14 @@ __global__ __launch_bounds__(64 * kGatedSpans) void gated_fold_kernel(GatedArgs 
 #pragma unroll
     for (int i = 0; i < NV; i++) { A[i] = 1.0; for (int r = 0; r < R; r++) H[r][i] = 0.0; }
     if (l.on)
-        for (long long n = 0; n < p.span; n += K) {
-            const long long s0 = sp.s0 + (BACK ? p.span - K - n : n);
-            if (s0 >= sp.s1) continue;
-            if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fold_batch<T, NV, R, K, BACK, HASV, true>(p, l, s0, A, H);
-            else gated_fold_batch<T, NV, R, K, BACK, HASV, false>(p, l, s0, A, H);
-        }
+        gated_formed(p.form, [&](auto form) {
+            for (long long n = 0; n < p.span; n += K) {
+                const long long s0 = sp.s0 + (BACK ? p.span - K - n : n);
+                if (s0 >= sp.s1) continue;
+                if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fold_batch<T, form.value, NV, R, K, BACK, HASV, true>(p, l, s0, A, H);
+                else gated_fold_batch<T, form.value, NV, R, K, BACK, HASV, false>(p, l, s0, A, H);
+            }
+        });
     const long long BD = p.groups * NV, at = sp.group * NV;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
@@ -211,7 +259,7 @@ __global__ __launch_bounds__(64 * kGatedSpans) void gated_fold_kernel(GatedArgs 
             for (int r = 0; r < R; r++) h[r] = 0.0;
             for (int w = 0; w < kGatedSpans; w++) {
                 const double aw = s_a[w][lane * NV + i];
-                a = gated_times(a, aw);
+                a = gated_bound(a * aw);
 #pragma unroll
                 for (int r = 0; r < R; r++) h[r] = gated_apply(aw, h[r], s_h[w][r][lane * NV + i]);
             }
@@ -240,7 +288,7 @@ __device__ __forceinline__ void gated_carry(const GatedArgs& p, const Span& sp, 
 #pragma unroll 4
             for (long long b = b0; b < b1; b++) {
                 const double ab = p.block_a[b * BD + at + i];
-                a = gated_times(a, ab);
+                a = gated_bound(a * ab);
 #pragma unroll
                 for (int r = 0; r < R; r++) c[r] = gated_apply(ab, c[r], p.block_h[(b * R + r) * BD + at + i]);
             }
@@ -287,20 +335,12 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
         for (int i = 0; i < NV; i++) h[r][i] = p.initial ? p.initial[out + r * p.D + i] : 0.0f;
     if (SPLIT) gated_carry<NV, R>(p, sp, l.on, h);
     if (!l.on) return;
-    for (long long s0 = sp.s0; s0 < sp.s1; s0 += K) {
-        if (p.marks) {
-            float* mk = p.marks + (s0 / K) * R * p.groups * NV + group * NV;
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                Pack<float, NV> o;
-#pragma unroll
-                for (int i = 0; i < NV; i++) o.v[i] = h[r][i];
-                *(Pack<float, NV>*)(mk + r * p.groups * NV) = o;
-            }
+    gated_formed(p.form, [&](auto form) {
+        for (long long s0 = sp.s0; s0 < sp.s1; s0 += K) {
+            if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fwd_batch<T, form.value, NV, R, K, SPLIT, true>(p, l, group, s0, h);
+            else gated_fwd_batch<T, form.value, NV, R, K, SPLIT, false>(p, l, group, s0, h);
         }
-        if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fwd_batch<T, NV, R, K, true>(p, l, s0, h);
-        else gated_fwd_batch<T, NV, R, K, false>(p, l, s0, h);
-    }
+    });
     if (!SPLIT || sp.index == p.blocks * kGatedSpans - 1)
 #pragma unroll
         for (int r = 0; r < R; r++)
@@ -308,7 +348,7 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
             for (int i = 0; i < NV; i++) p.last[out + r * p.D + i] = h[r][i];
 }
 
-template <typename T, int NV, int R, int K, bool HASD, bool WHOLE>
+template <typename T, int FORM, int NV, int R, int K, bool SPLIT, bool HASD, bool WHOLE>
 __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& l, long long group, long long s0, float (&c)[R][NV])
 {
     using P = Pack<T, NV>;
@@ -326,14 +366,17 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
     }
 #pragma unroll
     for (int k = 0; k < K; k++)
+    {
         if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
-            z[k] = *(const P*)(gp + dir * k * p.gate_t);
+            z[k] = *(const P*)gp;
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                x[k][r] = *(const P*)(xp + dir * k * p.x_t + r * p.x_r);
-                if (HASD) d[k][r] = *(const P*)(dp + dir * k * p.ds_t + r * p.ds_r);
+                x[k][r] = *(const P*)(xp + r * p.x_r);
+                if (HASD) d[k][r] = *(const P*)(dp + r * p.ds_r);
             }
         }
+        gp += dir * p.gate_t; xp += dir * p.x_t; dp += dir * p.ds_t;
+    }
     float before[K][R][NV];
 #pragma unroll
     for (int k = 0; k < K; k++) {
@@ -345,14 +388,15 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 float a, m;
-                gated_am(p.form, to_f(z[k].v[i]), a, m);
+                gated_am<FORM>(to_f(z[k].v[i]), a, m);
 #pragma unroll
                 for (int r = 0; r < R; r++) h[r][i] = __builtin_fmaf(a, h[r][i], m * to_f(x[k][r].v[i]));
             }
         }
     }
-    T* ogp = p.d_gate ? (T*)p.d_gate + (l.b * p.T + m0) * p.D + l.d : nullptr;
-    T* oxp = p.d_x ? (T*)p.d_x + ((l.b * p.T + m0) * R) * p.D + l.d : nullptr;
+    const long long m1 = m0 + dir * (K - 1);
+    T* ogp = (T*)p.d_gate + (l.b * p.T + m1) * p.D + l.d;                    // no d_gate, no d_x: not written
+    T* oxp = (T*)p.d_x + ((l.b * p.T + m1) * R) * p.D + l.d;
 #pragma unroll
     for (int k = K - 1; k >= 0; k--) {
         const bool in = WHOLE || (s0 + k >= l.lo && s0 + k < l.hi);
@@ -363,12 +407,12 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 float a, m, dz = 0.0f;
-                gated_am(p.form, to_f(z[k].v[i]), a, m);
+                gated_am<FORM>(to_f(z[k].v[i]), a, m);
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     const float g = c[r][i] + (HASD ? to_f(d[k][r].v[i]) : 0.0f);
                     const float h0 = before[k][r][i];
-                    dz = __builtin_fmaf(g, p.form == GSX_GATED_LINEAR ? h0 : p.form == GSX_GATED_BLEND ? to_f(x[k][r].v[i]) - h0 : -h0, dz);
+                    dz = __builtin_fmaf(g, FORM == GSX_GATED_LINEAR ? h0 : FORM == GSX_GATED_BLEND ? to_f(x[k][r].v[i]) - h0 : -h0, dz);
                     ox[r].v[i] = from_f<T>(m * g);
                     c[r][i] = a * g;
                 }
@@ -376,11 +420,12 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
             }
         }
         if (WHOLE || s0 + k < p.T) {
-            if (ogp) *(P*)(ogp + dir * k * p.D) = oz;
-            if (oxp)
+            if (p.d_gate) pack_store<!SPLIT>(ogp, oz);
+            if (p.d_x)
 #pragma unroll
-                for (int r = 0; r < R; r++) *(P*)(oxp + (dir * k * R + r) * p.D) = ox[r];
+                for (int r = 0; r < R; r++) pack_store<!SPLIT>(oxp + r * p.D, ox[r]);
         }
+        ogp -= dir * p.D; oxp -= dir * R * p.D;
     }
 }
 
@@ -401,11 +446,13 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
         for (int i = 0; i < NV; i++) c[r][i] = p.d_last ? p.d_last[out + r * p.D + i] : 0.0f;
     if (SPLIT) gated_carry<NV, R>(p, sp, l.on, c);
     if (!l.on) return;
-    for (long long n = (sp.s1 - sp.s0 + K - 1) / K; n > 0; n--) {
-        const long long s0 = sp.s0 + (n - 1) * K;
-        if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_bwd_batch<T, NV, R, K, HASD, true>(p, l, group, s0, c);
-        else gated_bwd_batch<T, NV, R, K, HASD, false>(p, l, group, s0, c);
-    }
+    gated_formed(p.form, [&](auto form) {
+        for (long long n = (sp.s1 - sp.s0 + K - 1) / K; n > 0; n--) {
+            const long long s0 = sp.s0 + (n - 1) * K;
+            if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_bwd_batch<T, form.value, NV, R, K, SPLIT, HASD, true>(p, l, group, s0, c);
+            else gated_bwd_batch<T, form.value, NV, R, K, SPLIT, HASD, false>(p, l, group, s0, c);
+        }
+    });
     if (p.d_initial && (!SPLIT || sp.index == p.blocks * kGatedSpans - 1))
 #pragma unroll
         for (int r = 0; r < R; r++)
@@ -422,12 +469,14 @@ __global__ __launch_bounds__(kBlock) void gated_step_kernel(float* __restrict__ 
     if (i >= n) return;                                                      // NV divides n
     Pack<float, NV> h = *(const Pack<float, NV>*)(state + i);
     const Pack<T, NV> z = *(const Pack<T, NV>*)(gate + i), v = *(const Pack<T, NV>*)(x + i);
+    gated_formed(form, [&](auto known) {
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-        float a, m;
-        gated_am(form, to_f(z.v[k]), a, m);
-        h.v[k] = __builtin_fmaf(a, h.v[k], m * to_f(v.v[k]));
-    }
+        for (int k = 0; k < NV; k++) {
+            float a, m;
+            gated_am<known.value>(to_f(z.v[k]), a, m);
+            h.v[k] = __builtin_fmaf(a, h.v[k], m * to_f(v.v[k]));
+        }
+    });
     *(Pack<float, NV>*)(state + i) = h;
 }
 
