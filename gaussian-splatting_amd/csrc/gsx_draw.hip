@@ -128,10 +128,14 @@ __device__ __forceinline__ double draw_exp(double x)
 __device__ __forceinline__ double draw_weight(float l, float top, double inv_t) { return draw_exp(((double)l - (double)top) * inv_t); }
 
 // bin of the first histogram: does not fall as l falls
+__device__ __forceinline__ float draw_depth(float l, float top, float scale)
+{
+    return fminf((top - l) * scale, (float)(kDrawBins - 1));         // NaN (-inf at an endless temperature): the last
+}
 __device__ __forceinline__ int draw_bin(float l, float top, float scale)
 {
     const float t = (top - l) * scale;
-    return t < (float)(kDrawBins - 1) ? (int)t : kDrawBins - 1;      // NaN (-inf at an endless temperature): the last
+    return t < (float)(kDrawBins - 1) ? (int)t : kDrawBins - 1;
 }
 
 // a weight as whole numbers: w = hi 2^-31 + lo 2^-63, to the nearest; sums of 2^27 of either fit 64 bits
@@ -219,6 +223,7 @@ struct Places {
     }
     __device__ __forceinline__ float finite_top(float top) { infinite = top == __builtin_inff(); return infinite ? 0.0f : top; }
     __device__ __forceinline__ int groups() const { return (V + off + 3) >> 2; }
+    __device__ __forceinline__ bool whole(int g) const { return 4 * g >= off && 4 * g + 4 <= V + off; }        // all four of its places are tokens
     // A group's load and what follows on it are apart, so that several loads are in flight: any use of one waits for it.  fetch() reads the nearest
     // group that lies in the row whole (rows here have more than 512 tokens); finish() reads the two at the ends token by token.
     __device__ __forceinline__ Four<T> fetch(int g) const
@@ -587,6 +592,24 @@ __device__ __forceinline__ void draw_near_add(u64* bins, float l, float top, flo
 __device__ __forceinline__ uint32_t draw_near_count(u64 v) { return (uint32_t)(v >> kDrawCountBit); }
 __device__ __forceinline__ u64 draw_near_mass(u64 v) { return v & ((1ull << kDrawCountBit) - 1); }
 
+// The 64-bit weights of a group's tokens at depths `t` (places outside the row weigh nothing): those in front of `lo` to `above`, and to the total all of them (kAll), those in
+// front of `upto` (kUpto) or none; -> those in front of lo that min_p keeps.  The kinds are the compiler's: as choices per token they took a tenth of the pass.
+enum DrawTotal { kNone, kAll, kUpto };
+template <int TOTAL, bool LEAST>
+__device__ __forceinline__ double draw_group_sums(const float (&l)[4], const float (&t)[4], float lo, float upto, float top, const DrawRow& set, double& above, double& total)
+{
+    double front = 0.0, kept = 0.0, all = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const double w = draw_weight(l[j], top, set.inv_t), f = t[j] < lo ? w : 0.0;
+        front += f;
+        if (LEAST) kept += f >= set.min_p ? f : 0.0;
+        if (TOTAL != kNone) all += TOTAL == kAll || t[j] < upto ? w : 0.0;
+    }
+    above += front; total += all;
+    return LEAST ? kept : front;
+}
+
 // where the cuts may end, from the histogram; c.near
 template <int NT, typename Count, typename Mass>
 __device__ __forceinline__ void draw_bracket(DrawCut& c, const Count& count, const Mass& mass, const DrawRow& set, long long V, bool by_k, bool by_p)
@@ -823,11 +846,12 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
     const int groups = row.groups();
     const DrawRow set = draw_row(a, r);
     float top = -__builtin_inff();
-    for (int g = tid; g < groups; g += 4 * NT) {
-        float l[4][4];
+    constexpr int kAhead = 2;                                        // groups in flight per thread, here and below: 256 rows of 131072 113 us with 2, 114 with 4, 121 with 8, 116 with 1
+    for (int g = tid; g < groups; g += kAhead * NT) {
+        float l[kAhead][4];
         row.load_many(g, NT, groups, l);
 #pragma unroll
-        for (int q = 0; q < 4; q++)
+        for (int q = 0; q < kAhead; q++)
 #pragma unroll
             for (int j = 0; j < 4; j++) top = fmaxf(top, l[q][j]);
     }
@@ -840,24 +864,12 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
     }
     const float raw_top = top;
     top = row.finite_top(top);
-    // f(l, i) for every token of the row, over all threads
-    auto tokens = [&](auto f) {
-        for (int g0 = 0; g0 < groups; g0 += 4 * NT) {
-            float l[4][4];
-            row.load_many(g0 + tid, NT, groups, l);
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (l[q][j] == l[q][j]) f(l[q][j], 4 * (g0 + q * NT + tid) + j - row.off);
-        }
-    };
     auto all_groups = [&](auto f) {                                  // every thread of a wave, also where the wave reaches beyond the row
-        for (int g0 = 0; g0 < groups; g0 += 4 * NT) {
-            float l[4][4];
+        for (int g0 = 0; g0 < groups; g0 += kAhead * NT) {
+            float l[kAhead][4];
             row.load_many(g0 + tid, NT, groups, l);
 #pragma unroll
-            for (int q = 0; q < 4; q++)
+            for (int q = 0; q < kAhead; q++)
                 if (g0 + q * NT < groups) f(l[q], g0 + q * NT + tid);
         }
     };
@@ -868,7 +880,15 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         for (int b = tid; b < kDrawBins; b += NT) hist.hi[b] = 0;
         __syncthreads();
         const float units = (float)(set.inv_t * 0x1.71547652b82fep+0);
-        tokens([&](float l, int) { draw_near_add(hist.hi, l, top, set.scale, units); });
+        all_groups([&](const float (&l)[4], int g) {
+            if (__all(row.whole(g)))                                 // no choice per token: 3 us of a row of 131072
+#pragma unroll
+                for (int j = 0; j < 4; j++) draw_near_add(hist.hi, l[j], top, set.scale, units);
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (l[j] == l[j]) draw_near_add(hist.hi, l[j], top, set.scale, units);
+        });
         __syncthreads();
         draw_bracket<NT>(c, [&](int b) { return draw_near_count(hist.hi[b]); }, [&](int b) { return draw_near_mass(hist.hi[b]); }, set, a.V, by_k, by_p);
         const int bk = c.near.bk, lo = by_p ? c.near.lo : bk, hi = by_p ? c.near.hi : bk;
@@ -876,37 +896,41 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
         if (PICK) for (int q = tid; q < kDrawWaveTiles; q += NT) { hist.hi[q] = 0; hist.lo[q] = 0; tile[q] = 0.0; }
         __syncthreads();
         // 64-bit weights: of all tokens for the total of a top p, in front of the bracket for its sum and for the tiles
-        const int sums_to = by_p ? (by_k ? bk - 1 : kDrawBins - 1) : lo - 1;
+        const float lo_t = (float)lo, hi_t = (float)(hi + 1), bk_t = (float)(by_k ? bk : kDrawBins), front = fminf(lo_t, bk_t);
         double above = 0.0, total = 0.0;
-        auto pass = [&](const float (&l)[4], int g) {
-            int b[4];
-            bool in[4], sums = false;
+        auto pass = [&](auto kind, auto least) {
+            all_groups([&](const float (&l)[4], int g) {
+                float t[4];
+                bool in[4], some = false, sums = kind == kAll;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                b[j] = l[j] == l[j] ? draw_bin(l[j], top, set.scale) : kDrawBins;
-                in[j] = (b[j] >= lo && b[j] <= hi) || (by_k && b[j] == bk);
-                sums |= b[j] <= sums_to;
-                if (in[j]) {
-                    const uint32_t slot = atomicAdd(&c.slots, 1u);
-                    if (slot < (uint32_t)(NT < kDrawCand ? NT : kDrawCand)) sh.cand.rank[slot] = draw_rank(l[j], 4 * g + j - row.off);
+                for (int j = 0; j < 4; j++) {
+                    t[j] = draw_depth(l[j], top, set.scale);
+                    in[j] = l[j] == l[j] && ((t[j] >= lo_t && t[j] < hi_t) || (t[j] >= bk_t && t[j] < bk_t + 1.0f));
+                    some |= in[j];
+                    sums |= t[j] < (kind == kUpto ? bk_t : front);
                 }
-            }
-            if (!__any(sums)) return;                                // its tile has been cleared
-            double sum = 0.0;
+                if (__any(some))
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const double w = draw_weight(l[j], top, set.inv_t);
-                total += b[j] <= sums_to ? w : 0.0;
-                const double front = b[j] <= sums_to && b[j] < lo ? w : 0.0;
-                above += front;
-                sum += front >= set.min_p ? front : 0.0;
-            }
-            if (PICK && lo > 0) {
-                sum = draw_wave_scan(sum);
-                if (lane == 63) tile[g >> 6] = sum;
-            }
+                    for (int j = 0; j < 4; j++)
+                        if (in[j]) {
+                            const uint32_t slot = atomicAdd(&c.slots, 1u);
+                            if (slot < (uint32_t)(NT < kDrawCand ? NT : kDrawCand)) sh.cand.rank[slot] = draw_rank(l[j], 4 * g + j - row.off);
+                        }
+                if (!__any(sums)) return;                            // its tile has been cleared
+                double sum = draw_group_sums<kind.value, least.value>(l, t, front, bk_t, top, set, above, total);
+                if (PICK && lo > 0) {
+                    sum = draw_wave_scan(sum);
+                    if (lane == 63) tile[g >> 6] = sum;
+                }
+            });
         };
-        all_groups(pass);
+        auto pass_of = [&](auto kind) {
+            if (set.min_p > 0.0) pass(kind, std::true_type{});
+            else pass(kind, std::false_type{});
+        };
+        if (!by_p) pass_of(std::integral_constant<int, kNone>{});
+        else if (by_k) pass_of(std::integral_constant<int, kUpto>{});
+        else pass_of(std::integral_constant<int, kAll>{});
         __syncthreads();
         if (by_p) draw_sums<NT>(above, total, c.wave_2);
         __syncthreads();
@@ -1148,7 +1172,8 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
     // a short list takes everything up to bin bk: the row ends in draw_floor_kernel then
     const bool listed = draw_all_listed(near, by_k);
     const int bk = near.bk, lo = listed ? 0 : by_p ? near.lo : bk, hi = listed ? bk : by_p ? near.hi : bk;
-    const int sums_to = listed || !by_p ? -1 : by_k ? bk - 1 : kDrawBins - 1;
+    const float lo_t = (float)lo, hi_t = (float)(hi + 1), bk_t = (float)(by_k ? bk : kDrawBins), front = fminf(lo_t, bk_t);
+    const bool apart = by_k && (bk < lo || bk > hi);
     const int lane = threadIdx.x & 63;
     u64* stash = s_list[threadIdx.x >> 6];
     double above = 0.0, total = 0.0;
@@ -1165,42 +1190,42 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
         if (lane == 0) at = atomicAdd(&a.list_n[r], (uint32_t)held);
         flush_to((uint32_t)__builtin_amdgcn_readfirstlane((int)at));
     };
-    draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], int g) {
-        int b[4];
-        bool in[4], sums = false, some = false;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            b[j] = l[j] == l[j] ? draw_bin(l[j], top, set.scale) : kDrawBins;
-            in[j] = (b[j] >= lo && b[j] <= hi) || (by_k && b[j] == bk);
-            sums |= b[j] <= sums_to;
-            some |= in[j];
-        }
-        if (__any(sums))
+    auto pass = [&](auto kind) {
+        draw_walk<kDrawWalk>(a, row, [&](const float (&l)[4], int g) {
+            float t[4];
+            bool in[4], some = false, sums = kind == kAll;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const double w = draw_weight(l[j], top, set.inv_t);
-                total += b[j] <= sums_to ? w : 0.0;
-                above += b[j] <= sums_to && b[j] < lo ? w : 0.0;
+                t[j] = draw_depth(l[j], top, set.scale);
+                in[j] = l[j] == l[j] && t[j] >= lo_t && t[j] < hi_t;
+                if (apart) in[j] = in[j] || (l[j] == l[j] && t[j] >= bk_t && t[j] < bk_t + 1.0f);
+                some |= in[j];
+                sums |= t[j] < bk_t;
             }
-        if (__any(some)) {
+            if (kind != kNone && __any(sums)) draw_group_sums<kind.value, false>(l, t, front, bk_t, top, set, above, total);
+            if (__any(some)) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const u64 who = __ballot(in[j]);
-                if (in[j]) stash[held + __popcll(who & ((1ull << lane) - 1))] = draw_rank(l[j], 4 * g + j - row.off);
-                held += __popcll(who);
+                for (int j = 0; j < 4; j++) {
+                    const u64 who = __ballot(in[j]);
+                    if (in[j]) stash[held + __popcll(who & ((1ull << lane) - 1))] = draw_rank(l[j], 4 * g + j - row.off);
+                    held += __popcll(who);
+                }
+                if (held > kStash - 256) flush();
             }
-            if (held > kStash - 256) flush();
-        }
-    });
+        });
+    };
+    if (listed || !by_p) pass(std::integral_constant<int, kNone>{});
+    else if (by_k) pass(std::integral_constant<int, kUpto>{});
+    else pass(std::integral_constant<int, kAll>{});
     // what is left, with one atomic for the workgroup: atomics on one address take some 10 ns each
     if (lane == 0) s_held[threadIdx.x >> 6] = (uint32_t)held;
     __syncthreads();
-    uint32_t front = 0, all = 0;
+    uint32_t ahead = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) { if (w == (int)(threadIdx.x >> 6)) front = all; all += s_held[w]; }
+    for (int w = 0; w < kWaves; w++) { if (w == (int)(threadIdx.x >> 6)) ahead = all; all += s_held[w]; }
     if (threadIdx.x == 0) s_held[kWaves] = all ? atomicAdd(&a.list_n[r], all) : 0;
     __syncthreads();
-    flush_to(s_held[kWaves] + front);
+    flush_to(s_held[kWaves] + ahead);
     draw_sums<kDrawWalk>(above, total, s_2);
     if (threadIdx.x == 0) {
         a.sums[(r * a.walkers + blockIdx.x) * 2] = above;
