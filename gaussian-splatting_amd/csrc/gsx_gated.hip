@@ -38,21 +38,20 @@ struct GatedArgs {
 template <typename T, int NV>
 struct alignas(sizeof(T) * NV) Pack { T v[NV]; };
 
-// Packs read or written past the caches (LAST).  A walk of whole columns reads what nothing will read soon and more than the caches hold: 1 M channels x 60 steps 142 us
-// through them, 118 past them; 32 layers of 800 x 800 forward 92, 70.  Its backward reads what the forward has left there and writes its gradients past it: 131, 114.
-// States are written through (118, past 131), and a split walk reads again what its fold has read.
-template <bool LAST, typename P>
+// What a walk reads for the last time and writes goes past the caches, which hold less than it: 1 M channels x 60 steps 146 us through them, 136 past them; 32 layers of
+// 800 x 800, both ways, 208 and 188.  What the fold of a split walk reads is read again by the walk, and stays: 96 channels x 100001 steps 42.5 us past the caches, 35.7
+// through them; so do the inputs of a split backward (8 x 2048 x 2048: 145, 141).
+template <bool PAST, typename P>
 __device__ __forceinline__ P pack_load(const void* at)
 {
     using W = std::conditional_t<sizeof(P) == 2, uint16_t, std::conditional_t<sizeof(P) == 4, uint32_t, unsigned long long>>;
-    return __builtin_bit_cast(P, LAST ? __builtin_nontemporal_load((const W*)at) : *(const W*)at);
+    return __builtin_bit_cast(P, PAST ? __builtin_nontemporal_load((const W*)at) : *(const W*)at);
 }
-template <bool LAST, typename P>
+template <typename P>
 __device__ __forceinline__ void pack_store(void* at, const P& p)
 {
     using W = std::conditional_t<sizeof(P) == 2, uint16_t, std::conditional_t<sizeof(P) == 4, uint32_t, unsigned long long>>;
-    const W w = __builtin_bit_cast(W, p);
-    if (LAST) __builtin_nontemporal_store(w, (W*)at); else *(W*)at = w;
+    __builtin_nontemporal_store(__builtin_bit_cast(W, p), (W*)at);
 }
 
 template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
@@ -101,7 +100,7 @@ __device__ __forceinline__ Lane lane_of(const GatedArgs& p, long long group)
     return l;
 }
 
-template <typename T, int FORM, int NV, int R, int K, bool SPLIT, bool WHOLE>
+template <typename T, int FORM, int NV, int R, int K, bool WHOLE>
 __device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& l, long long group, long long s0, float (&h)[R][NV])
 {
     using P = Pack<T, NV>;
@@ -113,9 +112,9 @@ __device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& 
     for (int k = 0; k < K; k++)
     {
         if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
-            z[k] = pack_load<!SPLIT, P>(gp);
+            z[k] = pack_load<true, P>(gp);
 #pragma unroll
-            for (int r = 0; r < R; r++) x[k][r] = pack_load<!SPLIT, P>(xp + r * p.x_r);
+            for (int r = 0; r < R; r++) x[k][r] = pack_load<true, P>(xp + r * p.x_r);
         }
         gp += dir * p.gate_t; xp += dir * p.x_t;                             // one step on: the multiples of a step would fill the scalar registers
     }
@@ -148,7 +147,7 @@ __device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& 
                 P o;
 #pragma unroll
                 for (int i = 0; i < NV; i++) o.v[i] = in ? from_f<T>(h[r][i]) : from_f<T>(0.0f);
-                *(P*)(sp + r * p.D) = o;
+                pack_store(sp + r * p.D, o);
             }
         }
         sp += dir * R * p.D;
@@ -337,8 +336,8 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
     if (!l.on) return;
     gated_formed(p.form, [&](auto form) {
         for (long long s0 = sp.s0; s0 < sp.s1; s0 += K) {
-            if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fwd_batch<T, form.value, NV, R, K, SPLIT, true>(p, l, group, s0, h);
-            else gated_fwd_batch<T, form.value, NV, R, K, SPLIT, false>(p, l, group, s0, h);
+            if (__all(s0 >= l.lo && s0 + K <= l.hi)) gated_fwd_batch<T, form.value, NV, R, K, true>(p, l, group, s0, h);
+            else gated_fwd_batch<T, form.value, NV, R, K, false>(p, l, group, s0, h);
         }
     });
     if (!SPLIT || sp.index == p.blocks * kGatedSpans - 1)
@@ -368,11 +367,11 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
     for (int k = 0; k < K; k++)
     {
         if (WHOLE || (s0 + k >= l.lo && s0 + k < l.hi)) {
-            z[k] = *(const P*)gp;
+            z[k] = pack_load<!SPLIT, P>(gp);
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                x[k][r] = *(const P*)(xp + r * p.x_r);
-                if (HASD) d[k][r] = *(const P*)(dp + r * p.ds_r);
+                x[k][r] = pack_load<!SPLIT, P>(xp + r * p.x_r);
+                if (HASD) d[k][r] = pack_load<!SPLIT, P>(dp + r * p.ds_r);
             }
         }
         gp += dir * p.gate_t; xp += dir * p.x_t; dp += dir * p.ds_t;
@@ -420,10 +419,10 @@ __device__ __forceinline__ void gated_bwd_batch(const GatedArgs& p, const Lane& 
             }
         }
         if (WHOLE || s0 + k < p.T) {
-            if (p.d_gate) pack_store<!SPLIT>(ogp, oz);
+            if (p.d_gate) pack_store(ogp, oz);
             if (p.d_x)
 #pragma unroll
-                for (int r = 0; r < R; r++) pack_store<!SPLIT>(oxp + r * p.D, ox[r]);
+                for (int r = 0; r < R; r++) pack_store(oxp + r * p.D, ox[r]);
         }
         ogp -= dir * p.D; oxp -= dir * R * p.D;
     }
