@@ -15,6 +15,9 @@
 // A histogram's 2048 bins are 1/64 of a unit of (top - l) / T wide: the tokens spread over hundreds of bins (few collisions in LDS), and the bin where
 // a cut falls holds few enough tokens to be ranked in LDS.  Where it does not (ties, extreme temperatures), narrower histograms of the 59-bit rank
 // (key, index) follow until it does: every row ends, whatever its values.
+// Measured, us a call and what bounds it: 640000 rows of 32, 4 draws each, 55 (short; issue, 475 instructions a wave of eight rows); one row of 5000 16 (row; a workgroup's chain
+// of passes); 256 rows of 131072 in 32 bits 117 (row; the top 16, the histogram 17, the pass of 64-bit weights 50 by issue, the decision 7, against 26 for the bytes);
+// 64 rows of 100003 in 16 bits 49 (parts; seven launches that wait for one another); one row of 1 M and 1 M draws 48, of 6 M with a top p 138 (parts; loads that wait).
 #include <type_traits>
 #include "gsx_common.h"
 
@@ -1233,6 +1236,8 @@ __global__ __launch_bounds__(kDrawWalk) void draw_part_pass_kernel(DrawArgs a)
     }
 }
 
+// Draws that the one workgroup of a row with a short list makes itself (512 at a time); of more the whole card makes them.  One row of 265754, k = 161: 8192 draws 38 us by the workgroup, 40 by the card; 54914: 66, 40.
+constexpr int64_t kDrawInFloor = 8192;
 // one workgroup per row: the cuts among the list's tokens, of any number; -> a.floors
 template <typename T>
 __global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
@@ -1270,7 +1275,7 @@ __global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
         if (tid == 0) c.slots = (uint32_t)n;
         __syncthreads();
         done = draw_decide<NT>(c, sh.cand, set, top, by_k, by_p, above, total, all_listed);
-        if (all_listed) {                                            // and its draws, from the kept ones in index order
+        if (all_listed && a.S <= kDrawInFloor) {                     // and its draws, from the kept ones in index order
             const u64 rank = tid < n ? sh.cand.rank[tid] : 0;
             const float l = draw_rank_logit(rank);
             const double lw = tid < n && rank >= c.floor_rank ? draw_weight(l, top, set.inv_t) : 0.0;
@@ -1339,7 +1344,7 @@ __global__ __launch_bounds__(kDrawExact) void draw_floor_kernel(DrawArgs a)
 
 // the masses of a part: inclusive sums behind every group, counted from the part's start
 template <typename T>
-__global__ __launch_bounds__(kDrawPart, 6) void draw_part_mass_kernel(DrawArgs a)
+__global__ __launch_bounds__(kDrawPart, 5) void draw_part_mass_kernel(DrawArgs a)
 {
     __shared__ double s_d[kDrawPart / 64];
     __shared__ float s_f[kDrawPart / 64];
@@ -1366,7 +1371,7 @@ __global__ __launch_bounds__(kDrawPart, 6) void draw_part_mass_kernel(DrawArgs a
 #pragma unroll
                 for (int j = 0; j < 4; j++) sum += draw_kept(l[q][j], 4 * (g0 + b + q * kDrawPart + tid) + j - row.off, floor, top, set);
                 span[q * kDrawPart + tid] = sum;
-                __builtin_amdgcn_sched_barrier(0);                   // one group's exps at a time: 80 registers, six waves a SIMD
+                __builtin_amdgcn_sched_barrier(0);                   // one group's exps at a time, for five waves a SIMD (six spill, and gain nothing)
             }
             __syncthreads();
             double w[4], all;

@@ -341,3 +341,10 @@ def test_more_rows_than_compute_units(R, V, S, cut):
     for r in rows:
         want, _ = oracle_row(logits[r].double().cpu().numpy(), u[r].cpu().numpy(), float(np.float32(cut.get("T", 1.0))), cut.get("k", 0), float(np.float32(cut.get("p", 1.0))), 0.0)
         assert np.array_equal(got[r], want), (r, got[r], want)
+
+
+@pytest.mark.parametrize("S", [8192, 8193, 30000])
+@pytest.mark.parametrize("cut", [dict(k=100), dict(k=161, p=0.6, m=0.07, T=0.35)], ids=str)
+def test_many_draws_from_few_tokens(S, cut):
+    logits, u = rand(S, 2, 100001, S, f64=True)
+    check(logits, u, **cut)
