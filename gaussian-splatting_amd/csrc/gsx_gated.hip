@@ -9,7 +9,10 @@
 // 4 / K bytes per element) and the backward runs each batch forward again from its mark, in registers.  It then reads gate, x and
 // the states' gradient, once each -- as much as a backward that reads `states` instead of x, and `states` need not exist.
 // Few channels and many steps: the steps are split into spans, one per wave.  A first kernel folds every span to the (A, H) of
-// h -> A h + H, and every workgroup's spans to one; the second begins each span from what the spans in front of it come to.
+// h -> A h + H, and every workgroup's spans to one; the second begins each span from what the spans in front of it come to.  One pass that hands
+// the state from workgroup to workgroup would read once, but its waves would wait for one another in a chain of hundreds.
+// Measured, with other inputs and outputs in turn, against a copy's 5.15 TB/s: 60 steps x 1 M channels in 32 bits 134 us (5.4 TB/s); 32 layers of 800 x 800 (3 planes in
+// 32 bits) 66 us forward (5.5) and 120 backward (5.7); split, 2 x 32768 x 512 in bf16, mean of the folds 31 us (4.3), walks 36 forward (5.8) and 62 backward (5.5).
 #include <type_traits>
 #include "gsx_common.h"
 

@@ -128,7 +128,8 @@ def gated_scan(gate, x, initial=None, lengths=None, form="linear", reverse=False
     return_states=False) is rounded once.
     lengths (B) int32: sequence b consists of its first lengths[b] steps; what lies behind is not read, states and gradients there are
     zero.  reverse: from step T - 1 (or lengths[b] - 1) down to 0.
-    Differentiable once in gate, x and initial; a gate expanded over a batch costs what its full size costs."""
+    Differentiable once in gate, x and initial; a gate expanded over a batch costs what its full size costs.  Can be captured into a graph; capture
+    its backward with torch.autograd.grad, or while no earlier graph of the same leaves is alive (torch would accumulate on that one's stream)."""
     _check_pair(gate, x, form)
     if gate.dim() != 3 or x.dim() not in (3, 4) or gate.shape != x.shape[:2] + x.shape[-1:]:
         raise ValueError(f"gate (B, T, D) and x (B, T, D) or (B, T, P, D) are wanted, got {tuple(gate.shape)} and {tuple(x.shape)}")
