@@ -1391,8 +1391,8 @@ __global__ __launch_bounds__(kDrawPart, 5) void draw_part_mass_kernel(DrawArgs a
 
 // Draws of a row in parts.  What bounds many of them is the chain of loads that wait for each other and the lines that these touch; so the sums behind every 1 / nodes of a
 // part lie in LDS, down to 16 groups where they fit, the sums behind every 16 groups lie side by side, and a draw reads one line of each kind of sums and one of tokens.
-// Measured: 1 M tokens and draws 35 us, 6 M tokens and 1 M draws 75 us (88 with the steps down to 16 groups in the sums behind each group); two draws of a thread side by
-// side 38 and 85, four 41 and 91: with 16 waves a CU the loads of one draw hide behind those of others, and the registers of more cost waves.
+// Measured: 1 M tokens and draws 36 us, 6 M tokens and 1 M draws 55 us (68 with the steps down to 16 groups in the sums behind each group); two draws of a thread side by
+// side 3 and 10 us more, four 6 and 15: with 16 waves a CU the loads of one draw hide behind those of others, and the registers of more cost waves.
 constexpr int kDrawMostParts = 2048;
 constexpr int kDrawMostNodes = 16384;
 constexpr int64_t kDrawManyDraws = 1 << 15;         // from here on the nodes' 128 KB are worth their loading (1 M tokens: 64 draws 20.7 us with them, 19.0 without; 32768: 25.6, 26.4)
