@@ -1810,7 +1810,8 @@ using namespace gsx;
 
 GSX_API size_t gsx_draw_workspace_bytes(const gsx_draw* s)
 {
-    return draw_check(s) == GSX_OK ? draw_layout(s).bytes : 0;
+    if (draw_check(s) != GSX_OK) return 0;
+    return s->R == 0 || s->S == 0 ? 256 : draw_layout(s).bytes;              // nothing to draw: no layout, which shares the card out over the rows
 }
 
 GSX_API int gsx_draw_indices(const gsx_draw* s, void* stream)

@@ -129,3 +129,14 @@ def test_structs_match_the_header():
         subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), os.path.join(d, "a.c"), "-o", os.path.join(d, "a")])
         got = [int(v) for v in subprocess.check_output([os.path.join(d, "a")], text=True).split()]
     assert got == [C.sizeof(L.GsxGated), L.GsxGated.d_initial.offset, C.sizeof(L.GsxDraw), L.GsxDraw.ws_bytes.offset]
+
+
+@pytest.mark.parametrize("V", [0, 10, 512, 513, 49152, 49153, 60000, 524284, 524285, 1 << 27])
+def test_workspace_of_a_batch_without_rows_or_draws(V):
+    """what a C caller asks for before a call that does nothing: a size, for every way that V alone would take"""
+    lib = L.lib()
+    for cut in (dict(), dict(top_k=5, top_p=0.5)):
+        s = dict(dtype=0, R=2, V=V, S=1, row_stride=V, temperature=1.0, top_p=1.0, min_p=0.0, top_k=0)
+        for none in (dict(R=0), dict(S=0), dict(R=0, S=0)):
+            d = L.GsxDraw(**dict(s, **cut, **none))
+            assert 0 < lib.gsx_draw_workspace_bytes(d) <= 256 and lib.gsx_draw_indices(d, None) == L.GSX_OK
