@@ -26,18 +26,20 @@ def _channels(t):
 
 # struct gsx_gated as bytes: filling the ctypes structure field by field takes several times as long
 _PACK = struct.Struct("4i3qQ2qQ3q5QQ3q4QQQ").pack
-_entry = {}
+_entry = None
 
 
 def _entries():
-    """(workspace, forward, backward) that take the packed struct"""
-    if not _entry:
-        lib = L.lib()
+    """(workspace, forward, backward) that take the packed struct; the table is whole before another thread can see it"""
+    global _entry
+    if _entry is None:
+        lib, entry = L.lib(), {}
         for name, argtypes, restype in (("gsx_gated_workspace_bytes", [C.c_char_p, C.c_int32], C.c_size_t),
                                         ("gsx_gated_scan_fwd", [C.c_char_p, C.c_void_p], C.c_int), ("gsx_gated_scan_bwd", [C.c_char_p, C.c_void_p], C.c_int)):
             fn = lib[name]                                       # a function object of its own: the binding's keeps its types
             fn.argtypes, fn.restype = argtypes, restype
-            _entry[name] = fn
+            entry[name] = fn
+        _entry = entry
     return _entry
 
 

@@ -140,3 +140,23 @@ def test_workspace_of_a_batch_without_rows_or_draws(V):
         for none in (dict(R=0), dict(S=0), dict(R=0, S=0)):
             d = L.GsxDraw(**dict(s, **cut, **none))
             assert 0 < lib.gsx_draw_workspace_bytes(d) <= 256 and lib.gsx_draw_indices(d, None) == L.GSX_OK
+
+
+def test_first_calls_of_two_threads(monkeypatch):
+    """a second thread that comes while the first one fills the table of entry points gets a whole table"""
+    import threading
+    from gaussian_splatting_amd import recurrence
+    real, seen, threads = L.lib(), [], []
+
+    class Slow:
+        def __getitem__(self, name):
+            if name == "gsx_gated_scan_bwd" and not threads:         # two of the three are in the first thread's hands
+                threads.append(threading.Thread(target=lambda: seen.append(set(recurrence._entries()))))
+                threads[0].start()
+                threads[0].join()
+            return real[name]
+    slow = Slow()
+    monkeypatch.setattr(L, "lib", lambda: slow)
+    monkeypatch.setattr(recurrence, "_entry", None)
+    want = {"gsx_gated_workspace_bytes", "gsx_gated_scan_fwd", "gsx_gated_scan_bwd"}
+    assert set(recurrence._entries()) == want and seen == [want]
