@@ -150,16 +150,16 @@ def gated_scan(gate, x, initial=None, lengths=None, form="linear", reverse=False
 
 def gated_step(state, gate, x, form="linear"):
     """One step in place on a 32-bit state that lives between calls (a served stream): state, gate, x of one shape, contiguous.  -> state.
-    Not differentiable (gated_scan with one step is)."""
+    Not differentiable (gated_scan with one step is): under grad mode, arguments that require a gradient are refused."""
     _check_pair(gate, x, form)
     shape = state.shape
     if state.dtype != torch.float32 or shape != x.shape or gate.shape != shape or state.device != x.device:
         raise ValueError(f"state (float32), gate and x must share a shape and a device, got {tuple(state.shape)} {state.dtype}, {tuple(gate.shape)}, {tuple(x.shape)}")
     if not state.is_contiguous():
         raise ValueError("gated_step writes the state in place: it must be contiguous")
+    if (state.requires_grad or gate.requires_grad or x.requires_grad) and torch.is_grad_enabled():
+        raise RuntimeError("gated_step writes the state in place and leaves no graph: state, gate and x must not require a gradient")
     _refuse_host(x, "recurrence")
-    if state.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("gated_step writes the state in place and leaves no graph: the state must not require a gradient")
     gate, x = gate.contiguous(), x.contiguous()
     dev = x.device
     with L.on_device(dev):

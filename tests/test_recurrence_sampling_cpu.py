@@ -160,3 +160,13 @@ def test_first_calls_of_two_threads(monkeypatch):
     monkeypatch.setattr(recurrence, "_entry", None)
     want = {"gsx_gated_workspace_bytes", "gsx_gated_scan_fwd", "gsx_gated_scan_bwd"}
     assert set(recurrence._entries()) == want and seen == [want]
+
+
+@pytest.mark.parametrize("which", [0, 1, 2], ids=["state", "gate", "x"])
+def test_step_refuses_to_drop_a_gradient(which):
+    args = [z(4), z(4), z(4)]
+    args[which].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="require a gradient"):
+        gated_step(*args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+        gated_step(*args)
