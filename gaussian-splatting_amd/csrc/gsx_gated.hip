@@ -463,9 +463,9 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
 }
 
 // One step in place, for a state that lives between calls: 12 bytes and more per element, and at a serving batch's size (64 x 2048)
-// nothing but the launch.
+// nothing but the launch.  The state may itself be the gate or the input: a lane reads its elements of all three before it writes.
 template <typename T, int NV>
-__global__ __launch_bounds__(kBlock) void gated_step_kernel(float* __restrict__ state, const T* __restrict__ gate, const T* __restrict__ x, long long n, int form)
+__global__ __launch_bounds__(kBlock) void gated_step_kernel(float* state, const T* gate, const T* x, long long n, int form)
 {
     const long long i = ((long long)blockIdx.x * kBlock + threadIdx.x) * NV;
     if (i >= n) return;                                                      // NV divides n
@@ -652,6 +652,9 @@ GSX_API int gsx_gated_step(int32_t dtype, int32_t form, int64_t n, float* state,
     if (n == 0) return GSX_OK;
     if (!state || !gate || !x) return GSX_E_INVALID;
     const uintptr_t e = size_of(dtype);
+    // an input that shares memory with the state at another place would be read by one lane and written by another
+    auto meets = [&](const void* p) { return (uintptr_t)p < (uintptr_t)state + (uintptr_t)n * 4 && (uintptr_t)state < (uintptr_t)p + (uintptr_t)n * e && !(p == state && e == 4); };
+    if (meets(gate) || meets(x)) return GSX_E_INVALID;
     const bool four = n % 4 == 0 && ((uintptr_t)state & 15) == 0 && ((uintptr_t)gate & (4 * e - 1)) == 0 && ((uintptr_t)x & (4 * e - 1)) == 0;
     const int64_t blocks = ceil_div(n, four ? 4 * kBlock : kBlock);
     if (blocks > 0x7fffffffll) return GSX_E_RANGE;

@@ -149,7 +149,8 @@ def gated_scan(gate, x, initial=None, lengths=None, form="linear", reverse=False
 
 
 def gated_step(state, gate, x, form="linear"):
-    """One step in place on a 32-bit state that lives between calls (a served stream): state, gate, x of one shape, contiguous.  -> state.
+    """One step in place on a 32-bit state that lives between calls (a served stream): state, gate, x of one shape, contiguous; gate and x may be
+    the state itself, but may not overlap it otherwise.  -> state.
     Not differentiable (gated_scan with one step is): under grad mode, arguments that require a gradient are refused."""
     _check_pair(gate, x, form)
     shape = state.shape

@@ -426,7 +426,8 @@ int gsx_merge_greedy_host(int32_t N, const uint32_t* offsets_host, const uint32_
  * them, d_states and d_last (each may be NULL: zeros), and writes d_gate (B x T x D), d_x (B x T x planes x D) and d_initial, all
  * contiguous, each NULL if not wanted.  No atomics: results are the same bits every time.
  * ws: gsx_gated_workspace_bytes of the struct as it is handed over otherwise (often 0), 256-byte aligned; each call may have its own.
- * gsx_gated_step: one step in place on n contiguous elements, for a state that lives between calls (a served stream). */
+ * gsx_gated_step: one step in place on n contiguous elements, for a state that lives between calls (a served stream).  gate and x may be the
+ * state itself (GSX_F32), but may not share memory with it otherwise (GSX_E_INVALID). */
 #define GSX_F32 0
 #define GSX_BF16 1
 #define GSX_F16 2

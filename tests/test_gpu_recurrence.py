@@ -415,3 +415,21 @@ def test_two_streams_at_once():
     for a, out in zip(alone, outs):
         for o in out:
             assert all(torch.equal(p, q) for p, q in zip(a, o))
+
+
+def test_step_beside_and_upon_its_own_state():
+    """gate and input next to the state in one buffer, and the state as its own gate or input; an overlap is refused"""
+    from gaussian_splatting_amd import gated_step
+    for n in (64, 67, 4096):
+        buf = torch.rand(3 * n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(n))
+        s, g, x = buf[n:2 * n], buf[:n], buf[2 * n:]
+        was = buf.double().clone()
+        for gate, inp in ((g, x), (s, x), (g, s), (s, s)):
+            buf.copy_(was.float())
+            z, v, h = gate.double(), inp.double(), s.double()
+            gated_step(s, gate, inp)
+            assert bool(((s.double() - (z * h + v)).abs() <= 4 * U * ((z * h).abs() + v.abs())).all())
+            assert torch.equal(buf[:n].double(), was[:n]) and torch.equal(buf[2 * n:].double(), was[2 * n:])
+        for gate, inp in ((buf[n - 1:2 * n - 1], x), (g, buf[n + 1:2 * n + 1])):
+            with pytest.raises(RuntimeError, match="gsx_gated_step"):
+                gated_step(s, gate, inp)

@@ -170,3 +170,13 @@ def test_step_refuses_to_drop_a_gradient(which):
         gated_step(*args)
     with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
         gated_step(*args)
+
+
+def test_step_refuses_inputs_that_overlap_the_state():
+    """addresses only: none of these calls reaches a device"""
+    lib, at, n = L.lib(), 1 << 20, 64
+    far = at + 4096
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        for other in (at + 4, at - 4, at + 4 * n - size, at - size * n + size) + ((at,) if size == 2 else ()):
+            assert lib.gsx_gated_step(dtype, 0, n, at, other, far, None) == L.GSX_E_INVALID, (dtype, other - at)
+            assert lib.gsx_gated_step(dtype, 0, n, at, far, other, None) == L.GSX_E_INVALID, (dtype, other - at)
