@@ -188,7 +188,22 @@ __device__ __forceinline__ DrawRow draw_row(const DrawArgs& a, long long r)
 __device__ __forceinline__ double draw_uniform(const DrawArgs& a, long long t)
 {
     const double u = a.uniforms_f64 ? ((const double*)a.uniforms)[t] : (double)((const float*)a.uniforms)[t];
-    return u >= 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;                     // NaN: 0
+    return u >= 0.0 ? (u < 1.0 ? u : 0x1.fffffffffffffp-1) : 0.0;    // NaN: 0; u total stays below the total, also when rounded
+}
+
+// Where rounding has led a draw to a place `q` (> 0) without weight: the place to try next, in front of it.  Sums at(i) of two orders of addition differ by some units of
+// 2^-53 (less than 2^-47 of them) where no weight lies between, so the last place with weight is the first whose sum comes that near to the one in front of q.
+// One by one, a thread would walk over a whole row whose kept tokens lie at its start.
+template <typename At>
+__device__ __forceinline__ int draw_back(const At& at, int q)
+{
+    const double least = at(q - 1) * (1.0 - 0x1p-47);
+    int a = 0, b = q - 1;
+    while (a < b) {
+        const int mid = (a + b) >> 1;
+        if (at(mid) >= least) b = mid; else a = mid + 1;
+    }
+    return a;
 }
 
 __device__ __forceinline__ double draw_kept(float l, int i, const DrawFloor& floor, float top, const DrawRow& set)
@@ -782,7 +797,7 @@ __device__ __forceinline__ void draw_row_draws(const DrawArgs& a, long long r, c
             const double want = draw_uniform(a, r * a.S + s) * total;
             const int lo = draw_place([&](int i) { return tile[i]; }, tiles, draw_power(tiles), want);
             // the first token in the tile that exceeds; where rounding leaves none, the last one with weight
-            for (int q = lo; q >= 0; q--) {
+            for (int q = lo;;) {
                 const int g = q * 64 + lane;
                 float l[4];
                 row.load(g, groups, l);
@@ -795,7 +810,11 @@ __device__ __forceinline__ void draw_row_draws(const DrawArgs& a, long long r, c
                     if (w[j] > 0.0) { any = j; if (hit < 0 && run > want) hit = j; }
                 }
                 const u64 hits = __ballot(hit >= 0), some = __ballot(any >= 0);
-                if (!some) continue;
+                if (!some) {
+                    if (q == 0) break;                               // not with a top that weighs 1
+                    q = draw_back([&](int i) { return tile[i]; }, q);
+                    continue;
+                }
                 const int who = hits ? __ffsll((long long)hits) - 1 : 63 - __clzll((long long)some);
                 if (lane == who) {
                     const int j = hits ? hit : any;
@@ -1019,10 +1038,11 @@ __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long
     const double want = draw_uniform(a, t) * total;
     const int lo = draw_place([&](int i) { return spans[i]; }, row.groups(), draw_power(row.groups()), want);
     int index = -1; float at_l = 0.0f;
-    for (int q = lo; q >= 0 && index < 0; q--) {
+    for (int q = lo;; q = draw_back([&](int i) { return spans[i]; }, q)) {
         float l[4];
         row.load(q, row.groups(), l);
         index = draw_in_group(row, q, l, q ? spans[q - 1] : 0.0, want, floor, top, set, at_l);
+        if (index >= 0 || q == 0) break;
     }
     a.indices[t] = index;
     if (a.logprobs) a.logprobs[t] = draw_logprob(at_l, top, set.inv_t, draw_log(total));
@@ -1483,7 +1503,8 @@ __global__ __launch_bounds__(kDrawPickers) void draw_part_pick_kernel(DrawArgs a
         float l[4], at_l = 0.0f;
         row.load(lo, groups, l);
         int index = draw_in_group(row, lo, l, run, want, floor, top, set, at_l);
-        for (int q = lo - 1; q >= 0 && index < 0; q--) {             // nothing there: rounding; the last one in front with weight
+        for (int q = lo; index < 0 && q > 0;) {                      // nothing there: rounding; the last one in front with weight
+            q = draw_back([&](int i) { return s_part[i >> part_log] + spans[i]; }, q);
             row.load(q, groups, l);
             index = draw_in_group(row, q, l, s_part[q >> part_log] + (q & (a.part - 1) ? spans[q - 1] : 0.0), want, floor, top, set, at_l);
         }

@@ -29,7 +29,7 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ret
     """logits (R, V) float32 / bfloat16 / float16, uniforms (R, S) float32 or float64 in [0, 1) -> indices (R, S) int64 (and their log
     probabilities, float32).  Tokens are ranked by (logit descending, index ascending); kept are the first top_k (0: all), of these the
     fewest whose mass reaches top_p of their mass, of these the ones at least min_p times as likely as the first.  A draw is the lowest
-    index whose inclusive kept mass, in index order, exceeds u times all kept mass.
+    index whose inclusive kept mass, in index order, exceeds u times all kept mass (u of 1 and more: the largest double below 1; below 0 and NaN: 0).
     temperature (0: the lowest index of the largest logit), top_k, top_p and min_p are numbers or tensors of one value per row.  NaN and -inf logits
     are masked; a row with nothing left, or with a value of its own out of range, gives -1 (and -inf).  float32 uniforms have 24 bits:
     take float64 where V is in the millions.  Not differentiable."""

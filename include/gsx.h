@@ -464,7 +464,7 @@ int gsx_gated_step(int32_t dtype, int32_t form, int64_t n, float* state, const v
  * (<= 0: off), top_p > 0 (>= 1: off), 0 <= min_p <= 1 (0: off).  Tokens are ranked by (logit descending, index ascending).  Kept are the
  * first top_k; of these the fewest whose mass reaches top_p of their mass; of these the ones whose probability is at least min_p
  * times the largest.
- * uniforms R x S, contiguous, floats or (uniforms_f64) doubles in [0, 1) (outside: clamped; NaN: 0).  24 random bits cannot tell 2^24 tokens apart: give
+ * uniforms R x S, contiguous, floats or (uniforms_f64) doubles in [0, 1) (below and NaN: 0; 1 and above: the largest double below 1).  24 random bits cannot tell 2^24 tokens apart: give
  * doubles where V is large.  indices[r][s] = the lowest index whose inclusive mass over the kept tokens, in index order, exceeds
  * u * (all kept mass); logprobs (nullable) = the log of its share of the kept mass.  A row with nothing left, or with settings of its own
  * out of range, gets -1 and -inf.  Masses are summed in 64 bits in a fixed order: the same bits every time.

@@ -348,3 +348,40 @@ def test_more_rows_than_compute_units(R, V, S, cut):
 def test_many_draws_from_few_tokens(S, cut):
     logits, u = rand(S, 2, 100001, S, f64=True)
     check(logits, u, **cut)
+
+
+NEAR_ONE = [1.0, 1 - 2.0 ** -53, 7.0, math.inf, 1 - 2.0 ** -52, 1 - 2.0 ** -50, 0.5]
+
+
+@pytest.mark.parametrize("R,V,S", [(2, 15000, 7), (2, 15000, 70), (130, 70000, 7), (130, 70000, 18), (2, 300000, 7), (1, 1100003, 40000)])
+@pytest.mark.parametrize("cut", [dict(k=700), dict(m=0.01)], ids=str)
+def test_numbers_of_one_where_the_kept_tokens_come_first(R, V, S, cut):
+    """a thread or a wave of the row (both sizes), of the pick kernel, of the parts: behind the last kept token all sums agree but for rounding"""
+    from gaussian_splatting_amd import sample
+    g = torch.Generator(device="cuda").manual_seed(V + S)
+    logits = torch.full((R, V), -30.0, device="cuda")
+    logits[:, :700] = torch.rand(R, 700, generator=g, device="cuda")
+    u = torch.rand(R, S, generator=g, device="cuda", dtype=torch.float64)
+    u[:, :7] = torch.tensor(NEAR_ONE, dtype=torch.float64, device="cuda")
+    got = sample(logits, u, top_k=cut.get("k", 0), min_p=cut.get("m", 0.0)).cpu().numpy()
+    for r in {0, R - 1}:
+        want, _ = oracle_row(logits[r].double().cpu().numpy(), u[r].cpu().numpy(), 1.0, cut.get("k", 0), 1.0, float(np.float32(cut.get("m", 0.0))))
+        assert want[0] == 699 and np.array_equal(got[r], want), (r, np.nonzero(got[r] != want)[0][:5])
+    u32 = u.float()
+    assert torch.equal(sample(logits, u32, top_k=cut.get("k", 0), min_p=cut.get("m", 0.0))[:, :4], torch.from_numpy(got[:, :4]).cuda())
+
+
+def test_a_number_of_one_and_the_longest_row():
+    """the kept tokens are the first of 2^27: the draw looks for the last of them, it does not walk there (33 million groups, seconds)"""
+    from gaussian_splatting_amd import sample
+    from gaussian_splatting_amd.sampling import MAX_V
+    logits = torch.full((1, MAX_V), -100.0, dtype=torch.bfloat16, device="cuda")
+    logits[:, :600] = 1.0
+    u = torch.tensor([[1.0, 1 - 2.0 ** -53, 0.5, 2.0]], dtype=torch.float64, device="cuda")
+    sample(logits, u * 0.5, top_k=600)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    got = sample(logits, u, top_k=600)
+    end.record()
+    assert got.tolist() == [[599, 599, 300, 599]]
+    assert start.elapsed_time(end) < 500.0                            # ms: a few for the passes
