@@ -26,6 +26,15 @@ constexpr int kBlock = 256;        // 4 wave64
 constexpr int kRecVec = GSX_REC_FLOATS / 4;      // float4s per rank-ordered record (its stride; the first three hold the record)
 constexpr int kWave = 64;
 
+// A launch's threads along one axis must stay below 2^32.  Where calls may have more workgroups, they lie in rows of kGridRow (of 1024 threads at most); a kernel
+// asks block_of() for its place and leaves what lies behind the last one alone.
+constexpr int64_t kGridRow = 1 << 21;
+constexpr int64_t kMostBlocks = kGridRow * 65535;
+inline dim3 grid_of(int64_t blocks) { return dim3((unsigned)(blocks < kGridRow ? blocks : kGridRow), (unsigned)((blocks + kGridRow - 1) / kGridRow)); }
+#ifdef __HIPCC__
+__device__ __forceinline__ long long block_of() { return (long long)blockIdx.y * kGridRow + blockIdx.x; }
+#endif
+
 // Instances per compositing chunk for a view of D instances (gsx_constants.h): one wave composites one chunk, so a small
 // view cut into 256-instance chunks is a few hundred waves on 4096 wave slots, each running its 256 splats alone -- the
 // kernels then take one chunk's latency whatever the size of the scene.  Shorter chunks for smaller views; the choice is

@@ -861,7 +861,8 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
     __shared__ std::conditional_t<EXACT, Fine, Cand> sh;
     __shared__ double tile[PICK ? kDrawWaveTiles : 1];
     __shared__ DrawCut c;
-    const long long r = blockIdx.x;
+    const long long r = block_of();
+    if (r >= a.R) return;
     const int tid = threadIdx.x, lane = tid & 63;
     if (!EXACT && a.cuts && tid == 0) a.left[r] = 0;
     Places<T> row(a, r);
@@ -996,8 +997,8 @@ __global__ __launch_bounds__(kDrawExact) void draw_exact_kernel(DrawArgs a)
     __shared__ union { DrawFine fine; DrawCand cand; } sh;
     __shared__ double tile[PICK ? kDrawWaveTiles : 1];
     __shared__ DrawCut c;
-    const long long r = blockIdx.x;
-    if (!a.left[r]) return;
+    const long long r = block_of();
+    if (r >= a.R || !a.left[r]) return;
     Places<T> row(a, r);
     const DrawRow set = draw_row(a, r);
     const float raw_top = a.tops[r], top = row.finite_top(raw_top);
@@ -1025,7 +1026,7 @@ __device__ __forceinline__ int draw_in_group(const Places<T>& row, int g, const 
 template <typename T>
 __global__ __launch_bounds__(kBlock) void draw_pick_kernel(DrawArgs a, long long n)
 {
-    const long long t = (long long)blockIdx.x * kBlock + threadIdx.x;
+    const long long t = block_of() * kBlock + threadIdx.x;
     if (t >= n) return;
     const long long r = t / a.S;
     const double total = a.total[r];
@@ -1558,7 +1559,7 @@ __global__ __launch_bounds__(kBlock) void draw_short_kernel(DrawArgs a)
     __shared__ double s_total[kBlock / 64][kRows], s_log[kBlock / 64][kRows], s_inv[kBlock / 64][kRows];
     __shared__ float s_top[kBlock / 64][kRows];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / W, j0 = (lane % W) * E;
-    const long long r0 = ((long long)blockIdx.x * (kBlock / 64) + wave) * kRows, r = r0 + sub;
+    const long long r0 = (block_of() * (kBlock / 64) + wave) * kRows, r = r0 + sub;
     const int V = (int)a.V;
     const bool on = r < a.R;
     const DrawRow set = draw_row(a, on ? r : a.R - 1);
@@ -1771,7 +1772,7 @@ static DrawLayout draw_layout(const gsx_draw* s)
 template <typename T, int W, int E>
 static void draw_short(const DrawArgs& a, hipStream_t stream)
 {
-    draw_short_kernel<T, W, E><<<dim3((unsigned)ceil_div(a.R, (kBlock / 64) * (64 / W))), dim3(kBlock), 0, stream>>>(a);
+    draw_short_kernel<T, W, E><<<grid_of(ceil_div(a.R, (kBlock / 64) * (64 / W))), dim3(kBlock), 0, stream>>>(a);
 }
 
 template <typename T>
@@ -1807,7 +1808,7 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
         GSX_LAUNCH_CHECK();
         return GSX_OK;
     }
-    const dim3 grid((unsigned)a.R);
+    const dim3 grid = grid_of(a.R);
     const bool small = a.V <= (a.R <= kDrawCus ? kDrawSmall : kDrawSmallOfMany);
     if (l.way == DrawLayout::kRow) {
         if (small) draw_row_kernel<T, kDrawExact, true, true><<<grid, dim3(kDrawExact), 0, stream>>>(a);
@@ -1819,7 +1820,7 @@ static int draw_run(const DrawArgs& a, const DrawLayout& l, hipStream_t stream)
         if (!small && l.cuts) draw_exact_kernel<T, false><<<grid, dim3(kDrawExact), 0, stream>>>(a);
         GSX_LAUNCH_CHECK();
         const int64_t n = a.R * a.S;
-        draw_pick_kernel<T><<<dim3((unsigned)ceil_div(n, kBlock)), dim3(kBlock), 0, stream>>>(a, n);
+        draw_pick_kernel<T><<<grid_of(ceil_div(n, kBlock)), dim3(kBlock), 0, stream>>>(a, n);
     }
     GSX_LAUNCH_CHECK();
     return GSX_OK;

@@ -326,7 +326,7 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
     constexpr int K = GatedBatch<R>::value;
     Span sp;
     if (SPLIT) sp = span_of<false>(p);
-    else { sp.group = (long long)blockIdx.x * (64 * kGatedWaves) + threadIdx.x; sp.s0 = 0; sp.s1 = p.T; }
+    else { sp.group = block_of() * (64 * kGatedWaves) + threadIdx.x; sp.s0 = 0; sp.s1 = p.T; }
     const long long group = sp.group;
     const Lane l = lane_of<NV>(p, group);
     const long long out = (l.b * R) * p.D + l.d;                             // in B x R x D
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
     constexpr int K = GatedBatch<R>::value;
     Span sp;
     if (SPLIT) sp = span_of<true>(p);
-    else { sp.group = (long long)blockIdx.x * (64 * kGatedWaves) + threadIdx.x; sp.s0 = 0; sp.s1 = p.T; }
+    else { sp.group = block_of() * (64 * kGatedWaves) + threadIdx.x; sp.s0 = 0; sp.s1 = p.T; }
     const long long group = sp.group;
     const Lane l = lane_of<NV>(p, group);
     const long long out = (l.b * R) * p.D + l.d;
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(64 * (SPLIT ? kGatedSpans : kGatedWaves)) void gate
 template <typename T, int NV>
 __global__ __launch_bounds__(kBlock) void gated_step_kernel(float* state, const T* gate, const T* x, long long n, int form)
 {
-    const long long i = ((long long)blockIdx.x * kBlock + threadIdx.x) * NV;
+    const long long i = (block_of() * kBlock + threadIdx.x) * NV;
     if (i >= n) return;                                                      // NV divides n
     Pack<float, NV> h = *(const Pack<float, NV>*)(state + i);
     const Pack<T, NV> z = *(const Pack<T, NV>*)(gate + i), v = *(const Pack<T, NV>*)(x + i);
@@ -559,9 +559,7 @@ static int gated_launch(const gsx_gated* s, const GatedPlan& g, bool backward, h
         p.span = g.span; p.blocks = g.blocks; p.columns = g.columns;
         p.span_a = (double*)(ws + g.span_a); p.span_h = (double*)(ws + g.span_h);
         p.block_a = (double*)(ws + g.block_a); p.block_h = (double*)(ws + g.block_h);
-        const int64_t grid = g.columns * g.blocks;
-        if (grid > 0x7fffffffll) return GSX_E_RANGE;
-        const dim3 dg((unsigned)grid), db(64 * kGatedSpans);
+        const dim3 dg((unsigned)(g.columns * g.blocks)), db(64 * kGatedSpans);           // some kGatedWant waves
         if (backward) {
             if (p.d_states) gated_fold_kernel<T, NV, R, true, true><<<dg, db, 0, stream>>>(p);
             else gated_fold_kernel<T, NV, R, true, false><<<dg, db, 0, stream>>>(p);
@@ -574,9 +572,9 @@ static int gated_launch(const gsx_gated* s, const GatedPlan& g, bool backward, h
             gated_fwd_kernel<T, NV, R, true><<<dg, db, 0, stream>>>(p);
         }
     } else {
-        const int64_t grid = ceil_div(p.groups, 64 * kGatedWaves);
-        if (grid > 0x7fffffffll) return GSX_E_RANGE;
-        const dim3 dg((unsigned)grid), db(64 * kGatedWaves);
+        const int64_t blocks = ceil_div(p.groups, 64 * kGatedWaves);
+        if (blocks > kMostBlocks) return GSX_E_RANGE;
+        const dim3 dg = grid_of(blocks), db(64 * kGatedWaves);
         if (backward && p.d_states) gated_bwd_kernel<T, NV, R, false, true><<<dg, db, 0, stream>>>(p);
         else if (backward) gated_bwd_kernel<T, NV, R, false, false><<<dg, db, 0, stream>>>(p);
         else gated_fwd_kernel<T, NV, R, false><<<dg, db, 0, stream>>>(p);
@@ -657,8 +655,8 @@ GSX_API int gsx_gated_step(int32_t dtype, int32_t form, int64_t n, float* state,
     if (meets(gate) || meets(x)) return GSX_E_INVALID;
     const bool four = n % 4 == 0 && ((uintptr_t)state & 15) == 0 && ((uintptr_t)gate & (4 * e - 1)) == 0 && ((uintptr_t)x & (4 * e - 1)) == 0;
     const int64_t blocks = ceil_div(n, four ? 4 * kBlock : kBlock);
-    if (blocks > 0x7fffffffll) return GSX_E_RANGE;
-    const dim3 grid((unsigned)blocks), block(kBlock);
+    if (blocks > kMostBlocks) return GSX_E_RANGE;
+    const dim3 grid = grid_of(blocks), block(kBlock);
     hipStream_t st = (hipStream_t)stream;
 #define GSX_STEP(T) do { if (four) gated_step_kernel<T, 4><<<grid, block, 0, st>>>(state, (const T*)gate, (const T*)x, n, form); \
                          else gated_step_kernel<T, 1><<<grid, block, 0, st>>>(state, (const T*)gate, (const T*)x, n, form); } while (0)

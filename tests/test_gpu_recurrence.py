@@ -433,3 +433,26 @@ def test_step_beside_and_upon_its_own_state():
         for gate, inp in ((buf[n - 1:2 * n - 1], x), (g, buf[n + 1:2 * n + 1])):
             with pytest.raises(RuntimeError, match="gsx_gated_step"):
                 gated_step(s, gate, inp)
+
+
+def test_more_lanes_than_one_axis_of_a_launch():
+    """more than 2^32 threads: every channel of every sequence, both ways, and one step.  One step of time, so the values are exact"""
+    from gaussian_splatting_amd import gated_scan, gated_step
+    B, D = 65537, 65536
+    x = torch.randn(1, 1, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).requires_grad_(True)
+    gate = torch.full((1, 1, D), 0.5, device="cuda").expand(B, 1, D)
+    _, last = gated_scan(gate, x.expand(B, 1, D), return_states=False)
+    for b in range(0, B, 4096):
+        assert bool((last[b:b + 4096] == x[0]).all()), b
+    (dx,) = torch.autograd.grad(last, x, torch.ones(1, D, device="cuda").expand(B, D))
+    assert bool((dx == float(B)).all())                              # a sum of B ones
+    del last, dx
+    n = (1 << 32) + 257                                              # odd: a lane per element
+    half = torch.full((n,), 0.5, dtype=torch.bfloat16, device="cuda")
+    state = torch.full((n,), 2.0, device="cuda")
+    state[-1] = 4.0
+    gated_step(state, half, half)
+    assert float(state[-1]) == 2.5
+    state[-1] = 1.5
+    for i in range(0, n, 1 << 28):
+        assert bool((state[i:i + (1 << 28)] == 1.5).all()), i

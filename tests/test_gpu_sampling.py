@@ -385,3 +385,27 @@ def test_a_number_of_one_and_the_longest_row():
     end.record()
     assert got.tolist() == [[599, 599, 300, 599]]
     assert start.elapsed_time(end) < 500.0                            # ms: a few for the passes
+
+
+def test_more_rows_and_draws_than_one_axis_of_a_launch():
+    """more than 2^32 threads in each kind of kernel: lanes of short rows, workgroups of rows, threads of draws"""
+    from gaussian_splatting_amd import sample
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for R, V in (((1 << 26) + 5, 200), ((1 << 23) + 3, 513)):
+        logits = 2 * torch.randn(1, V, generator=g, device="cuda")
+        u = torch.rand(R, 1, generator=g, device="cuda", dtype=torch.float64)
+        c = torch.cumsum(torch.exp(logits[0].double() - logits.max().double()), 0)
+        got = sample(logits.expand(R, V), u)
+        for r in range(0, R, 1 << 24):
+            want = torch.searchsorted(c, u[r:r + (1 << 24), 0] * c[-1], right=True)
+            assert torch.equal(got[r:r + (1 << 24), 0], want), (R, V, r)
+        del got, u
+    R, V = 600, 700
+    S = (1 << 32) // R + 9
+    logits = 2 * torch.randn(1, V, generator=g, device="cuda")
+    u = torch.rand(1, S, generator=g, device="cuda")
+    c = torch.cumsum(torch.exp(logits[0].double() - logits.max().double()), 0)
+    want = torch.searchsorted(c, u[0].double() * c[-1], right=True)
+    got = sample(logits.expand(R, V), u.expand(R, S))
+    for r in range(R):
+        assert torch.equal(got[r], want), r
