@@ -1759,7 +1759,8 @@ static DrawLayout draw_layout(const gsx_draw* s)
             if (l.walkers > kDrawFewWalkers) { l.row_n = take(R * kDrawBins * 4); l.row_m = take(R * kDrawBins * 8); }
             l.near = take(R * sizeof(DrawNear));
             l.sums = take(R * l.walkers * 16);
-            // room for every token of a few rows, a quarter of a million at least of each of many; what does not fit goes the exact way
+            // 2^24 / R tokens of each row, 4096 at least (131072 at the 128 rows up to which ordinary lengths come here; from 4096 rows on, all of more than 524284
+            // tokens, the 4096): a longer list is not kept, and one workgroup finds that row's cuts from the row itself
             int64_t most = (1ll << 24) / s->R;
             if (most < 4096) most = 4096;
             l.list_most = s->V < most ? s->V : most;

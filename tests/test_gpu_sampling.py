@@ -434,3 +434,17 @@ def test_dense_points_of_a_small_scene():
     want, _ = oracle_row(m.opacity.detach().double().cpu().numpy()[:, 0], u.cpu().numpy(), 1.0, 0, float(np.float32(0.9)), 0.0)
     want = torch.from_numpy(want).cuda()
     assert torch.equal(pts, torch.cat([m.positions[want], m.features[want]], 1))
+
+
+@pytest.mark.parametrize("R,V", [(4100, 524301), (128, 200001)])
+def test_lists_that_do_not_fit(R, V):
+    """many long rows, whose cuts lie among more tokens than the row's list has room for (4096, and 131072)"""
+    from gaussian_splatting_amd import sample
+    g = torch.Generator(device="cuda").manual_seed(R)
+    logits = torch.randn(R, V, generator=g, device="cuda", dtype=torch.bfloat16)
+    u = torch.rand(R, 5, generator=g, device="cuda", dtype=torch.float64)
+    for cut in (dict(T=300.0, p=0.6), dict(T=300.0, k=V // 2, p=0.9)):
+        got = sample(logits, u, temperature=cut["T"], top_k=cut.get("k", 0), top_p=cut["p"]).cpu().numpy()
+        for r in (0, R // 3, R - 1):
+            want, _ = oracle_row(logits[r].double().cpu().numpy(), u[r].cpu().numpy(), 300.0, cut.get("k", 0), float(np.float32(cut["p"])), 0.0)
+            assert np.array_equal(got[r], want), (r, cut, got[r], want)
