@@ -448,3 +448,20 @@ def test_lists_that_do_not_fit(R, V):
         for r in (0, R // 3, R - 1):
             want, _ = oracle_row(logits[r].double().cpu().numpy(), u[r].cpu().numpy(), 300.0, cut.get("k", 0), float(np.float32(cut["p"])), 0.0)
             assert np.array_equal(got[r], want), (r, cut, got[r], want)
+
+
+@pytest.mark.parametrize("R,V,S", [(2, 3001, 5), (2, 3001, 70), (300, 40001, 5), (2, 40001, 5), (2, 40001, 70), (129, 120001, 3), (2, 100001, 5), (2, 100001, 40000), (128, 300001, 3)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_long_ties_under_both_cuts(R, V, S, dtype):
+    """top-k and top-p together among more equal tokens than are ranked at once, through every kernel that finds a cut exactly: the row's own of 512 threads (3001,
+    300 x 40001), the one behind the row's of 1024 (2 x 40001, 129 x 120001), the one of rows in parts, from its list and (300001) from the row"""
+    from gaussian_splatting_amd import sample
+    g = torch.Generator(device="cuda").manual_seed(V)
+    logits = torch.randint(0, 2, (R, V), generator=g, device="cuda").to(DT[dtype])
+    u = torch.rand(R, S, generator=g, device="cuda", dtype=torch.float64)
+    rows = sorted({0, 1, R // 2, R - 1})
+    for k, p, m in ((V // 3, 0.5, 0.0), (V - V // 4, 0.8, 0.0), (V - 1, 0.97, 0.0), (2 * V // 3, 0.6, 0.5), (700, 0.9, 0.0)):
+        got = sample(logits, u, top_k=k, top_p=p, min_p=m).cpu().numpy()
+        for r in rows:
+            want, _ = oracle_row(logits[r].double().cpu().numpy(), u[r].cpu().numpy(), 1.0, k, float(np.float32(p)), float(np.float32(m)))
+            assert np.array_equal(got[r], want), (r, k, p, np.nonzero(got[r] != want)[0][:4])
