@@ -158,8 +158,13 @@ __device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& 
 }
 
 // A product of gates in 64 bits that stays finite: times a zero state it is a zero, times any other one it leaves 32 bits, as the walk would.  Four more gates of up to 2^128
-// reach 2^1012 at most, two products 2^1000.
-__device__ __forceinline__ double gated_bound(double A) { return fmin(fmax(A, -0x1p500), 0x1p500); }
+// reach 2^1012 at most, two products 2^1000.  And that stays off zero, unless a gate is one: an infinite state stays infinite, as in the walk, and any other one falls
+// below 32 bits all the same (2^128 2^-400).  Four more gates of 2^-149 at least leave 2^-996, two products 2^-800.
+__device__ __forceinline__ double gated_bound(double A)
+{
+    const double m = fmin(fabs(A), 0x1p500);
+    return copysign(A != 0.0 ? fmax(m, 0x1p-400) : 0.0, A);
+}
 
 // Folds steps [s0, s0 + K) to h -> A h + H, in 64 bits: H and A h may be far larger than the state that they add up to, and a 32-bit H would
 // then be less exact than the walk itself (its 64-bit FMA is as fast on this card as the 32-bit one).  Backward: c -> A c + H of c_t = a_t (d_t + c_(t+1)), from the last step to the first.

@@ -456,3 +456,29 @@ def test_more_lanes_than_one_axis_of_a_launch():
     state[-1] = 1.5
     for i in range(0, n, 1 << 28):
         assert bool((state[i:i + (1 << 28)] == 1.5).all()), i
+
+
+@pytest.mark.parametrize("form", ["linear", "blend", "over"])
+def test_infinities_stay_where_the_walk_has_them(form):
+    """an infinite state outlives gates whose product leaves 64 bits, also across spans that are walked apart; a zero gate makes it a NaN"""
+    from gaussian_splatting_amd import gated_scan
+    inf, T, D = float("inf"), 9001, 8
+    a = torch.full((1, T, D), 0.25, dtype=torch.float64, device="cuda")
+    a[:, 6000, 3] = 0.0
+    gate = (a if form == "linear" else 1 - a).float()
+    x = torch.ones(1, T, D, device="cuda")
+    x[:, 5, 0], x[:, 40, 1], x[:, 100, 2], x[:, 7, 3] = inf, -inf, float("nan"), inf
+    initial = torch.zeros(1, D, device="cuda")
+    initial[:, 4] = inf
+    d = torch.ones(1, T, D, device="cuda")
+    d[:, T - 3, 5], d[:, T - 500, 6], d[:, T - 70, 7] = inf, -inf, float("nan")
+    leaves = [v.requires_grad_(True) for v in (gate, x, initial)]
+    states, last = gated_scan(*leaves, form=form)
+    dx, di = torch.autograd.grad((states, last), leaves[1:], (d, torch.zeros_like(last)))
+    want = walk(form, gate.detach().double(), x.detach().double()[:, :, None], initial.detach().double()[:, None], None, False, d.double()[:, :, None], torch.zeros(1, 1, D, dtype=torch.float64, device="cuda"))
+    for got, w, what in ((states, want["states"][0][:, :, 0], "states"), (last, want["last"][0][:, 0], "last"), (dx, want["d_x"][0][:, :, 0], "d_x"), (di, want["d_initial"][0][:, 0], "d_initial")):
+        for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(kind(got), kind(w)), (what, kind.__name__, int((kind(got) != kind(w)).sum()))
+        ok = torch.isfinite(w)
+        # sums of positive terms that a gate of a quarter forgets: 4 U a step of at most 4 / 3 of the result, and one product
+        assert bool(((got.double() - w)[ok].abs() <= 16 * U * w[ok].abs()).all()), what
