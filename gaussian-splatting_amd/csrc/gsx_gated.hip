@@ -621,7 +621,9 @@ using namespace gsx;
 GSX_API int64_t gsx_gated_marks_floats(int64_t B, int64_t T, int32_t planes, int64_t D)
 {
     if (B < 0 || T < 0 || D < 0 || planes < 1 || planes > GSX_GATED_MAX_PLANES) return GSX_E_INVALID;
-    return ceil_div(T, planes == 1 ? GatedBatch<1>::value : GatedBatch<2>::value) * planes * B * D;
+    if (T >= (1ll << 40) || B >= (1ll << 31) || D >= (1ll << 31) || (B && D > (1ll << 40) / B)) return GSX_E_RANGE;        // as gated_check
+    const int64_t batches = ceil_div(T, planes == 1 ? GatedBatch<1>::value : GatedBatch<2>::value), each = planes * B * D;
+    return each && batches > (1ll << 60) / each ? (int64_t)GSX_E_RANGE : batches * each;
 }
 
 GSX_API size_t gsx_gated_workspace_bytes(const gsx_gated* s, int32_t backward)

@@ -74,7 +74,10 @@ class _GatedScan(torch.autograd.Function):
         head = _head(gate, x, h0, lengths, form, reverse)
         marks = None
         if want_grad:
-            marks = torch.empty(L.lib().gsx_gated_marks_floats(head[4], head[5], head[3], head[6]), dtype=torch.float32, device=dev)
+            n = L.lib().gsx_gated_marks_floats(head[4], head[5], head[3], head[6])
+            if n < 0:
+                L.check(n, "gsx_gated_marks_floats")
+            marks = torch.empty(n, dtype=torch.float32, device=dev)
         _call("gsx_gated_scan_fwd", 0, head, (states.data_ptr() if want_states else 0, last.data_ptr(), marks.data_ptr() if want_grad else 0,
                                               0, 0, 0, 0, 0, 0, 0, 0), dev)
         if want_grad:

@@ -422,7 +422,7 @@ int gsx_merge_greedy_host(int32_t N, const uint32_t* offsets_host, const uint32_
  * lengths: sequence b consists of steps 0 .. lengths[b] - 1 only (clamped to 0 .. T); the steps behind it are not read, change no
  * state, and get zeros in states, d_gate and d_x.
  * fwd writes states (NULL: not wanted), last and marks (NULL: no backward follows; else gsx_gated_marks_floats floats: the 32-bit
- * state in front of every batch of steps, from which bwd runs the batch again).  bwd reads gate, x, lengths and marks as fwd left
+ * state in front of every batch of steps, from which bwd runs the batch again; the size is negative where the arguments are refused).  bwd reads gate, x, lengths and marks as fwd left
  * them, d_states and d_last (each may be NULL: zeros), and writes d_gate (B x T x D), d_x (B x T x planes x D) and d_initial, all
  * contiguous, each NULL if not wanted.  No atomics: results are the same bits every time.
  * ws: gsx_gated_workspace_bytes of the struct as it is handed over otherwise (often 0), 256-byte aligned; each call may have its own.

@@ -162,6 +162,14 @@ def test_first_calls_of_two_threads(monkeypatch):
     assert set(recurrence._entries()) == want and seen == [want]
 
 
+def test_marks_beyond_64_bits_are_refused():
+    """inputs with strides of zero need no memory, so the size is the only thing that stands in the way of such a call"""
+    size = L.lib().gsx_gated_marks_floats
+    for args in ((1, 1 << 39, 1, 1 << 30), (1 << 20, (1 << 40) - 16, 4, 1 << 20), (1 << 20, 1 << 30, 1, 1 << 20), (1 << 31, 1, 1, 1), (1, 1 << 40, 1, 1), (1, 1, 1, 1 << 31), (1 << 21, 1, 1, 1 << 20)):
+        assert size(*args) == L.GSX_E_RANGE, args
+    assert size(1, (1 << 40) - 1, 1, 1) == 1 << 36 and size(1 << 20, 16, 1, 1 << 20) == 1 << 40 and size(0, 1 << 30, 4, 1 << 30) == 0
+
+
 @pytest.mark.parametrize("which", [0, 1, 2], ids=["state", "gate", "x"])
 def test_step_refuses_to_drop_a_gradient(which):
     args = [z(4), z(4), z(4)]
