@@ -1,10 +1,12 @@
 """Draws from softmax(logits / temperature) by given random numbers (csrc/gsx_draw.hip): what GaussianSplat.get_dense_points does with a
 scene's opacities (/root/reference/model/gaussian_splatting.py:420-443), with the cuts by rank, mass and share, for one row of
 millions of Gaussians as for many rows (a layer per pixel, a batch of a large alphabet)."""
+import math
 import torch
 from . import _lib as L
 from .recurrence import DTYPES, _ptr, _refuse_host
 
+WHOLE = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8, torch.bool)
 MAX_V = 1 << 27                                                  # GSX_DRAW_MAX_V
 
 
@@ -13,8 +15,8 @@ def _setting(v, name, R, device, dtype, ok, where):
     if torch.is_tensor(v):
         if v.shape != (R,) or v.device != device:
             raise ValueError(f"{name} must be a number or ({R},) on {device}, got {tuple(v.shape)} on {v.device}")
-        if dtype == torch.int32 and (v.is_floating_point() or v.is_complex()):
-            raise TypeError(f"{name} by row must be whole numbers, got {v.dtype}")
+        if dtype == torch.int32 and v.dtype not in WHOLE:
+            raise TypeError(f"{name} by row must be whole numbers of up to 64 bits with a sign, got {v.dtype}")
         v = v.detach()
         if v.dtype == torch.int64 and dtype == torch.int32:
             v = v.clamp(-1, MAX_V)                               # all tokens and more, where a cast alone would wrap
@@ -45,7 +47,7 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ret
         raise ValueError(f"a row may have {MAX_V} tokens, got {V}")
     dev = logits.device
     t, ts = _setting(temperature, "temperature", R, dev, torch.float32, lambda v: v >= 0, "0 or more")
-    k, ks = _setting(top_k, "top_k", R, dev, torch.int32, lambda v: 0 <= v == int(v), "a whole number, 0 or more")
+    k, ks = _setting(top_k, "top_k", R, dev, torch.int32, lambda v: 0 <= v < math.inf and v == int(v), "a whole number, 0 or more")
     p, ps = _setting(top_p, "top_p", R, dev, torch.float32, lambda v: v > 0, "above 0")
     m, ms = _setting(min_p, "min_p", R, dev, torch.float32, lambda v: 0 <= v <= 1, "in [0, 1]")
     _refuse_host(logits, "sampling")
