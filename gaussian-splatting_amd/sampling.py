@@ -6,7 +6,7 @@ import torch
 from . import _lib as L
 from .recurrence import DTYPES, _ptr, _refuse_host
 
-WHOLE = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8, torch.bool)
+WIDE = (torch.int64, torch.uint32, torch.uint64)
 MAX_V = 1 << 27                                                  # GSX_DRAW_MAX_V
 
 
@@ -15,11 +15,11 @@ def _setting(v, name, R, device, dtype, ok, where):
     if torch.is_tensor(v):
         if v.shape != (R,) or v.device != device:
             raise ValueError(f"{name} must be a number or ({R},) on {device}, got {tuple(v.shape)} on {v.device}")
-        if dtype == torch.int32 and v.dtype not in WHOLE:
-            raise TypeError(f"{name} by row must be whole numbers of up to 64 bits with a sign, got {v.dtype}")
+        if dtype == torch.int32 and (v.is_floating_point() or v.is_complex()):
+            raise TypeError(f"{name} by row must be whole numbers, got {v.dtype}")
         v = v.detach()
-        if v.dtype == torch.int64 and dtype == torch.int32:
-            v = v.clamp(-1, MAX_V)                               # all tokens and more, where a cast alone would wrap
+        if dtype == torch.int32 and v.dtype in WIDE:
+            v = v.to(torch.int64).clamp(-1, MAX_V)               # all tokens and more, where a cast alone would wrap (from 2^63 on it is negative: all)
         return 0, v.to(dtype).contiguous()
     if not ok(v):
         raise ValueError(f"{name} must be {where}, got {v}")

@@ -465,3 +465,11 @@ def test_long_ties_under_both_cuts(R, V, S, dtype):
         for r in rows:
             want, _ = oracle_row(logits[r].double().cpu().numpy(), u[r].cpu().numpy(), 1.0, k, float(np.float32(p)), float(np.float32(m)))
             assert np.array_equal(got[r], want), (r, k, p, np.nonzero(got[r] != want)[0][:4])
+
+
+@pytest.mark.parametrize("t,k", [(torch.uint64, [2 ** 32 + 3, 3, 0, 700]), (torch.uint32, [2 ** 31 + 5, 2 ** 32 - 1, 4, 0]), (torch.uint16, [65535, 2, 0, 100]), (torch.uint8, [255, 1, 0, 7])], ids=str)
+def test_ranks_by_row_of_unsigned_types(t, k):
+    from gaussian_splatting_amd import sample
+    logits, u = rand(13, 4, 700, 50)
+    want = torch.tensor([min(v, 700) for v in k], dtype=torch.int32, device="cuda")
+    assert torch.equal(sample(logits, u, top_k=torch.tensor(k, dtype=t).cuda()), sample(logits, u, top_k=want))

@@ -162,9 +162,9 @@ def test_first_calls_of_two_threads(monkeypatch):
     assert set(recurrence._entries()) == want and seen == [want]
 
 
-@pytest.mark.parametrize("k,err", [(math.inf, ValueError), (-math.inf, ValueError), (math.nan, ValueError), (torch.zeros(3, dtype=torch.uint64), TypeError), (torch.zeros(3, dtype=torch.uint32), TypeError)])
+@pytest.mark.parametrize("k,err", [(math.inf, ValueError), (-math.inf, ValueError), (math.nan, ValueError)])
 def test_ranks_that_are_no_numbers_of_tokens(k, err):
-    """an endless rank is no whole number, and unsigned ones would wrap on their way to 32 bits"""
+    """an endless rank is no whole number"""
     with pytest.raises(err, match="top_k"):
         sample(z(3, 5), z(3, 2), top_k=k)
 
