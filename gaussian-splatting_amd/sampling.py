@@ -6,12 +6,13 @@ import torch
 from . import _lib as L
 from .recurrence import DTYPES, _ptr, _refuse_host
 
+LEAST = 2.0 ** -126                                              # the smallest normal number of 32 bits
 WIDE = (torch.int64, torch.uint32, torch.uint64)
 MAX_V = 1 << 27                                                  # GSX_DRAW_MAX_V
 
 
-def _setting(v, name, R, device, dtype, ok, where):
-    """(number, tensor): a setting of all rows, or one per row"""
+def _setting(v, name, R, device, dtype, ok, where, positive=False):
+    """(number, tensor): a setting of all rows, or one per row; positive: one above 0 stays above 0 in 32 bits"""
     if torch.is_tensor(v):
         if v.shape != (R,) or v.device != device:
             raise ValueError(f"{name} must be a number or ({R},) on {device}, got {tuple(v.shape)} on {v.device}")
@@ -20,10 +21,12 @@ def _setting(v, name, R, device, dtype, ok, where):
         v = v.detach()
         if dtype == torch.int32 and v.dtype in WIDE:
             v = v.to(torch.int64).clamp(-1, MAX_V)               # all tokens and more, where a cast alone would wrap (from 2^63 on it is negative: all)
+        if positive and v.dtype == torch.float64:
+            v = torch.where(v > 0, v.clamp(min=LEAST), v)
         return 0, v.to(dtype).contiguous()
     if not ok(v):
         raise ValueError(f"{name} must be {where}, got {v}")
-    return v, None
+    return (max(v, LEAST) if positive and v > 0 else v), None
 
 
 @torch.no_grad()
@@ -32,7 +35,7 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ret
     probabilities, float32).  Tokens are ranked by (logit descending, index ascending); kept are the first top_k (0: all), of these the
     fewest whose mass reaches top_p of their mass, of these the ones at least min_p times as likely as the first.  A draw is the lowest
     index whose inclusive kept mass, in index order, exceeds u times all kept mass (u of 1 and more: the largest double below 1; below 0 and NaN: 0).
-    temperature (0: the lowest index of the largest logit), top_k, top_p and min_p are numbers or tensors of one value per row.  NaN and -inf logits
+    temperature (0: the lowest index of the largest logit), top_k, top_p and min_p are numbers or tensors of one value per row, taken in 32 bits (what is above 0 stays so).  NaN and -inf logits
     are masked; a row with nothing left, or with a value of its own out of range, gives -1 (and -inf).  float32 uniforms have 24 bits:
     take float64 where V is in the millions.  Not differentiable."""
     if logits.dim() != 2 or uniforms.dim() != 2 or uniforms.shape[0] != logits.shape[0]:
@@ -46,9 +49,9 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ret
     if V > MAX_V:
         raise ValueError(f"a row may have {MAX_V} tokens, got {V}")
     dev = logits.device
-    t, ts = _setting(temperature, "temperature", R, dev, torch.float32, lambda v: v >= 0, "0 or more")
+    t, ts = _setting(temperature, "temperature", R, dev, torch.float32, lambda v: v >= 0, "0 or more", positive=True)
     k, ks = _setting(top_k, "top_k", R, dev, torch.int32, lambda v: 0 <= v < math.inf and v == int(v), "a whole number, 0 or more")
-    p, ps = _setting(top_p, "top_p", R, dev, torch.float32, lambda v: v > 0, "above 0")
+    p, ps = _setting(top_p, "top_p", R, dev, torch.float32, lambda v: v > 0, "above 0", positive=True)
     m, ms = _setting(min_p, "min_p", R, dev, torch.float32, lambda v: 0 <= v <= 1, "in [0, 1]")
     _refuse_host(logits, "sampling")
     lib = L.lib()

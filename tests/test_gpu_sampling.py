@@ -473,3 +473,22 @@ def test_ranks_by_row_of_unsigned_types(t, k):
     logits, u = rand(13, 4, 700, 50)
     want = torch.tensor([min(v, 700) for v in k], dtype=torch.int32, device="cuda")
     assert torch.equal(sample(logits, u, top_k=torch.tensor(k, dtype=t).cuda()), sample(logits, u, top_k=want))
+
+
+@pytest.mark.parametrize("V", [6, 300, 5000, 17001, 70000])
+def test_settings_near_zero(V):
+    """a temperature that 32 bits round to 0 still shares the draws out among equal largest logits, and such a share still keeps the first token"""
+    from gaussian_splatting_amd import sample
+    logits, u = rand(V, 2, V, 400, f64=True)
+    ties = torch.tensor([1, V // 2, V - 2], device="cuda")
+    logits[:, ties] = 20.0
+    want = ties[(u * 3).floor().long()]
+    R = torch.full((2,), 1.0, dtype=torch.float64, device="cuda")
+    for T in (1e-50, 5e-324, 2.0 ** -149, 1e-40, 1e-37):
+        assert torch.equal(sample(logits, u, temperature=T), want), T
+        assert torch.equal(sample(logits, u, temperature=R * T), want), T
+        assert torch.equal(sample(logits, u, temperature=T, top_p=0.5), ties[(u * 2).floor().long()]), T
+        assert torch.equal(sample(logits, u, temperature=T, top_k=2), ties[(u * 2).floor().long()]), T
+    for p in (1e-50, 5e-324, 2.0 ** -149, 1e-40):
+        assert bool((sample(logits, u, top_p=p) == 1).all()) and bool((sample(logits, u, top_p=R * p) == 1).all()), p
+    assert bool((sample(logits, u, temperature=0.0) == 1).all()) and bool((sample(logits, u, temperature=R * 0) == 1).all()) and bool((sample(logits, u, top_p=R * 0) == -1).all())
