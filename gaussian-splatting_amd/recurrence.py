@@ -24,8 +24,14 @@ def _channels(t):
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _format(structure):
+    """the struct format of a ctypes structure: its fields one after the other, addresses as unsigned words"""
+    codes = {C.c_int32: "i", C.c_int64: "q", C.c_void_p: "Q", C.c_size_t: "Q"}
+    return "".join(f"{t._length_}{codes[t._type_]}" if hasattr(t, "_length_") else codes[t] for _, t in structure._fields_)
+
+
 # struct gsx_gated as bytes: filling the ctypes structure field by field takes several times as long
-_PACK = struct.Struct("4i3qQ2qQ3q5QQ3q4QQQ").pack
+_PACK = struct.Struct(_format(L.GsxGated)).pack
 _entry = None
 
 

@@ -195,3 +195,36 @@ def test_step_refuses_inputs_that_overlap_the_state():
         for other in (at + 4, at - 4, at + 4 * n - size, at - size * n + size) + ((at,) if size == 2 else ()):
             assert lib.gsx_gated_step(dtype, 0, n, at, other, far, None) == L.GSX_E_INVALID, (dtype, other - at)
             assert lib.gsx_gated_step(dtype, 0, n, at, far, other, None) == L.GSX_E_INVALID, (dtype, other - at)
+
+
+def test_what_is_packed_is_the_struct(monkeypatch):
+    """both directions of a scan up to the library's door, which is replaced: every field of the struct holds what it is named for"""
+    from gaussian_splatting_amd import recurrence
+    calls = []
+
+    def door(name):
+        def entry(packed, other):
+            assert len(packed) == C.sizeof(L.GsxGated)
+            calls.append((name, L.GsxGated.from_buffer_copy(packed)))
+            return 512 if name.endswith("bytes") else 0
+        return entry
+    monkeypatch.setattr(recurrence, "_entry", {n: door(n) for n in ("gsx_gated_workspace_bytes", "gsx_gated_scan_fwd", "gsx_gated_scan_bwd")})
+    monkeypatch.setattr(recurrence, "_refuse_host", lambda x, name: None)
+    monkeypatch.setattr(L, "stream_ptr", lambda dev: 0)
+    B, T, P, D = 2, 5, 3, 7
+    gate, x = z(T, B, D + 1, t=torch.bfloat16)[:, :, 1:].transpose(0, 1), z(B, T, P, D, t=torch.bfloat16)
+    initial, lengths = z(B, P, D), torch.tensor([3, 5], dtype=torch.int32)
+    leaves = [v.requires_grad_(True) for v in (gate, x, initial)]
+    states, last = gated_scan(*leaves, lengths=lengths, form="over", reverse=True)
+    grads = torch.autograd.grad((states, last), leaves, (z(B, T, P, D, t=torch.bfloat16), z(B, P, D)))
+    assert [n for n, _ in calls] == ["gsx_gated_workspace_bytes", "gsx_gated_scan_fwd", "gsx_gated_workspace_bytes", "gsx_gated_scan_bwd"]
+    (_, sized), (_, f), _, (_, b) = calls
+    assert sized.ws is None and sized.ws_bytes == 0
+    for s in (f, b):
+        assert (s.dtype, s.form, s.reverse, s.planes, s.B, s.T, s.D) == (1, 2, 1, P, B, T, D)
+        assert s.gate == gate.data_ptr() and list(s.gate_stride) == [D + 1, B * (D + 1)] and s.x == x.data_ptr() and list(s.x_stride) == [T * P * D, P * D, D]
+        assert s.lengths == lengths.data_ptr() and s.marks and s.ws and s.ws_bytes == 512
+    assert f.initial == initial.data_ptr() and f.states == states.data_ptr() and f.last == last.data_ptr() and f.marks == b.marks
+    assert not (f.d_states or f.d_last or f.d_gate or f.d_x or f.d_initial or b.initial or b.states or b.last)
+    assert b.d_states and list(b.d_states_stride) == [T * P * D, P * D, D] and b.d_last
+    assert [b.d_gate, b.d_x, b.d_initial] == [g.data_ptr() for g in grads]
