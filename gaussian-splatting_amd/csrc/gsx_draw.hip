@@ -15,7 +15,7 @@
 // A histogram's 2048 bins are 1/64 of a unit of (top - l) / T wide: the tokens spread over hundreds of bins (few collisions in LDS), and the bin where
 // a cut falls holds few enough tokens to be ranked in LDS.  Where it does not (ties, extreme temperatures), narrower histograms of the 59-bit rank
 // (key, index) follow until it does: every row ends, whatever its values.
-// Measured, us a call and what bounds it: 640000 rows of 32, 4 draws each, 55 (short; issue, 475 instructions a wave of eight rows); one row of 5000 16 (row; a workgroup's chain
+// Measured with three inputs in turn, us a call and what bounds it: 640000 rows of 32, 4 draws each, 55 (short; issue, 475 instructions a wave of eight rows); one row of 5000 16 (row; a workgroup's chain
 // of passes); 256 rows of 131072 in 32 bits 117 (row; the top 16, the histogram 17, the pass of 64-bit weights 50 by issue, the decision 7, against 26 for the bytes);
 // 64 rows of 100003 in 16 bits 49 (parts; seven launches that wait for one another); one row of 1 M and 1 M draws 48, of 6 M with a top p 138 (parts; loads that wait).
 #include <type_traits>
@@ -27,7 +27,8 @@ constexpr int kDrawBins = 2048;                     // of the first histogram
 constexpr float kDrawBinsPerUnit = 64.0f;
 constexpr int kDrawFine = 512;                      // bins of the narrower ones
 constexpr int kDrawCand = 1024;                     // tokens that are ranked in LDS
-// Which way, thread count and kernels a call takes; us a call, by length, rows and draws, of N(0, 2) logits in 32 bits cut to k = 50, p = 0.9:
+// Which way, thread count and kernels a call takes; us a call, by length, rows and draws, of N(0, 2) logits in 32 bits cut to k = 50, p = 0.9, one input
+// repeated in a graph (here and at the rules further down: a few per cent less than with inputs in turn, on both sides):
 // Longest row of the short way.  100000 rows of 500: 532, with a workgroup each 2866; one row of 500: 19 against 15.
 constexpr int kDrawShort = 512;
 // Longest row whose workgroup is of 512 threads and decides by itself in every case; 1024 threads read a longer one sooner while it has a CU to itself, and of more rows
@@ -599,7 +600,6 @@ __device__ __forceinline__ u64 draw_cuts(DrawCut& c, const DrawHist& hist, DrawF
 // of one bin), not where.  One pass then adds up the 64-bit weights of the tokens in front of the bracket, which are kept whatever
 // happens, and collects the tokens inside it and in the bin where the top k end; these few are ranked and decided exactly.  `false`: too
 // many of them, or the sums do not bear the bracket out; the longer way has no such limits.
-// mass(q, w): adds a weight that is kept for certain to tile q (all lanes of the wave call it, once per group).
 // A bin is one 64-bit word, one atomic per token: its tokens from bit 45 on, below the 32-bit weights in units of 2^-26 (2^19 tokens fit both).
 constexpr int kDrawCountBit = 45;
 constexpr int64_t kDrawMostInHist = 1 << 19;
@@ -727,8 +727,8 @@ __device__ __forceinline__ bool draw_decide(DrawCut& c, DrawCand& cand, const Dr
     return true;
 }
 
-// The cuts of a row exactly from the first histogram on: for rows that the quicker way cannot decide (ties, brackets of too many tokens), in kernels
-// of their own, whose registers would cost the others.
+// The cuts of a row exactly from the first histogram on: for rows that the quicker way cannot decide (ties, brackets of too many tokens).  The workgroups of 512 threads
+// (short enough rows, the floor of rows in parts) go on with it at once; behind those of 1024, whose registers it would not leave room for, a kernel of its own does.
 template <typename T, int NT>
 __device__ __forceinline__ u64 draw_exact_floor(const DrawArgs& a, const Places<T>& row, const DrawRow& set, float top, DrawCut& c, DrawHist& hist, DrawFine& fine, DrawCand& cand)
 {
@@ -870,7 +870,7 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(DrawArgs a)
     const int groups = row.groups();
     const DrawRow set = draw_row(a, r);
     float top = -__builtin_inff();
-    constexpr int kAhead = 2;                                        // groups in flight per thread, here and below: 256 rows of 131072 113 us with 2, 114 with 4, 121 with 8, 116 with 1
+    constexpr int kAhead = 2;                                        // groups in flight per thread, here and below: 256 rows of 131072, one input repeated, 113 us with 2, 114 with 4, 121 with 8, 116 with 1
     for (int g = tid; g < groups; g += kAhead * NT) {
         float l[kAhead][4];
         row.load_many(g, NT, groups, l);

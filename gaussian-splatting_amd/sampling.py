@@ -37,7 +37,7 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ret
     index whose inclusive kept mass, in index order, exceeds u times all kept mass (u of 1 and more: the largest double below 1; below 0 and NaN: 0).
     temperature (0: the lowest index of the largest logit), top_k, top_p and min_p are numbers or tensors of one value per row, taken in 32 bits (what is above 0 stays so).  NaN and -inf logits
     are masked; a row with nothing left, or with a value of its own out of range, gives -1 (and -inf).  float32 uniforms have 24 bits:
-    take float64 where V is in the millions.  Not differentiable."""
+    take float64 where V is in the millions.  V is 2^27 at most, 524284 for more than 65535 rows.  Not differentiable."""
     if logits.dim() != 2 or uniforms.dim() != 2 or uniforms.shape[0] != logits.shape[0]:
         raise ValueError(f"logits (R, V) and uniforms (R, S) are wanted, got {tuple(logits.shape)} and {tuple(uniforms.shape)}")
     if logits.dtype not in DTYPES or uniforms.dtype not in (torch.float32, torch.float64):

@@ -461,7 +461,7 @@ int gsx_gated_step(int32_t dtype, int32_t form, int64_t n, float* state, const v
  * GSX_DRAW_MAX_V tokens (multinomial stops at 2^24) and for many rows.
  * logits R x V of `dtype`, rows row_stride elements apart; NaN and -inf are masked tokens, never drawn; +inf takes all mass.
  * Per row (the array) or for all rows (the number, where the array is NULL): temperature >= 0 (0: the lowest index of the largest logit), top_k
- * (<= 0: off), top_p > 0 (>= 1: off), 0 <= min_p <= 1 (0: off).  Tokens are ranked by (logit descending, index ascending).  Kept are the
+ * (a number of 0, by row 0 and less: off), top_p > 0 (>= 1: off), 0 <= min_p <= 1 (0: off).  Tokens are ranked by (logit descending, index ascending).  Kept are the
  * first top_k; of these the fewest whose mass reaches top_p of their mass; of these the ones whose probability is at least min_p
  * times the largest.
  * uniforms R x S, contiguous, floats or (uniforms_f64) doubles in [0, 1) (below and NaN: 0; 1 and above: the largest double below 1).  24 random bits cannot tell 2^24 tokens apart: give
