@@ -12,7 +12,7 @@
 // h -> A h + H, and every workgroup's spans to one; the second begins each span from what the spans in front of it come to.  One pass that hands
 // the state from workgroup to workgroup would read once, but its waves would wait for one another in a chain of hundreds.
 // Measured, with other inputs and outputs in turn, against a copy's 5.15 TB/s: 60 steps x 1 M channels in 32 bits 134 us (5.4 TB/s); 32 layers of 800 x 800 (3 planes in
-// 32 bits) 66 us forward (5.5) and 120 backward (5.7); split, 2 x 32768 x 512 in bf16, mean of the folds 31 us (4.3), walks 36 forward (5.8) and 62 backward (5.5).
+// 32 bits) 66 us forward (5.5) and 120 backward (5.7); split, 2 x 32768 x 512 in bf16, mean of the folds 33 us (4.1), walks 35 forward (5.7) and 62 backward (5.4).
 #include <type_traits>
 #include "gsx_common.h"
 
@@ -159,7 +159,8 @@ __device__ __forceinline__ void gated_fwd_batch(const GatedArgs& p, const Lane& 
 
 // A product of gates in 64 bits that stays finite: times a zero state it is a zero, times any other one it leaves 32 bits, as the walk would.  Four more gates of up to 2^128
 // reach 2^1012 at most, two products 2^1000.  And that stays off zero, unless a gate is one: an infinite state stays infinite, as in the walk, and any other one falls
-// below 32 bits all the same (2^128 2^-400).  Four more gates of 2^-149 at least leave 2^-996, two products 2^-800.
+// below 32 bits all the same (2^128 2^-400).  Four more gates of 2^-149 at least leave 2^-996, two products 2^-800.  (2 x 32768 x 512 in bf16: 2 us of 164.  On the exponent's word, or once a batch where a
+// product has become small, it costs 4, in registers.)
 __device__ __forceinline__ double gated_bound(double A)
 {
     const double m = fmin(fabs(A), 0x1p500);
@@ -195,7 +196,7 @@ __device__ __forceinline__ void gated_fold_batch(const GatedArgs& p, const Lane&
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const double zd = (double)to_f(z[k].v[i]), a = FORM == GSX_GATED_LINEAR ? zd : 1.0 - zd;
-                A[i] = (q & 3) == 3 ? gated_bound(A[i] * a) : A[i] * a;
+                A[i] = !WHOLE || (q & 3) == 3 ? gated_bound(A[i] * a) : A[i] * a;       // a sequence may begin and end anywhere in a batch
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     const double vd = HASV ? (double)to_f(v[k][r].v[i]) : 0.0;
